@@ -376,6 +376,38 @@ int qmoe_moe_decode_workspace_size(const qmoe_moe_decode_desc* d, int64_t* bytes
 int qmoe_moe_decode(const qmoe_moe_decode_desc* d, void* workspace, int64_t ws_bytes, qmoe_stream_t stream);
 
 /*
+ * Rows of the vocabulary table: out[n] = round(scale * s[id] * w[id]), id =
+ * ids[n]. Replaces the gather + dequantize of `layers/adapter/quantization/
+ * fp8.py:1692-1698` (VllmFp8LinearMethodTPU.embedding) with one launch, and the
+ * plain gather of an unquantized table.
+ *   ids     : int32, or int64 with ids_i64 [N]; an id outside [0, V) gives a
+ *             row of NaN
+ *   w       : [V, ldw >= H] of `wtype`: 0 bf16, 1 f32, 3 e4m3fn, 4 int8, 5 e5m2
+ *   row_scale: f32 [V] for the 1-byte types (rounded to the output type before
+ *             the product, as the reference does), else NULL
+ *   out     : [N, ldo >= H] of `otype`: 0 bf16, 1 f32, 2 f16
+ * N < 2^24, V <= 2^27, H <= 2^20.
+ */
+int qmoe_vocab_lookup(const void* ids, int ids_i64, int64_t N, const void* w, int wtype, int64_t ldw,
+                      const float* row_scale, int64_t V, int64_t H, float scale, void* out, int otype, int64_t ldo,
+                      qmoe_stream_t stream);
+
+/*
+ * Gradient of the lookup with respect to the table (no counterpart in the
+ * reference, which serves only): dw[v] = round(scale * sum of grad[n] over
+ * ids[n] == v), float32 sums in the order of n whatever the launch (the result
+ * is bit-identical from call to call). Ids outside [0, V) and `padding_idx`
+ * (-1: none) add nothing. add = 0: every row of dw is written (zeros without a
+ * token); add = 1: the sums are added to the rows that have a token, the
+ * others are neither read nor written. grad [N, ldg >= H], dw [V, lddw >= H] of
+ * types 0 bf16 or 1 f32. The workspace needs no initialisation.
+ */
+int qmoe_vocab_lookup_grad_workspace_size(int64_t N, int64_t V, int64_t H, int64_t* bytes);
+int qmoe_vocab_lookup_grad(const void* ids, int ids_i64, int64_t N, const void* grad, int gtype, int64_t ldg, int64_t V,
+                           int64_t H, float scale, int64_t padding_idx, void* dw, int wtype, int64_t lddw, int add,
+                           void* workspace, int64_t ws_bytes, qmoe_stream_t stream);
+
+/*
  * Plain read of `bytes` (a multiple of 16, 16-byte aligned) at `src` by at
  * most `workgroups` 256-thread workgroups; `sink` receives at most one dword
  * per workgroup ([workgroups] uint32, normally untouched). No counterpart in

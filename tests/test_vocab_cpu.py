@@ -1,0 +1,85 @@
+"""The vocabulary operators without a GPU: shapes and types under fake
+tensors, and the refusals of the wrappers and of the C entry points."""
+
+import ctypes
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from qmoe import _capi, ops
+from qmoe.layers.vocab import embedding
+
+
+def test_lookup_fake_shapes_and_gradient():
+    with FakeTensorMode():
+        w = torch.empty((1000, 96), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+        ids = torch.empty((3, 5), dtype=torch.int32, device="cuda")
+        out = embedding(ids, w, scale=2.0, padding_idx=7)
+        assert out.shape == (3, 5, 96) and out.dtype == torch.bfloat16
+        assert out.requires_grad
+        dw = torch.ops.qmoe.vocab_lookup_grad(torch.empty_like(out), ids, 1000, 2.0, 7, torch.bfloat16)
+        assert dw.shape == w.shape and dw.dtype == w.dtype
+        q = torch.empty((1000, 96), dtype=torch.float8_e4m3fn, device="cuda")
+        out = embedding(ids, q, torch.empty((1000, 1), device="cuda"), out_dtype=torch.float32)
+        assert out.shape == (3, 5, 96) and out.dtype == torch.float32
+
+
+def test_lookup_refusals():
+    w, ids = torch.zeros((8, 16), dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="device tensors"):
+        embedding(ids, w)
+    with pytest.raises(ValueError, match="int32 or int64"):
+        embedding(ids.to(torch.int16), w)
+    with pytest.raises(ValueError, match="one scale per row"):
+        embedding(ids, w.to(torch.float8_e4m3fn))
+    with pytest.raises(ValueError, match="no row scales"):
+        embedding(ids, w, torch.ones(8))
+    with pytest.raises(ValueError, match="row scales must be"):
+        embedding(ids, w.to(torch.int8), torch.ones(7))
+    with pytest.raises(ValueError, match="contiguous"):
+        embedding(ids, w.t())
+    with pytest.raises(ValueError, match="bf16, f32"):
+        embedding(ids, w.to(torch.float16))
+    with pytest.raises(ValueError, match="padding_idx"):
+        embedding(ids, w, padding_idx=8)
+    with pytest.raises(ValueError, match="bf16, f16 or f32"):
+        embedding(ids, w, out_dtype=torch.float64)
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        q = w.float().requires_grad_()
+        embedding(ids, q.to(torch.float8_e4m3fn), torch.ones(8))
+    with pytest.raises(NotImplementedError, match="not f16"):
+        embedding(ids, w.clone().requires_grad_(), out_dtype=torch.float16)
+
+
+def test_lookup_grad_refusals():
+    g, ids = torch.zeros((3, 16)), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="device tensors"):
+        ops.vocab_lookup_grad(g, ids, 8)
+    with pytest.raises(ValueError, match="for ids of"):
+        ops.vocab_lookup_grad(g[:2], ids, 8)
+    with pytest.raises(ValueError, match="bf16 or f32"):
+        ops.vocab_lookup_grad(g.half(), ids, 8)
+    with pytest.raises(ValueError, match="padding_idx"):
+        ops.vocab_lookup_grad(g, ids, 8, padding_idx=-1)
+    with pytest.raises(ValueError, match="`into`"):
+        ops.vocab_lookup_grad(g, ids, 8, into=torch.zeros((7, 16)))
+    with pytest.raises(ValueError, match="not torch.float16"):
+        ops.vocab_lookup_grad(g, ids, 8, dtype=torch.float16)
+
+
+def test_lookup_entry_points_check_their_arguments():
+    lib, n = _capi.lib, ctypes.c_int64(0)
+    a = ctypes.c_void_p(0x1000)
+    call = lambda N=4, wt=0, ldw=64, rs=None, V=8, H=64, ot=0: lib.qmoe_vocab_lookup(  # noqa: E731
+        a, 1, N, a, wt, ldw, rs, V, H, 1.0, a, ot, 64, None)
+    assert call(N=-1) == 1 and call(N=1 << 24) == 1 and call(V=0) == 1 and call(ldw=63) == 1 and call(ot=3) == 1
+    assert call(wt=2) == 1 and call(wt=6) == 1
+    assert call(wt=3) == 1 and call(rs=a) == 1  # row scales exactly for 1-byte codes
+    assert call(N=0) == 0
+    assert lib.qmoe_vocab_lookup_grad_workspace_size(100, 50, 64, ctypes.byref(n)) == 0 and n.value > 0
+    assert lib.qmoe_vocab_lookup_grad_workspace_size(100, 0, 64, ctypes.byref(n)) == 1
+    grad = lambda gt=0, wt=0, ws=a, size=1 << 20, ldg=64: lib.qmoe_vocab_lookup_grad(  # noqa: E731
+        a, 1, 100, a, gt, ldg, 50, 64, 1.0, -1, a, wt, 64, 0, ws, size, None)
+    assert grad(gt=2) == 1 and grad(wt=3) == 1 and grad(ldg=63) == 1
+    assert grad(ws=None) == 2 and grad(size=n.value - 1) == 2

@@ -18,7 +18,7 @@ import torch  # noqa: F401  (its HIP runtime first; see above)
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libqmoe.so")
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 QMOE_OK = 0
 STATUS_TEXT = {
@@ -162,6 +162,14 @@ def _load():
     lib.qmoe_moe_decode_workspace_size.argtypes = [ctypes.POINTER(DecodeDesc), ctypes.POINTER(_i64)]
     lib.qmoe_moe_decode.restype = ctypes.c_int
     lib.qmoe_moe_decode.argtypes = [ctypes.POINTER(DecodeDesc), _vp, _i64, _vp]
+    lib.qmoe_vocab_lookup.restype = ctypes.c_int
+    lib.qmoe_vocab_lookup.argtypes = [_vp, ctypes.c_int, _i64, _vp, ctypes.c_int, _i64, _vp, _i64, _i64, _f32, _vp,
+                                      ctypes.c_int, _i64, _vp]
+    lib.qmoe_vocab_lookup_grad_workspace_size.restype = ctypes.c_int
+    lib.qmoe_vocab_lookup_grad_workspace_size.argtypes = [_i64, _i64, _i64, ctypes.POINTER(_i64)]
+    lib.qmoe_vocab_lookup_grad.restype = ctypes.c_int
+    lib.qmoe_vocab_lookup_grad.argtypes = [_vp, ctypes.c_int, _i64, _vp, ctypes.c_int, _i64, _i64, _i64, _f32, _i64, _vp,
+                                           ctypes.c_int, _i64, ctypes.c_int, _vp, _i64, _vp]
     lib.qmoe_stream_read.restype = ctypes.c_int
     lib.qmoe_stream_read.argtypes = [_vp, _i64, _i32, _vp, _vp]
     v = lib.qmoe_abi_version()
@@ -189,6 +197,9 @@ EXPORTED = (
     "qmoe_moe_combine",
     "qmoe_moe_decode_workspace_size",
     "qmoe_moe_decode",
+    "qmoe_vocab_lookup",
+    "qmoe_vocab_lookup_grad_workspace_size",
+    "qmoe_vocab_lookup_grad",
 )
 
 

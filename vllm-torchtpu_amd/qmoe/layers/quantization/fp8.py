@@ -37,6 +37,7 @@ import torch
 from qmoe import envs, ops
 from qmoe.layers.fused_moe import moe_forward
 from qmoe.layers.linear_common import KEEP_VLLM_LAYOUT_ATTR, quantized_matmul
+from qmoe.layers.vocab import embedding
 
 FP8 = torch.float8_e4m3fn
 # requantization targets (`fp8.py:122-127`); the short names are the ones
@@ -290,8 +291,11 @@ class Fp8LinearMethod:
     def embedding(self, layer, input_):
         """`fp8.py:1692-1698`: gather the rows of the ``[vocab, H]`` codes and
         their per-row scales, dequantize in the layer's dtype."""
-        flat = input_.reshape(-1)
         out_dtype = getattr(layer, "params_dtype", None) or getattr(layer, "orig_dtype", None) or torch.bfloat16
+        if (layer.weight.is_cuda and layer.weight_scale.dtype == torch.float32
+                and out_dtype in (torch.bfloat16, torch.float16, torch.float32)):
+            return embedding(input_, layer.weight, layer.weight_scale, out_dtype=out_dtype)
+        flat = input_.reshape(-1)
         w = torch.index_select(layer.weight, 0, flat).to(out_dtype)
         s = torch.index_select(layer.weight_scale.reshape(-1), 0, flat).to(out_dtype).unsqueeze(-1)
         return (w * s).reshape(*input_.shape, -1)

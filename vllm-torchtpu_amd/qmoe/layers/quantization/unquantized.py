@@ -8,6 +8,7 @@ import torch
 from qmoe import _capi, envs, ops
 from qmoe.layers.fused_moe import moe_forward
 from qmoe.layers.quantization.fp8 import _activation, _device, _param
+from qmoe.layers.vocab import embedding
 
 
 class UnquantizedLinearMethod:
@@ -27,6 +28,16 @@ class UnquantizedLinearMethod:
         if bias is not None:
             out = out + bias
         return out
+
+    def embedding(self, layer, input_):
+        """Rows of a bf16 ``[vocab, H]`` table (a `VocabParallelEmbedding` of an
+        unquantized checkpoint)."""
+        return embedding(input_, layer.weight)
+
+    def tie_weights(self, layer, embed_tokens):
+        """Share the embedding's table, as `fp8.py:1700-1704`."""
+        layer.weight = embed_tokens.weight
+        return layer
 
 
 class UnquantizedFusedMoEMethod:

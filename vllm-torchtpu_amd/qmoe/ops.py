@@ -638,3 +638,99 @@ def stream_read(buf, workgroups=2048, sink=None):
     check(lib.qmoe_stream_read(_ptr(buf), nbytes, workgroups, _ptr(sink), _stream(buf.device)), "stream_read")
     return sink
 
+
+
+# ---------------------------------------------------------------- vocabulary table
+
+_TABLE_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2, FP8: 3, torch.int8: 4, torch.float8_e5m2: 5}
+
+
+def _on_device(*ts):
+    """One device for every tensor given (None aside), made the current one
+    for the launches of a ``with`` block: the runtime launches on the current
+    device, whatever device the stream and the pointers belong to."""
+    _require_gpu(*ts)
+    devs = {t.device for t in ts if t is not None}
+    if len(devs) != 1:
+        raise ValueError(f"qmoe: tensors on different devices: {sorted(map(str, devs))}")
+    return torch.cuda.device(devs.pop())
+
+
+def _check_ids(ids, what):
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what} must be int32 or int64, got {ids.dtype}")
+    return ids.reshape(-1).contiguous()
+
+
+def _check_table(weight, weight_scale, what):
+    """A [V, H] table with contiguous rows: bf16 / f32, or 1-byte codes with one
+    float32 scale per row (returned as [V])."""
+    if weight.dim() != 2 or weight.dtype not in _TABLE_TYPES or weight.dtype == torch.float16:
+        raise ValueError(f"{what}: the table must be a [V, H] bf16, f32, e4m3, e5m2 or int8 tensor, got "
+                         f"{weight.dtype} {tuple(weight.shape)}")
+    if weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"{what}: empty table {tuple(weight.shape)}")
+    if weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]:
+        raise ValueError(f"{what}: the table's rows must be contiguous and apart, got strides {weight.stride()}")
+    coded = weight.element_size() == 1
+    if coded != (weight_scale is not None):
+        raise ValueError(f"{what}: a {weight.dtype} table takes {'one scale per row' if coded else 'no row scales'}")
+    if not coded:
+        return None
+    if weight_scale.dtype != torch.float32 or weight_scale.numel() != weight.shape[0]:
+        raise ValueError(f"{what}: row scales must be float32 [{weight.shape[0]}], got {weight_scale.dtype} "
+                         f"{tuple(weight_scale.shape)}")
+    return weight_scale.reshape(-1).contiguous()
+
+
+def vocab_lookup(ids, weight, weight_scale=None, scale=1.0, out_dtype=torch.bfloat16):
+    """Rows ``ids`` (any shape) of the table: round(scale * s * w) as
+    ``out_dtype`` (bf16, f16 or f32) ``[*ids.shape, H]``; see
+    include/qmoe.h `qmoe_vocab_lookup`. An id outside the table gives a row of
+    NaN."""
+    s = _check_table(weight, weight_scale, "vocab_lookup")
+    flat = _check_ids(ids, "vocab_lookup: ids")
+    if out_dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"vocab_lookup: the output is bf16, f16 or f32, not {out_dtype}")
+    V, H = weight.shape
+    with _on_device(flat, weight, s):
+        out = torch.empty((flat.numel(), H), dtype=out_dtype, device=weight.device)
+        check(lib.qmoe_vocab_lookup(_ptr(flat), int(flat.dtype == torch.int64), flat.numel(), _ptr(weight),
+                                    _TABLE_TYPES[weight.dtype], weight.stride(0), _ptr(s), V, H, float(scale),
+                                    _ptr(out), _TABLE_TYPES[out_dtype], H, _stream(weight.device)), "vocab_lookup")
+    return out.view(*ids.shape, H)
+
+
+def vocab_lookup_grad(grad, ids, vocab, scale=1.0, padding_idx=None, dtype=torch.bfloat16, into=None):
+    """Gradient of `vocab_lookup` with respect to a bf16 or f32 table: ``[vocab,
+    H]`` of ``dtype``, or with ``into`` (a table gradient to add to, e.g. that of
+    a tied output projection) only the rows that have a token, in place."""
+    if grad.dtype not in (torch.bfloat16, torch.float32) or grad.dim() < 1:
+        raise ValueError(f"vocab_lookup_grad: the gradient must be bf16 or f32 rows, got {grad.dtype}")
+    flat = _check_ids(ids, "vocab_lookup_grad: ids")
+    H = grad.shape[-1]
+    if tuple(grad.shape[:-1]) != tuple(ids.shape) or H == 0:
+        raise ValueError(f"vocab_lookup_grad: a gradient of {tuple(grad.shape)} for ids of {tuple(ids.shape)}")
+    g = grad.reshape(-1, H)
+    if g.numel() and (g.stride(1) != 1 or g.stride(0) < H):
+        g = g.contiguous()
+    if padding_idx is not None and not 0 <= padding_idx < vocab:
+        raise ValueError(f"vocab_lookup_grad: padding_idx {padding_idx} is outside the table of {vocab} rows")
+    if into is not None:
+        if into.dim() != 2 or tuple(into.shape) != (vocab, H) or into.dtype not in (torch.bfloat16, torch.float32) or \
+                into.stride(1) != 1 or into.stride(0) < H:
+            raise ValueError(f"vocab_lookup_grad: `into` must be a bf16 or f32 [{vocab}, {H}] tensor with contiguous rows")
+    elif dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"vocab_lookup_grad: the table's gradient is bf16 or f32, not {dtype}")
+    with _on_device(g, flat, into):
+        dw = into if into is not None else torch.empty((vocab, H), dtype=dtype, device=g.device)
+        need = ctypes.c_int64(0)
+        check(lib.qmoe_vocab_lookup_grad_workspace_size(flat.numel(), vocab, H, ctypes.byref(need)),
+              "vocab_lookup_grad (shape)")
+        ws, ws_n = _workspace(g.device, need.value)
+        check(lib.qmoe_vocab_lookup_grad(_ptr(flat), int(flat.dtype == torch.int64), flat.numel(), _ptr(g),
+                                         _TABLE_TYPES[g.dtype], g.stride(0) if g.numel() else H, vocab, H, float(scale),
+                                         -1 if padding_idx is None else int(padding_idx), _ptr(dw),
+                                         _TABLE_TYPES[dw.dtype], dw.stride(0), int(into is not None), _ptr(ws), ws_n,
+                                         _stream(g.device)), "vocab_lookup_grad")
+    return dw
