@@ -408,6 +408,48 @@ int qmoe_vocab_lookup_grad(const void* ids, int ids_i64, int64_t N, const void* 
                            void* workspace, int64_t ws_bytes, qmoe_stream_t stream);
 
 /*
+ * Softmax cross entropy of a projection onto the vocabulary table, without
+ * the [T, V] logits in memory (no counterpart in the reference, whose head is
+ * the full product of `layers/adapter/quantization/fp8.py:1679-1681`):
+ *   l[t, v] = s[v] x[t] . w[v],  lse[t] = log sum_v exp l[t, v],
+ *   loss[t] = lse[t] - l[t, target[t]]
+ *   x         : bf16 [T, ldx >= H]; w [V, ldw >= H] of `wtype`: 0 bf16, 3 e4m3fn,
+ *               4 int8, 5 e5m2; row_scale f32 [V] for the 1-byte types, else
+ *               NULL. H, ldx and ldw multiples of 8, x and bf16 w 16-byte
+ *               aligned, codes 8-byte aligned
+ *   targets   : int32, or int64 with targets_i64 [T]; ignore_index gives loss 0
+ *               (lse is computed all the same), any other target outside [0, V)
+ *               a NaN loss
+ *   loss, lse : f32 [T]
+ * T <= 2^20, V <= 2^24, H <= 2^16, ceil(V / 256) * ceil(T / 128) <= 2^22. The
+ * workspace needs no initialisation.
+ */
+int qmoe_vocab_loss_workspace_size(int64_t T, int64_t V, int64_t H, int wtype, int64_t* bytes);
+int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void* w, int wtype, int64_t ldw,
+                    const float* row_scale, int64_t V, int64_t H, const void* targets, int targets_i64,
+                    int64_t ignore_index, float* loss, float* lse, void* workspace, int64_t ws_bytes,
+                    qmoe_stream_t stream);
+
+/*
+ * Its gradients. g_loss, g_lse (optional): f32 [T] gradients of loss and lse;
+ * lse as qmoe_vocab_loss wrote it. With c[t] = (g_loss[t] where the target
+ * counts) + g_lse[t]: P[t, v] = exp(l - lse[t]) c[t] - [v == target[t]]
+ * g_loss[t], rounded to bf16; dx = P (s w) bf16 [T, lddx >= H], dw = P^T x bf16
+ * [V, lddw >= H] (bf16 tables only). Either may be NULL. A token with neither
+ * gradient leaves zeros in dx and nothing in dw, whatever its x holds. P and the
+ * logits exist for one piece of the vocabulary at a time. lddx, lddw multiples
+ * of 4, dx and dw 8-byte aligned. Every row of dx and dw is written; the sums'
+ * order is fixed.
+ */
+int qmoe_vocab_loss_grad_workspace_size(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw,
+                                        int64_t* bytes);
+int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const void* w, int wtype, int64_t ldw,
+                         const float* row_scale, int64_t V, int64_t H, const void* targets, int targets_i64,
+                         int64_t ignore_index, const float* lse, const float* g_loss, const float* g_lse, void* dx,
+                         int64_t lddx, void* dw, int64_t lddw, void* workspace, int64_t ws_bytes,
+                         qmoe_stream_t stream);
+
+/*
  * Plain read of `bytes` (a multiple of 16, 16-byte aligned) at `src` by at
  * most `workgroups` 256-thread workgroups; `sink` receives at most one dword
  * per workgroup ([workgroups] uint32, normally untouched). No counterpart in

@@ -8,7 +8,7 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from qmoe import _capi, ops
-from qmoe.layers.vocab import embedding
+from qmoe.layers.vocab import embedding, vocab_cross_entropy
 
 
 def test_lookup_fake_shapes_and_gradient():
@@ -83,3 +83,64 @@ def test_lookup_entry_points_check_their_arguments():
         a, 1, 100, a, gt, ldg, 50, 64, 1.0, -1, a, wt, 64, 0, ws, size, None)
     assert grad(gt=2) == 1 and grad(wt=3) == 1 and grad(ldg=63) == 1
     assert grad(ws=None) == 2 and grad(size=n.value - 1) == 2
+
+
+def test_loss_fake_shapes():
+    with FakeTensorMode():
+        x = torch.empty((3, 5, 96), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+        t = torch.empty((3, 5), dtype=torch.int64, device="cuda")
+        w = torch.empty((1000, 96), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+        loss, lse = vocab_cross_entropy(x, w, t)
+        assert loss.shape == lse.shape == (3, 5) and loss.dtype == lse.dtype == torch.float32 and loss.requires_grad
+        dx, dw = torch.ops.qmoe.vocab_loss_grad(x, w, t, lse, lse, None, None, -100, True, True)
+        assert dx.shape == x.shape and dw.shape == w.shape and dx.dtype == dw.dtype == torch.bfloat16
+        q = torch.empty((1000, 96), dtype=torch.int8, device="cuda")
+        assert vocab_cross_entropy(x.detach(), q, t, torch.empty(1000, device="cuda"))[0].shape == (3, 5)
+        with pytest.raises(ValueError, match="multiples of 8"):
+            vocab_cross_entropy(x.detach()[..., :95], w.detach()[:, :95], t)
+
+
+def test_loss_refusals():
+    x, w = torch.zeros((3, 16), dtype=torch.bfloat16), torch.zeros((8, 16), dtype=torch.bfloat16)
+    t = torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="device tensors"):
+        vocab_cross_entropy(x, w, t)
+    with pytest.raises(ValueError, match="hidden states must be bf16"):
+        vocab_cross_entropy(x.float(), w, t)
+    with pytest.raises(ValueError, match="hidden states must be bf16"):
+        vocab_cross_entropy(x[:, :8], w, t)
+    with pytest.raises(ValueError, match="targets of"):
+        vocab_cross_entropy(x, w, t[:2])
+    with pytest.raises(ValueError, match="int32 or int64"):
+        vocab_cross_entropy(x, w, t.float())
+    with pytest.raises(ValueError, match="must be bf16, e4m3"):
+        vocab_cross_entropy(x, w.float(), t)
+    with pytest.raises(ValueError, match="multiples of 8"):
+        vocab_cross_entropy(x[:, :12], w[:, :12], t)
+    with pytest.raises(ValueError, match="multiples of 8"):
+        vocab_cross_entropy(x, torch.zeros((8, 20), dtype=torch.bfloat16)[:, :16], t)
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        vocab_cross_entropy(x, torch.zeros(8 * 16 + 1, dtype=torch.bfloat16)[1:].view(8, 16), t)
+    with pytest.raises(ValueError, match="one scale per row"):
+        vocab_cross_entropy(x, w.to(torch.int8), t)
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        ops.vocab_loss_grad(x, w.to(torch.int8), t, torch.zeros(3), torch.zeros(3), weight_scale=torch.ones(8))
+    with pytest.raises(ValueError, match="g_loss must be"):
+        ops.vocab_loss_grad(x, w, t, torch.zeros(3), torch.zeros(2))
+
+
+def test_loss_entry_points_check_their_arguments():
+    lib, n, a = _capi.lib, ctypes.c_int64(0), ctypes.c_void_p(0x1000)
+    size = lambda T=100, V=500, H=64, wt=0: lib.qmoe_vocab_loss_workspace_size(T, V, H, wt, ctypes.byref(n))  # noqa: E731
+    assert size() == 0 and n.value > 0
+    assert size(H=60) == size(V=0) == size(T=-1) == size(wt=1) == size(T=1 << 20, V=1 << 24) == 1
+    assert lib.qmoe_vocab_loss_grad_workspace_size(100, 500, 64, 0, 1, 1, ctypes.byref(n)) == 0
+    need = n.value
+    loss = lambda x=a, ldx=64, wt=0, rs=None, ws=a, size=1 << 24, T=100: lib.qmoe_vocab_loss(  # noqa: E731
+        x, ldx, T, a, wt, 64, rs, 500, 64, a, 1, -100, a, a, ws, size, None)
+    assert loss(ldx=60) == loss(ldx=68) == loss(wt=1) == loss(wt=3) == loss(rs=a) == loss(x=ctypes.c_void_p(0x1008)) == 1
+    assert loss(ws=None) == loss(size=100) == 2 and loss(T=0) == 0
+    grad = lambda dx=a, dw=a, wt=0, rs=None, lddx=64, size=1 << 24, T=100: lib.qmoe_vocab_loss_grad(  # noqa: E731
+        a, 64, T, a, wt, 64, rs, 500, 64, a, 1, -100, a, a, None, dx, lddx, dw, 64, a, size, None)
+    assert grad(dx=None, dw=None) == grad(wt=4, rs=a) == grad(lddx=62) == grad(T=0) == 1
+    assert grad(size=need - 1) == 2

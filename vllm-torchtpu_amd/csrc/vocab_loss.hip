@@ -1,0 +1,753 @@
+// Softmax cross entropy of a projection onto the vocabulary table, in pieces
+// of the vocabulary, without keeping the logits:
+//
+//   l[t, v] = s[v] x[t] . w[v]       (s: one scale per row of a 1-byte table, else 1)
+//   lse[t]  = log sum_v exp l[t, v]
+//   loss[t] = lse[t] - l[t, target[t]], 0 where target[t] is the ignored index
+//
+// and with g the gradients of loss (of scored tokens) and h of lse
+//
+//   P[t, v] = exp(l[t, v] - lse[t]) (g[t] + h[t]) - [v == target[t]] g[t]
+//   dx[t]   = sum_v P[t, v] s[v] w[v],      dw[v] = sum_t P[t, v] x[t]
+//
+// What bounds it: four matrix products of 2 T V H operations on the bf16 matrix
+// cores (the logits twice: keeping them would take T V values), or, for few
+// tokens, one read of the table.
+//
+// Every product is one kernel: rows of two row-major bf16 operands against
+// each other along their contiguous axis, 256 "A" rows x 128 or 256 "B" rows
+// per workgroup, with the stage ring of gemm_t8.hip and an epilogue of its own:
+//   logits : A = table rows, B = tokens; per token and tile the maximum and the
+//            sum of exponentials (one pass), and the target's logit
+//   probs  : the same product again; P as [t][v], and as [v][t] for dw
+//   dx     : A = columns of the table piece (transposed once per piece), B = P
+//            rows; float32 sums added over the pieces
+//   dw     : A = columns of x (transposed once), B = P^T rows
+// Sums are float32; P is rounded to bf16 once, as the operand of the products.
+
+#include <algorithm>
+#include <type_traits>
+
+#include "../../include/qmoe.h"
+#include "gemm_tile.h"
+
+namespace {
+
+constexpr int kVThreads = 512;
+constexpr int kVN = 256;  // A rows of a tile
+
+enum { VE_LSE = 0, VE_PROB = 1, VE_SUM = 2, VE_STORE = 3 };
+
+struct VocabGemm {
+  const uint8_t* a;  // bf16 rows [na][lda bytes]
+  int64_t lda;
+  int na;
+  const uint8_t* b;  // bf16 rows [nb][ldb bytes]
+  int64_t ldb;
+  int nb;
+  int K;  // a multiple of 8
+  int n_tiles, m_tiles;
+  // logits / probs: A row r is table row v0 + r; B rows are tokens
+  const float* row_scale;  // of the piece (from v0 on), or nullptr
+  int64_t v0, V;
+  const void* targets;
+  int targets_i64;
+  int64_t ignore;
+  float2* part;     // [tiles of all pieces][nb] maximum and sum of exponentials
+  int part_tile;    // first tile of the piece
+  float* tgt;       // [nb] the target's logit
+  const float *lse, *g_loss, *g_lse;  // g_lse may be nullptr
+  uint16_t* p;      // [nb][ldp] P
+  int64_t ldp;
+  uint16_t* pt;     // [na rounded up][ldpt] P^T, or nullptr
+  int64_t ldpt;
+  // dx / dw: out[b row][a row]
+  float* sum;       // [nb][ldsum] float32 sums of the pieces before, or nullptr
+  int64_t ldsum;
+  int first, last;  // first / last piece
+  uint16_t* y;      // [nb][ldy]
+  int64_t ldy;
+};
+
+__device__ __align__(16) const uint32_t kVocabZero[4] = {0, 0, 0, 0};
+
+__device__ __forceinline__ int64_t load_target(const VocabGemm& p, int t) {
+  return p.targets_i64 ? static_cast<const int64_t*>(p.targets)[t]
+                       : (int64_t) static_cast<const int32_t*>(p.targets)[t];
+}
+
+__device__ __forceinline__ int vg_swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
+
+// Four 16-byte copies per lane from one scalar base, to `lds` + 0, 8, 16, 24 KB
+// (the scalar move gives the base its wait states, as in gemm_tile.h)
+__device__ __forceinline__ void vg_copy4(const uint8_t* base, const uint32_t (&off)[4], uint32_t lds) {
+  const uint8_t* b;
+  asm volatile(
+      "s_mov_b64 %0, %6\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\t"
+      "s_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %0\n\t"
+      "s_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %0\n\t"
+      "s_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %0"
+      : "=&s"(b)
+      : "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base)
+      : "m0", "scc", "memory");
+}
+__device__ __forceinline__ void vg_copy2(const uint8_t* base, const uint32_t (&off)[2], uint32_t lds) {
+  const uint8_t* b;
+  asm volatile(
+      "s_mov_b64 %0, %4\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\t"
+      "s_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %0"
+      : "=&s"(b)
+      : "s"(lds), "v"(off[0]), "v"(off[1]), "s"(base)
+      : "m0", "scc", "memory");
+}
+__device__ __forceinline__ void vg_copy(const uint8_t* base, const uint32_t (&off)[4], uint32_t lds) { vg_copy4(base, off, lds); }
+__device__ __forceinline__ void vg_copy(const uint8_t* base, const uint32_t (&off)[2], uint32_t lds) { vg_copy2(base, off, lds); }
+
+__device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* q) {
+  const uint64_t b = reinterpret_cast<uint64_t>(q);
+  return reinterpret_cast<const uint8_t*>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 |
+                                          (uint32_t)__builtin_amdgcn_readfirstlane((int)b));
+}
+
+// (maximum, sum of exponentials below it) of two disjoint sets; the base of the
+// exponentials is 0 where the maximum is infinite, so that infinite logits give
+// an infinite sum and a set without any (-inf, 0)
+__device__ __forceinline__ float lse_base(float m) { return fabsf(m) == __builtin_inff() ? 0.0f : m; }
+__device__ __forceinline__ float2 lse_merge(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x), base = lse_base(m);
+  // a sum is relative to its own base
+  const float sa = a.x == -__builtin_inff() ? a.y : a.y * __expf(lse_base(a.x) - base);
+  const float sb = b.x == -__builtin_inff() ? b.y : b.y * __expf(lse_base(b.x) - base);
+  return make_float2(m, sa + sb);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  union {
+    bf16x2 h;
+    uint32_t u;
+  } r;
+  r.h = __builtin_convertvector(f32x2{a, b}, bf16x2);
+  return r.u;
+}
+
+template <int EPI, int BM>
+__global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGemm p) {
+  constexpr int BN = kVN, NI = 2, MJ = BM / 64, RING = BM > 128 ? 2 : 3;
+  constexpr int WB = BN * 128, XB = BM * 128, STG = WB + XB;
+  __shared__ __align__(1024) uint8_t smem[RING * STG];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave & 3, wm = wave >> 2, rl = lane & 31, kh = lane >> 5;
+  int mt, nt;
+  if (!tile_dense(blockIdx.x, p.m_tiles, p.n_tiles, mt, nt)) return;
+  const int n0 = nt * BN, m0 = mt * BM;
+  const int arows = min(BN, p.na - n0), brows = min(BM, p.nb - m0);
+
+  // copies: one instruction = 8 rows x 128 bytes (lane -> row l >> 3, slot l & 7;
+  // the slot of chunk c of row r is c ^ vg_swz(r)); rows past the end repeat the
+  // last one (their products are dropped)
+  constexpr int WI = BN / 64, XI = BM / 64;
+  const int chunk16 = (lane & 7) ^ ((lane >> 3) ^ (wave & 1));
+  const uint8_t* abase = p.a + (int64_t)n0 * p.lda;
+  const uint8_t* bbase = p.b + (int64_t)m0 * p.ldb;
+  uint32_t aoff[WI], boff[XI];
+#pragma unroll
+  for (int j = 0; j < WI; ++j)
+    aoff[j] = (uint32_t)min((wave + 8 * j) * 8 + (lane >> 3), arows - 1) * (uint32_t)p.lda + chunk16 * 16;
+#pragma unroll
+  for (int j = 0; j < XI; ++j)
+    boff[j] = (uint32_t)min((wave + 8 * j) * 8 + (lane >> 3), brows - 1) * (uint32_t)p.ldb + chunk16 * 16;
+  const int KS = (p.K + 63) / 64;
+  const uint32_t cw = lds0 + wave * 1024;
+  auto copy_stage = [&](int s, int buf) {
+    const uint32_t d = __builtin_amdgcn_readfirstlane(cw + buf * STG);
+    const uint8_t* as = uniform_ptr(abase + (int64_t)s * 128);
+    const uint8_t* bs = uniform_ptr(bbase + (int64_t)s * 128);
+    if (s * 64 + 64 <= p.K) {
+      vg_copy(as, aoff, d);
+      vg_copy(bs, boff, d + WB);
+    } else {  // the last, partial stage: zeros behind the rows' ends
+      const bool in = s * 64 + chunk16 * 8 < p.K;
+      const uint8_t* z = reinterpret_cast<const uint8_t*>(kVocabZero);
+#pragma unroll
+      for (int j = 0; j < WI; ++j) lds_copy16(in ? as + aoff[j] : z, d + j * 8192);
+#pragma unroll
+      for (int j = 0; j < XI; ++j) lds_copy16(in ? bs + boff[j] : z, d + WB + j * 8192);
+    }
+  };
+
+  f32x16 acc[NI][MJ];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < MJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
+  // The K pipeline over the wavefront's first MJE 32-row B blocks (those with a
+  // row). Per stage: the first operands are in registers (read during the last
+  // MFMAs of the stage before); all but the last MFMA step run while the next
+  // step's operands are read; then the next stage's copies have landed ->
+  // barrier: everybody holds this stage's last operands, so that its buffer
+  // takes the copies of stage s + RING -> the last step, while the next stage's
+  // first operands are read.
+  auto pipeline = [&](auto mje_c) {
+    constexpr int MJE = decltype(mje_c)::value;
+#pragma unroll
+    for (int r = 0; r < RING; ++r)
+      if (r < KS) copy_stage(r, r);
+    auto landed = [&](bool ahead) {
+      if (ahead && RING == 3) wait_copies_upto<WI + XI>();
+      else wait_copies_upto<0>();
+    };
+    auto chunk = [&](const uint8_t* base, int row, int c) {
+      return *reinterpret_cast<const uint4*>(base + (row + rl) * 128 + ((c ^ vg_swz(rl)) * 16));
+    };
+    landed(false);
+    stage_barrier();
+    int buf = 0;
+    union B8 {
+      uint4 u;
+      bf16x8 v;
+    };
+    constexpr int MR = MJE > 0 ? MJE : 1;
+    B8 wf[2][NI], xf[2][MR];
+    auto read_q = [&](int b, int q) {
+      const uint8_t* sW = smem + b * STG;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) wf[q & 1][i].u = chunk(sW, wn * 64 + i * 32, 2 * q + kh);
+#pragma unroll
+      for (int j = 0; j < MJE; ++j) xf[q & 1][j].u = chunk(sW + WB, (2 * j + wm) * 32, 2 * q + kh);
+    };
+    auto mma = [&](int q) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < MJE; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[q & 1][i].v, xf[q & 1][j].v, acc[i][j], 0, 0, 0);
+    };
+    if constexpr (MJE > 0) read_q(0, 0);
+    for (int s = 0; s < KS; ++s) {
+      const int nb = buf == RING - 1 ? 0 : buf + 1;
+      if constexpr (MJE > 0) {
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+          read_q(buf, q + 1);
+          mma(q);
+        }
+      }
+      if (s + 1 < KS) landed(s + 2 < KS);
+      stage_barrier();
+      if (s + RING < KS) copy_stage(s + RING, buf);
+      asm volatile("" ::: "memory");
+      if constexpr (MJE > 0) {
+        if (s + 1 < KS) read_q(nb, 0);
+        mma(3);
+      }
+      buf = nb;
+    }
+  };
+  const int mje = max(0, (cdiv(brows, 32) - wm + 1) / 2);
+  if constexpr (MJ == 4) {
+    if (mje == 0) pipeline(std::integral_constant<int, 0>{});
+    else if (mje == 1) pipeline(std::integral_constant<int, 1>{});
+    else if (mje == 2) pipeline(std::integral_constant<int, 2>{});
+    else if (mje == 3) pipeline(std::integral_constant<int, 3>{});
+    else pipeline(std::integral_constant<int, 4>{});
+  } else {
+    if (mje == 0) pipeline(std::integral_constant<int, 0>{});
+    else if (mje == 1) pipeline(std::integral_constant<int, 1>{});
+    else pipeline(std::integral_constant<int, 2>{});
+  }
+  __syncthreads();  // every wavefront is done with the stage buffers
+
+  // ---- epilogues. Register quad q of block (i, j): A rows wn * 64 + i * 32 + q
+  // * 8 + kh * 4 + 0..3, B row (2 j + wm) * 32 + rl
+  auto arow = [&](int i, int q) { return wn * 64 + i * 32 + q * 8 + kh * 4; };
+  auto brow = [&](int j) { return (2 * j + wm) * 32 + rl; };
+  float* s_scale = reinterpret_cast<float*>(smem);
+  if constexpr (EPI == VE_LSE || EPI == VE_PROB) {
+    if (tid < BN) s_scale[tid] = p.row_scale ? p.row_scale[n0 + min(tid, arows - 1)] : 1.0f;
+    __syncthreads();
+  }
+  if constexpr (EPI == VE_LSE) {
+    float2* s_part = reinterpret_cast<float2*>(smem + 1024);  // [4 wn][BM]
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) {
+      const int tb = brow(j);
+      const bool valid = tb < brows;
+      const int64_t at = valid ? load_target(p, m0 + tb) - p.v0 - n0 : -1;  // the target's A row, if in the tile
+      float m = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int n = arow(i, q) + r;
+            const float l = n < arows ? acc[i][j][q * 4 + r] * s_scale[n] : -__builtin_inff();
+            acc[i][j][q * 4 + r] = l;
+            m = fmaxf(m, l);
+            if (n == at && n < arows) p.tgt[m0 + tb] = l;
+          }
+      const float base = lse_base(m);
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s += __expf(acc[i][j][r] - base);
+      const float2 mine = make_float2(m, s);
+      const float2 both = lse_merge(mine, make_float2(__shfl_xor(m, 32, 64), __shfl_xor(s, 32, 64)));
+      if (kh == 0) s_part[wn * BM + tb] = both;
+    }
+    __syncthreads();
+    if (tid < brows) {
+      float2 v = s_part[tid];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) v = lse_merge(v, s_part[w * BM + tid]);
+      p.part[(int64_t)(p.part_tile + nt) * p.nb + m0 + tid] = v;
+    }
+  } else if constexpr (EPI == VE_PROB) {
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) {
+      const int tb = brow(j), t = m0 + tb;
+      const bool valid = tb < brows;
+      float hot = 0.0f, coef = 0.0f, lse = 0.0f;
+      int64_t at = -1;
+      if (valid) {
+        const int64_t tg = load_target(p, t);
+        hot = tg == p.ignore ? 0.0f : (tg >= 0 && tg < p.V ? p.g_loss[t] : __builtin_nanf(""));
+        coef = hot + (p.g_lse ? p.g_lse[t] : 0.0f);
+        lse = p.lse[t];
+        at = tg - p.v0 - n0;
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        uint2 w[4];  // the quads as bf16: four A rows of this B row
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int n = arow(i, q) + r;
+            float e = 0.0f;
+            // a token without a gradient leaves zeros, whatever its logits are
+            if (n < arows && coef != 0.0f) e = __expf(acc[i][j][q * 4 + r] * s_scale[n] - lse) * coef;
+            if (n == at && n < arows) e -= hot;
+            v[r] = e;
+          }
+          // (P times the row scales is what multiplies the codes)
+          const float* sc = s_scale + arow(i, q);
+          w[q] = make_uint2(pack_bf16(v[0] * sc[0], v[1] * sc[1]), pack_bf16(v[2] * sc[2], v[3] * sc[3]));
+          if (p.pt) {
+            // 4 x 4 transposition over the lanes of a quad: lane k gets A row k of
+            // four consecutive tokens
+            const int k = lane & 3;
+            float o[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {  // from lane k ^ d its value of row k
+              const float send = (k ^ d) == 0 ? v[0] : ((k ^ d) == 1 ? v[1] : ((k ^ d) == 2 ? v[2] : v[3]));
+              const float got = d == 0 ? send : __shfl_xor(send, d, 64);
+              if ((k ^ d) == 0) o[0] = got;
+              if ((k ^ d) == 1) o[1] = got;
+              if ((k ^ d) == 2) o[2] = got;
+              if ((k ^ d) == 3) o[3] = got;
+            }
+            const int t4 = m0 + (tb & ~3);
+            if (t4 < p.ldpt)
+              *reinterpret_cast<uint2*>(p.pt + (int64_t)(n0 + arow(i, q) + k) * p.ldpt + t4) =
+                  make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
+          }
+        }
+        if (valid && p.p) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint2*>(p.p + (int64_t)t * p.ldp + n0 + arow(i, q)) = w[q];
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) {
+      const int t = m0 + brow(j);
+      if (brow(j) >= brows) continue;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = n0 + arow(i, q);
+          float v[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = acc[i][j][q * 4 + r];
+          if (n + 4 <= p.na) {
+            if constexpr (EPI == VE_SUM) {
+              float4* dst = reinterpret_cast<float4*>(p.sum + (int64_t)t * p.ldsum + n);
+              if (!p.first) {
+                const float4 o = *dst;
+                v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
+              }
+              if (!p.last) {
+                *dst = make_float4(v[0], v[1], v[2], v[3]);
+                continue;
+              }
+            }
+            *reinterpret_cast<uint2*>(p.y + (int64_t)t * p.ldy + n) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+          }
+        }
+    }
+  }
+}
+
+// Joins the tiles of a token (one wavefront): lse, loss
+__global__ __launch_bounds__(256) void vocab_loss_join_kernel(const float2* part, int tiles, int T, const float* tgt,
+                                                              const void* targets, int targets_i64, int64_t ignore,
+                                                              int64_t V, float* loss, float* lse) {
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (t >= T) return;
+  float2 v = make_float2(-__builtin_inff(), 0.0f);
+  for (int i = lane; i < tiles; i += 64) v = lse_merge(v, part[(int64_t)i * T + t]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = lse_merge(v, make_float2(__shfl_xor(v.x, o, 64), __shfl_xor(v.y, o, 64)));
+  if (lane) return;
+  const int64_t tg = targets_i64 ? static_cast<const int64_t*>(targets)[t]
+                                 : (int64_t) static_cast<const int32_t*>(targets)[t];
+  const float all = lse_base(v.x) + logf(v.y);
+  lse[t] = all;
+  loss[t] = tg == ignore ? 0.0f : (tg >= 0 && tg < V ? all - tgt[t] : __builtin_nanf(""));
+}
+
+// 4 e4m3 / int8 / e5m2 codes -> 4 bf16 (exact)
+template <int WT>
+__device__ __forceinline__ uint2 codes4_to_bf16(uint32_t c) {
+  float f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = (c >> (8 * i)) & 0xffu;
+    f[i] = WT == 3 ? e4m3_to_f32(b) : (WT == 4 ? (float)(int8_t)b : e5m2_to_f32(b));
+  }
+  return make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
+}
+
+// Rows of codes -> bf16 rows; 8 codes per thread
+template <int WT>
+__global__ __launch_bounds__(256) void vocab_expand_kernel(const uint8_t* w, int64_t ldw, int64_t rows, int H8,
+                                                           uint16_t* out, int64_t ldo) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * H8) return;
+  const int64_t r = i / H8;
+  const int c = (int)(i - r * H8) * 8;
+  const uint2 d = *reinterpret_cast<const uint2*>(w + r * ldw + c);
+  const uint2 lo = codes4_to_bf16<WT>(d.x), hi = codes4_to_bf16<WT>(d.y);
+  *reinterpret_cast<uint4*>(out + r * ldo + c) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+}
+
+// src rows [R][C] (bf16 or codes) -> out [C][ldo] bf16, columns R .. ldo - 1 zero;
+// with `targets` a row whose token has no gradient becomes zeros (whatever it
+// holds). 64 x 64 tiles through LDS.
+template <int WT>
+__global__ __launch_bounds__(256) void vocab_transpose_kernel(const uint8_t* src, int64_t ld, int R, int C,
+                                                              uint16_t* out, int64_t ldo, const void* targets,
+                                                              int targets_i64, int64_t ignore, const float* g_loss,
+                                                              const float* g_lse) {
+  __shared__ uint16_t tile[64][66];
+  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+  const int tid = threadIdx.x;
+  {
+    const int c = (tid & 7) * 8;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r = (tid >> 3) + 32 * k;
+      bool live = r0 + r < R && c0 + c < C;
+      if (live && targets) {
+        const int64_t tg = targets_i64 ? static_cast<const int64_t*>(targets)[r0 + r]
+                                       : (int64_t) static_cast<const int32_t*>(targets)[r0 + r];
+        live = (tg != ignore && g_loss[r0 + r] != 0.0f) || (g_lse && g_lse[r0 + r] != 0.0f);
+      }
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (live) {
+        if constexpr (WT == 0) {
+          v = *reinterpret_cast<const uint4*>(src + (int64_t)(r0 + r) * ld + (int64_t)(c0 + c) * 2);
+        } else {
+          const uint2 d = *reinterpret_cast<const uint2*>(src + (int64_t)(r0 + r) * ld + c0 + c);
+          const uint2 lo = codes4_to_bf16<WT>(d.x), hi = codes4_to_bf16<WT>(d.y);
+          v = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+      }
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) tile[r][c + i] = (uint16_t)(u[i / 2] >> (16 * (i & 1)));
+    }
+  }
+  __syncthreads();
+  const int r = (tid & 7) * 8;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int c = (tid >> 3) + 32 * k;
+    if (c0 + c >= C || r0 + r >= ldo) continue;
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = tile[r + 2 * i][c] | (uint32_t)tile[r + 2 * i + 1][c] << 16;
+    *reinterpret_cast<uint4*>(out + (int64_t)(c0 + c) * ldo + r0 + r) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// B-row tile height
+int vocab_bm(int nb) { return nb > 128 ? 256 : 128; }
+
+template <int EPI>
+void launch_gemm(VocabGemm g, hipStream_t st) {
+  const int bm = vocab_bm(g.nb);
+  g.n_tiles = cdiv(g.na, kVN);
+  g.m_tiles = cdiv(g.nb, bm);
+  const unsigned grid = (unsigned)(cdiv(g.n_tiles * g.m_tiles, kXcds) * kXcds);
+  if (bm == 256) hipLaunchKernelGGL((vocab_gemm_kernel<EPI, 256>), dim3(grid), dim3(kVThreads), 0, st, g);
+  else hipLaunchKernelGGL((vocab_gemm_kernel<EPI, 128>), dim3(grid), dim3(kVThreads), 0, st, g);
+}
+
+void launch_expand(int wt, const uint8_t* w, int64_t ldw, int64_t rows, int64_t H, uint16_t* out, hipStream_t st) {
+  const dim3 grid((unsigned)cdiv(rows * (H / 8), (int64_t)256));
+  if (wt == 3) hipLaunchKernelGGL(vocab_expand_kernel<3>, grid, dim3(256), 0, st, w, ldw, rows, (int)(H / 8), out, H);
+  else if (wt == 4) hipLaunchKernelGGL(vocab_expand_kernel<4>, grid, dim3(256), 0, st, w, ldw, rows, (int)(H / 8), out, H);
+  else hipLaunchKernelGGL(vocab_expand_kernel<5>, grid, dim3(256), 0, st, w, ldw, rows, (int)(H / 8), out, H);
+}
+
+struct LossArgs {
+  const void* x;
+  int64_t ldx, T;
+  const void* w;
+  int wtype;
+  int64_t ldw;
+  const float* row_scale;
+  int64_t V, H;
+  const void* targets;
+  int targets_i64;
+  int64_t ignore;
+};
+
+void launch_transpose(int wt, const uint8_t* src, int64_t ld, int64_t R, int64_t C, uint16_t* out, int64_t ldo,
+                      const LossArgs* mask, const float* g_loss, const float* g_lse, hipStream_t st) {
+  const dim3 grid((unsigned)cdiv(ldo, (int64_t)64), (unsigned)cdiv(C, (int64_t)64));
+  const void* tg = mask ? mask->targets : nullptr;
+  const int i64 = mask ? mask->targets_i64 : 0;
+  const int64_t ig = mask ? mask->ignore : 0;
+#define QMOE_TR(W) \
+  hipLaunchKernelGGL(vocab_transpose_kernel<W>, grid, dim3(256), 0, st, src, ld, (int)R, (int)C, out, ldo, tg, i64, ig, g_loss, g_lse)
+  if (wt == 0) QMOE_TR(0);
+  else if (wt == 3) QMOE_TR(3);
+  else if (wt == 4) QMOE_TR(4);
+  else QMOE_TR(5);
+#undef QMOE_TR
+}
+
+// sizes whose tile counts, and the threads of their grids, fit 32 bits
+constexpr int64_t kMaxTokens = (int64_t)1 << 20, kMaxVocab = (int64_t)1 << 24, kMaxHidden = (int64_t)1 << 16;
+
+bool loss_sizes_ok(int64_t T, int64_t V, int64_t H) {
+  return T >= 0 && T <= kMaxTokens && V > 0 && V <= kMaxVocab && H > 0 && H <= kMaxHidden && H % 8 == 0 &&
+         cdiv(V, (int64_t)kVN) * cdiv(T, (int64_t)128) <= ((int64_t)1 << 22);
+}
+
+int loss_args_ok(const LossArgs& a) {
+  if (!loss_sizes_ok(a.T, a.V, a.H)) return 0;
+  if (a.wtype != 0 && (a.wtype < 3 || a.wtype > 5)) return 0;
+  if (a.ldx < a.H || a.ldw < a.H || a.ldx % 8 || a.ldw % 8) return 0;
+  if (a.ldx >= (int64_t)1 << 22 || a.ldw >= (int64_t)1 << 22) return 0;  // 256 rows of a tile within 32-bit offsets
+  if (a.T == 0) return 1;
+  if (!a.x || !a.w || !a.targets || ((a.wtype != 0) != (a.row_scale != nullptr))) return 0;
+  if ((reinterpret_cast<uintptr_t>(a.x) & 15) || (reinterpret_cast<uintptr_t>(a.w) & (a.wtype ? 7 : 15))) return 0;
+  return 1;
+}
+
+// Table rows of a piece of the forward pass: all of a bf16 table (read where
+// it lies), about 128 MB of expanded rows of a 1-byte one
+int64_t loss_piece(int64_t V, int64_t H, int wtype) {
+  if (wtype == 0) return V;
+  return std::min(up(V, kVN), std::max<int64_t>(up((int64_t)(64 << 20) / H, kVN), kVN));
+}
+
+int64_t loss_layout(int64_t T, int64_t V, int64_t H, int wtype, int64_t (&off)[3]) {
+  int64_t at = 0;
+  off[0] = at;  // partial (maximum, sum) of every tile
+  at += up(cdiv(V, (int64_t)kVN) * T * 8, 256);
+  off[1] = at;  // the targets' logits
+  at += up(T * 4, 256);
+  off[2] = at;  // expanded rows
+  if (wtype) at += up(loss_piece(V, H, wtype) * H * 2, 256);
+  return at;
+}
+
+// Table rows of a piece of the gradients: P, P^T and the transposed (and for
+// codes the expanded) table rows of a piece take up to 128 MB each
+int64_t grad_piece(int64_t T, int64_t V, int64_t H) {
+  return std::min(up(V, kVN), std::max<int64_t>((int64_t)(64 << 20) / std::max(up(T, 64), H) / kVN * kVN, kVN));
+}
+
+// P, P^T, table piece transposed, x transposed, float32 sums, expanded rows
+int64_t grad_layout(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw, int64_t (&off)[6]) {
+  const int64_t Vc = grad_piece(T, V, H), Tp = up(T, 64);
+  const bool pieces = Vc < V;
+  int64_t at = 0;
+  off[0] = at;
+  if (need_dx) at += up(T * Vc * 2, 256);
+  off[1] = at;
+  if (need_dw) at += up(Vc * Tp * 2, 256);
+  off[2] = at;
+  if (need_dx) at += up(H * Vc * 2, 256);
+  off[3] = at;
+  if (need_dw) at += up(H * Tp * 2, 256);
+  off[4] = at;
+  if (need_dx && pieces) at += up(T * up(H, 4) * 4, 256);
+  off[5] = at;
+  if (wtype) at += up(Vc * H * 2, 256);
+  return at;
+}
+
+}  // namespace
+
+// See include/qmoe.h for the contracts.
+extern "C" int qmoe_vocab_loss_workspace_size(int64_t T, int64_t V, int64_t H, int wtype, int64_t* bytes) {
+  if (!loss_sizes_ok(T, V, H) || (wtype != 0 && (wtype < 3 || wtype > 5)) || !bytes) return QMOE_ERR_ARG;
+  int64_t off[3];
+  *bytes = loss_layout(T, V, H, wtype, off);
+  return QMOE_OK;
+}
+
+extern "C" int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void* w, int wtype, int64_t ldw,
+                               const float* row_scale, int64_t V, int64_t H, const void* targets, int targets_i64,
+                               int64_t ignore_index, float* loss, float* lse, void* workspace, int64_t ws_bytes,
+                               hipStream_t stream) {
+  const LossArgs a{x, ldx, T, w, wtype, ldw, row_scale, V, H, targets, targets_i64, ignore_index};
+  if (!loss_args_ok(a)) return QMOE_ERR_ARG;
+  if (T == 0) return QMOE_OK;
+  if (!loss || !lse) return QMOE_ERR_ARG;
+  int64_t off[3];
+  if (!workspace || ws_bytes < loss_layout(T, V, H, wtype, off)) return QMOE_ERR_WORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  VocabGemm g{};
+  g.b = static_cast<const uint8_t*>(x);
+  g.ldb = ldx * 2;
+  g.nb = (int)T;
+  g.K = (int)H;
+  g.V = V;
+  g.targets = targets;
+  g.targets_i64 = targets_i64;
+  g.ignore = ignore_index;
+  g.part = reinterpret_cast<float2*>(ws + off[0]);
+  g.tgt = reinterpret_cast<float*>(ws + off[1]);
+  const int64_t Vc = loss_piece(V, H, wtype);
+  for (int64_t v0 = 0; v0 < V; v0 += Vc) {
+    const uint8_t* rows = static_cast<const uint8_t*>(w) + v0 * ldw * (wtype ? 1 : 2);
+    const int64_t n = std::min(Vc, V - v0);
+    g.a = rows;
+    g.lda = ldw * 2;
+    if (wtype) {
+      uint16_t* e = reinterpret_cast<uint16_t*>(ws + off[2]);
+      launch_expand(wtype, rows, ldw, n, H, e, stream);
+      g.a = reinterpret_cast<const uint8_t*>(e);
+      g.lda = H * 2;
+    }
+    g.na = (int)n;
+    g.v0 = v0;
+    g.row_scale = row_scale ? row_scale + v0 : nullptr;
+    g.part_tile = (int)(v0 / kVN);
+    launch_gemm<VE_LSE>(g, stream);
+  }
+  hipLaunchKernelGGL(vocab_loss_join_kernel, dim3((unsigned)cdiv(T, (int64_t)4)), dim3(256), 0, stream, g.part,
+                     (int)cdiv(V, (int64_t)kVN), (int)T, g.tgt, targets, targets_i64, ignore_index, V, loss, lse);
+  return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
+}
+
+extern "C" int qmoe_vocab_loss_grad_workspace_size(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw,
+                                                   int64_t* bytes) {
+  if (!loss_sizes_ok(T, V, H) || (wtype != 0 && (wtype < 3 || wtype > 5)) || !bytes) return QMOE_ERR_ARG;
+  int64_t off[6];
+  *bytes = grad_layout(T, V, H, wtype, need_dx, need_dw, off);
+  return QMOE_OK;
+}
+
+extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const void* w, int wtype, int64_t ldw,
+                                    const float* row_scale, int64_t V, int64_t H, const void* targets, int targets_i64,
+                                    int64_t ignore_index, const float* lse, const float* g_loss, const float* g_lse,
+                                    void* dx, int64_t lddx, void* dw, int64_t lddw, void* workspace, int64_t ws_bytes,
+                                    hipStream_t stream) {
+  const LossArgs a{x, ldx, T, w, wtype, ldw, row_scale, V, H, targets, targets_i64, ignore_index};
+  if (!loss_args_ok(a) || T == 0 || !lse || !g_loss || (!dx && !dw)) return QMOE_ERR_ARG;
+  if (dw && wtype) return QMOE_ERR_ARG;  // codes have no gradient
+  if (dx && (lddx < H || lddx % 4 || (reinterpret_cast<uintptr_t>(dx) & 7))) return QMOE_ERR_ARG;
+  if (dw && (lddw < H || lddw % 4 || (reinterpret_cast<uintptr_t>(dw) & 7))) return QMOE_ERR_ARG;
+  int64_t off[6];
+  if (!workspace || ws_bytes < grad_layout(T, V, H, wtype, dx != nullptr, dw != nullptr, off)) return QMOE_ERR_WORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int64_t Vc = grad_piece(T, V, H), Tp = up(T, 64);
+  uint16_t* P = reinterpret_cast<uint16_t*>(ws + off[0]);
+  uint16_t* PT = reinterpret_cast<uint16_t*>(ws + off[1]);
+  uint16_t* WT = reinterpret_cast<uint16_t*>(ws + off[2]);
+  uint16_t* XT = reinterpret_cast<uint16_t*>(ws + off[3]);
+  if (dw) launch_transpose(0, static_cast<const uint8_t*>(x), ldx * 2, T, H, XT, Tp, &a, g_loss, g_lse, stream);
+  for (int64_t v0 = 0; v0 < V; v0 += Vc) {
+    const uint8_t* rows = static_cast<const uint8_t*>(w) + v0 * ldw * (wtype ? 1 : 2);
+    const int64_t n = std::min(Vc, V - v0), np = up(n, 64);
+    VocabGemm g{};
+    g.a = rows;
+    g.lda = ldw * 2;
+    if (wtype) {
+      uint16_t* e = reinterpret_cast<uint16_t*>(ws + off[5]);
+      launch_expand(wtype, rows, ldw, n, H, e, stream);
+      g.a = reinterpret_cast<const uint8_t*>(e);
+      g.lda = H * 2;
+    }
+    g.na = (int)n;
+    g.b = static_cast<const uint8_t*>(x);
+    g.ldb = ldx * 2;
+    g.nb = (int)T;
+    g.K = (int)H;
+    g.row_scale = row_scale ? row_scale + v0 : nullptr;
+    g.v0 = v0;
+    g.V = V;
+    g.targets = targets;
+    g.targets_i64 = targets_i64;
+    g.ignore = ignore_index;
+    g.lse = lse;
+    g.g_loss = g_loss;
+    g.g_lse = g_lse;
+    g.p = dx ? P : nullptr;
+    g.ldp = Vc;
+    g.pt = dw ? PT : nullptr;
+    g.ldpt = Tp;
+    launch_gemm<VE_PROB>(g, stream);
+    if (dx) {
+      launch_transpose(wtype, rows, ldw * (wtype ? 1 : 2), n, H, WT, np, nullptr, nullptr, nullptr, stream);
+      VocabGemm d{};
+      d.a = reinterpret_cast<const uint8_t*>(WT);
+      d.lda = np * 2;
+      d.na = (int)H;
+      d.b = reinterpret_cast<const uint8_t*>(P);
+      d.ldb = Vc * 2;
+      d.nb = (int)T;
+      d.K = (int)np;
+      d.sum = reinterpret_cast<float*>(ws + off[4]);
+      d.ldsum = up(H, 4);
+      d.first = v0 == 0;
+      d.last = v0 + Vc >= V;
+      d.y = static_cast<uint16_t*>(dx);
+      d.ldy = lddx;
+      launch_gemm<VE_SUM>(d, stream);
+    }
+    if (dw) {
+      VocabGemm d{};
+      d.a = reinterpret_cast<const uint8_t*>(XT);
+      d.lda = Tp * 2;
+      d.na = (int)H;
+      d.b = reinterpret_cast<const uint8_t*>(PT);
+      d.ldb = Tp * 2;
+      d.nb = (int)n;
+      d.K = (int)Tp;
+      d.y = static_cast<uint16_t*>(dw) + v0 * lddw;
+      d.ldy = lddw;
+      launch_gemm<VE_STORE>(d, stream);
+    }
+  }
+  return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
+}

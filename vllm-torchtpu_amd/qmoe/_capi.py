@@ -170,6 +170,17 @@ def _load():
     lib.qmoe_vocab_lookup_grad.restype = ctypes.c_int
     lib.qmoe_vocab_lookup_grad.argtypes = [_vp, ctypes.c_int, _i64, _vp, ctypes.c_int, _i64, _i64, _i64, _f32, _i64, _vp,
                                            ctypes.c_int, _i64, ctypes.c_int, _vp, _i64, _vp]
+    lib.qmoe_vocab_loss_workspace_size.restype = ctypes.c_int
+    lib.qmoe_vocab_loss_workspace_size.argtypes = [_i64, _i64, _i64, ctypes.c_int, ctypes.POINTER(_i64)]
+    lib.qmoe_vocab_loss.restype = ctypes.c_int
+    lib.qmoe_vocab_loss.argtypes = [_vp, _i64, _i64, _vp, ctypes.c_int, _i64, _vp, _i64, _i64, _vp, ctypes.c_int, _i64,
+                                    _vp, _vp, _vp, _i64, _vp]
+    lib.qmoe_vocab_loss_grad_workspace_size.restype = ctypes.c_int
+    lib.qmoe_vocab_loss_grad_workspace_size.argtypes = [_i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                                        ctypes.POINTER(_i64)]
+    lib.qmoe_vocab_loss_grad.restype = ctypes.c_int
+    lib.qmoe_vocab_loss_grad.argtypes = [_vp, _i64, _i64, _vp, ctypes.c_int, _i64, _vp, _i64, _i64, _vp, ctypes.c_int,
+                                         _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp]
     lib.qmoe_stream_read.restype = ctypes.c_int
     lib.qmoe_stream_read.argtypes = [_vp, _i64, _i32, _vp, _vp]
     v = lib.qmoe_abi_version()
@@ -200,6 +211,10 @@ EXPORTED = (
     "qmoe_vocab_lookup",
     "qmoe_vocab_lookup_grad_workspace_size",
     "qmoe_vocab_lookup_grad",
+    "qmoe_vocab_loss_workspace_size",
+    "qmoe_vocab_loss",
+    "qmoe_vocab_loss_grad_workspace_size",
+    "qmoe_vocab_loss_grad",
 )
 
 

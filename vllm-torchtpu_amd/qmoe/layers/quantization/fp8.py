@@ -37,7 +37,7 @@ import torch
 from qmoe import envs, ops
 from qmoe.layers.fused_moe import moe_forward
 from qmoe.layers.linear_common import KEEP_VLLM_LAYOUT_ATTR, quantized_matmul
-from qmoe.layers.vocab import embedding
+from qmoe.layers.vocab import embedding, vocab_cross_entropy
 
 FP8 = torch.float8_e4m3fn
 # requantization targets (`fp8.py:122-127`); the short names are the ones
@@ -299,6 +299,14 @@ class Fp8LinearMethod:
         w = torch.index_select(layer.weight, 0, flat).to(out_dtype)
         s = torch.index_select(layer.weight_scale.reshape(-1), 0, flat).to(out_dtype).unsqueeze(-1)
         return (w * s).reshape(*input_.shape, -1)
+
+    def cross_entropy(self, layer, x, targets, ignore_index=-100):
+        """(loss, lse) of the targets under softmax(apply(layer, x)) of an
+        embedding table used as the output projection, without the logits
+        (`qmoe.layers.vocab.vocab_cross_entropy`)."""
+        if not _is_embedding(layer):
+            raise NotImplementedError("cross_entropy takes an embedding table (bf16 activations, one scale per row)")
+        return vocab_cross_entropy(x, layer.weight, targets, layer.weight_scale, ignore_index)
 
     def tie_weights(self, layer, embed_tokens):
         """`fp8.py:1700-1704`: share the embedding's codes and scales."""

@@ -8,7 +8,7 @@ import torch
 from qmoe import _capi, envs, ops
 from qmoe.layers.fused_moe import moe_forward
 from qmoe.layers.quantization.fp8 import _activation, _device, _param
-from qmoe.layers.vocab import embedding
+from qmoe.layers.vocab import embedding, vocab_cross_entropy
 
 
 class UnquantizedLinearMethod:
@@ -33,6 +33,11 @@ class UnquantizedLinearMethod:
         """Rows of a bf16 ``[vocab, H]`` table (a `VocabParallelEmbedding` of an
         unquantized checkpoint)."""
         return embedding(input_, layer.weight)
+
+    def cross_entropy(self, layer, x, targets, ignore_index=-100):
+        """(loss, lse) of the targets under softmax(apply(layer, x)), without
+        the logits (`qmoe.layers.vocab.vocab_cross_entropy`)."""
+        return vocab_cross_entropy(x, layer.weight, targets, None, ignore_index)
 
     def tie_weights(self, layer, embed_tokens):
         """Share the embedding's table, as `fp8.py:1700-1704`."""

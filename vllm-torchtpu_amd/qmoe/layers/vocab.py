@@ -3,6 +3,8 @@
 ``embedding`` is the lookup behind the quant methods' ``embedding``
 (`layers/adapter/quantization/fp8.py:1692-1698`) with the scaling that some
 models put behind it, and its gradient for a bf16 or f32 table.
+``vocab_cross_entropy`` scores tokens against the output projection (the tied
+table of `fp8.py:1679-1681`) without the [T, V] logits, and its gradients.
 
 Both run as torch custom ops (``torch.ops.qmoe.vocab_lookup`` ...) under
 `torch.compile` and fake tensors, and straight on the C ABI in eager mode: the
@@ -10,7 +12,7 @@ op's dispatch takes longer than a decode step's lookup. Gradients come from
 `torch.autograd.Function`s around them.
 """
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -64,8 +66,11 @@ class _Embedding(torch.autograd.Function):
 
 
 def _lookup(ids, weight, weight_scale, scale, out_dtype):
-    fn = ops.vocab_lookup if _eager(ids, weight, weight_scale) else torch.ops.qmoe.vocab_lookup
-    return fn(ids, weight, weight_scale, scale, out_dtype)
+    if _eager(ids, weight, weight_scale):
+        return ops.vocab_lookup(ids, weight, weight_scale, scale, out_dtype)
+    ops._check_table(weight, weight_scale, "embedding")
+    ops._check_ids(ids, "embedding: ids")
+    return torch.ops.qmoe.vocab_lookup(ids, weight, weight_scale, scale, out_dtype)
 
 
 def embedding(ids, weight, weight_scale=None, scale=1.0, padding_idx=None, out_dtype=torch.bfloat16):
@@ -77,8 +82,6 @@ def embedding(ids, weight, weight_scale=None, scale=1.0, padding_idx=None, out_d
     outside the table gives a row of NaN. A bf16 or f32 table that requires a
     gradient gets one (in its own type, from float32 sums in token order, the
     same bits on every call); ``padding_idx`` names the row that gets none."""
-    ops._check_table(weight, weight_scale, "embedding")
-    ops._check_ids(ids, "embedding: ids")
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"embedding: padding_idx {padding_idx} is outside the table of {weight.shape[0]} rows")
     scale = float(scale)
@@ -89,3 +92,84 @@ def embedding(ids, weight, weight_scale=None, scale=1.0, padding_idx=None, out_d
             raise NotImplementedError("embedding: gradients flow through bf16 or f32 outputs, not f16")
         return _Embedding.apply(ids, weight, scale, padding_idx, out_dtype)
     return _lookup(ids, weight, weight_scale, scale, out_dtype)
+
+
+# ---------------------------------------------------------------- cross entropy
+
+
+@torch.library.custom_op("qmoe::vocab_loss", mutates_args=())
+def _loss_op(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, weight_scale: Optional[torch.Tensor],
+             ignore_index: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    return ops.vocab_loss(x, weight, targets, weight_scale, ignore_index)
+
+
+@_loss_op.register_fake
+def _(x, weight, targets, weight_scale, ignore_index):
+    return x.new_empty(targets.shape, dtype=torch.float32), x.new_empty(targets.shape, dtype=torch.float32)
+
+
+@torch.library.custom_op("qmoe::vocab_loss_grad", mutates_args=())
+def _loss_grad_op(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, g_loss: torch.Tensor,
+                  g_lse: Optional[torch.Tensor], weight_scale: Optional[torch.Tensor], ignore_index: int, need_x: bool,
+                  need_weight: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(a gradient that is not asked for comes back empty)"""
+    dx, dw = ops.vocab_loss_grad(x, weight, targets, lse, g_loss, g_lse, weight_scale, ignore_index, need_x, need_weight)
+    return (x.new_empty(0) if dx is None else dx), (x.new_empty(0) if dw is None else dw)
+
+
+@_loss_grad_op.register_fake
+def _(x, weight, targets, lse, g_loss, g_lse, weight_scale, ignore_index, need_x, need_weight):
+    return x.new_empty(x.shape if need_x else 0), x.new_empty(weight.shape if need_weight else 0)
+
+
+class _VocabCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, targets, weight_scale, ignore_index):
+        loss, lse = _loss(x, weight, targets, weight_scale, ignore_index)
+        ctx.save_for_backward(x, weight, targets, weight_scale, lse)
+        ctx.ignore_index = ignore_index
+        ctx.set_materialize_grads(False)
+        return loss, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_loss, g_lse):
+        x, weight, targets, weight_scale, lse = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[:2]
+        if g_loss is None and g_lse is None:
+            return None, None, None, None, None
+        if g_loss is None:
+            g_loss = torch.zeros_like(g_lse)
+        fn = ops.vocab_loss_grad if _eager(x, weight, g_loss, g_lse) else torch.ops.qmoe.vocab_loss_grad
+        dx, dw = fn(x, weight, targets, lse, g_loss, g_lse, weight_scale, ctx.ignore_index, need_x, need_w)
+        return (dx if need_x else None), (dw if need_w else None), None, None, None
+
+
+def _loss(x, weight, targets, weight_scale, ignore_index):
+    if _eager(x, weight, targets, weight_scale):
+        return ops.vocab_loss(x, weight, targets, weight_scale, ignore_index)
+    ops._check_loss(x, weight, targets, weight_scale, "vocab_cross_entropy")
+    return torch.ops.qmoe.vocab_loss(x, weight, targets, weight_scale, ignore_index)
+
+
+def vocab_cross_entropy(x, weight, targets, weight_scale=None, ignore_index=-100):
+    """Cross entropy of the targets (int32 or int64 [...]) under softmax(x .
+    w^T): (loss, lse), float32 of the targets' shape, without the logits in
+    memory. ``-loss`` is the targets' log-probability, ``lse`` the log of the
+    sum of exponentials.
+
+    ``x`` is bf16 [..., H]; ``weight`` [V, H] bf16, or 1-byte codes (e4m3, e5m2,
+    int8) with one float32 scale per row, the layout `Fp8LinearMethod` keeps an
+    embedding table in; H a multiple of 8. ``ignore_index`` marks tokens that
+    are not scored (loss 0, no gradient of the loss; padding rows may hold
+    anything); another target outside the table gives a NaN loss.
+
+    Differentiable in ``x`` and in a bf16 ``weight`` through both results
+    (gradients in bf16; a table of codes is frozen). The sums' order is fixed:
+    the same bits on every call."""
+    ignore_index = int(ignore_index)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        if weight.requires_grad and weight_scale is not None:
+            raise NotImplementedError("vocab_cross_entropy: no gradient for a table of 1-byte codes")
+        return _VocabCrossEntropy.apply(x, weight, targets, weight_scale, ignore_index)
+    return _loss(x, weight, targets, weight_scale, ignore_index)

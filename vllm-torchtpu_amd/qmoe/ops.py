@@ -734,3 +734,87 @@ def vocab_lookup_grad(grad, ids, vocab, scale=1.0, padding_idx=None, dtype=torch
                                          _TABLE_TYPES[dw.dtype], dw.stride(0), int(into is not None), _ptr(ws), ws_n,
                                          _stream(g.device)), "vocab_lookup_grad")
     return dw
+
+
+def _check_loss(x, weight, targets, weight_scale, what):
+    """Shapes, types and strides of the vocabulary loss's operands; returns
+    (targets [T], row scales [V] or None)."""
+    s = _check_table(weight, weight_scale, what)
+    if weight.dtype == torch.float32:
+        raise ValueError(f"{what}: the table must be bf16, e4m3, e5m2 or int8, got {weight.dtype}")
+    H = weight.shape[1]
+    if H % 8 or weight.stride(0) % 8:
+        raise ValueError(f"{what}: the table needs a width and a row stride in multiples of 8, got "
+                         f"{tuple(weight.shape)}, strides {weight.stride()}")
+    if x.dtype != torch.bfloat16 or x.dim() < 1 or x.shape[-1] != H:
+        raise ValueError(f"{what}: hidden states must be bf16 [..., {H}], got {x.dtype} {tuple(x.shape)}")
+    if tuple(targets.shape) != tuple(x.shape[:-1]):
+        raise ValueError(f"{what}: targets of {tuple(targets.shape)} for hidden states of {tuple(x.shape)}")
+    return _check_ids(targets, f"{what}: targets"), s
+
+
+def _loss_operands(x, weight, targets, weight_scale, what):
+    """`_check_loss` and the table's alignment, and the hidden rows [T, H] as
+    the kernels read them (copied where they are not 16-byte aligned)."""
+    t, s = _check_loss(x, weight, targets, weight_scale, what)
+    align = 16 if weight.dtype == torch.bfloat16 else 8
+    if weight.data_ptr() % align:
+        raise ValueError(f"{what}: the table must be {align}-byte aligned")
+    H = weight.shape[1]
+    x2 = x.reshape(-1, H)
+    if x2.numel() and (x2.stride(1) != 1 or x2.stride(0) < H or x2.stride(0) % 8 or x2.data_ptr() % 16):
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2, t, s
+
+
+def vocab_loss(x, weight, targets, weight_scale=None, ignore_index=-100):
+    """Softmax cross entropy of ``x`` [..., H] (bf16) projected onto the table
+    [V, H]: float32 (loss, log of the sum of exponentials), both of the
+    targets' shape; see include/qmoe.h `qmoe_vocab_loss`."""
+    x2, t, s = _loss_operands(x, weight, targets, weight_scale, "vocab_loss")
+    V, H = weight.shape
+    with _on_device(x2, weight, t, s):
+        T, dev = t.numel(), weight.device
+        loss, lse = torch.empty(targets.shape, device=dev), torch.empty(targets.shape, device=dev)
+        if T == 0:
+            return loss, lse
+        need, wt = ctypes.c_int64(0), _TABLE_TYPES[weight.dtype]
+        check(lib.qmoe_vocab_loss_workspace_size(T, V, H, wt, ctypes.byref(need)), "vocab_loss (shape)")
+        ws, ws_n = _workspace(dev, need.value)
+        check(lib.qmoe_vocab_loss(_ptr(x2), x2.stride(0), T, _ptr(weight), wt, weight.stride(0), _ptr(s), V, H, _ptr(t),
+                                  int(t.dtype == torch.int64), int(ignore_index), _ptr(loss), _ptr(lse), _ptr(ws), ws_n,
+                                  _stream(dev)), "vocab_loss")
+    return loss, lse
+
+
+def vocab_loss_grad(x, weight, targets, lse, g_loss, g_lse=None, weight_scale=None, ignore_index=-100, need_x=True,
+                    need_weight=True):
+    """Gradients of `vocab_loss`: (dx like ``x`` or None, dw bf16 [V, H] or None)
+    for the gradients of its two results; see include/qmoe.h
+    `qmoe_vocab_loss_grad`."""
+    x2, t, s = _loss_operands(x, weight, targets, weight_scale, "vocab_loss_grad")
+    if need_weight and weight.dtype != torch.bfloat16:
+        raise NotImplementedError("vocab_loss_grad: no gradient for a table of 1-byte codes")
+    V, H = weight.shape
+    for v, name in ((lse, "lse"), (g_loss, "g_loss"), (g_lse, "g_lse")):
+        if v is not None and (v.dtype != torch.float32 or tuple(v.shape) != tuple(targets.shape)):
+            raise ValueError(f"vocab_loss_grad: {name} must be float32 {tuple(targets.shape)}, got {v.dtype} "
+                             f"{tuple(v.shape)}")
+    lse, g_loss = lse.contiguous(), g_loss.contiguous()
+    g_lse = g_lse.contiguous() if g_lse is not None else None
+    with _on_device(x2, weight, t, s, lse, g_loss, g_lse):
+        T, dev = t.numel(), weight.device
+        dx = torch.empty((T, H), dtype=torch.bfloat16, device=dev) if need_x else None
+        dw = torch.empty((V, H), dtype=torch.bfloat16, device=dev) if need_weight else None
+        if T == 0 and dw is not None:
+            dw.zero_()
+        if T and (need_x or need_weight):
+            need, wt = ctypes.c_int64(0), _TABLE_TYPES[weight.dtype]
+            check(lib.qmoe_vocab_loss_grad_workspace_size(T, V, H, wt, int(need_x), int(need_weight), ctypes.byref(need)),
+                  "vocab_loss_grad (shape)")
+            ws, ws_n = _workspace(dev, need.value)
+            check(lib.qmoe_vocab_loss_grad(_ptr(x2), x2.stride(0), T, _ptr(weight), wt, weight.stride(0), _ptr(s), V, H,
+                                           _ptr(t), int(t.dtype == torch.int64), int(ignore_index), _ptr(lse),
+                                           _ptr(g_loss), _ptr(g_lse), _ptr(dx), H, _ptr(dw), H, _ptr(ws), ws_n,
+                                           _stream(dev)), "vocab_loss_grad")
+    return (dx.view(x.shape) if dx is not None else None), dw
