@@ -376,6 +376,59 @@ int qmoe_moe_decode_workspace_size(const qmoe_moe_decode_desc* d, int64_t* bytes
 int qmoe_moe_decode(const qmoe_moe_decode_desc* d, void* workspace, int64_t ws_bytes, qmoe_stream_t stream);
 
 /*
+ * A whole MoE layer for a few tokens (a decode step) in two launches: routing
+ * (qmoe_moe_route's rule, float32 weights), then for every route j of token t
+ *   h[t, j] = bf16(act(W13[e] x[t] + b13[e])),
+ *   out[t] = bf16(sum over j of w[t, j] (W2[e] h[t, j] + b2[e])),
+ * float32 sums in a fixed order, each weight bf16(code * scale) and bf16
+ * activations (the dequantize-before-matmul regime of
+ * `kernels/megablox/gmm_v2.py:452-462`). Replaces `layers/adapter/
+ * moe_routing.py:232-323` followed by `layers/core/fused_moe_gmm.py:592-728`
+ * for 1..16 tokens; against qmoe_moe_route_dispatch + qmoe_gemm (twice) +
+ * qmoe_moe_combine neither the routing weights nor the route outputs are
+ * rounded to bf16 before their sum.
+ */
+enum {
+  QMOE_FEW_MXFP4 = 0, /* e2m1 + e8m0 per 32 k */
+  QMOE_FEW_NVFP4 = 1, /* e2m1 + bf16 per 16 k */
+  QMOE_FEW_INT4 = 2,  /* offset-binary nibbles + bf16 per `group` k */
+  QMOE_FEW_FP8 = 3,   /* e4m3 + f32 per (row, 128 k) */
+  QMOE_FEW_BF16 = 4
+};
+typedef struct qmoe_moe_few_desc {
+  int32_t format;          /* QMOE_FEW_... */
+  int32_t group;           /* QMOE_FEW_INT4: k per scale (32, 64 or 128) */
+  const void* x;           /* bf16 [T][ldx] */
+  int64_t ldx;             /* a multiple of 8 */
+  int32_t T;               /* tokens, 1..16 */
+  int32_t H;               /* hidden size, a multiple of 32 (FP8: 128; INT4: group) */
+  int32_t I;               /* intermediate size, likewise */
+  int32_t E;               /* experts, 1..512 */
+  int32_t topk;            /* routes per token, T * topk <= 128 */
+  const void* router_logits; /* [T][E] bf16, or f32 with logits_f32 */
+  int32_t logits_f32;
+  int32_t scoring;         /* as qmoe_moe_route */
+  const float* correction_bias; /* [E] or NULL */
+  int32_t renormalize;
+  float routed_scaling_factor;
+  int32_t num_group;
+  int32_t topk_group;
+  int32_t skip_padded;     /* routes whose weight is 0 in bf16 are padding */
+  const void* w1;          /* [E][2I][H]: gate rows then up rows */
+  const void* w2;          /* [E][H][I] */
+  const void* w1_scale;    /* [E][2I][..]; NULL for QMOE_FEW_BF16 */
+  const void* w2_scale;    /* [E][H][..] */
+  const float* w1_bias;    /* [E][2I] or NULL */
+  const float* w2_bias;    /* [E][H] or NULL */
+  int32_t act;             /* QMOE_ACT_SILU ... */
+  float act_p0, act_p1;
+  void* out;               /* bf16 [T][ldo] */
+  int64_t ldo;             /* a multiple of 4 */
+} qmoe_moe_few_desc;
+int qmoe_moe_few_workspace_size(const qmoe_moe_few_desc* d, int64_t* bytes);
+int qmoe_moe_few(const qmoe_moe_few_desc* d, void* workspace, int64_t ws_bytes, qmoe_stream_t stream);
+
+/*
  * Rows of the vocabulary table: out[n] = round(scale * s[id] * w[id]), id =
  * ids[n]. Replaces the gather + dequantize of `layers/adapter/quantization/
  * fp8.py:1692-1698` (VllmFp8LinearMethodTPU.embedding) with one launch, and the

@@ -355,16 +355,17 @@ __device__ __forceinline__ void route_token(const void* __restrict__ logits, int
 }
 
 // route_token with the scoring rule and grouping chosen at run time (one
-// instantiation per slot count for a kernel that serves every rule)
+// instantiation per slot count for a kernel that serves every rule); weights
+// as bf16, or float32 with w_f32
 template <int S>
 __device__ __forceinline__ void route_token_any(int scoring, bool grouped, const void* __restrict__ logits,
                                                 int logits_f32, int64_t t, int E, int topk,
                                                 const float* __restrict__ bias, int renormalize, float rsf,
-                                                int num_group, int topk_group, uint16_t* __restrict__ out_w,
+                                                int num_group, int topk_group, void* __restrict__ out_w,
                                                 int32_t* __restrict__ out_ids, float* ch, int32_t* lds_ids,
-                                                uint16_t* lds_w) {
+                                                uint16_t* lds_w, int w_f32 = 0) {
 #define QMOE_ROUTE_CASE(SC, G)                                                                               \
-  route_token<S, SC, G>(logits, logits_f32, t, E, topk, bias, renormalize, rsf, num_group, topk_group, out_w, 0, \
+  route_token<S, SC, G>(logits, logits_f32, t, E, topk, bias, renormalize, rsf, num_group, topk_group, out_w, w_f32, \
                         out_ids, ch, lds_ids, lds_w)
   switch (scoring * 2 + (grouped ? 1 : 0)) {
     case 0: QMOE_ROUTE_CASE(0, false); break;

@@ -116,6 +116,42 @@ class DecodeDesc(ctypes.Structure):
     ]
 
 
+class FewDesc(ctypes.Structure):
+    """Mirror of `qmoe_moe_few_desc` (field order and types must match)."""
+
+    _fields_ = [
+        ("format", _i32),
+        ("group", _i32),
+        ("x", _vp),
+        ("ldx", _i64),
+        ("T", _i32),
+        ("H", _i32),
+        ("I", _i32),
+        ("E", _i32),
+        ("topk", _i32),
+        ("router_logits", _vp),
+        ("logits_f32", _i32),
+        ("scoring", _i32),
+        ("correction_bias", _vp),
+        ("renormalize", _i32),
+        ("routed_scaling_factor", _f32),
+        ("num_group", _i32),
+        ("topk_group", _i32),
+        ("skip_padded", _i32),
+        ("w1", _vp),
+        ("w2", _vp),
+        ("w1_scale", _vp),
+        ("w2_scale", _vp),
+        ("w1_bias", _vp),
+        ("w2_bias", _vp),
+        ("act", _i32),
+        ("act_p0", _f32),
+        ("act_p1", _f32),
+        ("out", _vp),
+        ("ldo", _i64),
+    ]
+
+
 def _load():
     if not os.path.exists(_LIB_PATH):
         raise ImportError(
@@ -162,6 +198,10 @@ def _load():
     lib.qmoe_moe_decode_workspace_size.argtypes = [ctypes.POINTER(DecodeDesc), ctypes.POINTER(_i64)]
     lib.qmoe_moe_decode.restype = ctypes.c_int
     lib.qmoe_moe_decode.argtypes = [ctypes.POINTER(DecodeDesc), _vp, _i64, _vp]
+    lib.qmoe_moe_few_workspace_size.restype = ctypes.c_int
+    lib.qmoe_moe_few_workspace_size.argtypes = [ctypes.POINTER(FewDesc), ctypes.POINTER(_i64)]
+    lib.qmoe_moe_few.restype = ctypes.c_int
+    lib.qmoe_moe_few.argtypes = [ctypes.POINTER(FewDesc), _vp, _i64, _vp]
     lib.qmoe_vocab_lookup.restype = ctypes.c_int
     lib.qmoe_vocab_lookup.argtypes = [_vp, ctypes.c_int, _i64, _vp, ctypes.c_int, _i64, _vp, _i64, _i64, _f32, _vp,
                                       ctypes.c_int, _i64, _vp]
@@ -208,6 +248,8 @@ EXPORTED = (
     "qmoe_moe_combine",
     "qmoe_moe_decode_workspace_size",
     "qmoe_moe_decode",
+    "qmoe_moe_few_workspace_size",
+    "qmoe_moe_few",
     "qmoe_vocab_lookup",
     "qmoe_vocab_lookup_grad_workspace_size",
     "qmoe_vocab_lookup_grad",

@@ -57,6 +57,11 @@ _READERS = {
     # `qmoe/layers/fused_moe_decode.py`), whatever the cap above allows (0:
     # the cap alone)
     "QMOE_DECODE_OP_MAX_TOKENS": lambda: _nonneg_int("QMOE_DECODE_OP_MAX_TOKENS", 16),
+    # this build only: MoE steps of at most this many tokens (0: none, 16 at
+    # most) with bf16 activations run the two-launch layer
+    # (`qmoe/layers/fused_moe.py`, few_token_moe): one rounding of a token's
+    # sum instead of one per expert
+    "QMOE_FEW_TOKEN_MOE": lambda: _nonneg_int("QMOE_FEW_TOKEN_MOE", 0),
     # this build only (no reference counterpart): 128x128-block FP8 checkpoints
     # keep their tiles at run time with per-(token, 128) e4m3 activations
     # (the blockwise W8A8 recipe of BASELINE configs 2 and 4) instead of the

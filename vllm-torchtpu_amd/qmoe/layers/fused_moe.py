@@ -245,6 +245,45 @@ def _(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk, scor
     return x.new_empty(x.shape, dtype=torch.bfloat16)
 
 
+@torch.library.custom_op("qmoe::few_token_moe", mutates_args=())
+def _few_token_moe_op(x: torch.Tensor, router_logits: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor,
+                      w1_scale: Optional[torch.Tensor], w2_scale: Optional[torch.Tensor],
+                      w1_bias: Optional[torch.Tensor], w2_bias: Optional[torch.Tensor], topk: int, activation: str,
+                      fmt: str, scoring_func: str, renormalize: bool, e_bias: Optional[torch.Tensor],
+                      routed_scaling_factor: float, num_expert_group: int, topk_group: int, skip: bool) -> torch.Tensor:
+    return ops.moe_few_tokens(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk, activation, fmt,
+                              scoring_func, renormalize, e_bias, routed_scaling_factor, num_expert_group, topk_group,
+                              skip)
+
+
+@_few_token_moe_op.register_fake
+def _(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk, activation, fmt, scoring_func, renormalize,
+      e_bias, routed_scaling_factor, num_expert_group, topk_group, skip):
+    return x.new_empty(x.shape, dtype=torch.bfloat16)
+
+
+def few_token_moe(hidden_states, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk, activation, *,
+                  weight_format=None, scoring_func="softmax", renormalize=True, e_score_correction_bias=None,
+                  routed_scaling_factor=1.0, num_expert_group=1, topk_group=1, skip_padded_tokens=False):
+    """A whole MoE layer -- routing and routed experts -- of 1..16 bf16 tokens
+    (at most 128 routes) in two launches: bf16 [T, H].
+
+    The bf16-activation formats of the table above (``mxfp4``, ``nvfp4``,
+    ``int4``, ``fp8_w8a16``, ``bf16``), `select_experts`'s routing rule and
+    arguments. Against `select_experts` + `fused_moe_gmm` the routing weights
+    stay float32 and a token's expert outputs are summed in float32 and rounded
+    once, instead of each being rounded to bf16 before the sum; steps of a
+    method's layer take it with ``QMOE_FEW_TOKEN_MOE`` (`moe_forward`)."""
+    fmt = weight_format or infer_weight_format(w1, w1_scale)
+    args = (hidden_states, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, int(topk), activation or "", fmt,
+            scoring_func, bool(renormalize), e_score_correction_bias, float(routed_scaling_factor),
+            int(num_expert_group or 1), int(topk_group or 1), bool(skip_padded_tokens))
+    if ops.eager_call(*args[:8], e_score_correction_bias):
+        return ops.moe_few_tokens(*args)
+    ops._check_few(*args[:12])
+    return torch.ops.qmoe.few_token_moe(*args)
+
+
 def moe_forward(layer, x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, weight_format,
                 skip_padded_tokens=None, input_ids=None):
     """Routing + routed experts of a MoE method's `apply_monolithic`
@@ -252,7 +291,10 @@ def moe_forward(layer, x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2
     `fused_moe_gmm`). A decode-size batch (1..16 bf16 tokens, at most 64
     routes) with the layer's own scoring takes the fused route + dispatch
     launch; anything else (a model-supplied routing function, hash routing,
-    larger batches) routes first and calls `fused_moe_gmm`."""
+    larger batches) routes first and calls `fused_moe_gmm`. With
+    ``QMOE_FEW_TOKEN_MOE`` set, such a batch of at most that many tokens runs
+    `few_token_moe` where it has the weight format."""
+    from qmoe import envs
     from qmoe.layers import moe_routing
 
     topk = layer.moe_config.experts_per_token
@@ -268,6 +310,12 @@ def moe_forward(layer, x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2
         return fused_moe_gmm(x, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk_weights, topk_ids, None, topk,
                              act, skip_padded_tokens=skip_padded_tokens, weight_format=weight_format)
     ops.act_code(act)
+    if T <= envs.QMOE_FEW_TOKEN_MOE and act and ops.few_token_moe_takes(T, topk, weight_format):
+        bias, rsf, ng, tg = moe_routing.routing_params(layer)
+        return few_token_moe(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk, act,
+                             weight_format=weight_format, scoring_func=layer.scoring_func, renormalize=layer.renormalize,
+                             e_score_correction_bias=bias, routed_scaling_factor=rsf, num_expert_group=ng, topk_group=tg,
+                             skip_padded_tokens=skip_padded_tokens)
     if _dense_expert_admitted(x, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, act, weight_format):
         skip_padded_tokens = True  # the dense-expert branch's coefficient mask, as in fused_moe_gmm
     bias, rsf, ng, tg = moe_routing.routing_params(layer)

@@ -19,12 +19,6 @@ import torch
 from qmoe import ops
 
 
-def _eager(*ts):
-    """Plain tensors outside of a trace: no dispatcher has to see the call."""
-    return not torch.compiler.is_compiling() and all(
-        t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in ts)
-
-
 # ---------------------------------------------------------------- lookup
 
 
@@ -61,12 +55,12 @@ class _Embedding(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         (ids,) = ctx.saved_tensors
-        fn = ops.vocab_lookup_grad if _eager(grad, ids) else torch.ops.qmoe.vocab_lookup_grad
+        fn = ops.vocab_lookup_grad if ops.eager_call(grad, ids) else torch.ops.qmoe.vocab_lookup_grad
         return None, fn(grad, ids, *ctx.args), None, None, None
 
 
 def _lookup(ids, weight, weight_scale, scale, out_dtype):
-    if _eager(ids, weight, weight_scale):
+    if ops.eager_call(ids, weight, weight_scale):
         return ops.vocab_lookup(ids, weight, weight_scale, scale, out_dtype)
     ops._check_table(weight, weight_scale, "embedding")
     ops._check_ids(ids, "embedding: ids")
@@ -140,13 +134,13 @@ class _VocabCrossEntropy(torch.autograd.Function):
             return None, None, None, None, None
         if g_loss is None:
             g_loss = torch.zeros_like(g_lse)
-        fn = ops.vocab_loss_grad if _eager(x, weight, g_loss, g_lse) else torch.ops.qmoe.vocab_loss_grad
+        fn = ops.vocab_loss_grad if ops.eager_call(x, weight, g_loss, g_lse) else torch.ops.qmoe.vocab_loss_grad
         dx, dw = fn(x, weight, targets, lse, g_loss, g_lse, weight_scale, ctx.ignore_index, need_x, need_w)
         return (dx if need_x else None), (dw if need_w else None), None, None, None
 
 
 def _loss(x, weight, targets, weight_scale, ignore_index):
-    if _eager(x, weight, targets, weight_scale):
+    if ops.eager_call(x, weight, targets, weight_scale):
         return ops.vocab_loss(x, weight, targets, weight_scale, ignore_index)
     ops._check_loss(x, weight, targets, weight_scale, "vocab_cross_entropy")
     return torch.ops.qmoe.vocab_loss(x, weight, targets, weight_scale, ignore_index)

@@ -43,6 +43,13 @@ def _stream(dev):
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
+def eager_call(*ts):
+    """Whether a call on these tensors runs at once (plain tensors outside of a
+    trace), so that no dispatcher has to see it."""
+    return not torch.compiler.is_compiling() and all(
+        t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in ts)
+
+
 def _require_gpu(*ts):
     for t in ts:
         if t is not None and t.device.type != "cuda":
@@ -638,6 +645,119 @@ def stream_read(buf, workgroups=2048, sink=None):
     check(lib.qmoe_stream_read(_ptr(buf), nbytes, workgroups, _ptr(sink), _stream(buf.device)), "stream_read")
     return sink
 
+
+
+# ---------------------------------------------------------------- few-token MoE
+
+FEW_MAX_TOKENS = 16
+FEW_MAX_ROUTES = 128
+# format: (code, weight type, k per stored element, scale type, k per scale; int4's group comes from its scales)
+_FEW_FORMATS = {
+    "mxfp4": (0, torch.uint8, 2, torch.uint8, 32),
+    "nvfp4": (1, torch.uint8, 2, torch.bfloat16, 16),
+    "int4": (2, torch.int32, 8, torch.bfloat16, 0),
+    "fp8_w8a16": (3, FP8, 1, torch.float32, 128),
+    "bf16": (4, torch.bfloat16, 1, None, 0),
+}
+
+
+def few_token_moe_takes(T, topk, fmt):
+    """Whether `moe_few_tokens` has a form for this step."""
+    return fmt in _FEW_FORMATS and 1 <= T <= FEW_MAX_TOKENS and T * topk <= FEW_MAX_ROUTES
+
+
+def _check_few(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk, activation, fmt, scoring_func):
+    """Shapes and types of a few-token MoE layer; returns (I, int4 group)."""
+    if fmt not in _FEW_FORMATS:
+        raise NotImplementedError(f"few-token MoE: weight format {fmt!r} is not one of {sorted(_FEW_FORMATS)}")
+    if scoring_func not in _SCORING:
+        raise NotImplementedError(f"FusedMoE does not support {scoring_func} scoring function for TPU.")
+    if act_code(activation or None)[0] == _capi.ACT_NONE:
+        raise ValueError("few-token MoE: a gate / up activation is required")
+    _, wdt, per, sdt, blk = _FEW_FORMATS[fmt]
+    if x.dim() != 2 or x.dtype != torch.bfloat16:
+        raise ValueError(f"few-token MoE: hidden states must be bf16 [T, H], got {x.dtype} {tuple(x.shape)}")
+    T, H = x.shape
+    if w1.dim() != 3 or w2.dim() != 3 or w1.dtype != wdt or w2.dtype != wdt:
+        raise ValueError(f"few-token MoE: {fmt} experts are {wdt} [E, 2I, H / {per}] and [E, H, I / {per}]")
+    E, I = w1.shape[0], w2.shape[2] * per
+    if tuple(w1.shape) != (E, 2 * I, H // per) or tuple(w2.shape) != (E, H, I // per) or H % per:
+        raise ValueError(f"few-token MoE: inconsistent shapes: hidden {tuple(x.shape)}, w1 {tuple(w1.shape)}, "
+                         f"w2 {tuple(w2.shape)}")
+    if tuple(router_logits.shape) != (T, E):
+        raise ValueError(f"few-token MoE: router logits must be [{T}, {E}], got {tuple(router_logits.shape)}")
+    if not 1 <= T <= FEW_MAX_TOKENS or not 1 <= topk <= E or T * topk > FEW_MAX_ROUTES:
+        raise ValueError(f"few-token MoE takes 1..{FEW_MAX_TOKENS} tokens, topk <= experts and at most {FEW_MAX_ROUTES} "
+                         f"routes, got T={T}, topk={topk}, E={E}")
+    group = 0
+    for w, s, n, k, name in ((w1, w1_scale, 2 * I, H, "w1_scale"), (w2, w2_scale, H, I, "w2_scale")):
+        if not w.is_contiguous():
+            raise ValueError("few-token MoE: expert weights must be contiguous")
+        if sdt is None:
+            if s is not None:
+                raise ValueError(f"few-token MoE: {fmt} experts have no scales")
+            continue
+        b = blk
+        if fmt == "int4":
+            b = k // s.shape[-1] if s is not None and s.dim() == 3 and s.shape[-1] else 0
+            if b not in (32, 64, 128) or (group and b != group):
+                raise ValueError("few-token MoE: int4 scales are per group of 32, 64 or 128 k, the same in both matrices")
+            group = b
+        if s is None or s.element_size() != sdt.itemsize or (sdt.itemsize > 1 and s.dtype != sdt) or k % b or \
+                tuple(s.shape) != (E, n, k // b) or not s.is_contiguous():
+            raise ValueError(f"few-token MoE: {name} must be contiguous {sdt} [{E}, {n}, {k} / {b}]")
+    for b, n, name in ((w1_bias, 2 * I, "w1_bias"), (w2_bias, H, "w2_bias")):
+        if b is not None and b.numel() != E * n:
+            raise ValueError(f"few-token MoE: {name} must hold [{E}, {n}] values, got {tuple(b.shape)}")
+    mult = 128 if fmt == "fp8_w8a16" else max(32, group)
+    if H % mult or I % mult:
+        raise ValueError(f"few-token MoE: {fmt} needs H and I in multiples of {mult}, got {H}, {I}")
+    return I, group
+
+
+def moe_few_tokens(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk, activation, fmt,
+                   scoring_func="softmax", renormalize=True, bias=None, routed_scaling_factor=1.0, num_expert_group=1,
+                   topk_group=1, skip_padded_tokens=False):
+    """Routing and experts of 1..16 tokens in two launches -> bf16 [T, H]; see
+    include/qmoe.h `qmoe_moe_few`. Weights and scales in the layouts of
+    `qmoe.layers.fused_moe` (formats mxfp4, nvfp4, int4, fp8_w8a16, bf16)."""
+    I, group = _check_few(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk, activation, fmt,
+                          scoring_func)
+    act, p0, p1 = act_code(activation)
+    if bias is not None and bias.numel() != w1.shape[0]:
+        raise ValueError(f"few-token MoE: the correction bias must hold {w1.shape[0]} values")
+    with _on_device(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, bias):
+        if x.stride(1) != 1 or x.stride(0) < x.shape[1] or x.stride(0) % 8 or x.data_ptr() % 16:
+            x = x.clone(memory_format=torch.contiguous_format)
+        lg = router_logits
+        if lg.dtype not in (torch.bfloat16, torch.float32):
+            lg = lg.float()
+        lg = lg.contiguous()
+        f32 = lambda t: t.float().contiguous() if t is not None else None  # noqa: E731
+        b, b1, b2 = f32(bias), f32(w1_bias), f32(w2_bias)
+        out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+        d = _capi.FewDesc()
+        d.format, d.group = _FEW_FORMATS[fmt][0], group
+        d.x, d.ldx = x.data_ptr(), x.stride(0)
+        d.T, d.H, d.I, d.E, d.topk = x.shape[0], x.shape[1], I, w1.shape[0], topk
+        d.router_logits, d.logits_f32 = lg.data_ptr(), int(lg.dtype == torch.float32)
+        d.scoring = _SCORING[scoring_func]
+        d.correction_bias = b.data_ptr() if b is not None else None
+        d.renormalize, d.routed_scaling_factor = int(bool(renormalize)), float(routed_scaling_factor)
+        d.num_group, d.topk_group = int(num_expert_group or 1), int(topk_group or 1)
+        d.skip_padded = int(bool(skip_padded_tokens))
+        d.w1, d.w2 = w1.data_ptr(), w2.data_ptr()
+        d.w1_scale = w1_scale.data_ptr() if w1_scale is not None else None
+        d.w2_scale = w2_scale.data_ptr() if w2_scale is not None else None
+        d.w1_bias = b1.data_ptr() if b1 is not None else None
+        d.w2_bias = b2.data_ptr() if b2 is not None else None
+        d.act, d.act_p0, d.act_p1 = act, p0, p1
+        d.out, d.ldo = out.data_ptr(), out.stride(0)
+        need = ctypes.c_int64(0)
+        check(lib.qmoe_moe_few_workspace_size(ctypes.byref(d), ctypes.byref(need)), "moe_few_tokens (shape)")
+        ws, ws_n = _workspace(x.device, need.value)
+        check(lib.qmoe_moe_few(ctypes.byref(d), _ptr(ws), ws_n, _stream(x.device)), "moe_few_tokens")
+    return out
 
 
 # ---------------------------------------------------------------- vocabulary table
