@@ -491,7 +491,7 @@ int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void* w, int wt
  * [V, lddw >= H] (bf16 tables only). Either may be NULL. A token with neither
  * gradient leaves zeros in dx and nothing in dw, whatever its x holds. P and the
  * logits exist for one piece of the vocabulary at a time. lddx, lddw multiples
- * of 4, dx and dw 8-byte aligned. Every row of dx and dw is written; the sums'
+ * of 8, dx and dw 16-byte aligned. Every row of dx and dw is written; the sums'
  * order is fixed.
  */
 int qmoe_vocab_loss_grad_workspace_size(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw,

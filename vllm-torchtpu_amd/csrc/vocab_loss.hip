@@ -130,6 +130,199 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return r.u;
 }
 
+// The epilogues. A tile's wavefront (wn, wm), wn < WN, wm < 2, holds NI x MJ
+// blocks of 32 x 32: register quad q of block (i, j) is A rows (wn NI + i) 32 + 8
+// q + 4 kh .. + 3 and B row (2 j + wm) 32 + rl, rl = lane % 32, kh = lane / 32.
+// The logits are reduced in registers; the others pass 64 B rows at a time
+// through LDS (A row n of B row t at n ^ 4 f(t)), so that a thread stores 8
+// consecutive values. `smem`: 74 KB of LDS that no copy or read uses any more.
+// opaque_*: a value the compiler takes for a new one, so that what depends on
+// it (64 row scales, masks or addresses) is not kept for all MJ rounds at once.
+__device__ __forceinline__ int opaque_s(int v) {
+  asm volatile("" : "+s"(v));
+  return v;
+}
+__device__ __forceinline__ int opaque_v(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+__device__ __forceinline__ int vg_row_swz(int t) { return 4 * ((t ^ (t >> 3)) & 15); }
+
+template <int EPI, int BM, int WN, int NI, int MJ>
+__device__ __forceinline__ void vocab_epilogue(const VocabGemm& p, f32x16 (&acc)[NI][MJ], uint8_t* smem, int nt, int m0,
+                                               int arows, int brows, int wn, int wm) {
+  constexpr int BN = WN * NI * 32, THREADS = WN * 128;
+  static_assert(BN == kVN, "tile height");
+  const int tid = threadIdx.x, lane = tid & 63, rl = lane & 31, kh = lane >> 5, n0 = nt * BN;
+  float* s_scale = reinterpret_cast<float*>(smem);
+  float* reg = reinterpret_cast<float*>(smem + 9216);  // [64][BN]
+  if constexpr (EPI == VE_LSE || EPI == VE_PROB) {
+    for (int i = tid; i < BN; i += THREADS) s_scale[i] = p.row_scale ? p.row_scale[n0 + min(i, arows - 1)] : 1.0f;
+    __syncthreads();
+  }
+  if constexpr (EPI == VE_LSE) {
+    float2* s_part = reinterpret_cast<float2*>(smem + 1024);  // [WN][BM]
+    constexpr float kLog2e = 1.4426950408889634f;
+    const bool plain = p.row_scale == nullptr && arows == BN;  // neither scales nor rows to leave out
+    const int n1 = wn * NI * 32 + kh * 4;
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) {
+      const int tb = (2 * j + wm) * 32 + rl;
+      float m = -__builtin_inff(), s = 0.0f;
+      if (!plain) {
+        const int lim = opaque_s(arows);
+        const float* sc = s_scale + opaque_v(n1);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int n = i * 32 + q * 8 + r;
+              acc[i][j][q * 4 + r] = n1 + n < lim ? acc[i][j][q * 4 + r] * sc[n] : -__builtin_inff();
+            }
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+      const float base = lse_base(m), b2 = base * kLog2e;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], kLog2e, -b2));
+      // the target's logit, if its row is one of this lane's
+      if (tb < brows) {
+        const int64_t at = load_target(p, m0 + tb) - p.v0 - n0 - n1;
+        if (at >= 0 && at < NI * 32 && at < arows - n1 && (at & 4) == 0) {
+          float l = 0.0f;
+#pragma unroll
+          for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) l = (int)at == i * 32 + (r / 4) * 8 + r % 4 ? acc[i][j][r] : l;
+          p.tgt[m0 + tb] = l;
+        }
+      }
+      const float2 both = lse_merge(make_float2(m, s), make_float2(__shfl_xor(m, 32, 64), __shfl_xor(s, 32, 64)));
+      if (kh == 0) s_part[wn * BM + tb] = both;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
+    for (int t = tid; t < brows; t += THREADS) {
+      float2 v = s_part[t];
+#pragma unroll
+      for (int w = 1; w < WN; ++w) v = lse_merge(v, s_part[w * BM + t]);
+      p.part[(int64_t)(p.part_tile + nt) * p.nb + m0 + t] = v;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) {
+    const int tl = wm * 32 + rl, tb = 64 * j + tl;  // B row of the 64, of the tile
+    // (P^T wants zeros up to its row length, a multiple of 64, too)
+    if (64 * j >= brows) break;
+    if (j) __syncthreads();  // the rows before have been read
+    const int n1 = opaque_v(wn * NI * 32 + kh * 4);
+    if constexpr (EPI == VE_PROB) {
+      const bool valid = tb < brows;
+      float hot = 0.0f, coef = 0.0f, lse2 = 0.0f;
+      int at = -1;
+      if (valid) {
+        const int t = m0 + tb;
+        const int64_t tg = load_target(p, t);
+        hot = tg == p.ignore ? 0.0f : (tg >= 0 && tg < p.V ? p.g_loss[t] : __builtin_nanf(""));
+        coef = hot + (p.g_lse ? p.g_lse[t] : 0.0f);
+        lse2 = p.lse[t] * 1.4426950408889634f;
+        const int64_t in = tg - p.v0 - n0;
+        at = in >= 0 && in < arows ? (int)in : -1;
+      }
+      const int lim = opaque_s(arows);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int n = n1 + i * 32 + q * 8 + r;
+            // a token without a gradient leaves zeros, whatever its logits are
+            float e = __builtin_amdgcn_exp2f(fmaf(acc[i][j][q * 4 + r] * s_scale[n], 1.4426950408889634f, -lse2)) * coef;
+            e = n < lim && coef != 0.0f ? e : 0.0f;
+            v[r] = n == at ? e - hot : e;
+          }
+          const int n = n1 + i * 32 + q * 8;
+          *reinterpret_cast<float4*>(reg + tl * BN + (n ^ vg_row_swz(tl))) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = n1 + i * 32 + q * 8;
+          float v[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            v[r] = acc[i][j][q * 4 + r];
+          }
+          *reinterpret_cast<float4*>(reg + tl * BN + (n ^ vg_row_swz(tl))) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+    }
+    __syncthreads();
+    // 8 consecutive A rows of a B row per thread
+    constexpr int CH = BN / 8;
+    const int c = (tid % CH) * 8;
+    if (EPI != VE_PROB || p.p) {
+#pragma unroll 2
+      for (int t = tid / CH; t < 64; t += THREADS / CH) {
+        const int64_t row = m0 + 64 * j + t;
+        if (64 * j + t >= brows) break;
+        const float4 lo = *reinterpret_cast<const float4*>(reg + t * BN + (c ^ vg_row_swz(t)));
+        const float4 hi = *reinterpret_cast<const float4*>(reg + t * BN + ((c + 4) ^ vg_row_swz(t)));
+        float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        if constexpr (EPI == VE_PROB) {
+          // P times the row scales is what multiplies the codes
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] *= s_scale[c + k];
+          *reinterpret_cast<uint4*>(p.p + row * p.ldp + n0 + c) = make_uint4(
+              pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+        } else if (c < arows) {  // (A rows come in multiples of 8)
+          if constexpr (EPI == VE_SUM) {
+            float4* dst = reinterpret_cast<float4*>(p.sum + row * p.ldsum + n0 + c);
+            if (!p.first) {
+              const float4 a = dst[0], b = dst[1];
+              v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
+              v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+            }
+            if (!p.last) {
+              dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+              dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+              continue;
+            }
+          }
+          *reinterpret_cast<uint4*>(p.y + row * p.ldy + n0 + c) = make_uint4(
+              pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+        }
+      }
+    }
+    if constexpr (EPI == VE_PROB) {
+      if (p.pt) {
+        // 8 consecutive B rows of an A row per thread
+        const int tg8 = (tid & 7) * 8;
+        const int64_t t0 = m0 + 64 * j + tg8;
+#pragma unroll 2
+        for (int n = tid >> 3; n < BN; n += THREADS / 8) {
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = reg[(tg8 + k) * BN + (n ^ vg_row_swz(tg8 + k))];
+          if (n < arows)
+            *reinterpret_cast<uint4*>(p.pt + (int64_t)(n0 + n) * p.ldpt + t0) = make_uint4(
+                pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+        }
+      }
+    }
+  }
+}
+
 template <int EPI, int BM>
 __global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGemm p) {
   constexpr int BN = kVN, NI = 2, MJ = BM / 64, RING = BM > 128 ? 2 : 3;
@@ -261,141 +454,151 @@ __global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGem
   }
   __syncthreads();  // every wavefront is done with the stage buffers
 
-  // ---- epilogues. Register quad q of block (i, j): A rows wn * 64 + i * 32 + q
-  // * 8 + kh * 4 + 0..3, B row (2 j + wm) * 32 + rl
-  auto arow = [&](int i, int q) { return wn * 64 + i * 32 + q * 8 + kh * 4; };
-  auto brow = [&](int j) { return (2 * j + wm) * 32 + rl; };
-  float* s_scale = reinterpret_cast<float*>(smem);
-  if constexpr (EPI == VE_LSE || EPI == VE_PROB) {
-    if (tid < BN) s_scale[tid] = p.row_scale ? p.row_scale[n0 + min(tid, arows - 1)] : 1.0f;
+  vocab_epilogue<EPI, BM, 4, NI, MJ>(p, acc, smem, nt, m0, arows, brows, wn, wm);
+}
+
+// The same product in tiles of 256 x 256 by four wavefronts of 4 x 4 blocks (one
+// per SIMD, the sums in accumulation registers). A wavefront of 64 x 128 reads
+// 24 KB of operands from LDS per 32 MFMAs, one of 128 x 128 32 KB per 64: with
+// eight of the former per CU the reads and the copies' writes fill LDS's 128
+// bytes per cycle, which is what bounds that kernel.
+//
+// Stages of 64 k: 32 KB of A rows and 32 KB of B rows, in a ring of five such
+// slots (all of LDS): A(s), B(s), A(s + 1), B(s + 1), A(s + 2). At the barrier of
+// stage s every wavefront holds its last operands, and the stage's two slots
+// take B(s + 2) and A(s + 3). Their copies go out four per MFMA step and one at a
+// time between the MFMAs: four wavefronts' copies at once would keep the
+// address unit busy, and the matrix cores idle, for half a step. Whole
+// 128-byte lines per row: with 64-byte rows in a ring of four smaller stages the
+// second half of a line is asked for while the first is pending, and the L1
+// stalls on it (dw of 4096 tokens, 16384 x 4096: 458 us; these: see above).
+// TAIL: K is not a multiple of 64 (an instance of its own: the extra stage costs
+// the others registers).
+constexpr int kBThreads = 256;
+
+template <int EPI, bool TAIL>
+__global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm p) {
+  constexpr int BN = kVN, BM = 256, NI = 4, MJ = 4;
+  constexpr uint32_t SLOT = BN * 128, RING = 5 * SLOT;
+  __shared__ __align__(1024) uint8_t smem[RING];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave & 1, wm = wave >> 1, rl = lane & 31, kh = lane >> 5;
+  int mt, nt;
+  if (!tile_dense(blockIdx.x, p.m_tiles, p.n_tiles, mt, nt)) return;
+  const int n0 = nt * BN, m0 = mt * BM;
+  const int arows = min(BN, p.na - n0), brows = min(BM, p.nb - m0);
+
+  // copies: one instruction = 8 rows x 128 bytes (lane -> row l >> 3, slot l & 7;
+  // the slot of chunk c of row r is c ^ vg_swz(r)); wavefront w moves the row
+  // groups w, w + 4, ... of both operands; rows past the end repeat the last
+  // one (their products are dropped)
+  const int chunk16 = (lane & 7) ^ ((lane >> 3) ^ (wave & 1));
+  const uint8_t* abase = p.a + (int64_t)n0 * p.lda;
+  const uint8_t* bbase = p.b + (int64_t)m0 * p.ldb;
+  uint32_t aoff[8], boff[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int r = (wave + 4 * j) * 8 + (lane >> 3);
+    aoff[j] = (uint32_t)min(r, arows - 1) * (uint32_t)p.lda + chunk16 * 16;
+    boff[j] = (uint32_t)min(r, brows - 1) * (uint32_t)p.ldb + chunk16 * 16;
+  }
+  const int KF = p.K / 64;  // whole stages
+  const uint32_t cw = lds0 + wave * 1024;
+  union B8 {
+    uint4 u;
+    bf16x8 v;
+  };
+  B8 wf[2][NI], xf[2][MJ];
+  // operand reads of step q of a stage: lane -> row l & 31, chunk 2 q + kh
+  const uint32_t wpo = (uint32_t)(wn * NI * 4096 + rl * 128), xpo = (uint32_t)(wm * 4096 + rl * 128);
+  auto read_w = [&](uint32_t slot, int q) {
+    const uint8_t* b = smem + slot + wpo + ((2 * q + kh) ^ vg_swz(rl)) * 16;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) wf[q & 1][i].u = *reinterpret_cast<const uint4*>(b + i * 4096);
+  };
+  auto read_x = [&](uint32_t slot, int q) {
+    const uint8_t* b = smem + slot + xpo + ((2 * q + kh) ^ vg_swz(rl)) * 16;
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) xf[q & 1][j].u = *reinterpret_cast<const uint4*>(b + j * 8192);
+  };
+  f32x16 acc[NI][MJ];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < MJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+  auto mma_row = [&](int q, int i) {
+#pragma unroll
+    for (int j = 0; j < MJ; ++j)
+      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[q & 1][i].v, xf[q & 1][j].v, acc[i][j], 0, 0, 0);
+  };
+  if (KF > 0) {
+    // (stages past the last one copy it again, into slots nobody reads)
+    auto src = [&](const uint8_t* base, int s) { return uniform_ptr(base + (int64_t)min(s, KF - 1) * 128); };
+    auto dst = [&](uint32_t slot) { return (uint32_t)__builtin_amdgcn_readfirstlane(cw + slot); };
+    auto wrap = [](uint32_t slot) { return slot >= RING ? slot - RING : slot; };
+#pragma unroll
+    for (int j = 0; j < 8; ++j) lds_copy16(src(abase, 0), aoff[j], dst(0) + j * 4096);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) lds_copy16(src(bbase, 0), boff[j], dst(SLOT) + j * 4096);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) lds_copy16(src(abase, 1), aoff[j], dst(2 * SLOT) + j * 4096);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) lds_copy16(src(bbase, 1), boff[j], dst(3 * SLOT) + j * 4096);
+    wait_copies_upto<12>();  // the first stage
+    stage_barrier();
+    read_w(0, 0);
+    read_x(SLOT, 0);
+    uint32_t sa = 0;  // slot of A(s); B(s), A(s + 1), ... follow
+    for (int s = 0; s < KF; ++s) {
+      const uint32_t sb = wrap(sa + SLOT), sa1 = wrap(sa + 2 * SLOT), sb1 = wrap(sa + 3 * SLOT), sa2 = wrap(sa + 4 * SLOT);
+      const uint8_t *b1 = src(bbase, s + 1), *a2 = src(abase, s + 2), *b2 = src(bbase, s + 2);
+      const uint32_t db1 = dst(sb1) + 16384, da2 = dst(sa2), db2 = dst(sa);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (q == 3) {
+          wait_copies_upto<8>();  // stage s + 1 has landed
+          stage_barrier();        // and everybody holds this stage's last operands
+        }
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          if (i == 0) read_w(q < 3 ? sa : sa1, (q + 1) & 3);
+          if (i == 1) read_x(q < 3 ? sb : sb1, (q + 1) & 3);
+          if (q == 0) lds_copy16(b1, boff[4 + i], db1 + i * 4096);
+          else if (q < 3) lds_copy16(a2, aoff[4 * (q - 1) + i], da2 + (4 * (q - 1) + i) * 4096);
+          else lds_copy16(b2, boff[i], db2 + i * 4096);
+          mma_row(q, i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      sa = sa1;
+    }
+    wait_copies_upto<0>();
     __syncthreads();
   }
-  if constexpr (EPI == VE_LSE) {
-    float2* s_part = reinterpret_cast<float2*>(smem + 1024);  // [4 wn][BM]
+  if constexpr (TAIL) {  // the last, partial stage: zeros behind the rows' ends
+    const uint8_t *as = abase + (int64_t)KF * 128, *bs = bbase + (int64_t)KF * 128;
+    const bool in = KF * 64 + chunk16 * 8 < p.K;
+    const uint8_t* z = reinterpret_cast<const uint8_t*>(kVocabZero);
 #pragma unroll
-    for (int j = 0; j < MJ; ++j) {
-      const int tb = brow(j);
-      const bool valid = tb < brows;
-      const int64_t at = valid ? load_target(p, m0 + tb) - p.v0 - n0 : -1;  // the target's A row, if in the tile
-      float m = -__builtin_inff();
+    for (int j = 0; j < 8; ++j) {
+      lds_copy16(in ? as + aoff[j] : z, cw + j * 4096);
+      lds_copy16(in ? bs + boff[j] : z, cw + SLOT + j * 4096);
+    }
+    wait_copies_upto<0>();
+    __syncthreads();
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
+    for (int q = 0; q < 4; ++q) {
+      read_w(0, q);
+      read_x(SLOT, q);
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int n = arow(i, q) + r;
-            const float l = n < arows ? acc[i][j][q * 4 + r] * s_scale[n] : -__builtin_inff();
-            acc[i][j][q * 4 + r] = l;
-            m = fmaxf(m, l);
-            if (n == at && n < arows) p.tgt[m0 + tb] = l;
-          }
-      const float base = lse_base(m);
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s += __expf(acc[i][j][r] - base);
-      const float2 mine = make_float2(m, s);
-      const float2 both = lse_merge(mine, make_float2(__shfl_xor(m, 32, 64), __shfl_xor(s, 32, 64)));
-      if (kh == 0) s_part[wn * BM + tb] = both;
+      for (int i = 0; i < NI; ++i) mma_row(q, i);
     }
     __syncthreads();
-    if (tid < brows) {
-      float2 v = s_part[tid];
-#pragma unroll
-      for (int w = 1; w < 4; ++w) v = lse_merge(v, s_part[w * BM + tid]);
-      p.part[(int64_t)(p.part_tile + nt) * p.nb + m0 + tid] = v;
-    }
-  } else if constexpr (EPI == VE_PROB) {
-#pragma unroll
-    for (int j = 0; j < MJ; ++j) {
-      const int tb = brow(j), t = m0 + tb;
-      const bool valid = tb < brows;
-      float hot = 0.0f, coef = 0.0f, lse = 0.0f;
-      int64_t at = -1;
-      if (valid) {
-        const int64_t tg = load_target(p, t);
-        hot = tg == p.ignore ? 0.0f : (tg >= 0 && tg < p.V ? p.g_loss[t] : __builtin_nanf(""));
-        coef = hot + (p.g_lse ? p.g_lse[t] : 0.0f);
-        lse = p.lse[t];
-        at = tg - p.v0 - n0;
-      }
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        uint2 w[4];  // the quads as bf16: four A rows of this B row
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float v[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int n = arow(i, q) + r;
-            float e = 0.0f;
-            // a token without a gradient leaves zeros, whatever its logits are
-            if (n < arows && coef != 0.0f) e = __expf(acc[i][j][q * 4 + r] * s_scale[n] - lse) * coef;
-            if (n == at && n < arows) e -= hot;
-            v[r] = e;
-          }
-          // (P times the row scales is what multiplies the codes)
-          const float* sc = s_scale + arow(i, q);
-          w[q] = make_uint2(pack_bf16(v[0] * sc[0], v[1] * sc[1]), pack_bf16(v[2] * sc[2], v[3] * sc[3]));
-          if (p.pt) {
-            // 4 x 4 transposition over the lanes of a quad: lane k gets A row k of
-            // four consecutive tokens
-            const int k = lane & 3;
-            float o[4];
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {  // from lane k ^ d its value of row k
-              const float send = (k ^ d) == 0 ? v[0] : ((k ^ d) == 1 ? v[1] : ((k ^ d) == 2 ? v[2] : v[3]));
-              const float got = d == 0 ? send : __shfl_xor(send, d, 64);
-              if ((k ^ d) == 0) o[0] = got;
-              if ((k ^ d) == 1) o[1] = got;
-              if ((k ^ d) == 2) o[2] = got;
-              if ((k ^ d) == 3) o[3] = got;
-            }
-            const int t4 = m0 + (tb & ~3);
-            if (t4 < p.ldpt)
-              *reinterpret_cast<uint2*>(p.pt + (int64_t)(n0 + arow(i, q) + k) * p.ldpt + t4) =
-                  make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
-          }
-        }
-        if (valid && p.p) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint2*>(p.p + (int64_t)t * p.ldp + n0 + arow(i, q)) = w[q];
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < MJ; ++j) {
-      const int t = m0 + brow(j);
-      if (brow(j) >= brows) continue;
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = n0 + arow(i, q);
-          float v[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = acc[i][j][q * 4 + r];
-          if (n + 4 <= p.na) {
-            if constexpr (EPI == VE_SUM) {
-              float4* dst = reinterpret_cast<float4*>(p.sum + (int64_t)t * p.ldsum + n);
-              if (!p.first) {
-                const float4 o = *dst;
-                v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
-              }
-              if (!p.last) {
-                *dst = make_float4(v[0], v[1], v[2], v[3]);
-                continue;
-              }
-            }
-            *reinterpret_cast<uint2*>(p.y + (int64_t)t * p.ldy + n) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-          }
-        }
-    }
   }
+  vocab_epilogue<EPI, BM, 2, NI, MJ>(p, acc, smem, nt, m0, arows, brows, wn, wm);
 }
 
 // Joins the tiles of a token (one wavefront): lse, loss
@@ -441,7 +644,8 @@ __global__ __launch_bounds__(256) void vocab_expand_kernel(const uint8_t* w, int
   *reinterpret_cast<uint4*>(out + r * ldo + c) = make_uint4(lo.x, lo.y, hi.x, hi.y);
 }
 
-// src rows [R][C] (bf16 or codes) -> out [C][ldo] bf16, columns R .. ldo - 1 zero;
+// src rows [R][C] (bf16 or codes) -> out [C][ldo] bf16, columns R .. zero up to the
+// next multiple of 64;
 // with `targets` a row whose token has no gradient becomes zeros (whatever it
 // holds). 64 x 64 tiles through LDS.
 template <int WT>
@@ -483,7 +687,7 @@ __global__ __launch_bounds__(256) void vocab_transpose_kernel(const uint8_t* src
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int c = (tid >> 3) + 32 * k;
-    if (c0 + c >= C || r0 + r >= ldo) continue;
+    if (c0 + c >= C) continue;
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) u[i] = tile[r + 2 * i][c] | (uint32_t)tile[r + 2 * i + 1][c] << 16;
@@ -502,7 +706,9 @@ void launch_gemm(VocabGemm g, hipStream_t st) {
   g.n_tiles = cdiv(g.na, kVN);
   g.m_tiles = cdiv(g.nb, bm);
   const unsigned grid = (unsigned)(cdiv(g.n_tiles * g.m_tiles, kXcds) * kXcds);
-  if (bm == 256) hipLaunchKernelGGL((vocab_gemm_kernel<EPI, 256>), dim3(grid), dim3(kVThreads), 0, st, g);
+  constexpr bool kTails = EPI == VE_LSE || EPI == VE_PROB;  // (the K of dx and dw is a multiple of 64)
+  if (bm == 256 && kTails && g.K % 64) hipLaunchKernelGGL((vocab_big_kernel<EPI, kTails>), dim3(grid), dim3(kBThreads), 0, st, g);
+  else if (bm == 256) hipLaunchKernelGGL((vocab_big_kernel<EPI, false>), dim3(grid), dim3(kBThreads), 0, st, g);
   else hipLaunchKernelGGL((vocab_gemm_kernel<EPI, 128>), dim3(grid), dim3(kVThreads), 0, st, g);
 }
 
@@ -527,8 +733,8 @@ struct LossArgs {
 };
 
 void launch_transpose(int wt, const uint8_t* src, int64_t ld, int64_t R, int64_t C, uint16_t* out, int64_t ldo,
-                      const LossArgs* mask, const float* g_loss, const float* g_lse, hipStream_t st) {
-  const dim3 grid((unsigned)cdiv(ldo, (int64_t)64), (unsigned)cdiv(C, (int64_t)64));
+                      int64_t width, const LossArgs* mask, const float* g_loss, const float* g_lse, hipStream_t st) {
+  const dim3 grid((unsigned)cdiv(width, (int64_t)64), (unsigned)cdiv(C, (int64_t)64));
   const void* tg = mask ? mask->targets : nullptr;
   const int i64 = mask ? mask->targets_i64 : 0;
   const int64_t ig = mask ? mask->ignore : 0;
@@ -584,17 +790,21 @@ int64_t grad_piece(int64_t T, int64_t V, int64_t H) {
   return std::min(up(V, kVN), std::max<int64_t>((int64_t)(64 << 20) / std::max(up(T, 64), H) / kVN * kVN, kVN));
 }
 
+// Row pitch (bf16) of a buffer of n columns, n a multiple of 64: an odd number of
+// 128-byte lines, so that the rows of a tile do not share memory channels
+int64_t odd_pitch(int64_t n) { return n % 128 ? n : n + 64; }
+
 // P, P^T, table piece transposed, x transposed, float32 sums, expanded rows
 int64_t grad_layout(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw, int64_t (&off)[6]) {
-  const int64_t Vc = grad_piece(T, V, H), Tp = up(T, 64);
+  const int64_t Vc = grad_piece(T, V, H), Vp = odd_pitch(Vc), Tp = odd_pitch(up(T, 64));
   const bool pieces = Vc < V;
   int64_t at = 0;
   off[0] = at;
-  if (need_dx) at += up(T * Vc * 2, 256);
+  if (need_dx) at += up(T * Vp * 2, 256);
   off[1] = at;
   if (need_dw) at += up(Vc * Tp * 2, 256);
   off[2] = at;
-  if (need_dx) at += up(H * Vc * 2, 256);
+  if (need_dx) at += up(H * Vp * 2, 256);
   off[3] = at;
   if (need_dw) at += up(H * Tp * 2, 256);
   off[4] = at;
@@ -675,17 +885,17 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
   const LossArgs a{x, ldx, T, w, wtype, ldw, row_scale, V, H, targets, targets_i64, ignore_index};
   if (!loss_args_ok(a) || T == 0 || !lse || !g_loss || (!dx && !dw)) return QMOE_ERR_ARG;
   if (dw && wtype) return QMOE_ERR_ARG;  // codes have no gradient
-  if (dx && (lddx < H || lddx % 4 || (reinterpret_cast<uintptr_t>(dx) & 7))) return QMOE_ERR_ARG;
-  if (dw && (lddw < H || lddw % 4 || (reinterpret_cast<uintptr_t>(dw) & 7))) return QMOE_ERR_ARG;
+  if (dx && (lddx < H || lddx % 8 || (reinterpret_cast<uintptr_t>(dx) & 15))) return QMOE_ERR_ARG;
+  if (dw && (lddw < H || lddw % 8 || (reinterpret_cast<uintptr_t>(dw) & 15))) return QMOE_ERR_ARG;
   int64_t off[6];
   if (!workspace || ws_bytes < grad_layout(T, V, H, wtype, dx != nullptr, dw != nullptr, off)) return QMOE_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const int64_t Vc = grad_piece(T, V, H), Tp = up(T, 64);
+  const int64_t Vc = grad_piece(T, V, H), Vp = odd_pitch(Vc), Tw = up(T, 64), Tp = odd_pitch(Tw);
   uint16_t* P = reinterpret_cast<uint16_t*>(ws + off[0]);
   uint16_t* PT = reinterpret_cast<uint16_t*>(ws + off[1]);
   uint16_t* WT = reinterpret_cast<uint16_t*>(ws + off[2]);
   uint16_t* XT = reinterpret_cast<uint16_t*>(ws + off[3]);
-  if (dw) launch_transpose(0, static_cast<const uint8_t*>(x), ldx * 2, T, H, XT, Tp, &a, g_loss, g_lse, stream);
+  if (dw) launch_transpose(0, static_cast<const uint8_t*>(x), ldx * 2, T, H, XT, Tp, Tw, &a, g_loss, g_lse, stream);
   for (int64_t v0 = 0; v0 < V; v0 += Vc) {
     const uint8_t* rows = static_cast<const uint8_t*>(w) + v0 * ldw * (wtype ? 1 : 2);
     const int64_t n = std::min(Vc, V - v0), np = up(n, 64);
@@ -713,18 +923,18 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
     g.g_loss = g_loss;
     g.g_lse = g_lse;
     g.p = dx ? P : nullptr;
-    g.ldp = Vc;
+    g.ldp = Vp;
     g.pt = dw ? PT : nullptr;
     g.ldpt = Tp;
     launch_gemm<VE_PROB>(g, stream);
     if (dx) {
-      launch_transpose(wtype, rows, ldw * (wtype ? 1 : 2), n, H, WT, np, nullptr, nullptr, nullptr, stream);
+      launch_transpose(wtype, rows, ldw * (wtype ? 1 : 2), n, H, WT, Vp, np, nullptr, nullptr, nullptr, stream);
       VocabGemm d{};
       d.a = reinterpret_cast<const uint8_t*>(WT);
-      d.lda = np * 2;
+      d.lda = Vp * 2;
       d.na = (int)H;
       d.b = reinterpret_cast<const uint8_t*>(P);
-      d.ldb = Vc * 2;
+      d.ldb = Vp * 2;
       d.nb = (int)T;
       d.K = (int)np;
       d.sum = reinterpret_cast<float*>(ws + off[4]);
@@ -743,7 +953,7 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
       d.b = reinterpret_cast<const uint8_t*>(PT);
       d.ldb = Tp * 2;
       d.nb = (int)n;
-      d.K = (int)Tp;
+      d.K = (int)Tw;
       d.y = static_cast<uint16_t*>(dw) + v0 * lddw;
       d.ldy = lddw;
       launch_gemm<VE_STORE>(d, stream);
