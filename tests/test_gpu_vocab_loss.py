@@ -188,13 +188,16 @@ def test_gradient_through_a_coded_table(dev, dtype, T, V, H):
         ops.vocab_loss_grad(x, w, t, loss.detach(), g, weight_scale=s)
 
 
-def test_gradients_over_several_pieces(dev):
-    """More table rows than one piece (the wide rows make the pieces short)."""
-    x, w, _, t = _case(dev, 70, 1500, 65536)
-    g = torch.randn(70, device=dev)
-    _, lse = vocab_cross_entropy(x, w, t)
-    dx, dw = ops.vocab_loss_grad(x, w, t, lse, g)
-    _check_grads(dx, dw, x, w, None, t, g, None)
+@pytest.mark.parametrize("T,V,H,dtype", [(70, 1500, 65536, BF16), (33, 3000, 32768, BF16), (33, 3000, 32768, I8),
+                                         (150, 2500, 32776, E4)])
+def test_gradients_over_several_pieces(dev, T, V, H, dtype):
+    """More table rows than one piece (the wide rows make the pieces short),
+    with and without a K split of dx."""
+    x, w, s, t = _case(dev, T, V, H, dtype)
+    g = torch.randn(T, device=dev)
+    _, lse = vocab_cross_entropy(x, w, t, s)
+    dx, dw = ops.vocab_loss_grad(x, w, t, lse, g, weight_scale=s, need_weight=dtype == BF16)
+    _check_grads(dx, dw, x, w, s, t, g, None)
 
 
 def test_gradients_by_differences(dev):

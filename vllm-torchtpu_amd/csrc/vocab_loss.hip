@@ -39,7 +39,7 @@ constexpr int kVN = 256;  // A rows of a tile
 enum { VE_LSE = 0, VE_PROB = 1, VE_SUM = 2, VE_STORE = 3 };
 
 struct VocabGemm {
-  const uint8_t* a;  // bf16 rows [na][lda bytes]
+  const uint8_t* a;  // rows [na][lda bytes] of bf16, or codes where the kernel says so
   int64_t lda;
   int na;
   const uint8_t* b;  // bf16 rows [nb][ldb bytes]
@@ -65,6 +65,8 @@ struct VocabGemm {
   float* sum;       // [nb][ldsum] float32 sums of the pieces before, or nullptr
   int64_t ldsum;
   int first, last;  // first / last piece
+  int kslice;       // K split: slice z takes the K range from z * kslice on ...
+  float* slices;    // ... and leaves its sums in [z][nb][ldsum]; kslice 0: no split
   uint16_t* y;      // [nb][ldy]
   int64_t ldy;
 };
@@ -77,31 +79,6 @@ __device__ __forceinline__ int64_t load_target(const VocabGemm& p, int t) {
 }
 
 __device__ __forceinline__ int vg_swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
-
-// Four 16-byte copies per lane from one scalar base, to `lds` + 0, 8, 16, 24 KB
-// (the scalar move gives the base its wait states, as in gemm_tile.h)
-__device__ __forceinline__ void vg_copy4(const uint8_t* base, const uint32_t (&off)[4], uint32_t lds) {
-  const uint8_t* b;
-  asm volatile(
-      "s_mov_b64 %0, %6\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\t"
-      "s_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %0\n\t"
-      "s_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %0\n\t"
-      "s_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %0"
-      : "=&s"(b)
-      : "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base)
-      : "m0", "scc", "memory");
-}
-__device__ __forceinline__ void vg_copy2(const uint8_t* base, const uint32_t (&off)[2], uint32_t lds) {
-  const uint8_t* b;
-  asm volatile(
-      "s_mov_b64 %0, %4\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\t"
-      "s_add_u32 m0, m0, 0x2000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %0"
-      : "=&s"(b)
-      : "s"(lds), "v"(off[0]), "v"(off[1]), "s"(base)
-      : "m0", "scc", "memory");
-}
-__device__ __forceinline__ void vg_copy(const uint8_t* base, const uint32_t (&off)[4], uint32_t lds) { vg_copy4(base, off, lds); }
-__device__ __forceinline__ void vg_copy(const uint8_t* base, const uint32_t (&off)[2], uint32_t lds) { vg_copy2(base, off, lds); }
 
 __device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* q) {
   const uint64_t b = reinterpret_cast<uint64_t>(q);
@@ -323,12 +300,69 @@ __device__ __forceinline__ void vocab_epilogue(const VocabGemm& p, f32x16 (&acc)
   }
 }
 
-template <int EPI, int BM>
-__global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGemm p) {
-  constexpr int BN = kVN, NI = 2, MJ = BM / 64, RING = BM > 128 ? 2 : 3;
-  constexpr int WB = BN * 128, XB = BM * 128, STG = WB + XB;
+// This workgroup's slice of a K split (dx only)
+template <int EPI>
+__device__ __forceinline__ void take_slice(VocabGemm& p) {
+  if constexpr (EPI == VE_SUM) {
+    if (p.kslice) {
+      const int k0 = blockIdx.y * p.kslice;
+      p.a += (int64_t)k0 * 2;
+      p.b += (int64_t)k0 * 2;
+      p.K = min(p.kslice, p.K - k0);
+      p.sum = p.slices + (int64_t)blockIdx.y * p.nb * p.ldsum;
+      p.first = 1, p.last = 0;
+    }
+  }
+}
+
+// 8 codes of a chunk as bf16 (exact)
+template <int AT>
+__device__ __forceinline__ bf16x8 codes8_to_bf16(uint32_t lo, uint32_t hi) {
+  union {
+    bf16x2 h[4];
+    bf16x8 v;
+  } r;
+  if constexpr (AT == 3) {
+    r.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, 1.0f, false);
+    r.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, 1.0f, true);
+    r.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, 1.0f, false);
+    r.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, 1.0f, true);
+  } else if constexpr (AT == 5) {
+    r.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8((int)lo, 1.0f, false);
+    r.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8((int)lo, 1.0f, true);
+    r.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8((int)hi, 1.0f, false);
+    r.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8((int)hi, 1.0f, true);
+  } else {
+    // n + 128 by the byte conversions, then - 128
+    const uint32_t u = lo ^ 0x80808080u, w = hi ^ 0x80808080u;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      r.h[k] = __builtin_convertvector(
+          f32x2{(float)((u >> (16 * k)) & 0xffu) - 128.0f, (float)((u >> (16 * k + 8)) & 0xffu) - 128.0f}, bf16x2);
+      r.h[2 + k] = __builtin_convertvector(
+          f32x2{(float)((w >> (16 * k)) & 0xffu) - 128.0f, (float)((w >> (16 * k + 8)) & 0xffu) - 128.0f}, bf16x2);
+    }
+  }
+  return r.v;
+}
+
+// Tiles of 256 A rows x BM B rows (64 or 128) by eight wavefronts, two per SIMD,
+// for problems that the 256 x 256 tiles below would leave CUs idle or pad, and
+// for few tokens, where reading the table is all that counts: with codes (AT 3
+// e4m3, 4 int8, 5 e5m2) the table is read as it is stored and expanded
+// between LDS and the matrix cores. Stages of 64 k of every row in a ring of
+// as many as fit.
+template <int EPI, int BM, int AT>
+__global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGemm args) {
+  constexpr int BN = kVN, NI = 2, MJ = BM / 64;
+  constexpr int AB = AT ? 64 : 128;  // bytes of an A row per stage
+  constexpr int WB = BN * AB, STG = WB + BM * 128;
+  constexpr int RING = 163840 / STG < 6 ? 163840 / STG : 6;
   __shared__ __align__(1024) uint8_t smem[RING * STG];
+  static_assert(RING >= 3 && RING * STG >= 9216 + 65536, "ring, epilogue region");
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
+  VocabGemm p = args;
+  take_slice<EPI>(p);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave & 3, wm = wave >> 2, rl = lane & 31, kh = lane >> 5;
   int mt, nt;
@@ -337,36 +371,36 @@ __global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGem
   const int arows = min(BN, p.na - n0), brows = min(BM, p.nb - m0);
 
   // copies: one instruction = 8 rows x 128 bytes (lane -> row l >> 3, slot l & 7;
-  // the slot of chunk c of row r is c ^ vg_swz(r)); rows past the end repeat the
-  // last one (their products are dropped)
-  constexpr int WI = BN / 64, XI = BM / 64;
-  const int chunk16 = (lane & 7) ^ ((lane >> 3) ^ (wave & 1));
+  // the slot of chunk c of row r is c ^ vg_swz(r)) or, of codes, 16 rows x 64
+  // bytes (lane -> row l >> 2, slot l & 3, chunk c at c ^ (r / 4) % 4); wavefront w
+  // moves the groups w, w + 8, ... of both operands; rows past the end repeat
+  // the last one (their products are dropped)
+  constexpr int WI = WB / 8192, XI = BM / 64;
+  const int xchunk = (lane & 7) ^ ((lane >> 3) ^ (wave & 1));
+  const int achunk = AT ? (lane & 3) ^ ((lane >> 4) & 3) : xchunk;
   const uint8_t* abase = p.a + (int64_t)n0 * p.lda;
   const uint8_t* bbase = p.b + (int64_t)m0 * p.ldb;
   uint32_t aoff[WI], boff[XI];
 #pragma unroll
-  for (int j = 0; j < WI; ++j)
-    aoff[j] = (uint32_t)min((wave + 8 * j) * 8 + (lane >> 3), arows - 1) * (uint32_t)p.lda + chunk16 * 16;
+  for (int j = 0; j < WI; ++j) {
+    const int r = AT ? (wave + 8 * j) * 16 + (lane >> 2) : (wave + 8 * j) * 8 + (lane >> 3);
+    aoff[j] = (uint32_t)min(r, arows - 1) * (uint32_t)p.lda + achunk * 16;
+  }
 #pragma unroll
   for (int j = 0; j < XI; ++j)
-    boff[j] = (uint32_t)min((wave + 8 * j) * 8 + (lane >> 3), brows - 1) * (uint32_t)p.ldb + chunk16 * 16;
-  const int KS = (p.K + 63) / 64;
+    boff[j] = (uint32_t)min((wave + 8 * j) * 8 + (lane >> 3), brows - 1) * (uint32_t)p.ldb + xchunk * 16;
+  const int KF = p.K / 64;  // whole stages
   const uint32_t cw = lds0 + wave * 1024;
-  auto copy_stage = [&](int s, int buf) {
-    const uint32_t d = __builtin_amdgcn_readfirstlane(cw + buf * STG);
-    const uint8_t* as = uniform_ptr(abase + (int64_t)s * 128);
-    const uint8_t* bs = uniform_ptr(bbase + (int64_t)s * 128);
-    if (s * 64 + 64 <= p.K) {
-      vg_copy(as, aoff, d);
-      vg_copy(bs, boff, d + WB);
-    } else {  // the last, partial stage: zeros behind the rows' ends
-      const bool in = s * 64 + chunk16 * 8 < p.K;
-      const uint8_t* z = reinterpret_cast<const uint8_t*>(kVocabZero);
+  // stage s to slot `slot` (stages past the last one copy it again, into slots
+  // nobody reads)
+  auto copy_stage = [&](int s, int slot) {
+    const uint32_t d = __builtin_amdgcn_readfirstlane(cw + slot * STG);
+    const int k = min(s, KF - 1);
+    const uint8_t *as = uniform_ptr(abase + (int64_t)k * AB), *bs = uniform_ptr(bbase + (int64_t)k * 128);
 #pragma unroll
-      for (int j = 0; j < WI; ++j) lds_copy16(in ? as + aoff[j] : z, d + j * 8192);
+    for (int j = 0; j < WI; ++j) lds_copy16(as, aoff[j], d + j * 8192);
 #pragma unroll
-      for (int j = 0; j < XI; ++j) lds_copy16(in ? bs + boff[j] : z, d + WB + j * 8192);
-    }
+    for (int j = 0; j < XI; ++j) lds_copy16(bs, boff[j], d + WB + j * 8192);
   };
 
   f32x16 acc[NI][MJ];
@@ -377,84 +411,114 @@ __global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGem
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
-  // The K pipeline over the wavefront's first MJE 32-row B blocks (those with a
-  // row). Per stage: the first operands are in registers (read during the last
-  // MFMAs of the stage before); all but the last MFMA step run while the next
-  // step's operands are read; then the next stage's copies have landed ->
-  // barrier: everybody holds this stage's last operands, so that its buffer
-  // takes the copies of stage s + RING -> the last step, while the next stage's
-  // first operands are read.
-  auto pipeline = [&](auto mje_c) {
-    constexpr int MJE = decltype(mje_c)::value;
+  // operand reads and MFMAs of step q (16 k). bf16: lane -> row l & 31, chunk 2 q
+  // + kh of both operands. Codes: a 16-byte chunk, 2 (q / 2) + kh, holds the
+  // lane's codes of two steps, so the B chunk is 4 (q / 2) + 2 kh + q % 2.
+  union B8 {
+    uint4 u;
+    bf16x8 v;
+  };
+  B8 wf[2][NI], xf[2][MJ];
+  auto read_q = [&](int slot, int q) {
+    const uint8_t* sW = smem + slot * STG;
+    if constexpr (AT) {
+      if (q % 2 == 0)
 #pragma unroll
-    for (int r = 0; r < RING; ++r)
-      if (r < KS) copy_stage(r, r);
-    auto landed = [&](bool ahead) {
-      if (ahead && RING == 3) wait_copies_upto<WI + XI>();
-      else wait_copies_upto<0>();
-    };
-    auto chunk = [&](const uint8_t* base, int row, int c) {
-      return *reinterpret_cast<const uint4*>(base + (row + rl) * 128 + ((c ^ vg_swz(rl)) * 16));
-    };
-    landed(false);
-    stage_barrier();
-    int buf = 0;
-    union B8 {
-      uint4 u;
-      bf16x8 v;
-    };
-    constexpr int MR = MJE > 0 ? MJE : 1;
-    B8 wf[2][NI], xf[2][MR];
-    auto read_q = [&](int b, int q) {
-      const uint8_t* sW = smem + b * STG;
-#pragma unroll
-      for (int i = 0; i < NI; ++i) wf[q & 1][i].u = chunk(sW, wn * 64 + i * 32, 2 * q + kh);
-#pragma unroll
-      for (int j = 0; j < MJE; ++j) xf[q & 1][j].u = chunk(sW + WB, (2 * j + wm) * 32, 2 * q + kh);
-    };
-    auto mma = [&](int q) {
+        for (int i = 0; i < NI; ++i)
+          wf[q / 2][i].u = *reinterpret_cast<const uint4*>(sW + (wn * 64 + i * 32 + rl) * 64 +
+                                                            (((2 * (q / 2) + kh) ^ (rl >> 2)) & 3) * 16);
+    } else {
 #pragma unroll
       for (int i = 0; i < NI; ++i)
+        wf[q & 1][i].u =
+            *reinterpret_cast<const uint4*>(sW + (wn * 64 + i * 32 + rl) * 128 + ((2 * q + kh) ^ vg_swz(rl)) * 16);
+    }
+    const int c = AT ? 4 * (q / 2) + 2 * kh + (q & 1) : 2 * q + kh;
 #pragma unroll
-        for (int j = 0; j < MJE; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[q & 1][i].v, xf[q & 1][j].v, acc[i][j], 0, 0, 0);
-    };
-    if constexpr (MJE > 0) read_q(0, 0);
-    for (int s = 0; s < KS; ++s) {
-      const int nb = buf == RING - 1 ? 0 : buf + 1;
-      if constexpr (MJE > 0) {
+    for (int j = 0; j < MJ; ++j)
+      xf[q & 1][j].u =
+          *reinterpret_cast<const uint4*>(sW + WB + ((2 * j + wm) * 32 + rl) * 128 + (c ^ vg_swz(rl)) * 16);
+  };
+  auto mma = [&](int q) {
 #pragma unroll
-        for (int q = 0; q < 3; ++q) {
-          read_q(buf, q + 1);
-          mma(q);
-        }
+    for (int i = 0; i < NI; ++i) {
+      bf16x8 a;
+      if constexpr (AT) {
+        const uint4 c = wf[q / 2][i].u;
+        a = q & 1 ? codes8_to_bf16<AT>(c.z, c.w) : codes8_to_bf16<AT>(c.x, c.y);
+      } else {
+        a = wf[q & 1][i].v;
       }
-      if (s + 1 < KS) landed(s + 2 < KS);
-      stage_barrier();
-      if (s + RING < KS) copy_stage(s + RING, buf);
-      asm volatile("" ::: "memory");
-      if constexpr (MJE > 0) {
-        if (s + 1 < KS) read_q(nb, 0);
-        mma(3);
-      }
-      buf = nb;
+#pragma unroll
+      for (int j = 0; j < MJ; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, xf[q & 1][j].v, acc[i][j], 0, 0, 0);
     }
   };
-  const int mje = max(0, (cdiv(brows, 32) - wm + 1) / 2);
-  if constexpr (MJ == 4) {
-    if (mje == 0) pipeline(std::integral_constant<int, 0>{});
-    else if (mje == 1) pipeline(std::integral_constant<int, 1>{});
-    else if (mje == 2) pipeline(std::integral_constant<int, 2>{});
-    else if (mje == 3) pipeline(std::integral_constant<int, 3>{});
-    else pipeline(std::integral_constant<int, 4>{});
-  } else {
-    if (mje == 0) pipeline(std::integral_constant<int, 0>{});
-    else if (mje == 1) pipeline(std::integral_constant<int, 1>{});
-    else pipeline(std::integral_constant<int, 2>{});
+  // Per stage: all but the last MFMA step run while the next step's operands are
+  // read; then the next stage's copies have landed -> barrier: everybody holds
+  // this stage's last operands, so that its slot takes the copies of stage s +
+  // RING -> the last step, while the next stage's first operands are read.
+  if (KF > 0) {
+#pragma unroll
+    for (int r = 0; r < RING; ++r) copy_stage(r, r);
+    wait_copies_upto<(RING - 1) * (WI + XI)>();
+    stage_barrier();
+    read_q(0, 0);
+    int slot = 0;
+    for (int s = 0; s < KF; ++s) {
+      const int next = slot == RING - 1 ? 0 : slot + 1;
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        read_q(slot, q + 1);
+        mma(q);
+      }
+      wait_copies_upto<(RING - 2) * (WI + XI)>();
+      stage_barrier();
+      copy_stage(s + RING, slot);
+      asm volatile("" ::: "memory");
+      read_q(next, 0);
+      mma(3);
+      slot = next;
+    }
+    wait_copies_upto<0>();
+    __syncthreads();
   }
-  __syncthreads();  // every wavefront is done with the stage buffers
-
+  // the last, partial stage: zeros behind the rows' ends (K is a multiple of 16
+  // for codes, 8 else; that of dx and dw of 64)
+  if ((EPI == VE_LSE || EPI == VE_PROB) && p.K % 64) {
+    const uint8_t *as = abase + (int64_t)KF * AB, *bs = bbase + (int64_t)KF * 128;
+    const bool ain = KF * 64 + achunk * (AT ? 16 : 8) < p.K, bin = KF * 64 + xchunk * 8 < p.K;
+    const uint8_t* z = reinterpret_cast<const uint8_t*>(kVocabZero);
+#pragma unroll
+    for (int j = 0; j < WI; ++j) lds_copy16(ain ? as + aoff[j] : z, cw + j * 8192);
+#pragma unroll
+    for (int j = 0; j < XI; ++j) lds_copy16(bin ? bs + boff[j] : z, cw + WB + j * 8192);
+    wait_copies_upto<0>();
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      read_q(0, q);
+      mma(q);
+    }
+    __syncthreads();
+  }
   vocab_epilogue<EPI, BM, 4, NI, MJ>(p, acc, smem, nt, m0, arows, brows, wn, wm);
+}
+
+// The slices of a K split and the pieces before -> the running sums, or, after
+// the last piece, dx
+__global__ __launch_bounds__(256) void vocab_slices_kernel(const VocabGemm p, int slices) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, n = (int64_t)p.nb * p.ldsum;
+  if (i >= n) return;
+  const int64_t row = i / p.ldsum;
+  const int c = (int)(i - row * p.ldsum);
+  float4 v = p.first ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *reinterpret_cast<const float4*>(p.sum + i);
+  for (int z = 0; z < slices; ++z) {
+    const float4 a = *reinterpret_cast<const float4*>(p.slices + z * n + i);
+    v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
+  }
+  if (!p.last) *reinterpret_cast<float4*>(p.sum + i) = v;
+  else *reinterpret_cast<uint2*>(p.y + row * p.ldy + c) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
 
 // The same product in tiles of 256 x 256 by four wavefronts of 4 x 4 blocks (one
@@ -477,11 +541,13 @@ __global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGem
 constexpr int kBThreads = 256;
 
 template <int EPI, bool TAIL>
-__global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm p) {
+__global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm args) {
   constexpr int BN = kVN, BM = 256, NI = 4, MJ = 4;
   constexpr uint32_t SLOT = BN * 128, RING = 5 * SLOT;
   __shared__ __align__(1024) uint8_t smem[RING];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
+  VocabGemm p = args;
+  take_slice<EPI>(p);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave & 1, wm = wave >> 1, rl = lane & 31, kh = lane >> 5;
   int mt, nt;
@@ -697,19 +763,39 @@ __global__ __launch_bounds__(256) void vocab_transpose_kernel(const uint8_t* src
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// B-row tile height
-int vocab_bm(int nb) { return nb > 128 ? 256 : 128; }
+// Tile of a problem of na A rows and nb B rows, by the rounds over the 256 CUs
+// that it takes: 256 x 256 (big), or 256 x 128 / 64.
+int vocab_bm(int64_t na, int64_t nb) {
+  const int64_t n = cdiv(na, (int64_t)kVN);
+  if (nb <= 64) return 64;
+  if (nb <= 128) return 128;
+  auto rounds = [&](int64_t bm) { return cdiv(n * cdiv(nb, bm), (int64_t)256); };
+  return rounds(256) * 150 <= rounds(128) * 100 ? 256 : 128;
+}
 
+template <int EPI, int BM, int AT>
+void launch_small(const VocabGemm& g, dim3 grid, hipStream_t st) {
+  hipLaunchKernelGGL((vocab_gemm_kernel<EPI, BM, AT>), grid, dim3(kVThreads), 0, st, g);
+}
+
+// at: type of the A rows, 0 bf16 or the codes' table type (logits and probs)
 template <int EPI>
-void launch_gemm(VocabGemm g, hipStream_t st) {
-  const int bm = vocab_bm(g.nb);
+void launch_gemm(VocabGemm g, int at, int bm, int slices, hipStream_t st) {
+  constexpr bool kLogits = EPI == VE_LSE || EPI == VE_PROB;
   g.n_tiles = cdiv(g.na, kVN);
   g.m_tiles = cdiv(g.nb, bm);
-  const unsigned grid = (unsigned)(cdiv(g.n_tiles * g.m_tiles, kXcds) * kXcds);
-  constexpr bool kTails = EPI == VE_LSE || EPI == VE_PROB;  // (the K of dx and dw is a multiple of 64)
-  if (bm == 256 && kTails && g.K % 64) hipLaunchKernelGGL((vocab_big_kernel<EPI, kTails>), dim3(grid), dim3(kBThreads), 0, st, g);
-  else if (bm == 256) hipLaunchKernelGGL((vocab_big_kernel<EPI, false>), dim3(grid), dim3(kBThreads), 0, st, g);
-  else hipLaunchKernelGGL((vocab_gemm_kernel<EPI, 128>), dim3(grid), dim3(kVThreads), 0, st, g);
+  const dim3 grid((unsigned)(cdiv(g.n_tiles * g.m_tiles, kXcds) * kXcds), (unsigned)slices);
+  if (bm == 256) {
+    // (the K of dx and dw is a multiple of 64)
+    if (kLogits && g.K % 64) hipLaunchKernelGGL((vocab_big_kernel<EPI, kLogits>), grid, dim3(kBThreads), 0, st, g);
+    else hipLaunchKernelGGL((vocab_big_kernel<EPI, false>), grid, dim3(kBThreads), 0, st, g);
+  } else if (at == 0) {
+    bm == 128 ? launch_small<EPI, 128, 0>(g, grid, st) : launch_small<EPI, 64, 0>(g, grid, st);
+  } else if constexpr (kLogits) {
+    if (at == 3) bm == 128 ? launch_small<EPI, 128, 3>(g, grid, st) : launch_small<EPI, 64, 3>(g, grid, st);
+    else if (at == 4) bm == 128 ? launch_small<EPI, 128, 4>(g, grid, st) : launch_small<EPI, 64, 4>(g, grid, st);
+    else bm == 128 ? launch_small<EPI, 128, 5>(g, grid, st) : launch_small<EPI, 64, 5>(g, grid, st);
+  }
 }
 
 void launch_expand(int wt, const uint8_t* w, int64_t ldw, int64_t rows, int64_t H, uint16_t* out, hipStream_t st) {
@@ -750,6 +836,8 @@ void launch_transpose(int wt, const uint8_t* src, int64_t ld, int64_t R, int64_t
 // sizes whose tile counts, and the threads of their grids, fit 32 bits
 constexpr int64_t kMaxTokens = (int64_t)1 << 20, kMaxVocab = (int64_t)1 << 24, kMaxHidden = (int64_t)1 << 16;
 
+constexpr int64_t kDirectTokens = 512;
+
 bool loss_sizes_ok(int64_t T, int64_t V, int64_t H) {
   return T >= 0 && T <= kMaxTokens && V > 0 && V <= kMaxVocab && H > 0 && H <= kMaxHidden && H % 8 == 0 &&
          cdiv(V, (int64_t)kVN) * cdiv(T, (int64_t)128) <= ((int64_t)1 << 22);
@@ -766,11 +854,18 @@ int loss_args_ok(const LossArgs& a) {
   return 1;
 }
 
+// Whether codes go to the tiles as they are stored: whole 16-byte chunks, and
+// not so many tokens that expanding a piece first, for the 256 x 256 tiles, is
+// the shorter way
+bool codes_direct(const void* w, int64_t ldw, int64_t H, int64_t T) {
+  return T <= kDirectTokens && H % 16 == 0 && ldw % 16 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+}
+
 // Table rows of a piece of the forward pass: all of a bf16 table (read where
-// it lies), about 128 MB of expanded rows of a 1-byte one
-int64_t loss_piece(int64_t V, int64_t H, int wtype) {
-  if (wtype == 0) return V;
-  return std::min(up(V, kVN), std::max<int64_t>(up((int64_t)(64 << 20) / H, kVN), kVN));
+// it lies), 16 or 128 MB of expanded rows of a 1-byte one
+int64_t loss_piece(int64_t T, int64_t V, int64_t H) {
+  const int64_t values = T <= 128 ? 8 << 20 : 64 << 20;
+  return std::min(up(V, kVN), std::max<int64_t>(up(values / H, kVN), kVN));
 }
 
 int64_t loss_layout(int64_t T, int64_t V, int64_t H, int wtype, int64_t (&off)[3]) {
@@ -780,7 +875,7 @@ int64_t loss_layout(int64_t T, int64_t V, int64_t H, int wtype, int64_t (&off)[3
   off[1] = at;  // the targets' logits
   at += up(T * 4, 256);
   off[2] = at;  // expanded rows
-  if (wtype) at += up(loss_piece(V, H, wtype) * H * 2, 256);
+  if (wtype) at += up(loss_piece(T, V, H) * H * 2, 256);
   return at;
 }
 
@@ -794,8 +889,25 @@ int64_t grad_piece(int64_t T, int64_t V, int64_t H) {
 // 128-byte lines, so that the rows of a tile do not share memory channels
 int64_t odd_pitch(int64_t n) { return n % 128 ? n : n + 64; }
 
-// P, P^T, table piece transposed, x transposed, float32 sums, expanded rows
-int64_t grad_layout(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw, int64_t (&off)[6]) {
+// dx of a piece: T x H outputs, a K axis as long as the piece. Tile height by
+// the padded rows' cost, and as many K slices as fill the CUs, of at least 512
+// (333 tokens, H 2880, pieces of 23296 rows: 24 tiles of 256 x 256 without a
+// split 458 us).
+struct DxPlan {
+  int bm, slices, kslice;
+};
+DxPlan dx_plan(int64_t T, int64_t H, int64_t K) {
+  DxPlan d{};
+  d.bm = T <= 64 ? 64 : (T <= 128 || cdiv(T, (int64_t)256) * 150 > cdiv(T, (int64_t)128) * 100 ? 128 : 256);
+  const int64_t tiles = cdiv(H, (int64_t)kVN) * cdiv(T, (int64_t)d.bm);
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(256 / tiles, K / 512));
+  d.kslice = (int)up(cdiv(K, want), 64);
+  d.slices = (int)cdiv(K, (int64_t)d.kslice);
+  return d;
+}
+
+// P, P^T, table piece transposed, x transposed, float32 sums, K slices, expanded rows
+int64_t grad_layout(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw, int64_t (&off)[7]) {
   const int64_t Vc = grad_piece(T, V, H), Vp = odd_pitch(Vc), Tp = odd_pitch(up(T, 64));
   const bool pieces = Vc < V;
   int64_t at = 0;
@@ -808,8 +920,13 @@ int64_t grad_layout(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int
   off[3] = at;
   if (need_dw) at += up(H * Tp * 2, 256);
   off[4] = at;
-  if (need_dx && pieces) at += up(T * up(H, 4) * 4, 256);
+  if (need_dx && pieces) at += up(T * H * 4, 256);
   off[5] = at;
+  if (need_dx) {
+    const DxPlan d = dx_plan(T, H, up(std::min(Vc, V), 64));
+    if (d.slices > 1) at += up(d.slices * T * H * 4, 256);
+  }
+  off[6] = at;
   if (wtype) at += up(Vc * H * 2, 256);
   return at;
 }
@@ -846,13 +963,14 @@ extern "C" int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void
   g.ignore = ignore_index;
   g.part = reinterpret_cast<float2*>(ws + off[0]);
   g.tgt = reinterpret_cast<float*>(ws + off[1]);
-  const int64_t Vc = loss_piece(V, H, wtype);
+  const bool direct = wtype && codes_direct(w, ldw, H, T);
+  const int64_t Vc = wtype && !direct ? loss_piece(T, V, H) : V;
   for (int64_t v0 = 0; v0 < V; v0 += Vc) {
     const uint8_t* rows = static_cast<const uint8_t*>(w) + v0 * ldw * (wtype ? 1 : 2);
     const int64_t n = std::min(Vc, V - v0);
     g.a = rows;
-    g.lda = ldw * 2;
-    if (wtype) {
+    g.lda = ldw * (wtype ? 1 : 2);
+    if (wtype && !direct) {
       uint16_t* e = reinterpret_cast<uint16_t*>(ws + off[2]);
       launch_expand(wtype, rows, ldw, n, H, e, stream);
       g.a = reinterpret_cast<const uint8_t*>(e);
@@ -862,7 +980,7 @@ extern "C" int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void
     g.v0 = v0;
     g.row_scale = row_scale ? row_scale + v0 : nullptr;
     g.part_tile = (int)(v0 / kVN);
-    launch_gemm<VE_LSE>(g, stream);
+    launch_gemm<VE_LSE>(g, direct ? wtype : 0, direct ? std::min(vocab_bm(n, T), 128) : vocab_bm(n, T), 1, stream);
   }
   hipLaunchKernelGGL(vocab_loss_join_kernel, dim3((unsigned)cdiv(T, (int64_t)4)), dim3(256), 0, stream, g.part,
                      (int)cdiv(V, (int64_t)kVN), (int)T, g.tgt, targets, targets_i64, ignore_index, V, loss, lse);
@@ -872,7 +990,7 @@ extern "C" int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void
 extern "C" int qmoe_vocab_loss_grad_workspace_size(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw,
                                                    int64_t* bytes) {
   if (!loss_sizes_ok(T, V, H) || (wtype != 0 && (wtype < 3 || wtype > 5)) || !bytes) return QMOE_ERR_ARG;
-  int64_t off[6];
+  int64_t off[7];
   *bytes = grad_layout(T, V, H, wtype, need_dx, need_dw, off);
   return QMOE_OK;
 }
@@ -887,7 +1005,7 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
   if (dw && wtype) return QMOE_ERR_ARG;  // codes have no gradient
   if (dx && (lddx < H || lddx % 8 || (reinterpret_cast<uintptr_t>(dx) & 15))) return QMOE_ERR_ARG;
   if (dw && (lddw < H || lddw % 8 || (reinterpret_cast<uintptr_t>(dw) & 15))) return QMOE_ERR_ARG;
-  int64_t off[6];
+  int64_t off[7];
   if (!workspace || ws_bytes < grad_layout(T, V, H, wtype, dx != nullptr, dw != nullptr, off)) return QMOE_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int64_t Vc = grad_piece(T, V, H), Vp = odd_pitch(Vc), Tw = up(T, 64), Tp = odd_pitch(Tw);
@@ -895,15 +1013,16 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
   uint16_t* PT = reinterpret_cast<uint16_t*>(ws + off[1]);
   uint16_t* WT = reinterpret_cast<uint16_t*>(ws + off[2]);
   uint16_t* XT = reinterpret_cast<uint16_t*>(ws + off[3]);
+  const bool direct = wtype && codes_direct(w, ldw, H, T);
   if (dw) launch_transpose(0, static_cast<const uint8_t*>(x), ldx * 2, T, H, XT, Tp, Tw, &a, g_loss, g_lse, stream);
   for (int64_t v0 = 0; v0 < V; v0 += Vc) {
     const uint8_t* rows = static_cast<const uint8_t*>(w) + v0 * ldw * (wtype ? 1 : 2);
     const int64_t n = std::min(Vc, V - v0), np = up(n, 64);
     VocabGemm g{};
     g.a = rows;
-    g.lda = ldw * 2;
-    if (wtype) {
-      uint16_t* e = reinterpret_cast<uint16_t*>(ws + off[5]);
+    g.lda = ldw * (wtype ? 1 : 2);
+    if (wtype && !direct) {
+      uint16_t* e = reinterpret_cast<uint16_t*>(ws + off[6]);
       launch_expand(wtype, rows, ldw, n, H, e, stream);
       g.a = reinterpret_cast<const uint8_t*>(e);
       g.lda = H * 2;
@@ -926,7 +1045,7 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
     g.ldp = Vp;
     g.pt = dw ? PT : nullptr;
     g.ldpt = Tp;
-    launch_gemm<VE_PROB>(g, stream);
+    launch_gemm<VE_PROB>(g, direct ? wtype : 0, direct ? std::min(vocab_bm(n, T), 128) : vocab_bm(n, T), 1, stream);
     if (dx) {
       launch_transpose(wtype, rows, ldw * (wtype ? 1 : 2), n, H, WT, Vp, np, nullptr, nullptr, nullptr, stream);
       VocabGemm d{};
@@ -938,12 +1057,20 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
       d.nb = (int)T;
       d.K = (int)np;
       d.sum = reinterpret_cast<float*>(ws + off[4]);
-      d.ldsum = up(H, 4);
+      d.ldsum = H;
       d.first = v0 == 0;
       d.last = v0 + Vc >= V;
       d.y = static_cast<uint16_t*>(dx);
       d.ldy = lddx;
-      launch_gemm<VE_SUM>(d, stream);
+      const DxPlan plan = dx_plan(T, H, up(std::min(Vc, V), 64));
+      const int slices = (int)cdiv(np, (int64_t)plan.kslice);
+      if (slices > 1) {
+        d.kslice = plan.kslice;
+        d.slices = reinterpret_cast<float*>(ws + off[5]);
+      }
+      launch_gemm<VE_SUM>(d, 0, plan.bm, slices, stream);
+      if (slices > 1)
+        hipLaunchKernelGGL(vocab_slices_kernel, dim3((unsigned)cdiv(T * H / 4, (int64_t)256)), dim3(256), 0, stream, d, slices);
     }
     if (dw) {
       VocabGemm d{};
@@ -956,7 +1083,7 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
       d.K = (int)Tw;
       d.y = static_cast<uint16_t*>(dw) + v0 * lddw;
       d.ldy = lddw;
-      launch_gemm<VE_STORE>(d, stream);
+      launch_gemm<VE_STORE>(d, 0, vocab_bm(H, n), 1, stream);
     }
   }
   return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
