@@ -10,18 +10,23 @@
 //
 //  * Launch 1: every workgroup routes the tokens itself (a few microseconds
 //    that replace a launch and its result's way through memory), then takes its
-//    share of the (active expert, 16 gate rows + their 16 up rows) items.
-//    Launch 2: a workgroup owns 16 output columns and walks the active
-//    experts, so that the weighted sum stays in registers.
-//  * Weights are read in granules of 16 rows x 64 bytes, a wavefront's load
-//    instruction each (4 adjacent lanes per row segment), and turned into MFMA
-//    operand order through 1 KB of LDS per granule; the K axis is dealt to
-//    the wavefronts in pairs of granules (one 128-byte line per row), several
-//    steps in flight per wavefront. Tokens are the other MFMA operand's 16
-//    columns; a column without a token loads nothing, and what it holds stays
-//    in its column.
+//    share of the (slot, 16 gate rows + their 16 up rows) items; a slot is up to
+//    kRows tokens of one expert (experts with more have several slots, which
+//    read the weights again, from L2). Launch 2: a workgroup owns 16 output
+//    columns and walks the slots, so that the weighted sum stays in registers.
+//  * Weights are read as whole 128-byte lines of 16 rows, two load instructions
+//    of 8 rows each, and turned into MFMA operand order through 2 KB of LDS per
+//    wavefront. (64 bytes of 16 rows per instruction, the other half of each
+//    line by the next one: the L1 stalled on pending lines 37 % of the time.)
+//    The K axis is dealt to the wavefronts line by line, several in flight.
+//  * A 16-byte chunk of 4-bit codes feeds four MFMAs, each with 8 tokens'
+//    values per lane. The 16 columns of the other operand hold all four for
+//    kRows = 4 tokens (column 4 r + i: token r's values for MFMA i) in one
+//    load, instead of one load per MFMA; each MFMA has its own sums, of which
+//    only its own columns count, and the four columns are added at the end.
+//    (8-bit codes: two MFMAs, 8 tokens; bf16: one, 16.)
 //  * Sums are float32: per wavefront, then over the wavefronts in order; in
-//    launch 2 over the experts in ascending order per wavefront.
+//    launch 2 over the slots in ascending order per wavefront.
 
 #include <algorithm>
 
@@ -35,6 +40,14 @@ namespace {
 enum { FF_MX = 0, FF_NV = 1, FF_I4 = 2, FF_F8 = 3, FF_BF = 4 };
 
 constexpr int kFewTokens = 16, kFewRoutes = 128, kFewExperts = 512;
+
+// What follows from the tokens' routes (route: t * topk + j)
+struct FewTables {
+  int32_t num;                             // slots
+  float w[kFewRoutes];                     // route -> weight
+  int16_t active[kFewRoutes];              // slot -> expert, ascending
+  int16_t route[kFewRoutes * kFewTokens];  // (slot, row < kRows) -> route or -1, rows of a slot together
+};
 
 struct FewParams {
   const uint16_t* x;  // bf16 [T][ldx]
@@ -51,8 +64,7 @@ struct FewParams {
   float act_p0, act_p1;
   int group_shift;  // FF_I4: log2 of the k per scale
   uint16_t* h;      // bf16 [T topk][I]
-  int32_t* ids;     // [T topk] routes of launch 1
-  float* wts;
+  FewTables* tables;  // from launch 1 to launch 2
   uint16_t* out;    // bf16 [T][ldo]
   int64_t ldo;
 };
@@ -61,7 +73,8 @@ struct FewParams {
 template <int F>
 struct Fmt {
   static constexpr int kCodes = F == FF_F8 ? 16 : (F == FF_BF ? 8 : 32);
-  static constexpr int kMfma = kCodes / 8;  // 16x16x32 MFMAs per granule
+  static constexpr int kMfma = kCodes / 8;  // 16x16x32 MFMAs per chunk
+  static constexpr int kRows = 16 / kMfma;  // tokens of a slot
   QMOE_HD static int row_bytes(int K) { return F == FF_BF ? 2 * K : (F == FF_F8 ? K : K / 2); }
   // bytes of a row's scales
   QMOE_HD static int scale_bytes(int K, int group_shift) {
@@ -73,13 +86,14 @@ using qmoe_stream::kOob;
 using qmoe_stream::make_rsrc;
 using qmoe_stream::rsrc_t;
 
-// One step of a wavefront: NT granules (16 rows x 64 bytes each), their
-// scales and the tokens' values at the same k
+// One step of a wavefront: a 128-byte line of 16 rows for each of NT tiles
+// (lane -> row 8 v + l / 8, chunk l % 8), their scales (lane -> row l % 16, chunks 2
+// kg and 2 kg + 1, kg = l / 16) and the tokens' values for those two chunks
 template <int F, int NT>
 struct Step {
-  uint4 w[NT];
-  uint32_t s[NT];
-  uint4 x[Fmt<F>::kMfma];
+  uint4 w[NT][2];
+  uint2 s[NT];
+  uint4 x[2];
 };
 
 __device__ __forceinline__ uint4 load16(rsrc_t r, uint32_t off) {
@@ -87,14 +101,24 @@ __device__ __forceinline__ uint4 load16(rsrc_t r, uint32_t off) {
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// The scale word of the lane's chunk (row r = lane & 15, chunk c of its row)
+// The scales of the lane's chunks c and c + 1 (c even) of the row at row_off:
+// FF_MX two bytes, FF_NV two pairs of bf16, FF_I4 a bf16 each, FF_F8 one float32
 template <int F>
-__device__ __forceinline__ uint32_t load_scale(rsrc_t r, uint32_t row_off, int c, int group_shift, bool in) {
-  if constexpr (F == FF_MX) return __builtin_amdgcn_raw_buffer_load_b8(r, in ? row_off + c : kOob, 0, 0);
-  else if constexpr (F == FF_NV) return __builtin_amdgcn_raw_buffer_load_b32(r, in ? row_off + c * 4 : kOob, 0, 0);
-  else if constexpr (F == FF_I4) return __builtin_amdgcn_raw_buffer_load_b16(r, in ? row_off + ((c * 32) >> group_shift) * 2 : kOob, 0, 0);
-  else if constexpr (F == FF_F8) return __builtin_amdgcn_raw_buffer_load_b32(r, in ? row_off + (c >> 3) * 4 : kOob, 0, 0);
-  else return 0;
+__device__ __forceinline__ uint2 load_scales(rsrc_t r, uint32_t row_off, int c, int group_shift, bool in) {
+  uint2 s = make_uint2(0, 0);
+  if constexpr (F == FF_MX) {
+    s.x = __builtin_amdgcn_raw_buffer_load_b8(r, in ? row_off + c : kOob, 0, 0);
+    s.y = __builtin_amdgcn_raw_buffer_load_b8(r, in ? row_off + c + 1 : kOob, 0, 0);
+  } else if constexpr (F == FF_NV) {
+    s.x = __builtin_amdgcn_raw_buffer_load_b32(r, in ? row_off + c * 4 : kOob, 0, 0);
+    s.y = __builtin_amdgcn_raw_buffer_load_b32(r, in ? row_off + c * 4 + 4 : kOob, 0, 0);
+  } else if constexpr (F == FF_I4) {
+    s.x = __builtin_amdgcn_raw_buffer_load_b16(r, in ? row_off + ((c * 32) >> group_shift) * 2 : kOob, 0, 0);
+    s.y = __builtin_amdgcn_raw_buffer_load_b16(r, in ? row_off + (((c + 1) * 32) >> group_shift) * 2 : kOob, 0, 0);
+  } else if constexpr (F == FF_F8) {
+    s.x = s.y = __builtin_amdgcn_raw_buffer_load_b32(r, in ? row_off + (c >> 3) * 4 : kOob, 0, 0);
+  }
+  return s;
 }
 
 union Bf8 {
@@ -141,110 +165,155 @@ __device__ __forceinline__ uint4 expand8(const uint4& c, int i, uint32_t s) {
   else return c;
 }
 
-// acc[t] += granule t . tokens. `tr`: this wavefront's LDS, NT KB. Row r's
-// 16-byte chunk c lies at slot c ^ (r / 4), so that neither the writes (4
-// chunks of a row by 4 adjacent lanes) nor the reads (one chunk of 16 rows)
-// meet in a bank.
+// acc[t][i] += line t . tokens, MFMA i of each chunk. `tr`: this wavefront's LDS,
+// 2 KB per tile. Row r's chunk c lies at slot c ^ (r / 2), so that neither the
+// writes (the 8 chunks of a row by 8 adjacent lanes) nor the reads (one chunk of
+// 16 rows) meet in a bank.
 template <int F, int NT>
-__device__ __forceinline__ void consume(const Step<F, NT>& st, uint4* tr, f32x4 (&acc)[NT]) {
-  const int lane = threadIdx.x & 63, wr = lane >> 2, r = lane & 15, kg = lane >> 4;
+__device__ __forceinline__ void consume(const Step<F, NT>& st, uint4* tr, f32x4 (&acc)[NT][Fmt<F>::kMfma]) {
+  const int lane = threadIdx.x & 63, r = lane & 15, kg = lane >> 4;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) tr[t * 64 + wr * 4 + ((lane & 3) ^ (wr >> 2))] = st.w[t];
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const int row = 8 * v + (lane >> 3);
+      tr[t * 128 + row * 8 + ((lane & 7) ^ (row >> 1))] = st.w[t][v];
+    }
   qmoe_moe::wave_lds_sync();
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const uint4 c = tr[t * 64 + r * 4 + (kg ^ (r >> 2))];
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int i = 0; i < Fmt<F>::kMfma; ++i) {
-      Bf8 a, b;
-      a.u = expand8<F>(c, i, st.s[t]);
-      b.u = st.x[i];
-      acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, acc[t], 0, 0, 0);
+    for (int u = 0; u < 2; ++u) {
+      const uint4 c = tr[t * 128 + r * 8 + ((2 * kg + u) ^ (r >> 1))];
+      Bf8 b;
+      b.u = st.x[u];
+#pragma unroll
+      for (int i = 0; i < Fmt<F>::kMfma; ++i) {
+        Bf8 a;
+        a.u = expand8<F>(c, i, u ? st.s[t].y : st.s[t].x);
+        acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, acc[t][i], 0, 0, 0);
+      }
     }
-  }
   qmoe_moe::wave_lds_sync();  // the slots are free for the next step
 }
 
-// The routes of the tokens and what follows from them, in LDS
-struct FewRoutes {
-  int32_t ids[kFewRoutes];
-  float w[kFewRoutes];
-  uint32_t mask[kFewExperts / 32];  // experts with a route
-  int16_t active[kFewRoutes];       // experts with a route, ascending
-  int16_t route[kFewRoutes][kFewTokens];  // (active slot, token) -> route or -1
-  int num;                          // active experts
-};
+// The sums of the lane's token, from the kMfma columns it is spread over
+template <int M>
+__device__ __forceinline__ f32x4 own_sums(const f32x4 (&acc)[M]) {
+  const int i = threadIdx.x & (M - 1);
+  f32x4 v = acc[0];
+#pragma unroll
+  for (int k = 1; k < M; ++k)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = i == k ? acc[k][q] : v[q];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (M >= 2) v[q] += qmoe_route::dpp_f<0xB1>(v[q]);
+    if constexpr (M >= 4) v[q] += qmoe_route::dpp_f<0x4E>(v[q]);
+  }
+  return v;
+}
 
-// From ids / w (visible to the workgroup) to the rest; every thread calls
-__device__ __forceinline__ void few_active(FewRoutes& s, const FewParams& p) {
+// From the routes (ids and tb.w, visible to the workgroup) to the tables; every
+// thread calls. Slots in ascending order of (expert, token).
+template <int ROWS>
+__device__ __forceinline__ void few_tables(FewTables& tb, const int32_t* ids, uint32_t* tokens, int32_t* first,
+                                           const FewParams& p) {
   const int tid = threadIdx.x, R = p.T * p.topk;
   auto valid = [&](int r) {
-    const int id = s.ids[r];
-    return id >= 0 && id < p.E && !(p.skip && (f32_to_bf16(s.w[r]) & 0x7fffu) == 0);
+    return ids[r] >= 0 && ids[r] < p.E && !(p.skip && (f32_to_bf16(tb.w[r]) & 0x7fffu) == 0);
   };
-  if (tid < kFewExperts / 32) s.mask[tid] = 0;
-  for (int i = tid; i < kFewRoutes * kFewTokens; i += blockDim.x) (&s.route[0][0])[i] = -1;
+  if (p.T == 1 && !p.skip) {  // a token's experts are distinct: a slot each
+    if (tid < R) {
+      tb.active[tid] = (int16_t)ids[tid];
+      tb.route[tid * ROWS] = (int16_t)tid;
+#pragma unroll
+      for (int i = 1; i < ROWS; ++i) tb.route[tid * ROWS + i] = -1;
+    }
+    if (tid == 0) tb.num = R;
+    __syncthreads();
+    return;
+  }
+  for (int i = tid; i < kFewExperts; i += blockDim.x) tokens[i] = 0;
+  for (int i = tid; i < R * ROWS; i += blockDim.x) tb.route[i] = -1;
   __syncthreads();
-  if (tid < R && valid(tid)) atomicOr(&s.mask[s.ids[tid] >> 5], 1u << (s.ids[tid] & 31));
+  if (tid < R && valid(tid)) atomicOr(&tokens[ids[tid]], 1u << (tid / p.topk));
+  __syncthreads();
+  if (tid < 64) {  // slots before an expert's first: lane l owns experts 8 l .. 8 l + 7
+    int n[8], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      n[j] = (__popc(tokens[tid * 8 + j]) + ROWS - 1) / ROWS;
+      sum += n[j];
+    }
+    int total;
+    int at = qmoe_moe::wave_excl_scan(sum, tid, total);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      first[tid * 8 + j] = at;
+      at += n[j];
+    }
+    if (tid == 0) tb.num = total;
+  }
   __syncthreads();
   if (tid < R && valid(tid)) {
-    const int id = s.ids[tid];
-    int slot = __popc(s.mask[id >> 5] & ((1u << (id & 31)) - 1u));
-    for (int i = 0; i < (id >> 5); ++i) slot += __popc(s.mask[i]);
-    s.active[slot] = (int16_t)id;
-    s.route[slot][tid / p.topk] = (int16_t)tid;
-  }
-  if (tid == 0) {
-    int n = 0;
-    for (int i = 0; i < kFewExperts / 32; ++i) n += __popc(s.mask[i]);
-    s.num = n;
+    const int e = ids[tid], rank = __popc(tokens[e] & ((1u << (tid / p.topk)) - 1u)), slot = first[e] + rank / ROWS;
+    if (rank % ROWS == 0) tb.active[slot] = (int16_t)e;
+    tb.route[slot * ROWS + rank % ROWS] = (int16_t)tid;
   }
   __syncthreads();
 }
 
-// The wavefront's i-th granule of a row of `granules`: pairs dealt in turn
-template <int NW>
-__device__ __forceinline__ int granule_of(int wave, int i) { return (i >> 1) * 2 * NW + wave * 2 + (i & 1); }
-
-constexpr int kUpWaves = 4, kUpAhead = 4;
+constexpr int kUpWaves = 4, kUpAhead = 3;
 
 template <int F, int S>
 __global__ __launch_bounds__(kUpWaves * 64) void few_up_kernel(const FewParams p) {
-  __shared__ FewRoutes s;
-  __shared__ float choice[kUpWaves][qmoe_route::kChoiceLds];
-  __shared__ __align__(16) uint4 tr[kUpWaves][2 * 64];
-  __shared__ __align__(16) f32x4 red[kUpWaves][2][64];
+  constexpr int ROWS = Fmt<F>::kRows, M = Fmt<F>::kMfma;
+  __shared__ FewTables tb;
+  __shared__ int32_t ids[kFewRoutes];
+  __shared__ union {
+    float choice[kUpWaves][qmoe_route::kChoiceLds];
+    struct {
+      uint32_t tokens[kFewExperts];
+      int32_t first[kFewExperts];
+    } t;
+  } tmp;
+  __shared__ __align__(16) uint4 tr[kUpWaves][2 * 128];
+  __shared__ __align__(16) f32x4 red[2][kUpWaves][2][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int R = p.T * p.topk;
   for (int t = wave; t < p.T; t += kUpWaves)
     qmoe_route::route_token_any<S>(p.scoring, p.grouped, p.logits, p.logits_f32, t, p.E, p.topk, p.correction,
-                                   p.renormalize, p.rsf, p.num_group, p.topk_group, s.w, s.ids, choice[wave], nullptr,
+                                   p.renormalize, p.rsf, p.num_group, p.topk_group, tb.w, ids, tmp.choice[wave], nullptr,
                                    nullptr, 1);
   __syncthreads();
-  if (blockIdx.x == 0 && tid < R) {
-    p.ids[tid] = s.ids[tid];
-    p.wts[tid] = s.w[tid];
+  few_tables<ROWS>(tb, ids, tmp.t.tokens, tmp.t.first, p);
+  const int num = __builtin_amdgcn_readfirstlane(tb.num);
+  if (blockIdx.x == 0) {
+    if (tid == 0) p.tables->num = num;
+    if (tid < R) p.tables->w[tid] = tb.w[tid];
+    if (tid < num) p.tables->active[tid] = tb.active[tid];
+    for (int i = tid; i < num * ROWS; i += kUpWaves * 64) p.tables->route[i] = tb.route[i];
   }
-  few_active(s, p);
 
-  const int tiles = p.I / 16, items = __builtin_amdgcn_readfirstlane(s.num) * tiles;
+  const int tiles = p.I / 16, items = num * tiles;
   const int it0 = (int)((int64_t)blockIdx.x * items / gridDim.x), it1 = (int)((int64_t)(blockIdx.x + 1) * items / gridDim.x);
   if (it0 >= it1) return;
-  const int rb = Fmt<F>::row_bytes(p.H), sb = Fmt<F>::scale_bytes(p.H, p.group_shift), granules = (rb + 63) / 64;
+  const int rb = Fmt<F>::row_bytes(p.H), sb = Fmt<F>::scale_bytes(p.H, p.group_shift);
   // steps per item, the same for every wavefront (those past a row's end load
   // nothing and add zeros)
-  const int chunks = (cdiv(granules, 2 * kUpWaves) * 2 + kUpAhead - 1) / kUpAhead;
+  const int chunks = cdiv(cdiv(cdiv(rb, 128), kUpWaves), kUpAhead);
   const int r = lane & 15, kg = lane >> 4;
   const rsrc_t xr = make_rsrc(p.x, (int64_t)p.T * p.ldx * 2);
 
-  // where the loads are: item, chunk of it
+  // where the loads are
   rsrc_t wr[2], sr[2];
-  uint32_t xrow = kOob;  // byte offset of the lane's token row
+  uint32_t xrow = kOob;  // byte offset of the column's token, at its MFMA's values
   auto seek = [&](int item) {
     const int slot = item / tiles, tile = item - slot * tiles;
-    const int e = __builtin_amdgcn_readfirstlane(s.active[slot]);
-    const int route = s.route[slot][r];  // column r: token r, where it takes this expert
-    xrow = route >= 0 ? (uint32_t)(r * p.ldx * 2) : kOob;
+    const int e = __builtin_amdgcn_readfirstlane(tb.active[slot]);
+    const int route = tb.route[slot * ROWS + r / M];
+    xrow = route >= 0 ? (uint32_t)((route / p.topk) * p.ldx * 2) + (r % M) * 16 : kOob;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int64_t row = (int64_t)e * 2 * p.I + t * p.I + tile * 16;
@@ -253,24 +322,27 @@ __global__ __launch_bounds__(kUpWaves * 64) void few_up_kernel(const FewParams p
     }
   };
   Step<F, 2> st[kUpAhead];
+  const uint32_t wlane = (uint32_t)((lane >> 3) * rb + (lane & 7) * 16), slane = (uint32_t)(r * sb);
   auto issue = [&](Step<F, 2>& d, int i, bool live) {
-    const int g = granule_of<kUpWaves>(wave, i);
-    const int lc = g * 4 + (lane & 3), mc = g * 4 + kg;  // chunk of the row: as loaded, as multiplied
-    const bool lin = live && lc * 16 < rb, min_ = live && mc * 16 < rb;
+    const int line = (wave + kUpWaves * i) * 128;  // byte of the row
+    const bool lin = live && line + (lane & 7) * 16 < rb;
+    const int c = line / 16 + 2 * kg;  // the first chunk that the lane multiplies
+    const bool in = live && c * 16 < rb;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      d.w[t] = load16(wr[t], lin ? (uint32_t)((lane >> 2) * rb + lc * 16) : kOob);
-      d.s[t] = load_scale<F>(sr[t], (uint32_t)(r * sb), mc, p.group_shift, min_);
+#pragma unroll
+      for (int v = 0; v < 2; ++v) d.w[t][v] = load16(wr[t], lin ? wlane + (uint32_t)(8 * v * rb + line) : kOob);
+      d.s[t] = load_scales<F>(sr[t], slane, c, p.group_shift, in);
     }
 #pragma unroll
-    for (int k = 0; k < Fmt<F>::kMfma; ++k)
-      d.x[k] = load16(xr, min_ ? xrow + (uint32_t)((mc * Fmt<F>::kCodes + k * 8) * 2) : kOob);
+    for (int u = 0; u < 2; ++u)
+      d.x[u] = load16(xr, live && (c + u) * 16 < rb ? xrow + (uint32_t)((c + u) * Fmt<F>::kCodes * 2) : kOob);
   };
   seek(it0);
 #pragma unroll
   for (int u = 0; u < kUpAhead; ++u) issue(st[u], u, true);
   for (int item = it0; item < it1; ++item) {
-    f32x4 acc[2] = {};
+    f32x4 acc[2][M] = {};
     for (int c = 0; c < chunks; ++c) {
       const bool more = c + 1 < chunks, next = item + 1 < it1;
       if (!more && next) seek(item + 1);
@@ -281,22 +353,24 @@ __global__ __launch_bounds__(kUpWaves * 64) void few_up_kernel(const FewParams p
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    // sums of the wavefronts in order, bias, activation
-    red[wave][0][lane] = acc[0];
-    red[wave][1][lane] = acc[1];
+    // the wavefronts' sums in order, bias, activation (by one wavefront, while
+    // the others go on: the next item's sums lie elsewhere)
+    f32x4(&rd)[kUpWaves][2][64] = red[item & 1];
+    rd[wave][0][lane] = own_sums<M>(acc[0]);
+    rd[wave][1][lane] = own_sums<M>(acc[1]);
     stage_barrier();
-    if (wave == 0) {
+    if (wave == item % kUpWaves && r % M == 0) {
       const int slot = item / tiles, n0 = (item - slot * tiles) * 16 + kg * 4;
-      const int route = s.route[slot][r];
-      f32x4 g = red[0][0][lane], u = red[0][1][lane];
+      const int route = tb.route[slot * ROWS + r / M];
+      f32x4 g = rd[0][0][lane], u = rd[0][1][lane];
 #pragma unroll
       for (int w = 1; w < kUpWaves; ++w) {
-        g += red[w][0][lane];
-        u += red[w][1][lane];
+        g += rd[w][0][lane];
+        u += rd[w][1][lane];
       }
       if (route >= 0) {
         if (p.b1) {
-          const float* b = p.b1 + (int64_t)s.active[slot] * 2 * p.I + n0;
+          const float* b = p.b1 + (int64_t)tb.active[slot] * 2 * p.I + n0;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             g[q] += b[q];
@@ -310,101 +384,116 @@ __global__ __launch_bounds__(kUpWaves * 64) void few_up_kernel(const FewParams p
             make_uint2(o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16);
       }
     }
-    stage_barrier();  // the sums have been read
   }
 }
 
-constexpr int kDownWaves = 8, kDownAhead = 6;
+constexpr int kDownAhead = 4;
 
-template <int F>
-__global__ __launch_bounds__(kDownWaves * 64) void few_down_kernel(const FewParams p) {
-  __shared__ FewRoutes s;
-  __shared__ __align__(16) uint4 tr[kDownWaves][64];
-  __shared__ __align__(16) f32x4 red[kDownWaves][64];
+// NW wavefronts: 16 where there are no more output tiles than CUs, else 8 (two
+// workgroups per CU)
+template <int F, int NW>
+__global__ __launch_bounds__(NW * 64) void few_down_kernel(const FewParams p) {
+  constexpr int ROWS = Fmt<F>::kRows, M = Fmt<F>::kMfma;
+  __shared__ FewTables tb;
+  __shared__ __align__(16) uint4 tr[NW][128];
+  __shared__ __align__(16) f32x4 tot[NW][64];  // [token][4 columns x 4]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int R = p.T * p.topk;
-  if (tid < R) {
-    s.ids[tid] = p.ids[tid];
-    s.w[tid] = p.wts[tid];
-  }
-  few_active(s, p);
-  const int num = __builtin_amdgcn_readfirstlane(s.num), n0 = blockIdx.x * 16;
-  const int rb = Fmt<F>::row_bytes(p.I), sb = Fmt<F>::scale_bytes(p.I, p.group_shift), granules = (rb + 63) / 64;
+  const int num = __builtin_amdgcn_readfirstlane(p.tables->num);
+  if (tid < R) tb.w[tid] = p.tables->w[tid];
+  if (tid < num) tb.active[tid] = p.tables->active[tid];
+  for (int i = tid; i < num * ROWS; i += NW * 64) tb.route[i] = p.tables->route[i];
+  __syncthreads();
+  const int n0 = blockIdx.x * 16;
+  const int rb = Fmt<F>::row_bytes(p.I), sb = Fmt<F>::scale_bytes(p.I, p.group_shift), lines = cdiv(rb, 128);
   const int r = lane & 15, kg = lane >> 4;
   const rsrc_t hr = make_rsrc(p.h, (int64_t)R * p.I * 2);
 
-  // the wavefront's i-th step is granule granule_of(wave, i) of all experts' rows
-  // laid end to end
-  const int total = num * granules;
-  struct At {
-    int slot, g;
+  // the wavefront's i-th step is line wave + NW i of all slots' rows laid end to
+  // end; a cursor goes over them for the loads, another for the products
+  struct Cursor {
+    int slot, line;
   };
-  auto at = [&](int i) {
-    const int L = granule_of<kDownWaves>(wave, i), slot = L / granules;
-    return At{slot, L - slot * granules};
+  auto settle = [&](Cursor& c) {
+    while (c.line >= lines) {
+      c.line -= lines;
+      ++c.slot;
+    }
   };
   Step<F, 1> st[kDownAhead];
-  auto issue = [&](Step<F, 1>& d, int i) {
-    const At a = at(i);
-    const bool live = a.slot < num;
-    const int e = live ? __builtin_amdgcn_readfirstlane(s.active[a.slot]) : 0;
-    const int route = live ? s.route[a.slot][r] : -1;
+  const uint32_t wlane = (uint32_t)((lane >> 3) * rb + (lane & 7) * 16), slane = (uint32_t)(r * sb);
+  auto issue = [&](Step<F, 1>& d, Cursor& at) {
+    settle(at);
+    const bool live = at.slot < num;
+    const int e = live ? __builtin_amdgcn_readfirstlane(tb.active[at.slot]) : 0;
+    const int route = live ? tb.route[at.slot * ROWS + r / M] : -1;
     const int64_t row = (int64_t)e * p.H + n0;
     const rsrc_t wr = make_rsrc(p.w2 + row * rb, (int64_t)16 * rb);
     const rsrc_t sr = make_rsrc(static_cast<const uint8_t*>(p.s2) + row * sb, (int64_t)16 * sb);
-    const int lc = a.g * 4 + (lane & 3), mc = a.g * 4 + kg;
-    const bool lin = live && lc * 16 < rb, min_ = live && mc * 16 < rb;
-    d.w[0] = load16(wr, lin ? (uint32_t)((lane >> 2) * rb + lc * 16) : kOob);
-    d.s[0] = load_scale<F>(sr, (uint32_t)(r * sb), mc, p.group_shift, min_);
+    const int line = at.line * 128, c = line / 16 + 2 * kg;
+    const bool lin = live && line + (lane & 7) * 16 < rb;
 #pragma unroll
-    for (int k = 0; k < Fmt<F>::kMfma; ++k)
-      d.x[k] = load16(hr, min_ && route >= 0 ? (uint32_t)(((int64_t)route * p.I + mc * Fmt<F>::kCodes + k * 8) * 2) : kOob);
+    for (int v = 0; v < 2; ++v) d.w[0][v] = load16(wr, lin ? wlane + (uint32_t)(8 * v * rb + line) : kOob);
+    d.s[0] = load_scales<F>(sr, slane, c, p.group_shift, live && c * 16 < rb);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      d.x[u] = load16(hr, route >= 0 && (c + u) * 16 < rb
+                              ? (uint32_t)(((int64_t)route * p.I + (c + u) * Fmt<F>::kCodes + (r % M) * 8) * 2)
+                              : kOob);
+    at.line += NW;
   };
-  f32x4 sum = {}, acc[1] = {};
+  tot[wave][lane] = f32x4{};
+  f32x4 acc[1][M] = {};
+  // the slot's sums, weighted, into its tokens' (this wavefront's, in LDS)
   auto flush = [&](int slot) {
-    const int route = s.route[slot][r];
-    const float w = route >= 0 ? s.w[route] : 0.0f;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (route >= 0) sum[q] += w * acc[0][q];
-      acc[0][q] = 0.0f;
+    const f32x4 v = own_sums<M>(acc[0]);
+    const int route = tb.route[slot * ROWS + r / M];
+    if (route >= 0 && r % M == 0) {
+      const float w = tb.w[route];
+      f32x4& t = tot[wave][route / p.topk * 4 + kg];
+      t = t + w * v;
     }
-  };
 #pragma unroll
-  for (int u = 0; u < kDownAhead; ++u) issue(st[u], u);
+    for (int i = 0; i < M; ++i) acc[0][i] = f32x4{};
+  };
+  Cursor ahead{0, wave}, now{0, wave};
+#pragma unroll
+  for (int u = 0; u < kDownAhead; ++u) issue(st[u], ahead);
   int slot = -1;
-  for (int i0 = 0; granule_of<kDownWaves>(wave, i0) < total; i0 += kDownAhead) {
+  settle(now);
+  while (now.slot < num) {
 #pragma unroll
     for (int u = 0; u < kDownAhead; ++u) {
-      const At a = at(i0 + u);
-      if (a.slot < num) {
-        if (a.slot != slot && slot >= 0) flush(slot);
-        slot = a.slot;
+      if (now.slot < num) {
+        if (now.slot != slot && slot >= 0) flush(slot);
+        slot = now.slot;
         consume<F, 1>(st[u], tr[wave], acc);
       }
-      issue(st[u], i0 + u + kDownAhead);
+      issue(st[u], ahead);
+      now.line += NW;
+      settle(now);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
   if (slot >= 0) flush(slot);
   if (p.b2)
-    for (int k = wave; k < num; k += kDownWaves) {
-      const int route = s.route[k][r];
-      const float* b = p.b2 + (int64_t)s.active[k] * p.H + n0 + kg * 4;
-      if (route >= 0)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) sum[q] += s.w[route] * b[q];
+    for (int k = wave; k < num; k += NW) {
+      const int route = tb.route[k * ROWS + r / M];
+      if (route >= 0 && r % M == 0) {
+        const float* b = p.b2 + (int64_t)tb.active[k] * p.H + n0 + kg * 4;
+        f32x4& t = tot[wave][route / p.topk * 4 + kg];
+        t = t + tb.w[route] * f32x4{b[0], b[1], b[2], b[3]};
+      }
     }
-  red[wave][lane] = sum;
   __syncthreads();
-  if (wave == 0 && r < p.T) {
-    f32x4 v = red[0][lane];
+  if (tid < p.T * 4) {  // token tid / 4, columns 4 (tid % 4) .. + 3
+    f32x4 v = tot[0][tid];
 #pragma unroll
-    for (int w = 1; w < kDownWaves; ++w) v += red[w][lane];
+    for (int w = 1; w < NW; ++w) v += tot[w][tid];
     uint16_t o[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) o[q] = f32_to_bf16(v[q]);
-    *reinterpret_cast<uint2*>(p.out + (int64_t)r * p.ldo + n0 + kg * 4) =
+    *reinterpret_cast<uint2*>(p.out + (int64_t)(tid >> 2) * p.ldo + n0 + (tid & 3) * 4) =
         make_uint2(o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16);
   }
 }
@@ -412,7 +501,7 @@ __global__ __launch_bounds__(kDownWaves * 64) void few_down_kernel(const FewPara
 template <int F, int S>
 void launch_up(const FewParams& p, hipStream_t st) {
   const int64_t items = (int64_t)std::min(p.E, p.T * p.topk) * (p.I / 16);
-  hipLaunchKernelGGL((few_up_kernel<F, S>), dim3((unsigned)std::min<int64_t>(items, 768)), dim3(kUpWaves * 64), 0, st, p);
+  hipLaunchKernelGGL((few_up_kernel<F, S>), dim3((unsigned)std::min<int64_t>(items, 512)), dim3(kUpWaves * 64), 0, st, p);
 }
 
 template <int F>
@@ -421,14 +510,15 @@ void launch_few(const FewParams& p, hipStream_t st) {
   if (S <= 2) launch_up<F, 2>(p, st);
   else if (S == 4) launch_up<F, 4>(p, st);
   else launch_up<F, 8>(p, st);
-  hipLaunchKernelGGL((few_down_kernel<F>), dim3((unsigned)(p.H / 16)), dim3(kDownWaves * 64), 0, st, p);
+  const dim3 grid((unsigned)(p.H / 16));
+  if (p.H / 16 <= 256) hipLaunchKernelGGL((few_down_kernel<F, 16>), grid, dim3(16 * 64), 0, st, p);
+  else hipLaunchKernelGGL((few_down_kernel<F, 8>), grid, dim3(8 * 64), 0, st, p);
 }
 
-int64_t few_layout(int64_t R, int64_t I, int64_t (&off)[3]) {
+int64_t few_layout(int64_t R, int64_t I, int64_t (&off)[2]) {
   off[0] = 0;
   off[1] = (R * I * 2 + 255) / 256 * 256;
-  off[2] = off[1] + (R * 4 + 255) / 256 * 256;
-  return off[2] + (R * 4 + 255) / 256 * 256;
+  return off[1] + ((int64_t)sizeof(FewTables) + 255) / 256 * 256;
 }
 
 int few_ok(const qmoe_moe_few_desc* d) {
@@ -450,7 +540,7 @@ int few_ok(const qmoe_moe_few_desc* d) {
 // See include/qmoe.h for the contract.
 extern "C" int qmoe_moe_few_workspace_size(const qmoe_moe_few_desc* d, int64_t* bytes) {
   if (!few_ok(d) || !bytes) return QMOE_ERR_ARG;
-  int64_t off[3];
+  int64_t off[2];
   *bytes = few_layout((int64_t)d->T * d->topk, d->I, off);
   return QMOE_OK;
 }
@@ -463,7 +553,7 @@ extern "C" int qmoe_moe_few(const qmoe_moe_few_desc* d, void* workspace, int64_t
   if (!aligned(d->x, 16) || !aligned(d->w1, 16) || !aligned(d->w2, 16) || !aligned(d->out, 8) ||
       !aligned(d->w1_scale, 4) || !aligned(d->w2_scale, 4) || !aligned(d->w1_bias, 4) || !aligned(d->w2_bias, 4))
     return QMOE_ERR_ARG;
-  int64_t off[3];
+  int64_t off[2];
   const int64_t R = (int64_t)d->T * d->topk;
   if (!workspace || ws_bytes < few_layout(R, d->I, off)) return QMOE_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -487,8 +577,7 @@ extern "C" int qmoe_moe_few(const qmoe_moe_few_desc* d, void* workspace, int64_t
   p.act = d->act, p.act_p0 = d->act_p0, p.act_p1 = d->act_p1;
   p.group_shift = d->format == FF_I4 ? __builtin_ctz(d->group) : 0;
   p.h = reinterpret_cast<uint16_t*>(ws + off[0]);
-  p.ids = reinterpret_cast<int32_t*>(ws + off[1]);
-  p.wts = reinterpret_cast<float*>(ws + off[2]);
+  p.tables = reinterpret_cast<FewTables*>(ws + off[1]);
   p.out = static_cast<uint16_t*>(d->out);
   p.ldo = d->ldo;
   switch (d->format) {
