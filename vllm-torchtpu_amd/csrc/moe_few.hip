@@ -267,7 +267,7 @@ __device__ __forceinline__ void few_tables(FewTables& tb, const int32_t* ids, ui
 constexpr int kUpWaves = 4, kUpAhead = 3;
 
 template <int F, int S>
-__global__ __launch_bounds__(kUpWaves * 64) void few_up_kernel(const FewParams p) {
+__global__ __launch_bounds__(kUpWaves * 64, 3) void few_up_kernel(const FewParams p) {
   constexpr int ROWS = Fmt<F>::kRows, M = Fmt<F>::kMfma;
   __shared__ FewTables tb;
   __shared__ int32_t ids[kFewRoutes];
@@ -341,7 +341,23 @@ __global__ __launch_bounds__(kUpWaves * 64) void few_up_kernel(const FewParams p
   seek(it0);
 #pragma unroll
   for (int u = 0; u < kUpAhead; ++u) issue(st[u], u, true);
+  typedef const float __attribute__((address_space(4))) CFloat;
   for (int item = it0; item < it1; ++item) {
+    const int slot = item / tiles, tile = item - slot * tiles;
+    // the item's biases by scalar loads, in time for its end: a vector load's
+    // wait there would drain the next item's weight loads
+    float bg[16], bu[16];
+    if (p.b1) {
+      CFloat* b = (CFloat*)(uintptr_t)(p.b1 + (int64_t)__builtin_amdgcn_readfirstlane(tb.active[slot]) * 2 * p.I + tile * 16);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        bg[k] = b[k];
+        bu[k] = b[p.I + k];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) bg[k] = bu[k] = 0.0f;
+    }
     f32x4 acc[2][M] = {};
     for (int c = 0; c < chunks; ++c) {
       const bool more = c + 1 < chunks, next = item + 1 < it1;
@@ -360,8 +376,7 @@ __global__ __launch_bounds__(kUpWaves * 64) void few_up_kernel(const FewParams p
     rd[wave][1][lane] = own_sums<M>(acc[1]);
     stage_barrier();
     if (wave == item % kUpWaves && r % M == 0) {
-      const int slot = item / tiles, n0 = (item - slot * tiles) * 16 + kg * 4;
-      const int route = tb.route[slot * ROWS + r / M];
+      const int n0 = tile * 16 + kg * 4, route = tb.route[slot * ROWS + r / M];
       f32x4 g = rd[0][0][lane], u = rd[0][1][lane];
 #pragma unroll
       for (int w = 1; w < kUpWaves; ++w) {
@@ -369,13 +384,10 @@ __global__ __launch_bounds__(kUpWaves * 64) void few_up_kernel(const FewParams p
         u += rd[w][1][lane];
       }
       if (route >= 0) {
-        if (p.b1) {
-          const float* b = p.b1 + (int64_t)tb.active[slot] * 2 * p.I + n0;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            g[q] += b[q];
-            u[q] += b[p.I + q];
-          }
+        for (int q = 0; q < 4; ++q) {
+          g[q] += kg == 0 ? bg[q] : (kg == 1 ? bg[4 + q] : (kg == 2 ? bg[8 + q] : bg[12 + q]));
+          u[q] += kg == 0 ? bu[q] : (kg == 1 ? bu[4 + q] : (kg == 2 ? bu[8 + q] : bu[12 + q]));
         }
         uint16_t o[4];
 #pragma unroll
@@ -399,10 +411,13 @@ __global__ __launch_bounds__(NW * 64) void few_down_kernel(const FewParams p) {
   __shared__ __align__(16) f32x4 tot[NW][64];  // [token][4 columns x 4]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int R = p.T * p.topk;
+  // (every entry that a slot could have, so that no load waits for their number)
   const int num = __builtin_amdgcn_readfirstlane(p.tables->num);
-  if (tid < R) tb.w[tid] = p.tables->w[tid];
-  if (tid < num) tb.active[tid] = p.tables->active[tid];
-  for (int i = tid; i < num * ROWS; i += NW * 64) tb.route[i] = p.tables->route[i];
+  if (tid < R) {
+    tb.w[tid] = p.tables->w[tid];
+    tb.active[tid] = p.tables->active[tid];
+  }
+  for (int i = tid; i < R * ROWS; i += NW * 64) tb.route[i] = p.tables->route[i];
   __syncthreads();
   const int n0 = blockIdx.x * 16;
   const int rb = Fmt<F>::row_bytes(p.I), sb = Fmt<F>::scale_bytes(p.I, p.group_shift), lines = cdiv(rb, 128);
@@ -456,9 +471,25 @@ __global__ __launch_bounds__(NW * 64) void few_down_kernel(const FewParams p) {
 #pragma unroll
     for (int i = 0; i < M; ++i) acc[0][i] = f32x4{};
   };
+  // biases: the wavefront's first slot's is loaded ahead of the weights
+  auto bias_of = [&](int k) {
+    const float* b = p.b2 + (int64_t)tb.active[k] * p.H + n0 + kg * 4;
+    return f32x4{b[0], b[1], b[2], b[3]};
+  };
+  auto add_bias = [&](int k, f32x4 b) {
+    const int route = tb.route[k * ROWS + r / M];
+    if (route >= 0 && r % M == 0) {
+      f32x4& t = tot[wave][route / p.topk * 4 + kg];
+      t = t + tb.w[route] * b;
+    }
+  };
+  const bool biased = p.b2 && wave < num;
+  f32x4 first_bias = {};
+  if (biased) first_bias = bias_of(wave);
   Cursor ahead{0, wave}, now{0, wave};
 #pragma unroll
   for (int u = 0; u < kDownAhead; ++u) issue(st[u], ahead);
+  if (biased) add_bias(wave, first_bias);
   int slot = -1;
   settle(now);
   while (now.slot < num) {
@@ -477,14 +508,7 @@ __global__ __launch_bounds__(NW * 64) void few_down_kernel(const FewParams p) {
   }
   if (slot >= 0) flush(slot);
   if (p.b2)
-    for (int k = wave; k < num; k += NW) {
-      const int route = tb.route[k * ROWS + r / M];
-      if (route >= 0 && r % M == 0) {
-        const float* b = p.b2 + (int64_t)tb.active[k] * p.H + n0 + kg * 4;
-        f32x4& t = tot[wave][route / p.topk * 4 + kg];
-        t = t + tb.w[route] * f32x4{b[0], b[1], b[2], b[3]};
-      }
-    }
+    for (int k = wave + NW; k < num; k += NW) add_bias(k, bias_of(k));
   __syncthreads();
   if (tid < p.T * 4) {  // token tid / 4, columns 4 (tid % 4) .. + 3
     f32x4 v = tot[0][tid];
@@ -501,7 +525,7 @@ __global__ __launch_bounds__(NW * 64) void few_down_kernel(const FewParams p) {
 template <int F, int S>
 void launch_up(const FewParams& p, hipStream_t st) {
   const int64_t items = (int64_t)std::min(p.E, p.T * p.topk) * (p.I / 16);
-  hipLaunchKernelGGL((few_up_kernel<F, S>), dim3((unsigned)std::min<int64_t>(items, 512)), dim3(kUpWaves * 64), 0, st, p);
+  hipLaunchKernelGGL((few_up_kernel<F, S>), dim3((unsigned)std::min<int64_t>(items, 768)), dim3(kUpWaves * 64), 0, st, p);
 }
 
 template <int F>
