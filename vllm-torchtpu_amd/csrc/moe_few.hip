@@ -86,40 +86,58 @@ using qmoe_stream::kOob;
 using qmoe_stream::make_rsrc;
 using qmoe_stream::rsrc_t;
 
+__device__ __forceinline__ uint4 load16(rsrc_t r, uint32_t off) {
+  const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// The words that hold the scales of the lane's chunks c and c + 1 (c even) of
+// the row at row_off, and where in them: FF_MX a byte each, FF_I4 a bf16, FF_NV a
+// pair of bf16, FF_F8 one float32. (Whole, aligned words: the compiler extends a
+// narrower load right behind it, where it waits for every load in flight.)
+template <int F>
+struct Scales {
+  uint32_t w[2];
+};
+template <int F>
+__device__ __forceinline__ uint32_t scale_off(uint32_t row_off, int c, int group_shift) {
+  return row_off + (F == FF_MX ? c : (F == FF_NV ? c * 4 : (F == FF_I4 ? ((c * 32) >> group_shift) * 2 : (c >> 3) * 4)));
+}
+template <int F>
+__device__ __forceinline__ Scales<F> load_scales(rsrc_t r, uint32_t row_off, int c, int group_shift, bool in) {
+  Scales<F> s;
+  if constexpr (F == FF_BF) {
+    s.w[0] = s.w[1] = 0;
+  } else {
+    const uint32_t a = scale_off<F>(row_off, c, group_shift) & ~3u, b = scale_off<F>(row_off, c + 1, group_shift) & ~3u;
+    s.w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, in ? a : kOob, 0, 0);
+    if constexpr (F == FF_F8) s.w[1] = s.w[0];
+    // (mostly the same word: no request then)
+    else s.w[1] = __builtin_amdgcn_raw_buffer_load_b32(r, in && b != a ? b : kOob, 0, 0);
+  }
+  return s;
+}
+// Scale of chunk c + u from its words, as expand8 takes it
+template <int F>
+__device__ __forceinline__ uint32_t scale_of(const uint32_t (&w)[2], uint32_t row_off, int c, int u, int group_shift) {
+  if constexpr (F == FF_MX || F == FF_I4) {
+    const uint32_t a = scale_off<F>(row_off, c, group_shift), o = scale_off<F>(row_off, c + u, group_shift);
+    const uint32_t word = u && (o & ~3u) != (a & ~3u) ? w[1] : w[0];
+    return (word >> ((o & 3u) * 8)) & (F == FF_MX ? 0xffu : 0xffffu);
+  } else {
+    return w[u];
+  }
+}
+
 // One step of a wavefront: a 128-byte line of 16 rows for each of NT tiles
 // (lane -> row 8 v + l / 8, chunk l % 8), their scales (lane -> row l % 16, chunks 2
 // kg and 2 kg + 1, kg = l / 16) and the tokens' values for those two chunks
 template <int F, int NT>
 struct Step {
   uint4 w[NT][2];
-  uint2 s[NT];
+  Scales<F> s[NT];
   uint4 x[2];
 };
-
-__device__ __forceinline__ uint4 load16(rsrc_t r, uint32_t off) {
-  const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
-  return make_uint4(v[0], v[1], v[2], v[3]);
-}
-
-// The scales of the lane's chunks c and c + 1 (c even) of the row at row_off:
-// FF_MX two bytes, FF_NV two pairs of bf16, FF_I4 a bf16 each, FF_F8 one float32
-template <int F>
-__device__ __forceinline__ uint2 load_scales(rsrc_t r, uint32_t row_off, int c, int group_shift, bool in) {
-  uint2 s = make_uint2(0, 0);
-  if constexpr (F == FF_MX) {
-    s.x = __builtin_amdgcn_raw_buffer_load_b8(r, in ? row_off + c : kOob, 0, 0);
-    s.y = __builtin_amdgcn_raw_buffer_load_b8(r, in ? row_off + c + 1 : kOob, 0, 0);
-  } else if constexpr (F == FF_NV) {
-    s.x = __builtin_amdgcn_raw_buffer_load_b32(r, in ? row_off + c * 4 : kOob, 0, 0);
-    s.y = __builtin_amdgcn_raw_buffer_load_b32(r, in ? row_off + c * 4 + 4 : kOob, 0, 0);
-  } else if constexpr (F == FF_I4) {
-    s.x = __builtin_amdgcn_raw_buffer_load_b16(r, in ? row_off + ((c * 32) >> group_shift) * 2 : kOob, 0, 0);
-    s.y = __builtin_amdgcn_raw_buffer_load_b16(r, in ? row_off + (((c + 1) * 32) >> group_shift) * 2 : kOob, 0, 0);
-  } else if constexpr (F == FF_F8) {
-    s.x = s.y = __builtin_amdgcn_raw_buffer_load_b32(r, in ? row_off + (c >> 3) * 4 : kOob, 0, 0);
-  }
-  return s;
-}
 
 union Bf8 {
   uint4 u;
@@ -165,13 +183,24 @@ __device__ __forceinline__ uint4 expand8(const uint4& c, int i, uint32_t s) {
   else return c;
 }
 
-// acc[t][i] += line t . tokens, MFMA i of each chunk. `tr`: this wavefront's LDS,
+// acc[t][i] += line t . tokens, MFMA i of each chunk; `first`: the line's first
+// chunk of the row, row_off: the lane's scale row. `tr`: this wavefront's LDS,
 // 2 KB per tile. Row r's chunk c lies at slot c ^ (r / 2), so that neither the
 // writes (the 8 chunks of a row by 8 adjacent lanes) nor the reads (one chunk of
 // 16 rows) meet in a bank.
 template <int F, int NT>
-__device__ __forceinline__ void consume(const Step<F, NT>& st, uint4* tr, f32x4 (&acc)[NT][Fmt<F>::kMfma]) {
+__device__ __forceinline__ void consume(const Step<F, NT>& st, uint4* tr, uint32_t row_off, int first, int group_shift,
+                                        f32x4 (&acc)[NT][Fmt<F>::kMfma]) {
   const int lane = threadIdx.x & 63, r = lane & 15, kg = lane >> 4;
+  // the scale words are taken as loaded only here: their conversions, moved up
+  // to the loads of the step before, would wait for every load in flight
+  uint32_t sc[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    sc[t][0] = st.s[t].w[0];
+    sc[t][1] = st.s[t].w[1];
+    if constexpr (F != FF_BF) asm volatile("" : "+v"(sc[t][0]), "+v"(sc[t][1]));
+  }
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -185,12 +214,13 @@ __device__ __forceinline__ void consume(const Step<F, NT>& st, uint4* tr, f32x4 
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const uint4 c = tr[t * 128 + r * 8 + ((2 * kg + u) ^ (r >> 1))];
+      const uint32_t scale = scale_of<F>(sc[t], row_off, first + 2 * kg, u, group_shift);
       Bf8 b;
       b.u = st.x[u];
 #pragma unroll
       for (int i = 0; i < Fmt<F>::kMfma; ++i) {
         Bf8 a;
-        a.u = expand8<F>(c, i, u ? st.s[t].y : st.s[t].x);
+        a.u = expand8<F>(c, i, scale);
         acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, acc[t][i], 0, 0, 0);
       }
     }
@@ -339,8 +369,12 @@ __global__ __launch_bounds__(kUpWaves * 64, 3) void few_up_kernel(const FewParam
       d.x[u] = load16(xr, live && (c + u) * 16 < rb ? xrow + (uint32_t)((c + u) * Fmt<F>::kCodes * 2) : kOob);
   };
   seek(it0);
+  // (in this order: the loop's waits count the loads behind a step's own)
 #pragma unroll
-  for (int u = 0; u < kUpAhead; ++u) issue(st[u], u, true);
+  for (int u = 0; u < kUpAhead; ++u) {
+    issue(st[u], u, true);
+    __builtin_amdgcn_sched_barrier(0);
+  }
   typedef const float __attribute__((address_space(4))) CFloat;
   for (int item = it0; item < it1; ++item) {
     const int slot = item / tiles, tile = item - slot * tiles;
@@ -364,7 +398,7 @@ __global__ __launch_bounds__(kUpWaves * 64, 3) void few_up_kernel(const FewParam
       if (!more && next) seek(item + 1);
 #pragma unroll
       for (int u = 0; u < kUpAhead; ++u) {
-        consume<F, 2>(st[u], tr[wave], acc);
+        consume<F, 2>(st[u], tr[wave], slane, (wave + kUpWaves * (c * kUpAhead + u)) * 8, p.group_shift, acc);
         issue(st[u], (more ? (c + 1) * kUpAhead : 0) + u, more || next);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -488,7 +522,10 @@ __global__ __launch_bounds__(NW * 64) void few_down_kernel(const FewParams p) {
   if (biased) first_bias = bias_of(wave);
   Cursor ahead{0, wave}, now{0, wave};
 #pragma unroll
-  for (int u = 0; u < kDownAhead; ++u) issue(st[u], ahead);
+  for (int u = 0; u < kDownAhead; ++u) {
+    issue(st[u], ahead);
+    __builtin_amdgcn_sched_barrier(0);
+  }
   if (biased) add_bias(wave, first_bias);
   int slot = -1;
   settle(now);
@@ -498,7 +535,7 @@ __global__ __launch_bounds__(NW * 64) void few_down_kernel(const FewParams p) {
       if (now.slot < num) {
         if (now.slot != slot && slot >= 0) flush(slot);
         slot = now.slot;
-        consume<F, 1>(st[u], tr[wave], acc);
+        consume<F, 1>(st[u], tr[wave], slane, now.line * 8, p.group_shift, acc);
       }
       issue(st[u], ahead);
       now.line += NW;

@@ -5,6 +5,7 @@ layouts on the host, and launches the HIP kernels on the current stream via
 `_capi`. There is no CPU path: a CPU tensor is a ValueError.
 """
 
+import contextlib
 import ctypes
 import math
 
@@ -43,11 +44,16 @@ def _stream(dev):
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
+_PLAIN = frozenset((type(None), torch.Tensor, torch.nn.Parameter))
+
+
 def eager_call(*ts):
     """Whether a call on these tensors runs at once (plain tensors outside of a
     trace), so that no dispatcher has to see it."""
-    return not torch.compiler.is_compiling() and all(
-        t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in ts)
+    for t in ts:
+        if type(t) not in _PLAIN:
+            return False
+    return not torch.compiler.is_compiling()
 
 
 def _require_gpu(*ts):
@@ -675,44 +681,54 @@ def _check_few(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, t
     if act_code(activation or None)[0] == _capi.ACT_NONE:
         raise ValueError("few-token MoE: a gate / up activation is required")
     _, wdt, per, sdt, blk = _FEW_FORMATS[fmt]
-    if x.dim() != 2 or x.dtype != torch.bfloat16:
+    if x.dim() != 2 or x.dtype is not torch.bfloat16:
         raise ValueError(f"few-token MoE: hidden states must be bf16 [T, H], got {x.dtype} {tuple(x.shape)}")
     T, H = x.shape
-    if w1.dim() != 3 or w2.dim() != 3 or w1.dtype != wdt or w2.dtype != wdt:
+    if w1.dim() != 3 or w2.dim() != 3 or w1.dtype is not wdt or w2.dtype is not wdt:
         raise ValueError(f"few-token MoE: {fmt} experts are {wdt} [E, 2I, H / {per}] and [E, H, I / {per}]")
-    E, I = w1.shape[0], w2.shape[2] * per
-    if tuple(w1.shape) != (E, 2 * I, H // per) or tuple(w2.shape) != (E, H, I // per) or H % per:
+    E, n1, _ = w1.shape
+    I = w2.shape[2] * per
+    if w1.shape != (E, 2 * I, H // per) or w2.shape != (E, H, I // per) or H % per:
         raise ValueError(f"few-token MoE: inconsistent shapes: hidden {tuple(x.shape)}, w1 {tuple(w1.shape)}, "
                          f"w2 {tuple(w2.shape)}")
-    if tuple(router_logits.shape) != (T, E):
+    if router_logits.shape != (T, E):
         raise ValueError(f"few-token MoE: router logits must be [{T}, {E}], got {tuple(router_logits.shape)}")
     if not 1 <= T <= FEW_MAX_TOKENS or not 1 <= topk <= E or T * topk > FEW_MAX_ROUTES:
         raise ValueError(f"few-token MoE takes 1..{FEW_MAX_TOKENS} tokens, topk <= experts and at most {FEW_MAX_ROUTES} "
                          f"routes, got T={T}, topk={topk}, E={E}")
+    if not w1.is_contiguous() or not w2.is_contiguous():
+        raise ValueError("few-token MoE: expert weights must be contiguous")
     group = 0
-    for w, s, n, k, name in ((w1, w1_scale, 2 * I, H, "w1_scale"), (w2, w2_scale, H, I, "w2_scale")):
-        if not w.is_contiguous():
-            raise ValueError("few-token MoE: expert weights must be contiguous")
-        if sdt is None:
-            if s is not None:
-                raise ValueError(f"few-token MoE: {fmt} experts have no scales")
-            continue
-        b = blk
-        if fmt == "int4":
-            b = k // s.shape[-1] if s is not None and s.dim() == 3 and s.shape[-1] else 0
-            if b not in (32, 64, 128) or (group and b != group):
-                raise ValueError("few-token MoE: int4 scales are per group of 32, 64 or 128 k, the same in both matrices")
-            group = b
-        if s is None or s.element_size() != sdt.itemsize or (sdt.itemsize > 1 and s.dtype != sdt) or k % b or \
-                tuple(s.shape) != (E, n, k // b) or not s.is_contiguous():
-            raise ValueError(f"few-token MoE: {name} must be contiguous {sdt} [{E}, {n}, {k} / {b}]")
-    for b, n, name in ((w1_bias, 2 * I, "w1_bias"), (w2_bias, H, "w2_bias")):
+    if sdt is None:
+        if w1_scale is not None or w2_scale is not None:
+            raise ValueError(f"few-token MoE: {fmt} experts have no scales")
+    else:
+        for s, n, k, name in ((w1_scale, n1, H, "w1_scale"), (w2_scale, H, I, "w2_scale")):
+            b = blk
+            if fmt == "int4":
+                b = k // s.shape[-1] if s is not None and s.dim() == 3 and s.shape[-1] else 0
+                if b not in (32, 64, 128) or (group and b != group):
+                    raise ValueError("few-token MoE: int4 scales are per group of 32, 64 or 128 k, the same in both "
+                                     "matrices")
+                group = b
+            if s is None or (s.dtype is not sdt and (fmt != "mxfp4" or s.element_size() != 1)) or k % b or \
+                    s.shape != (E, n, k // b) or not s.is_contiguous():
+                raise ValueError(f"few-token MoE: {name} must be contiguous {sdt} [{E}, {n}, {k} / {b}]")
+    for b, n, name in ((w1_bias, n1, "w1_bias"), (w2_bias, H, "w2_bias")):
         if b is not None and b.numel() != E * n:
             raise ValueError(f"few-token MoE: {name} must hold [{E}, {n}] values, got {tuple(b.shape)}")
-    mult = 128 if fmt == "fp8_w8a16" else max(32, group)
+    mult = 128 if fmt == "fp8_w8a16" else (group if group > 32 else 32)
     if H % mult or I % mult:
         raise ValueError(f"few-token MoE: {fmt} needs H and I in multiples of {mult}, got {H}, {I}")
     return I, group
+
+
+def _addr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _f32_flat(t):
+    return t if t is None or (t.dtype is torch.float32 and t.is_contiguous()) else t.float().contiguous()
 
 
 def moe_few_tokens(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk, activation, fmt,
@@ -724,83 +740,91 @@ def moe_few_tokens(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bia
     I, group = _check_few(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk, activation, fmt,
                           scoring_func)
     act, p0, p1 = act_code(activation)
-    if bias is not None and bias.numel() != w1.shape[0]:
-        raise ValueError(f"few-token MoE: the correction bias must hold {w1.shape[0]} values")
+    T, H = x.shape
+    E = w1.shape[0]
+    if bias is not None and bias.numel() != E:
+        raise ValueError(f"few-token MoE: the correction bias must hold {E} values")
     with _on_device(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, bias):
-        if x.stride(1) != 1 or x.stride(0) < x.shape[1] or x.stride(0) % 8 or x.data_ptr() % 16:
+        dev = x.device
+        ldx = x.stride(0)
+        if x.stride(1) != 1 or ldx < H or ldx % 8 or x.data_ptr() % 16:
             x = x.clone(memory_format=torch.contiguous_format)
+            ldx = H
         lg = router_logits
-        if lg.dtype not in (torch.bfloat16, torch.float32):
+        if lg.dtype not in _GRAD_TYPES:
             lg = lg.float()
-        lg = lg.contiguous()
-        f32 = lambda t: t.float().contiguous() if t is not None else None  # noqa: E731
-        b, b1, b2 = f32(bias), f32(w1_bias), f32(w2_bias)
-        out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
-        d = _capi.FewDesc()
-        d.format, d.group = _FEW_FORMATS[fmt][0], group
-        d.x, d.ldx = x.data_ptr(), x.stride(0)
-        d.T, d.H, d.I, d.E, d.topk = x.shape[0], x.shape[1], I, w1.shape[0], topk
-        d.router_logits, d.logits_f32 = lg.data_ptr(), int(lg.dtype == torch.float32)
-        d.scoring = _SCORING[scoring_func]
-        d.correction_bias = b.data_ptr() if b is not None else None
-        d.renormalize, d.routed_scaling_factor = int(bool(renormalize)), float(routed_scaling_factor)
-        d.num_group, d.topk_group = int(num_expert_group or 1), int(topk_group or 1)
-        d.skip_padded = int(bool(skip_padded_tokens))
-        d.w1, d.w2 = w1.data_ptr(), w2.data_ptr()
-        d.w1_scale = w1_scale.data_ptr() if w1_scale is not None else None
-        d.w2_scale = w2_scale.data_ptr() if w2_scale is not None else None
-        d.w1_bias = b1.data_ptr() if b1 is not None else None
-        d.w2_bias = b2.data_ptr() if b2 is not None else None
-        d.act, d.act_p0, d.act_p1 = act, p0, p1
-        d.out, d.ldo = out.data_ptr(), out.stride(0)
+        lg, b, b1, b2 = lg.contiguous(), _f32_flat(bias), _f32_flat(w1_bias), _f32_flat(w2_bias)
+        out = torch.empty((T, H), dtype=torch.bfloat16, device=dev)
+        d = _capi.FewDesc(_FEW_FORMATS[fmt][0], group, x.data_ptr(), ldx, T, H, I, E, topk, lg.data_ptr(),
+                          lg.dtype is torch.float32, _SCORING[scoring_func], _addr(b), bool(renormalize),
+                          routed_scaling_factor, num_expert_group or 1, topk_group or 1, bool(skip_padded_tokens),
+                          w1.data_ptr(), w2.data_ptr(), _addr(w1_scale), _addr(w2_scale), _addr(b1), _addr(b2), act, p0, p1,
+                          out.data_ptr(), H)
+        ref = ctypes.byref(d)
         need = ctypes.c_int64(0)
-        check(lib.qmoe_moe_few_workspace_size(ctypes.byref(d), ctypes.byref(need)), "moe_few_tokens (shape)")
-        ws, ws_n = _workspace(x.device, need.value)
-        check(lib.qmoe_moe_few(ctypes.byref(d), _ptr(ws), ws_n, _stream(x.device)), "moe_few_tokens")
+        check(lib.qmoe_moe_few_workspace_size(ref, ctypes.byref(need)), "moe_few_tokens (shape)")
+        ws, ws_n = _workspace(dev, need.value)
+        check(lib.qmoe_moe_few(ref, ws.data_ptr(), ws_n, torch.cuda.current_stream(dev).cuda_stream), "moe_few_tokens")
     return out
 
 
 # ---------------------------------------------------------------- vocabulary table
 
 _TABLE_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2, FP8: 3, torch.int8: 4, torch.float8_e5m2: 5}
+_OUT_TYPES = frozenset((torch.bfloat16, torch.float16, torch.float32))
+_GRAD_TYPES = frozenset((torch.bfloat16, torch.float32))
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _on_device(*ts):
     """One device for every tensor given (None aside), made the current one
     for the launches of a ``with`` block: the runtime launches on the current
     device, whatever device the stream and the pointers belong to."""
-    _require_gpu(*ts)
-    devs = {t.device for t in ts if t is not None}
-    if len(devs) != 1:
-        raise ValueError(f"qmoe: tensors on different devices: {sorted(map(str, devs))}")
-    return torch.cuda.device(devs.pop())
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        d = t.device
+        if dev is None:
+            dev = d
+            if d.type != "cuda":
+                raise ValueError(f"qmoe kernels need device tensors, got a {d} tensor")
+        elif d != dev:
+            raise ValueError(f"qmoe kernels need device tensors, all on one device, got {dev} and {d}")
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _check_ids(ids, what):
-    if ids.dtype not in (torch.int32, torch.int64):
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise ValueError(f"{what} must be int32 or int64, got {ids.dtype}")
-    return ids.reshape(-1).contiguous()
+    return ids if ids.dim() == 1 and ids.is_contiguous() else ids.reshape(-1).contiguous()
 
 
 def _check_table(weight, weight_scale, what):
     """A [V, H] table with contiguous rows: bf16 / f32, or 1-byte codes with one
     float32 scale per row (returned as [V])."""
-    if weight.dim() != 2 or weight.dtype not in _TABLE_TYPES or weight.dtype == torch.float16:
+    dtype, shape = weight.dtype, weight.shape
+    if len(shape) != 2 or dtype not in _TABLE_TYPES or dtype is torch.float16:
         raise ValueError(f"{what}: the table must be a [V, H] bf16, f32, e4m3, e5m2 or int8 tensor, got "
-                         f"{weight.dtype} {tuple(weight.shape)}")
-    if weight.shape[0] == 0 or weight.shape[1] == 0:
-        raise ValueError(f"{what}: empty table {tuple(weight.shape)}")
-    if weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]:
-        raise ValueError(f"{what}: the table's rows must be contiguous and apart, got strides {weight.stride()}")
-    coded = weight.element_size() == 1
+                         f"{dtype} {tuple(shape)}")
+    V, H = shape
+    if V == 0 or H == 0:
+        raise ValueError(f"{what}: empty table {tuple(shape)}")
+    strides = weight.stride()
+    if strides[1] != 1 or strides[0] < H:
+        raise ValueError(f"{what}: the table's rows must be contiguous and apart, got strides {strides}")
+    coded = _TABLE_TYPES[dtype] >= 3
     if coded != (weight_scale is not None):
-        raise ValueError(f"{what}: a {weight.dtype} table takes {'one scale per row' if coded else 'no row scales'}")
+        raise ValueError(f"{what}: a {dtype} table takes {'one scale per row' if coded else 'no row scales'}")
     if not coded:
         return None
-    if weight_scale.dtype != torch.float32 or weight_scale.numel() != weight.shape[0]:
-        raise ValueError(f"{what}: row scales must be float32 [{weight.shape[0]}], got {weight_scale.dtype} "
+    if weight_scale.dtype is not torch.float32 or weight_scale.numel() != V:
+        raise ValueError(f"{what}: row scales must be float32 [{V}], got {weight_scale.dtype} "
                          f"{tuple(weight_scale.shape)}")
-    return weight_scale.reshape(-1).contiguous()
+    return weight_scale if weight_scale.dim() == 1 and weight_scale.is_contiguous() else \
+        weight_scale.reshape(-1).contiguous()
 
 
 def vocab_lookup(ids, weight, weight_scale=None, scale=1.0, out_dtype=torch.bfloat16):
@@ -810,49 +834,53 @@ def vocab_lookup(ids, weight, weight_scale=None, scale=1.0, out_dtype=torch.bflo
     NaN."""
     s = _check_table(weight, weight_scale, "vocab_lookup")
     flat = _check_ids(ids, "vocab_lookup: ids")
-    if out_dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    if out_dtype not in _OUT_TYPES:
         raise ValueError(f"vocab_lookup: the output is bf16, f16 or f32, not {out_dtype}")
     V, H = weight.shape
+    n = flat.shape[0]
     with _on_device(flat, weight, s):
-        out = torch.empty((flat.numel(), H), dtype=out_dtype, device=weight.device)
-        check(lib.qmoe_vocab_lookup(_ptr(flat), int(flat.dtype == torch.int64), flat.numel(), _ptr(weight),
-                                    _TABLE_TYPES[weight.dtype], weight.stride(0), _ptr(s), V, H, float(scale),
-                                    _ptr(out), _TABLE_TYPES[out_dtype], H, _stream(weight.device)), "vocab_lookup")
-    return out.view(*ids.shape, H)
+        dev = weight.device
+        out = torch.empty((n, H), dtype=out_dtype, device=dev)
+        check(lib.qmoe_vocab_lookup(flat.data_ptr(), flat.dtype is torch.int64, n, weight.data_ptr(),
+                                    _TABLE_TYPES[weight.dtype], weight.stride(0), s.data_ptr() if s is not None else None,
+                                    V, H, scale, out.data_ptr(), _TABLE_TYPES[out_dtype], H,
+                                    torch.cuda.current_stream(dev).cuda_stream), "vocab_lookup")
+    return out if ids.dim() == 1 else out.view(*ids.shape, H)
 
 
 def vocab_lookup_grad(grad, ids, vocab, scale=1.0, padding_idx=None, dtype=torch.bfloat16, into=None):
     """Gradient of `vocab_lookup` with respect to a bf16 or f32 table: ``[vocab,
     H]`` of ``dtype``, or with ``into`` (a table gradient to add to, e.g. that of
     a tied output projection) only the rows that have a token, in place."""
-    if grad.dtype not in (torch.bfloat16, torch.float32) or grad.dim() < 1:
+    if grad.dtype not in _GRAD_TYPES or grad.dim() < 1:
         raise ValueError(f"vocab_lookup_grad: the gradient must be bf16 or f32 rows, got {grad.dtype}")
     flat = _check_ids(ids, "vocab_lookup_grad: ids")
     H = grad.shape[-1]
-    if tuple(grad.shape[:-1]) != tuple(ids.shape) or H == 0:
+    if grad.shape[:-1] != ids.shape or H == 0:
         raise ValueError(f"vocab_lookup_grad: a gradient of {tuple(grad.shape)} for ids of {tuple(ids.shape)}")
-    g = grad.reshape(-1, H)
-    if g.numel() and (g.stride(1) != 1 or g.stride(0) < H):
+    g = grad if grad.dim() == 2 else grad.reshape(-1, H)
+    n = flat.shape[0]
+    if n and (g.stride(1) != 1 or g.stride(0) < H):
         g = g.contiguous()
     if padding_idx is not None and not 0 <= padding_idx < vocab:
         raise ValueError(f"vocab_lookup_grad: padding_idx {padding_idx} is outside the table of {vocab} rows")
     if into is not None:
-        if into.dim() != 2 or tuple(into.shape) != (vocab, H) or into.dtype not in (torch.bfloat16, torch.float32) or \
+        if into.dim() != 2 or into.shape != (vocab, H) or into.dtype not in _GRAD_TYPES or \
                 into.stride(1) != 1 or into.stride(0) < H:
             raise ValueError(f"vocab_lookup_grad: `into` must be a bf16 or f32 [{vocab}, {H}] tensor with contiguous rows")
-    elif dtype not in (torch.bfloat16, torch.float32):
+    elif dtype not in _GRAD_TYPES:
         raise ValueError(f"vocab_lookup_grad: the table's gradient is bf16 or f32, not {dtype}")
     with _on_device(g, flat, into):
-        dw = into if into is not None else torch.empty((vocab, H), dtype=dtype, device=g.device)
+        dev = g.device
+        dw = into if into is not None else torch.empty((vocab, H), dtype=dtype, device=dev)
         need = ctypes.c_int64(0)
-        check(lib.qmoe_vocab_lookup_grad_workspace_size(flat.numel(), vocab, H, ctypes.byref(need)),
-              "vocab_lookup_grad (shape)")
-        ws, ws_n = _workspace(g.device, need.value)
-        check(lib.qmoe_vocab_lookup_grad(_ptr(flat), int(flat.dtype == torch.int64), flat.numel(), _ptr(g),
-                                         _TABLE_TYPES[g.dtype], g.stride(0) if g.numel() else H, vocab, H, float(scale),
-                                         -1 if padding_idx is None else int(padding_idx), _ptr(dw),
-                                         _TABLE_TYPES[dw.dtype], dw.stride(0), int(into is not None), _ptr(ws), ws_n,
-                                         _stream(g.device)), "vocab_lookup_grad")
+        check(lib.qmoe_vocab_lookup_grad_workspace_size(n, vocab, H, ctypes.byref(need)), "vocab_lookup_grad (shape)")
+        ws, ws_n = _workspace(dev, need.value)
+        check(lib.qmoe_vocab_lookup_grad(flat.data_ptr(), flat.dtype is torch.int64, n, g.data_ptr(),
+                                         _TABLE_TYPES[g.dtype], g.stride(0) if n else H, vocab, H, scale,
+                                         -1 if padding_idx is None else padding_idx, dw.data_ptr(),
+                                         _TABLE_TYPES[dw.dtype], dw.stride(0), into is not None, ws.data_ptr(), ws_n,
+                                         torch.cuda.current_stream(dev).cuda_stream), "vocab_lookup_grad")
     return dw
 
 
