@@ -14,15 +14,19 @@
 // cores (the logits twice: keeping them would take T V values), or, for few
 // tokens, one read of the table.
 //
-// Every product is one kernel: rows of two row-major bf16 operands against
-// each other along their contiguous axis, 256 "A" rows x 128 or 256 "B" rows
-// per workgroup, with the stage ring of gemm_t8.hip and an epilogue of its own:
+// Every product is the same tile, 256 "A" rows x 64, 128 or 256 "B" rows per
+// workgroup, with the stage ring of gemm_t8.hip and an epilogue of its own:
 //   logits : A = table rows, B = tokens; per token and tile the maximum and the
 //            sum of exponentials (one pass), and the target's logit
-//   probs  : the same product again; P as [t][v], and as [v][t] for dw
-//   dx     : A = columns of the table piece (transposed once per piece), B = P
-//            rows; float32 sums added over the pieces
-//   dw     : A = columns of x (transposed once), B = P^T rows
+//   probs  : the same product again; P as [t][v]
+//   dx     : A = columns of the table piece, B = P rows; float32 sums added over
+//            the pieces
+//   dw     : A = columns of x (transposed once), B = columns of P
+// Rows run along K, the contiguous axis, or, of the table in dx and of P in dw,
+// across it: those are copied as they lie, 64 K rows of a stage, and transposed
+// on their way from LDS to registers by ds_read_b64_tr_b16. (With a transposed
+// copy of each table piece and P stored both ways instead: 892 us against 766 at
+// 333 tokens x 50021 x 2880, 14.26 ms against 14.15 at 4096 x 131072 x 4096.)
 // Sums are float32; P is rounded to bf16 once, as the operand of the products.
 
 #include <algorithm>
@@ -59,11 +63,10 @@ struct VocabGemm {
   const float *lse, *g_loss, *g_lse;  // g_lse may be nullptr
   uint16_t* p;      // [nb][ldp] P
   int64_t ldp;
-  uint16_t* pt;     // [na rounded up][ldpt] P^T, or nullptr
-  int64_t ldpt;
   // dx / dw: out[b row][a row]
   float* sum;       // [nb][ldsum] float32 sums of the pieces before, or nullptr
   int64_t ldsum;
+  int kr;           // K rows of the operand that lies across K: those from kr on meet zeros
   int first, last;  // first / last piece
   int kslice;       // K split: slice z takes the K range from z * kslice on ...
   float* slices;    // ... and leaves its sums in [z][nb][ldsum]; kslice 0: no split
@@ -76,6 +79,37 @@ __device__ __align__(16) const uint32_t kVocabZero[4] = {0, 0, 0, 0};
 __device__ __forceinline__ int64_t load_target(const VocabGemm& p, int t) {
   return p.targets_i64 ? static_cast<const int64_t*>(p.targets)[t]
                        : (int64_t) static_cast<const int32_t*>(p.targets)[t];
+}
+
+// Which operand lies across K, rows of 256 or BM columns, and how it passes
+// through LDS. ds_read_b64_tr_b16: lane 4 r + c of 16 gives the address of row r's
+// elements 4 c .. + 3, lane i receives column i of the 4 rows. An MFMA operand is
+// two of them (k + 4) per lane; the 4 rows of an access lie in different 64-byte
+// blocks, for which the 16-byte chunk c of row k is stored at c ^ tr_swz.
+constexpr bool tr_a(int epi) { return epi == VE_SUM; }
+constexpr bool tr_b(int epi) { return epi == VE_STORE; }
+template <int RB>  // bytes of a row
+__device__ __forceinline__ int tr_swz(int k) {
+  return 4 * (RB == 128 ? (k >> 1) & 1 : k & 3);
+}
+// Byte of the lane's first 4 x 4 of k 0 .. 15 of columns 0 .. 31; those of columns
+// 32 f .. are at this ^ 64 f
+template <int RB>
+__device__ __forceinline__ uint32_t tr_lane(int lane) {
+  const int k = 8 * (lane >> 5) + ((lane & 15) >> 2);
+  return (uint32_t)(k * RB + ((32 * ((lane >> 4) & 1) + 8 * (lane & 3)) ^ (tr_swz<RB>(k) * 16)));
+}
+template <int RB>
+__device__ __forceinline__ uint4 tr_read(const uint8_t* at) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4* Lds;
+  union {
+    s16x4 h[2];
+    uint4 u;
+  } r;
+  r.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(void*)at);
+  r.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(void*)(at + 4 * RB));
+  return r.u;
 }
 
 __device__ __forceinline__ int vg_swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
@@ -196,7 +230,6 @@ __device__ __forceinline__ void vocab_epilogue(const VocabGemm& p, f32x16 (&acc)
 #pragma unroll
   for (int j = 0; j < MJ; ++j) {
     const int tl = wm * 32 + rl, tb = 64 * j + tl;  // B row of the 64, of the tile
-    // (P^T wants zeros up to its row length, a multiple of 64, too)
     if (64 * j >= brows) break;
     if (j) __syncthreads();  // the rows before have been read
     const int n1 = opaque_v(wn * NI * 32 + kh * 4);
@@ -248,53 +281,35 @@ __device__ __forceinline__ void vocab_epilogue(const VocabGemm& p, f32x16 (&acc)
     // 8 consecutive A rows of a B row per thread
     constexpr int CH = BN / 8;
     const int c = (tid % CH) * 8;
-    if (EPI != VE_PROB || p.p) {
 #pragma unroll 2
-      for (int t = tid / CH; t < 64; t += THREADS / CH) {
-        const int64_t row = m0 + 64 * j + t;
-        if (64 * j + t >= brows) break;
-        const float4 lo = *reinterpret_cast<const float4*>(reg + t * BN + (c ^ vg_row_swz(t)));
-        const float4 hi = *reinterpret_cast<const float4*>(reg + t * BN + ((c + 4) ^ vg_row_swz(t)));
-        float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        if constexpr (EPI == VE_PROB) {
-          // P times the row scales is what multiplies the codes
+    for (int t = tid / CH; t < 64; t += THREADS / CH) {
+      const int64_t row = m0 + 64 * j + t;
+      if (64 * j + t >= brows) break;
+      const float4 lo = *reinterpret_cast<const float4*>(reg + t * BN + (c ^ vg_row_swz(t)));
+      const float4 hi = *reinterpret_cast<const float4*>(reg + t * BN + ((c + 4) ^ vg_row_swz(t)));
+      float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      if constexpr (EPI == VE_PROB) {
+        // P times the row scales is what multiplies the codes
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] *= s_scale[c + k];
-          *reinterpret_cast<uint4*>(p.p + row * p.ldp + n0 + c) = make_uint4(
-              pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-        } else if (c < arows) {  // (A rows come in multiples of 8)
-          if constexpr (EPI == VE_SUM) {
-            float4* dst = reinterpret_cast<float4*>(p.sum + row * p.ldsum + n0 + c);
-            if (!p.first) {
-              const float4 a = dst[0], b = dst[1];
-              v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
-              v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
-            }
-            if (!p.last) {
-              dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-              dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-              continue;
-            }
+        for (int k = 0; k < 8; ++k) v[k] *= s_scale[c + k];
+        *reinterpret_cast<uint4*>(p.p + row * p.ldp + n0 + c) = make_uint4(
+            pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+      } else if (c < arows) {  // (A rows come in multiples of 8)
+        if constexpr (EPI == VE_SUM) {
+          float4* dst = reinterpret_cast<float4*>(p.sum + row * p.ldsum + n0 + c);
+          if (!p.first) {
+            const float4 a = dst[0], b = dst[1];
+            v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
+            v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
           }
-          *reinterpret_cast<uint4*>(p.y + row * p.ldy + n0 + c) = make_uint4(
-              pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+          if (!p.last) {
+            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+            continue;
+          }
         }
-      }
-    }
-    if constexpr (EPI == VE_PROB) {
-      if (p.pt) {
-        // 8 consecutive B rows of an A row per thread
-        const int tg8 = (tid & 7) * 8;
-        const int64_t t0 = m0 + 64 * j + tg8;
-#pragma unroll 2
-        for (int n = tid >> 3; n < BN; n += THREADS / 8) {
-          float v[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = reg[(tg8 + k) * BN + (n ^ vg_row_swz(tg8 + k))];
-          if (n < arows)
-            *reinterpret_cast<uint4*>(p.pt + (int64_t)(n0 + n) * p.ldpt + t0) = make_uint4(
-                pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-        }
+        *reinterpret_cast<uint4*>(p.y + row * p.ldy + n0 + c) = make_uint4(
+            pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
       }
     }
   }
@@ -306,9 +321,10 @@ __device__ __forceinline__ void take_slice(VocabGemm& p) {
   if constexpr (EPI == VE_SUM) {
     if (p.kslice) {
       const int k0 = blockIdx.y * p.kslice;
-      p.a += (int64_t)k0 * 2;
+      p.a += k0 * p.lda;
       p.b += (int64_t)k0 * 2;
       p.K = min(p.kslice, p.K - k0);
+      p.kr -= k0;
       p.sum = p.slices + (int64_t)blockIdx.y * p.nb * p.ldsum;
       p.first = 1, p.last = 0;
     }
@@ -355,6 +371,7 @@ __device__ __forceinline__ bf16x8 codes8_to_bf16(uint32_t lo, uint32_t hi) {
 template <int EPI, int BM, int AT>
 __global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGemm args) {
   constexpr int BN = kVN, NI = 2, MJ = BM / 64;
+  constexpr bool TRA = tr_a(EPI), TRB = tr_b(EPI);
   constexpr int AB = AT ? 64 : 128;  // bytes of an A row per stage
   constexpr int WB = BN * AB, STG = WB + BM * 128;
   constexpr int RING = 163840 / STG < 6 ? 163840 / STG : 6;
@@ -381,14 +398,28 @@ __global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGem
   const uint8_t* abase = p.a + (int64_t)n0 * p.lda;
   const uint8_t* bbase = p.b + (int64_t)m0 * p.ldb;
   uint32_t aoff[WI], boff[XI];
+  // the operand across K: an instruction is 1 KB of K rows; K rows past the last
+  // repeat it, by the bytes from the stage's first row that a lane stays below
+  constexpr int TB = TRA ? BN * 2 : BM * 2, TL = TB / 16;  // bytes, lanes of a K row
+  const int trow = lane / TL, tchunk = (lane % TL) ^ tr_swz<TB>(wave * (64 / TL) + trow);
+  const uint32_t tcol = TRA ? (uint32_t)min(tchunk, arows / 8 - 1) * 16 : (uint32_t)tchunk * 16;
+  const int64_t tld = TRA ? p.lda : p.ldb;
+  if constexpr (TRA) abase = p.a + n0 * 2;
+  if constexpr (TRB) bbase = p.b + m0 * 2;
+  const int64_t astep = TRA ? 64 * p.lda : AB, bstep = TRB ? 64 * p.ldb : 128;
 #pragma unroll
   for (int j = 0; j < WI; ++j) {
+    if constexpr (TRA) {
+      aoff[j] = (uint32_t)((wave + 8 * j) * (64 / TL) + trow) * (uint32_t)tld + tcol;
+      continue;
+    }
     const int r = AT ? (wave + 8 * j) * 16 + (lane >> 2) : (wave + 8 * j) * 8 + (lane >> 3);
     aoff[j] = (uint32_t)min(r, arows - 1) * (uint32_t)p.lda + achunk * 16;
   }
 #pragma unroll
   for (int j = 0; j < XI; ++j)
-    boff[j] = (uint32_t)min((wave + 8 * j) * 8 + (lane >> 3), brows - 1) * (uint32_t)p.ldb + xchunk * 16;
+    boff[j] = TRB ? (uint32_t)((wave + 8 * j) * (64 / TL) + trow) * (uint32_t)tld + tcol
+                  : (uint32_t)min((wave + 8 * j) * 8 + (lane >> 3), brows - 1) * (uint32_t)p.ldb + xchunk * 16;
   const int KF = p.K / 64;  // whole stages
   const uint32_t cw = lds0 + wave * 1024;
   // stage s to slot `slot` (stages past the last one copy it again, into slots
@@ -396,11 +427,13 @@ __global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGem
   auto copy_stage = [&](int s, int slot) {
     const uint32_t d = __builtin_amdgcn_readfirstlane(cw + slot * STG);
     const int k = min(s, KF - 1);
-    const uint8_t *as = uniform_ptr(abase + (int64_t)k * AB), *bs = uniform_ptr(bbase + (int64_t)k * 128);
+    const uint8_t *as = uniform_ptr(abase + k * astep), *bs = uniform_ptr(bbase + k * bstep);
+    uint32_t end = 0;
+    if constexpr (TRA || TRB) end = (uint32_t)min(63, p.kr - 64 * k - 1) * (uint32_t)tld + tcol;
 #pragma unroll
-    for (int j = 0; j < WI; ++j) lds_copy16(as, aoff[j], d + j * 8192);
+    for (int j = 0; j < WI; ++j) lds_copy16(as, TRA ? min(aoff[j], end) : aoff[j], d + j * 8192);
 #pragma unroll
-    for (int j = 0; j < XI; ++j) lds_copy16(bs, boff[j], d + WB + j * 8192);
+    for (int j = 0; j < XI; ++j) lds_copy16(bs, TRB ? min(boff[j], end) : boff[j], d + WB + j * 8192);
   };
 
   f32x16 acc[NI][MJ];
@@ -419,9 +452,13 @@ __global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGem
     bf16x8 v;
   };
   B8 wf[2][NI], xf[2][MJ];
+  const uint32_t tlane = tr_lane<TB>(lane);
   auto read_q = [&](int slot, int q) {
     const uint8_t* sW = smem + slot * STG;
-    if constexpr (AT) {
+    if constexpr (TRA) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) wf[q & 1][i].u = tr_read<TB>(sW + q * 16 * TB + (tlane ^ (wn * NI + i) * 64));
+    } else if constexpr (AT) {
       if (q % 2 == 0)
 #pragma unroll
         for (int i = 0; i < NI; ++i)
@@ -436,7 +473,8 @@ __global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGem
     const int c = AT ? 4 * (q / 2) + 2 * kh + (q & 1) : 2 * q + kh;
 #pragma unroll
     for (int j = 0; j < MJ; ++j)
-      xf[q & 1][j].u =
+      if constexpr (TRB) xf[q & 1][j].u = tr_read<TB>(sW + WB + q * 16 * TB + (tlane ^ (2 * j + wm) * 64));
+      else xf[q & 1][j].u =
           *reinterpret_cast<const uint4*>(sW + WB + ((2 * j + wm) * 32 + rl) * 128 + (c ^ vg_swz(rl)) * 16);
   };
   auto mma = [&](int q) {
@@ -544,6 +582,8 @@ template <int EPI, bool TAIL>
 __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm args) {
   constexpr int BN = kVN, BM = 256, NI = 4, MJ = 4;
   constexpr uint32_t SLOT = BN * 128, RING = 5 * SLOT;
+  constexpr bool TRA = tr_a(EPI), TRB = tr_b(EPI);
+  constexpr int TB = 512;  // bytes of a K row of the operand across K
   __shared__ __align__(1024) uint8_t smem[RING];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
   VocabGemm p = args;
@@ -562,12 +602,21 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
   const int chunk16 = (lane & 7) ^ ((lane >> 3) ^ (wave & 1));
   const uint8_t* abase = p.a + (int64_t)n0 * p.lda;
   const uint8_t* bbase = p.b + (int64_t)m0 * p.ldb;
+  // (the operand across K: 2 K rows per instruction; K rows past the last repeat
+  // it, by the bytes from the stage's first row that a lane stays below)
+  const int trow = lane >> 5, tchunk = (lane & 31) ^ tr_swz<TB>(2 * wave + trow);
+  const uint32_t tcol = TRA ? (uint32_t)min(tchunk, arows / 8 - 1) * 16 : (uint32_t)tchunk * 16;
+  if constexpr (TRA) abase = p.a + n0 * 2;
+  if constexpr (TRB) bbase = p.b + m0 * 2;
+  const int64_t astep = TRA ? 64 * p.lda : 128, bstep = TRB ? 64 * p.ldb : 128;
+  const uint32_t tld = (uint32_t)(TRA ? p.lda : p.ldb);
   uint32_t aoff[8], boff[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int r = (wave + 4 * j) * 8 + (lane >> 3);
-    aoff[j] = (uint32_t)min(r, arows - 1) * (uint32_t)p.lda + chunk16 * 16;
-    boff[j] = (uint32_t)min(r, brows - 1) * (uint32_t)p.ldb + chunk16 * 16;
+    const uint32_t t = (uint32_t)(2 * (wave + 4 * j) + trow) * tld + tcol;
+    aoff[j] = TRA ? t : (uint32_t)min(r, arows - 1) * (uint32_t)p.lda + chunk16 * 16;
+    boff[j] = TRB ? t : (uint32_t)min(r, brows - 1) * (uint32_t)p.ldb + chunk16 * 16;
   }
   const int KF = p.K / 64;  // whole stages
   const uint32_t cw = lds0 + wave * 1024;
@@ -578,12 +627,23 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
   B8 wf[2][NI], xf[2][MJ];
   // operand reads of step q of a stage: lane -> row l & 31, chunk 2 q + kh
   const uint32_t wpo = (uint32_t)(wn * NI * 4096 + rl * 128), xpo = (uint32_t)(wm * 4096 + rl * 128);
+  const uint32_t tlane = tr_lane<TB>(lane) ^ (TRA ? wn * NI * 64 : wm * 64);
   auto read_w = [&](uint32_t slot, int q) {
+    if constexpr (TRA) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) wf[q & 1][i].u = tr_read<TB>(smem + slot + q * 16 * TB + (tlane ^ i * 64));
+      return;
+    }
     const uint8_t* b = smem + slot + wpo + ((2 * q + kh) ^ vg_swz(rl)) * 16;
 #pragma unroll
     for (int i = 0; i < NI; ++i) wf[q & 1][i].u = *reinterpret_cast<const uint4*>(b + i * 4096);
   };
   auto read_x = [&](uint32_t slot, int q) {
+    if constexpr (TRB) {
+#pragma unroll
+      for (int j = 0; j < MJ; ++j) xf[q & 1][j].u = tr_read<TB>(smem + slot + q * 16 * TB + (tlane ^ j * 128));
+      return;
+    }
     const uint8_t* b = smem + slot + xpo + ((2 * q + kh) ^ vg_swz(rl)) * 16;
 #pragma unroll
     for (int j = 0; j < MJ; ++j) xf[q & 1][j].u = *reinterpret_cast<const uint4*>(b + j * 8192);
@@ -602,17 +662,25 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
   };
   if (KF > 0) {
     // (stages past the last one copy it again, into slots nobody reads)
-    auto src = [&](const uint8_t* base, int s) { return uniform_ptr(base + (int64_t)min(s, KF - 1) * 128); };
+    auto asrc = [&](int s) { return uniform_ptr(abase + min(s, KF - 1) * astep); };
+    auto bsrc = [&](int s) { return uniform_ptr(bbase + min(s, KF - 1) * bstep); };
+    auto end_of = [&](int s) { return (uint32_t)min(63, p.kr - 64 * min(s, KF - 1) - 1) * tld + tcol; };
+    auto copy_a = [&](const uint8_t* base, int j, uint32_t end, uint32_t to) {
+      lds_copy16(base, TRA ? min(aoff[j], end) : aoff[j], to);
+    };
+    auto copy_b = [&](const uint8_t* base, int j, uint32_t end, uint32_t to) {
+      lds_copy16(base, TRB ? min(boff[j], end) : boff[j], to);
+    };
     auto dst = [&](uint32_t slot) { return (uint32_t)__builtin_amdgcn_readfirstlane(cw + slot); };
     auto wrap = [](uint32_t slot) { return slot >= RING ? slot - RING : slot; };
 #pragma unroll
-    for (int j = 0; j < 8; ++j) lds_copy16(src(abase, 0), aoff[j], dst(0) + j * 4096);
+    for (int j = 0; j < 8; ++j) copy_a(asrc(0), j, end_of(0), dst(0) + j * 4096);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) lds_copy16(src(bbase, 0), boff[j], dst(SLOT) + j * 4096);
+    for (int j = 0; j < 8; ++j) copy_b(bsrc(0), j, end_of(0), dst(SLOT) + j * 4096);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) lds_copy16(src(abase, 1), aoff[j], dst(2 * SLOT) + j * 4096);
+    for (int j = 0; j < 8; ++j) copy_a(asrc(1), j, end_of(1), dst(2 * SLOT) + j * 4096);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) lds_copy16(src(bbase, 1), boff[j], dst(3 * SLOT) + j * 4096);
+    for (int j = 0; j < 4; ++j) copy_b(bsrc(1), j, end_of(1), dst(3 * SLOT) + j * 4096);
     wait_copies_upto<12>();  // the first stage
     stage_barrier();
     read_w(0, 0);
@@ -620,7 +688,8 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
     uint32_t sa = 0;  // slot of A(s); B(s), A(s + 1), ... follow
     for (int s = 0; s < KF; ++s) {
       const uint32_t sb = wrap(sa + SLOT), sa1 = wrap(sa + 2 * SLOT), sb1 = wrap(sa + 3 * SLOT), sa2 = wrap(sa + 4 * SLOT);
-      const uint8_t *b1 = src(bbase, s + 1), *a2 = src(abase, s + 2), *b2 = src(bbase, s + 2);
+      const uint8_t *b1 = bsrc(s + 1), *a2 = asrc(s + 2), *b2 = bsrc(s + 2);
+      const uint32_t e1 = end_of(s + 1), e2 = end_of(s + 2);
       const uint32_t db1 = dst(sb1) + 16384, da2 = dst(sa2), db2 = dst(sa);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -632,9 +701,9 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
         for (int i = 0; i < NI; ++i) {
           if (i == 0) read_w(q < 3 ? sa : sa1, (q + 1) & 3);
           if (i == 1) read_x(q < 3 ? sb : sb1, (q + 1) & 3);
-          if (q == 0) lds_copy16(b1, boff[4 + i], db1 + i * 4096);
-          else if (q < 3) lds_copy16(a2, aoff[4 * (q - 1) + i], da2 + (4 * (q - 1) + i) * 4096);
-          else lds_copy16(b2, boff[i], db2 + i * 4096);
+          if (q == 0) copy_b(b1, 4 + i, e1, db1 + i * 4096);
+          else if (q < 3) copy_a(a2, 4 * (q - 1) + i, e2, da2 + (4 * (q - 1) + i) * 4096);
+          else copy_b(b2, i, e2, db2 + i * 4096);
           mma_row(q, i);
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -710,11 +779,9 @@ __global__ __launch_bounds__(256) void vocab_expand_kernel(const uint8_t* w, int
   *reinterpret_cast<uint4*>(out + r * ldo + c) = make_uint4(lo.x, lo.y, hi.x, hi.y);
 }
 
-// src rows [R][C] (bf16 or codes) -> out [C][ldo] bf16, columns R .. zero up to the
-// next multiple of 64;
-// with `targets` a row whose token has no gradient becomes zeros (whatever it
-// holds). 64 x 64 tiles through LDS.
-template <int WT>
+// x rows [R][C] -> out [C][ldo] bf16, columns R .. zero up to the next multiple of
+// 64; a row whose token has no gradient becomes zeros (whatever it holds). 64 x
+// 64 tiles through LDS.
 __global__ __launch_bounds__(256) void vocab_transpose_kernel(const uint8_t* src, int64_t ld, int R, int C,
                                                               uint16_t* out, int64_t ldo, const void* targets,
                                                               int targets_i64, int64_t ignore, const float* g_loss,
@@ -728,21 +795,13 @@ __global__ __launch_bounds__(256) void vocab_transpose_kernel(const uint8_t* src
     for (int k = 0; k < 2; ++k) {
       const int r = (tid >> 3) + 32 * k;
       bool live = r0 + r < R && c0 + c < C;
-      if (live && targets) {
+      if (live) {
         const int64_t tg = targets_i64 ? static_cast<const int64_t*>(targets)[r0 + r]
                                        : (int64_t) static_cast<const int32_t*>(targets)[r0 + r];
         live = (tg != ignore && g_loss[r0 + r] != 0.0f) || (g_lse && g_lse[r0 + r] != 0.0f);
       }
       uint4 v = make_uint4(0, 0, 0, 0);
-      if (live) {
-        if constexpr (WT == 0) {
-          v = *reinterpret_cast<const uint4*>(src + (int64_t)(r0 + r) * ld + (int64_t)(c0 + c) * 2);
-        } else {
-          const uint2 d = *reinterpret_cast<const uint2*>(src + (int64_t)(r0 + r) * ld + c0 + c);
-          const uint2 lo = codes4_to_bf16<WT>(d.x), hi = codes4_to_bf16<WT>(d.y);
-          v = make_uint4(lo.x, lo.y, hi.x, hi.y);
-        }
-      }
+      if (live) v = *reinterpret_cast<const uint4*>(src + (int64_t)(r0 + r) * ld + (int64_t)(c0 + c) * 2);
       const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) tile[r][c + i] = (uint16_t)(u[i / 2] >> (16 * (i & 1)));
@@ -778,7 +837,7 @@ void launch_small(const VocabGemm& g, dim3 grid, hipStream_t st) {
   hipLaunchKernelGGL((vocab_gemm_kernel<EPI, BM, AT>), grid, dim3(kVThreads), 0, st, g);
 }
 
-// at: type of the A rows, 0 bf16 or the codes' table type (logits and probs)
+// at: type of the A rows, 0 bf16 or the codes' table type (logits)
 template <int EPI>
 void launch_gemm(VocabGemm g, int at, int bm, int slices, hipStream_t st) {
   constexpr bool kLogits = EPI == VE_LSE || EPI == VE_PROB;
@@ -791,7 +850,7 @@ void launch_gemm(VocabGemm g, int at, int bm, int slices, hipStream_t st) {
     else hipLaunchKernelGGL((vocab_big_kernel<EPI, false>), grid, dim3(kBThreads), 0, st, g);
   } else if (at == 0) {
     bm == 128 ? launch_small<EPI, 128, 0>(g, grid, st) : launch_small<EPI, 64, 0>(g, grid, st);
-  } else if constexpr (kLogits) {
+  } else if constexpr (EPI == VE_LSE) {
     if (at == 3) bm == 128 ? launch_small<EPI, 128, 3>(g, grid, st) : launch_small<EPI, 64, 3>(g, grid, st);
     else if (at == 4) bm == 128 ? launch_small<EPI, 128, 4>(g, grid, st) : launch_small<EPI, 64, 4>(g, grid, st);
     else bm == 128 ? launch_small<EPI, 128, 5>(g, grid, st) : launch_small<EPI, 64, 5>(g, grid, st);
@@ -818,19 +877,11 @@ struct LossArgs {
   int64_t ignore;
 };
 
-void launch_transpose(int wt, const uint8_t* src, int64_t ld, int64_t R, int64_t C, uint16_t* out, int64_t ldo,
-                      int64_t width, const LossArgs* mask, const float* g_loss, const float* g_lse, hipStream_t st) {
-  const dim3 grid((unsigned)cdiv(width, (int64_t)64), (unsigned)cdiv(C, (int64_t)64));
-  const void* tg = mask ? mask->targets : nullptr;
-  const int i64 = mask ? mask->targets_i64 : 0;
-  const int64_t ig = mask ? mask->ignore : 0;
-#define QMOE_TR(W) \
-  hipLaunchKernelGGL(vocab_transpose_kernel<W>, grid, dim3(256), 0, st, src, ld, (int)R, (int)C, out, ldo, tg, i64, ig, g_loss, g_lse)
-  if (wt == 0) QMOE_TR(0);
-  else if (wt == 3) QMOE_TR(3);
-  else if (wt == 4) QMOE_TR(4);
-  else QMOE_TR(5);
-#undef QMOE_TR
+void launch_transpose(const LossArgs& a, uint16_t* out, int64_t ldo, const float* g_loss, const float* g_lse,
+                      hipStream_t st) {
+  hipLaunchKernelGGL(vocab_transpose_kernel, dim3((unsigned)cdiv(a.T, (int64_t)64), (unsigned)cdiv(a.H, (int64_t)64)),
+                     dim3(256), 0, st, static_cast<const uint8_t*>(a.x), a.ldx * 2, (int)a.T, (int)a.H, out, ldo,
+                     a.targets, a.targets_i64, a.ignore, g_loss, g_lse);
 }
 
 // sizes whose tile counts, and the threads of their grids, fit 32 bits
@@ -879,10 +930,11 @@ int64_t loss_layout(int64_t T, int64_t V, int64_t H, int wtype, int64_t (&off)[3
   return at;
 }
 
-// Table rows of a piece of the gradients: P, P^T and the transposed (and for
-// codes the expanded) table rows of a piece take up to 128 MB each
-int64_t grad_piece(int64_t T, int64_t V, int64_t H) {
-  return std::min(up(V, kVN), std::max<int64_t>((int64_t)(64 << 20) / std::max(up(T, 64), H) / kVN * kVN, kVN));
+// Table rows of a piece of the gradients: P, and for codes the expanded rows, of
+// a piece take up to 128 MB each
+int64_t grad_piece(int64_t T, int64_t V, int64_t H, int wtype) {
+  const int64_t width = std::max<int64_t>(up(T, 64), wtype ? H : 0);
+  return std::min(up(V, kVN), std::max<int64_t>((int64_t)(64 << 20) / width / kVN * kVN, kVN));
 }
 
 // Row pitch (bf16) of a buffer of n columns, n a multiple of 64: an odd number of
@@ -906,27 +958,23 @@ DxPlan dx_plan(int64_t T, int64_t H, int64_t K) {
   return d;
 }
 
-// P, P^T, table piece transposed, x transposed, float32 sums, K slices, expanded rows
-int64_t grad_layout(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw, int64_t (&off)[7]) {
-  const int64_t Vc = grad_piece(T, V, H), Vp = odd_pitch(Vc), Tp = odd_pitch(up(T, 64));
+// P, x transposed, float32 sums, K slices, expanded rows
+int64_t grad_layout(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw, int64_t (&off)[5]) {
+  const int64_t Vc = grad_piece(T, V, H, wtype), Vp = odd_pitch(Vc), Tp = odd_pitch(up(T, 64));
   const bool pieces = Vc < V;
   int64_t at = 0;
   off[0] = at;
-  if (need_dx) at += up(T * Vp * 2, 256);
+  at += up(T * Vp * 2, 256);
   off[1] = at;
-  if (need_dw) at += up(Vc * Tp * 2, 256);
-  off[2] = at;
-  if (need_dx) at += up(H * Vp * 2, 256);
-  off[3] = at;
   if (need_dw) at += up(H * Tp * 2, 256);
-  off[4] = at;
+  off[2] = at;
   if (need_dx && pieces) at += up(T * H * 4, 256);
-  off[5] = at;
+  off[3] = at;
   if (need_dx) {
     const DxPlan d = dx_plan(T, H, up(std::min(Vc, V), 64));
     if (d.slices > 1) at += up(d.slices * T * H * 4, 256);
   }
-  off[6] = at;
+  off[4] = at;
   if (wtype) at += up(Vc * H * 2, 256);
   return at;
 }
@@ -990,7 +1038,7 @@ extern "C" int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void
 extern "C" int qmoe_vocab_loss_grad_workspace_size(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw,
                                                    int64_t* bytes) {
   if (!loss_sizes_ok(T, V, H) || (wtype != 0 && (wtype < 3 || wtype > 5)) || !bytes) return QMOE_ERR_ARG;
-  int64_t off[7];
+  int64_t off[5];
   *bytes = grad_layout(T, V, H, wtype, need_dx, need_dw, off);
   return QMOE_OK;
 }
@@ -1005,24 +1053,21 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
   if (dw && wtype) return QMOE_ERR_ARG;  // codes have no gradient
   if (dx && (lddx < H || lddx % 8 || (reinterpret_cast<uintptr_t>(dx) & 15))) return QMOE_ERR_ARG;
   if (dw && (lddw < H || lddw % 8 || (reinterpret_cast<uintptr_t>(dw) & 15))) return QMOE_ERR_ARG;
-  int64_t off[7];
+  int64_t off[5];
   if (!workspace || ws_bytes < grad_layout(T, V, H, wtype, dx != nullptr, dw != nullptr, off)) return QMOE_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const int64_t Vc = grad_piece(T, V, H), Vp = odd_pitch(Vc), Tw = up(T, 64), Tp = odd_pitch(Tw);
+  const int64_t Vc = grad_piece(T, V, H, wtype), Vp = odd_pitch(Vc), Tw = up(T, 64), Tp = odd_pitch(Tw);
   uint16_t* P = reinterpret_cast<uint16_t*>(ws + off[0]);
-  uint16_t* PT = reinterpret_cast<uint16_t*>(ws + off[1]);
-  uint16_t* WT = reinterpret_cast<uint16_t*>(ws + off[2]);
-  uint16_t* XT = reinterpret_cast<uint16_t*>(ws + off[3]);
-  const bool direct = wtype && codes_direct(w, ldw, H, T);
-  if (dw) launch_transpose(0, static_cast<const uint8_t*>(x), ldx * 2, T, H, XT, Tp, Tw, &a, g_loss, g_lse, stream);
+  uint16_t* XT = reinterpret_cast<uint16_t*>(ws + off[1]);
+  if (dw) launch_transpose(a, XT, Tp, g_loss, g_lse, stream);
   for (int64_t v0 = 0; v0 < V; v0 += Vc) {
     const uint8_t* rows = static_cast<const uint8_t*>(w) + v0 * ldw * (wtype ? 1 : 2);
     const int64_t n = std::min(Vc, V - v0), np = up(n, 64);
     VocabGemm g{};
     g.a = rows;
     g.lda = ldw * (wtype ? 1 : 2);
-    if (wtype && !direct) {
-      uint16_t* e = reinterpret_cast<uint16_t*>(ws + off[6]);
+    if (wtype) {
+      uint16_t* e = reinterpret_cast<uint16_t*>(ws + off[4]);
       launch_expand(wtype, rows, ldw, n, H, e, stream);
       g.a = reinterpret_cast<const uint8_t*>(e);
       g.lda = H * 2;
@@ -1041,22 +1086,20 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
     g.lse = lse;
     g.g_loss = g_loss;
     g.g_lse = g_lse;
-    g.p = dx ? P : nullptr;
+    g.p = P;
     g.ldp = Vp;
-    g.pt = dw ? PT : nullptr;
-    g.ldpt = Tp;
-    launch_gemm<VE_PROB>(g, direct ? wtype : 0, direct ? std::min(vocab_bm(n, T), 128) : vocab_bm(n, T), 1, stream);
+    launch_gemm<VE_PROB>(g, 0, vocab_bm(n, T), 1, stream);
     if (dx) {
-      launch_transpose(wtype, rows, ldw * (wtype ? 1 : 2), n, H, WT, Vp, np, nullptr, nullptr, nullptr, stream);
       VocabGemm d{};
-      d.a = reinterpret_cast<const uint8_t*>(WT);
-      d.lda = Vp * 2;
+      d.a = g.a;
+      d.lda = g.lda;
       d.na = (int)H;
       d.b = reinterpret_cast<const uint8_t*>(P);
       d.ldb = Vp * 2;
       d.nb = (int)T;
       d.K = (int)np;
-      d.sum = reinterpret_cast<float*>(ws + off[4]);
+      d.kr = (int)n;
+      d.sum = reinterpret_cast<float*>(ws + off[2]);
       d.ldsum = H;
       d.first = v0 == 0;
       d.last = v0 + Vc >= V;
@@ -1066,7 +1109,7 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
       const int slices = (int)cdiv(np, (int64_t)plan.kslice);
       if (slices > 1) {
         d.kslice = plan.kslice;
-        d.slices = reinterpret_cast<float*>(ws + off[5]);
+        d.slices = reinterpret_cast<float*>(ws + off[3]);
       }
       launch_gemm<VE_SUM>(d, 0, plan.bm, slices, stream);
       if (slices > 1)
@@ -1077,10 +1120,11 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
       d.a = reinterpret_cast<const uint8_t*>(XT);
       d.lda = Tp * 2;
       d.na = (int)H;
-      d.b = reinterpret_cast<const uint8_t*>(PT);
-      d.ldb = Tp * 2;
+      d.b = reinterpret_cast<const uint8_t*>(P);
+      d.ldb = Vp * 2;
       d.nb = (int)n;
       d.K = (int)Tw;
+      d.kr = (int)T;
       d.y = static_cast<uint16_t*>(dw) + v0 * lddw;
       d.ldy = lddw;
       launch_gemm<VE_STORE>(d, 0, vocab_bm(H, n), 1, stream);
