@@ -578,12 +578,13 @@ __global__ __launch_bounds__(256) void vocab_slices_kernel(const VocabGemm p, in
 // the others registers).
 constexpr int kBThreads = 256;
 
-template <int EPI, bool TAIL>
+template <int EPI, int BM, bool TAIL>
 __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm args) {
-  constexpr int BN = kVN, BM = 256, NI = 4, MJ = 4;
+  constexpr int BN = kVN, NI = 4, MJ = BM / 64, BI = 2 * MJ;  // BI: a wavefront's copies of B rows per stage
   constexpr uint32_t SLOT = BN * 128, RING = 5 * SLOT;
   constexpr bool TRA = tr_a(EPI), TRB = tr_b(EPI);
   constexpr int TB = 512;  // bytes of a K row of the operand across K
+  static_assert(!TRB || BM == 256, "K rows of 512 bytes");
   __shared__ __align__(1024) uint8_t smem[RING];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
   VocabGemm p = args;
@@ -676,12 +677,12 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
 #pragma unroll
     for (int j = 0; j < 8; ++j) copy_a(asrc(0), j, end_of(0), dst(0) + j * 4096);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) copy_b(bsrc(0), j, end_of(0), dst(SLOT) + j * 4096);
+    for (int j = 0; j < BI; ++j) copy_b(bsrc(0), j, end_of(0), dst(SLOT) + j * 4096);
 #pragma unroll
     for (int j = 0; j < 8; ++j) copy_a(asrc(1), j, end_of(1), dst(2 * SLOT) + j * 4096);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) copy_b(bsrc(1), j, end_of(1), dst(3 * SLOT) + j * 4096);
-    wait_copies_upto<12>();  // the first stage
+    for (int j = 0; j < BI / 2; ++j) copy_b(bsrc(1), j, end_of(1), dst(3 * SLOT) + j * 4096);
+    wait_copies_upto<8 + BI / 2>();  // the first stage
     stage_barrier();
     read_w(0, 0);
     read_x(SLOT, 0);
@@ -690,7 +691,7 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
       const uint32_t sb = wrap(sa + SLOT), sa1 = wrap(sa + 2 * SLOT), sb1 = wrap(sa + 3 * SLOT), sa2 = wrap(sa + 4 * SLOT);
       const uint8_t *b1 = bsrc(s + 1), *a2 = asrc(s + 2), *b2 = bsrc(s + 2);
       const uint32_t e1 = end_of(s + 1), e2 = end_of(s + 2);
-      const uint32_t db1 = dst(sb1) + 16384, da2 = dst(sa2), db2 = dst(sa);
+      const uint32_t db1 = dst(sb1) + BI / 2 * 4096, da2 = dst(sa2), db2 = dst(sa);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if (q == 3) {
@@ -701,9 +702,9 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
         for (int i = 0; i < NI; ++i) {
           if (i == 0) read_w(q < 3 ? sa : sa1, (q + 1) & 3);
           if (i == 1) read_x(q < 3 ? sb : sb1, (q + 1) & 3);
-          if (q == 0) copy_b(b1, 4 + i, e1, db1 + i * 4096);
-          else if (q < 3) copy_a(a2, 4 * (q - 1) + i, e2, da2 + (4 * (q - 1) + i) * 4096);
-          else copy_b(b2, i, e2, db2 + i * 4096);
+          if (q == 1 || q == 2) copy_a(a2, 4 * (q - 1) + i, e2, da2 + (4 * (q - 1) + i) * 4096);
+          else if (i < BI / 2 && q == 0) copy_b(b1, BI / 2 + i, e1, db1 + i * 4096);
+          else if (i < BI / 2) copy_b(b2, i, e2, db2 + i * 4096);
           mma_row(q, i);
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -720,7 +721,7 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       lds_copy16(in ? as + aoff[j] : z, cw + j * 4096);
-      lds_copy16(in ? bs + boff[j] : z, cw + SLOT + j * 4096);
+      if (j < BI) lds_copy16(in ? bs + boff[j] : z, cw + SLOT + j * 4096);
     }
     wait_copies_upto<0>();
     __syncthreads();
@@ -822,14 +823,18 @@ __global__ __launch_bounds__(256) void vocab_transpose_kernel(const uint8_t* src
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
+// Cost of a tile: 256 x 256 and 256 x 192 by four wavefronts, 256 x 128 by eight
+int tile_cost(int bm) { return bm == 256 ? 150 : (bm == 192 ? 122 : 100); }
+
 // Tile of a problem of na A rows and nb B rows, by the rounds over the 256 CUs
-// that it takes: 256 x 256 (big), or 256 x 128 / 64.
-int vocab_bm(int64_t na, int64_t nb) {
+// that it takes
+int vocab_bm(int64_t na, int64_t nb, bool dw = false) {
   const int64_t n = cdiv(na, (int64_t)kVN);
   if (nb <= 64) return 64;
   if (nb <= 128) return 128;
-  auto rounds = [&](int64_t bm) { return cdiv(n * cdiv(nb, bm), (int64_t)256); };
-  return rounds(256) * 150 <= rounds(128) * 100 ? 256 : 128;
+  auto cost = [&](int bm) { return cdiv(n * cdiv(nb, (int64_t)bm), (int64_t)256) * tile_cost(bm); };
+  const int big = dw || cost(256) <= cost(192) ? 256 : 192;
+  return cost(big) <= cost(128) ? big : 128;
 }
 
 template <int EPI, int BM, int AT>
@@ -846,8 +851,12 @@ void launch_gemm(VocabGemm g, int at, int bm, int slices, hipStream_t st) {
   const dim3 grid((unsigned)(cdiv(g.n_tiles * g.m_tiles, kXcds) * kXcds), (unsigned)slices);
   if (bm == 256) {
     // (the K of dx and dw is a multiple of 64)
-    if (kLogits && g.K % 64) hipLaunchKernelGGL((vocab_big_kernel<EPI, kLogits>), grid, dim3(kBThreads), 0, st, g);
-    else hipLaunchKernelGGL((vocab_big_kernel<EPI, false>), grid, dim3(kBThreads), 0, st, g);
+    if (kLogits && g.K % 64) hipLaunchKernelGGL((vocab_big_kernel<EPI, 256, kLogits>), grid, dim3(kBThreads), 0, st, g);
+    else hipLaunchKernelGGL((vocab_big_kernel<EPI, 256, false>), grid, dim3(kBThreads), 0, st, g);
+  } else if (!tr_b(EPI) && bm == 192) {
+    constexpr int E = tr_b(EPI) ? VE_SUM : EPI;
+    if (kLogits && g.K % 64) hipLaunchKernelGGL((vocab_big_kernel<E, 192, kLogits>), grid, dim3(kBThreads), 0, st, g);
+    else hipLaunchKernelGGL((vocab_big_kernel<E, 192, false>), grid, dim3(kBThreads), 0, st, g);
   } else if (at == 0) {
     bm == 128 ? launch_small<EPI, 128, 0>(g, grid, st) : launch_small<EPI, 64, 0>(g, grid, st);
   } else if constexpr (EPI == VE_LSE) {
@@ -950,7 +959,9 @@ struct DxPlan {
 };
 DxPlan dx_plan(int64_t T, int64_t H, int64_t K) {
   DxPlan d{};
-  d.bm = T <= 64 ? 64 : (T <= 128 || cdiv(T, (int64_t)256) * 150 > cdiv(T, (int64_t)128) * 100 ? 128 : 256);
+  auto cost = [&](int bm) { return cdiv(T, (int64_t)bm) * tile_cost(bm); };
+  const int big = cost(256) <= cost(192) ? 256 : 192;
+  d.bm = T <= 64 ? 64 : (T <= 128 || cost(128) < cost(big) ? 128 : big);
   const int64_t tiles = cdiv(H, (int64_t)kVN) * cdiv(T, (int64_t)d.bm);
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(256 / tiles, K / 512));
   d.kslice = (int)up(cdiv(K, want), 64);
@@ -1127,7 +1138,7 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
       d.kr = (int)T;
       d.y = static_cast<uint16_t*>(dw) + v0 * lddw;
       d.ldy = lddw;
-      launch_gemm<VE_STORE>(d, 0, vocab_bm(H, n), 1, stream);
+      launch_gemm<VE_STORE>(d, 0, vocab_bm(H, n, true), 1, stream);
     }
   }
   return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
