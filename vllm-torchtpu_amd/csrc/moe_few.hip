@@ -294,9 +294,10 @@ __device__ __forceinline__ void few_tables(FewTables& tb, const int32_t* ids, ui
   __syncthreads();
 }
 
-constexpr int kUpWaves = 4, kUpAhead = 3;
+constexpr int kUpWaves = 4;
 
-template <int F, int S>
+// A: steps in flight per wavefront
+template <int F, int S, int A>
 __global__ __launch_bounds__(kUpWaves * 64, 3) void few_up_kernel(const FewParams p) {
   constexpr int ROWS = Fmt<F>::kRows, M = Fmt<F>::kMfma;
   __shared__ FewTables tb;
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(kUpWaves * 64, 3) void few_up_kernel(const FewParam
   const int rb = Fmt<F>::row_bytes(p.H), sb = Fmt<F>::scale_bytes(p.H, p.group_shift);
   // steps per item, the same for every wavefront (those past a row's end load
   // nothing and add zeros)
-  const int chunks = cdiv(cdiv(cdiv(rb, 128), kUpWaves), kUpAhead);
+  const int chunks = cdiv(cdiv(cdiv(rb, 128), kUpWaves), A);
   const int r = lane & 15, kg = lane >> 4;
   const rsrc_t xr = make_rsrc(p.x, (int64_t)p.T * p.ldx * 2);
 
@@ -351,7 +352,7 @@ __global__ __launch_bounds__(kUpWaves * 64, 3) void few_up_kernel(const FewParam
       sr[t] = make_rsrc(static_cast<const uint8_t*>(p.s1) + row * sb, (int64_t)16 * sb);
     }
   };
-  Step<F, 2> st[kUpAhead];
+  Step<F, 2> st[A];
   const uint32_t wlane = (uint32_t)((lane >> 3) * rb + (lane & 7) * 16), slane = (uint32_t)(r * sb);
   auto issue = [&](Step<F, 2>& d, int i, bool live) {
     const int line = (wave + kUpWaves * i) * 128;  // byte of the row
@@ -371,7 +372,7 @@ __global__ __launch_bounds__(kUpWaves * 64, 3) void few_up_kernel(const FewParam
   seek(it0);
   // (in this order: the loop's waits count the loads behind a step's own)
 #pragma unroll
-  for (int u = 0; u < kUpAhead; ++u) {
+  for (int u = 0; u < A; ++u) {
     issue(st[u], u, true);
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -397,9 +398,9 @@ __global__ __launch_bounds__(kUpWaves * 64, 3) void few_up_kernel(const FewParam
       const bool more = c + 1 < chunks, next = item + 1 < it1;
       if (!more && next) seek(item + 1);
 #pragma unroll
-      for (int u = 0; u < kUpAhead; ++u) {
-        consume<F, 2>(st[u], tr[wave], slane, (wave + kUpWaves * (c * kUpAhead + u)) * 8, p.group_shift, acc);
-        issue(st[u], (more ? (c + 1) * kUpAhead : 0) + u, more || next);
+      for (int u = 0; u < A; ++u) {
+        consume<F, 2>(st[u], tr[wave], slane, (wave + kUpWaves * (c * A + u)) * 8, p.group_shift, acc);
+        issue(st[u], (more ? (c + 1) * A : 0) + u, more || next);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -433,13 +434,11 @@ __global__ __launch_bounds__(kUpWaves * 64, 3) void few_up_kernel(const FewParam
   }
 }
 
-constexpr int kDownAhead = 4;
+constexpr int kDownAhead = 2, kDownWaves = 8;
 
-// NW wavefronts: 16 where there are no more output tiles than CUs, else 8 (two
-// workgroups per CU)
-template <int F, int NW>
-__global__ __launch_bounds__(NW * 64) void few_down_kernel(const FewParams p) {
-  constexpr int ROWS = Fmt<F>::kRows, M = Fmt<F>::kMfma;
+template <int F>
+__global__ __launch_bounds__(kDownWaves * 64) void few_down_kernel(const FewParams p) {
+  constexpr int NW = kDownWaves, ROWS = Fmt<F>::kRows, M = Fmt<F>::kMfma;
   __shared__ FewTables tb;
   __shared__ __align__(16) uint4 tr[NW][128];
   __shared__ __align__(16) f32x4 tot[NW][64];  // [token][4 columns x 4]
@@ -561,8 +560,17 @@ __global__ __launch_bounds__(NW * 64) void few_down_kernel(const FewParams p) {
 
 template <int F, int S>
 void launch_up(const FewParams& p, hipStream_t st) {
+  // as many workgroups as fit (three per CU; 512 or 1536 instead: 118 or 119 us for
+  // 113 with 16 tokens, MXFP4, 128 x 2880 x 2880; 207 or 212 for 189 with 8, NVFP4,
+  // 256 x 2048 x 7168)
   const int64_t items = (int64_t)std::min(p.E, p.T * p.topk) * (p.I / 16);
-  hipLaunchKernelGGL((few_up_kernel<F, S>), dim3((unsigned)std::min<int64_t>(items, 768)), dim3(kUpWaves * 64), 0, st, p);
+  const dim3 grid((unsigned)std::min<int64_t>(items, 768)), block(kUpWaves * 64);
+  // three steps in flight, or two where three leave more of them empty (the NVFP4
+  // case, 7 lines per wavefront: 189 us by three, 176 by two; the MXFP4 one, 3
+  // lines: 113 and 121; four: 210, 162)
+  const int lines = cdiv(cdiv(Fmt<F>::row_bytes(p.H), 128), kUpWaves);
+  if (cdiv(lines, 2) * 2 < cdiv(lines, 3) * 3) hipLaunchKernelGGL((few_up_kernel<F, S, 2>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((few_up_kernel<F, S, 3>), grid, block, 0, st, p);
 }
 
 template <int F>
@@ -571,9 +579,7 @@ void launch_few(const FewParams& p, hipStream_t st) {
   if (S <= 2) launch_up<F, 2>(p, st);
   else if (S == 4) launch_up<F, 4>(p, st);
   else launch_up<F, 8>(p, st);
-  const dim3 grid((unsigned)(p.H / 16));
-  if (p.H / 16 <= 256) hipLaunchKernelGGL((few_down_kernel<F, 16>), grid, dim3(16 * 64), 0, st, p);
-  else hipLaunchKernelGGL((few_down_kernel<F, 8>), grid, dim3(8 * 64), 0, st, p);
+  hipLaunchKernelGGL((few_down_kernel<F>), dim3((unsigned)(p.H / 16)), dim3(kDownWaves * 64), 0, st, p);
 }
 
 int64_t few_layout(int64_t R, int64_t I, int64_t (&off)[2]) {

@@ -823,14 +823,17 @@ __global__ __launch_bounds__(256) void vocab_transpose_kernel(const uint8_t* src
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Cost of a tile: 256 x 256 and 256 x 192 by four wavefronts, 256 x 128 by eight
-int tile_cost(int bm) { return bm == 256 ? 150 : (bm == 192 ? 122 : 100); }
+// What a round of tiles over the 256 CUs costs: 256 x 256 and 256 x 192 by four
+// wavefronts, 256 x 128 by eight. (333 tokens x 50021 x 2880, 2, 2 and 3 rounds:
+// logits 142, 118, 136 us; probabilities 162, 128, 147.)
+int tile_cost(int bm) { return bm == 256 ? 160 : (bm == 192 ? 130 : 100); }
 
-// Tile of a problem of na A rows and nb B rows, by the rounds over the 256 CUs
-// that it takes
+// Tile of a problem of na A rows and nb B rows, by the rounds that it takes. (dw
+// has no 192 and no 64: K rows of P are copied by 256 or 512 bytes. 333 tokens,
+// H 2880: 178 us by 256 x 256, 195 by 256 x 128.)
 int vocab_bm(int64_t na, int64_t nb, bool dw = false) {
   const int64_t n = cdiv(na, (int64_t)kVN);
-  if (nb <= 64) return 64;
+  if (nb <= 64 && !dw) return 64;
   if (nb <= 128) return 128;
   auto cost = [&](int bm) { return cdiv(n * cdiv(nb, (int64_t)bm), (int64_t)256) * tile_cost(bm); };
   const int big = dw || cost(256) <= cost(192) ? 256 : 192;
@@ -858,7 +861,9 @@ void launch_gemm(VocabGemm g, int at, int bm, int slices, hipStream_t st) {
     if (kLogits && g.K % 64) hipLaunchKernelGGL((vocab_big_kernel<E, 192, kLogits>), grid, dim3(kBThreads), 0, st, g);
     else hipLaunchKernelGGL((vocab_big_kernel<E, 192, false>), grid, dim3(kBThreads), 0, st, g);
   } else if (at == 0) {
-    bm == 128 ? launch_small<EPI, 128, 0>(g, grid, st) : launch_small<EPI, 64, 0>(g, grid, st);
+    if constexpr (EPI == VE_SUM) launch_small<EPI, 64, 0>(g, grid, st);
+    else if constexpr (EPI == VE_STORE) launch_small<EPI, 128, 0>(g, grid, st);
+    else bm == 128 ? launch_small<EPI, 128, 0>(g, grid, st) : launch_small<EPI, 64, 0>(g, grid, st);
   } else if constexpr (EPI == VE_LSE) {
     if (at == 3) bm == 128 ? launch_small<EPI, 128, 3>(g, grid, st) : launch_small<EPI, 64, 3>(g, grid, st);
     else if (at == 4) bm == 128 ? launch_small<EPI, 128, 4>(g, grid, st) : launch_small<EPI, 64, 4>(g, grid, st);
@@ -896,7 +901,7 @@ void launch_transpose(const LossArgs& a, uint16_t* out, int64_t ldo, const float
 // sizes whose tile counts, and the threads of their grids, fit 32 bits
 constexpr int64_t kMaxTokens = (int64_t)1 << 20, kMaxVocab = (int64_t)1 << 24, kMaxHidden = (int64_t)1 << 16;
 
-constexpr int64_t kDirectTokens = 512;
+constexpr int64_t kDirectTokens = 1536;
 
 bool loss_sizes_ok(int64_t T, int64_t V, int64_t H) {
   return T >= 0 && T <= kMaxTokens && V > 0 && V <= kMaxVocab && H > 0 && H <= kMaxHidden && H % 8 == 0 &&
@@ -916,16 +921,16 @@ int loss_args_ok(const LossArgs& a) {
 
 // Whether codes go to the tiles as they are stored: whole 16-byte chunks, and
 // not so many tokens that expanding a piece first, for the 256 x 256 tiles, is
-// the shorter way
+// the shorter way (e4m3, 131072 x 4096: 512 tokens 0.54 ms as they are, 0.86
+// expanded; 1024 1.07, 1.22; 1536 1.61, 1.78; 2048 2.15, 2.14)
 bool codes_direct(const void* w, int64_t ldw, int64_t H, int64_t T) {
   return T <= kDirectTokens && H % 16 == 0 && ldw % 16 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
 }
 
-// Table rows of a piece of the forward pass: all of a bf16 table (read where
-// it lies), 16 or 128 MB of expanded rows of a 1-byte one
-int64_t loss_piece(int64_t T, int64_t V, int64_t H) {
-  const int64_t values = T <= 128 ? 8 << 20 : 64 << 20;
-  return std::min(up(V, kVN), std::max<int64_t>(up(values / H, kVN), kVN));
+// Table rows of a piece of the forward pass where codes are expanded first: 128
+// MB of them
+int64_t loss_piece(int64_t V, int64_t H) {
+  return std::min(up(V, kVN), std::max<int64_t>((int64_t)(64 << 20) / H / kVN * kVN, kVN));
 }
 
 int64_t loss_layout(int64_t T, int64_t V, int64_t H, int wtype, int64_t (&off)[3]) {
@@ -935,7 +940,7 @@ int64_t loss_layout(int64_t T, int64_t V, int64_t H, int wtype, int64_t (&off)[3
   off[1] = at;  // the targets' logits
   at += up(T * 4, 256);
   off[2] = at;  // expanded rows
-  if (wtype) at += up(loss_piece(T, V, H) * H * 2, 256);
+  if (wtype) at += up(loss_piece(V, H) * H * 2, 256);
   return at;
 }
 
@@ -946,22 +951,19 @@ int64_t grad_piece(int64_t T, int64_t V, int64_t H, int wtype) {
   return std::min(up(V, kVN), std::max<int64_t>((int64_t)(64 << 20) / width / kVN * kVN, kVN));
 }
 
-// Row pitch (bf16) of a buffer of n columns, n a multiple of 64: an odd number of
-// 128-byte lines, so that the rows of a tile do not share memory channels
-int64_t odd_pitch(int64_t n) { return n % 128 ? n : n + 64; }
-
-// dx of a piece: T x H outputs, a K axis as long as the piece. Tile height by
-// the padded rows' cost, and as many K slices as fill the CUs, of at least 512
-// (333 tokens, H 2880, pieces of 23296 rows: 24 tiles of 256 x 256 without a
-// split 458 us).
+// dx of a piece: T x H outputs, a K axis as long as the piece. As many K slices
+// as fill the CUs, of at least 512 (V 50021, H 2880 without the split: 489 us at
+// 64 tokens, 685 at 333; with it 87 and 104). Tile height by the padded rows'
+// cost; 64 by eight wavefronts up to 64 tokens (1, 64 tokens: 72, 87 us; of 192:
+// 84, 94), and above no 128 by eight (100, 333 tokens: 98, 200 us; of 192: 100,
+// 104): eight wavefronts' transposed reads keep LDS busy.
 struct DxPlan {
   int bm, slices, kslice;
 };
 DxPlan dx_plan(int64_t T, int64_t H, int64_t K) {
   DxPlan d{};
   auto cost = [&](int bm) { return cdiv(T, (int64_t)bm) * tile_cost(bm); };
-  const int big = cost(256) <= cost(192) ? 256 : 192;
-  d.bm = T <= 64 ? 64 : (T <= 128 || cost(128) < cost(big) ? 128 : big);
+  d.bm = T <= 64 ? 64 : (cost(256) <= cost(192) ? 256 : 192);
   const int64_t tiles = cdiv(H, (int64_t)kVN) * cdiv(T, (int64_t)d.bm);
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(256 / tiles, K / 512));
   d.kslice = (int)up(cdiv(K, want), 64);
@@ -971,13 +973,13 @@ DxPlan dx_plan(int64_t T, int64_t H, int64_t K) {
 
 // P, x transposed, float32 sums, K slices, expanded rows
 int64_t grad_layout(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw, int64_t (&off)[5]) {
-  const int64_t Vc = grad_piece(T, V, H, wtype), Vp = odd_pitch(Vc), Tp = odd_pitch(up(T, 64));
+  const int64_t Vc = grad_piece(T, V, H, wtype), Tw = up(T, 64);
   const bool pieces = Vc < V;
   int64_t at = 0;
   off[0] = at;
-  at += up(T * Vp * 2, 256);
+  at += up(T * Vc * 2, 256);
   off[1] = at;
-  if (need_dw) at += up(H * Tp * 2, 256);
+  if (need_dw) at += up(H * Tw * 2, 256);
   off[2] = at;
   if (need_dx && pieces) at += up(T * H * 4, 256);
   off[3] = at;
@@ -1023,7 +1025,7 @@ extern "C" int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void
   g.part = reinterpret_cast<float2*>(ws + off[0]);
   g.tgt = reinterpret_cast<float*>(ws + off[1]);
   const bool direct = wtype && codes_direct(w, ldw, H, T);
-  const int64_t Vc = wtype && !direct ? loss_piece(T, V, H) : V;
+  const int64_t Vc = wtype && !direct ? loss_piece(V, H) : V;
   for (int64_t v0 = 0; v0 < V; v0 += Vc) {
     const uint8_t* rows = static_cast<const uint8_t*>(w) + v0 * ldw * (wtype ? 1 : 2);
     const int64_t n = std::min(Vc, V - v0);
@@ -1067,10 +1069,10 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
   int64_t off[5];
   if (!workspace || ws_bytes < grad_layout(T, V, H, wtype, dx != nullptr, dw != nullptr, off)) return QMOE_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const int64_t Vc = grad_piece(T, V, H, wtype), Vp = odd_pitch(Vc), Tw = up(T, 64), Tp = odd_pitch(Tw);
+  const int64_t Vc = grad_piece(T, V, H, wtype), Tw = up(T, 64);
   uint16_t* P = reinterpret_cast<uint16_t*>(ws + off[0]);
   uint16_t* XT = reinterpret_cast<uint16_t*>(ws + off[1]);
-  if (dw) launch_transpose(a, XT, Tp, g_loss, g_lse, stream);
+  if (dw) launch_transpose(a, XT, Tw, g_loss, g_lse, stream);
   for (int64_t v0 = 0; v0 < V; v0 += Vc) {
     const uint8_t* rows = static_cast<const uint8_t*>(w) + v0 * ldw * (wtype ? 1 : 2);
     const int64_t n = std::min(Vc, V - v0), np = up(n, 64);
@@ -1098,7 +1100,7 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
     g.g_loss = g_loss;
     g.g_lse = g_lse;
     g.p = P;
-    g.ldp = Vp;
+    g.ldp = Vc;
     launch_gemm<VE_PROB>(g, 0, vocab_bm(n, T), 1, stream);
     if (dx) {
       VocabGemm d{};
@@ -1106,7 +1108,7 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
       d.lda = g.lda;
       d.na = (int)H;
       d.b = reinterpret_cast<const uint8_t*>(P);
-      d.ldb = Vp * 2;
+      d.ldb = Vc * 2;
       d.nb = (int)T;
       d.K = (int)np;
       d.kr = (int)n;
@@ -1129,10 +1131,10 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
     if (dw) {
       VocabGemm d{};
       d.a = reinterpret_cast<const uint8_t*>(XT);
-      d.lda = Tp * 2;
+      d.lda = Tw * 2;
       d.na = (int)H;
       d.b = reinterpret_cast<const uint8_t*>(P);
-      d.ldb = Vp * 2;
+      d.ldb = Vc * 2;
       d.nb = (int)n;
       d.K = (int)Tw;
       d.kr = (int)T;
