@@ -364,9 +364,10 @@ __device__ __forceinline__ bf16x8 codes8_to_bf16(uint32_t lo, uint32_t hi) {
 
 // Tiles of 256 A rows x BM B rows (64 or 128) by eight wavefronts, two per SIMD,
 // for problems that the 256 x 256 tiles below would leave CUs idle or pad, and
-// for few tokens, where reading the table is all that counts: with codes (AT 3
-// e4m3, 4 int8, 5 e5m2) the table is read as it is stored and expanded
-// between LDS and the matrix cores. Stages of 64 k of every row in a ring of
+// for few tokens, where reading the table is all that counts (one token, 131072
+// x 4096 bf16: 169 us, 6.4 TB/s; 16 tokens, 131072 x 7168 e4m3: 177 us, 5.3
+// TB/s): with codes (AT 3 e4m3, 4 int8, 5 e5m2) the table is read as it is stored
+// and expanded between LDS and the matrix cores. Stages of 64 k of every row in a ring of
 // as many as fit.
 template <int EPI, int BM, int AT>
 __global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGemm args) {
@@ -559,8 +560,8 @@ __global__ __launch_bounds__(256) void vocab_slices_kernel(const VocabGemm p, in
   else *reinterpret_cast<uint2*>(p.y + row * p.ldy + c) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
 
-// The same product in tiles of 256 x 256 by four wavefronts of 4 x 4 blocks (one
-// per SIMD, the sums in accumulation registers). A wavefront of 64 x 128 reads
+// The same product in tiles of 256 x 256 (or 192: 4 x 3 blocks) by four wavefronts
+// of 4 x 4 blocks (one per SIMD, the sums in accumulation registers). A wavefront of 64 x 128 reads
 // 24 KB of operands from LDS per 32 MFMAs, one of 128 x 128 32 KB per 64: with
 // eight of the former per CU the reads and the copies' writes fill LDS's 128
 // bytes per cycle, which is what bounds that kernel.
@@ -573,16 +574,23 @@ __global__ __launch_bounds__(256) void vocab_slices_kernel(const VocabGemm p, in
 // address unit busy, and the matrix cores idle, for half a step. Whole
 // 128-byte lines per row: with 64-byte rows in a ring of four smaller stages the
 // second half of a line is asked for while the first is pending, and the L1
-// stalls on it (dw of 4096 tokens, 16384 x 4096: 458 us; these: see above).
+// stalls on it (dw of 4096 tokens, 16384 x 4096: 458 us; by lines 417). Codes
+// (AT) take 64 bytes of a row and are expanded on their way to the matrix cores.
+//
+// 4096 tokens: logits of 131072 x 4096 3.11 ms, 1.41 PFLOP/s; of 16384 rows the
+// probabilities 454 us, 1.21 PFLOP/s (their stores wait for nothing, but no
+// product runs meanwhile), dx 397, 1.38, dw 418, 1.31. A plain product of 8192 on
+// each side by the library reaches 1.25 to 1.54 on the same card.
 // TAIL: K is not a multiple of 64 (an instance of its own: the extra stage costs
 // the others registers).
 constexpr int kBThreads = 256;
 
-template <int EPI, int BM, bool TAIL>
+template <int EPI, int BM, int AT, bool TAIL>
 __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm args) {
   constexpr int BN = kVN, NI = 4, MJ = BM / 64, BI = 2 * MJ;  // BI: a wavefront's copies of B rows per stage
   constexpr uint32_t SLOT = BN * 128, RING = 5 * SLOT;
   constexpr bool TRA = tr_a(EPI), TRB = tr_b(EPI);
+  constexpr int AB = AT ? 64 : 128, AI = AT ? 4 : 8;  // bytes of an A row per stage, a wavefront's copies of them
   constexpr int TB = 512;  // bytes of a K row of the operand across K
   static_assert(!TRB || BM == 256, "K rows of 512 bytes");
   __shared__ __align__(1024) uint8_t smem[RING];
@@ -600,7 +608,7 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
   // the slot of chunk c of row r is c ^ vg_swz(r)); wavefront w moves the row
   // groups w, w + 4, ... of both operands; rows past the end repeat the last
   // one (their products are dropped)
-  const int chunk16 = (lane & 7) ^ ((lane >> 3) ^ (wave & 1));
+  const int chunk16 = (lane & 7) ^ ((lane >> 3) ^ (wave & 1)), achunk = (lane & 3) ^ ((lane >> 4) & 3);
   const uint8_t* abase = p.a + (int64_t)n0 * p.lda;
   const uint8_t* bbase = p.b + (int64_t)m0 * p.ldb;
   // (the operand across K: 2 K rows per instruction; K rows past the last repeat
@@ -609,7 +617,7 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
   const uint32_t tcol = TRA ? (uint32_t)min(tchunk, arows / 8 - 1) * 16 : (uint32_t)tchunk * 16;
   if constexpr (TRA) abase = p.a + n0 * 2;
   if constexpr (TRB) bbase = p.b + m0 * 2;
-  const int64_t astep = TRA ? 64 * p.lda : 128, bstep = TRB ? 64 * p.ldb : 128;
+  const int64_t astep = TRA ? 64 * p.lda : AB, bstep = TRB ? 64 * p.ldb : 128;
   const uint32_t tld = (uint32_t)(TRA ? p.lda : p.ldb);
   uint32_t aoff[8], boff[8];
 #pragma unroll
@@ -617,6 +625,10 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
     const int r = (wave + 4 * j) * 8 + (lane >> 3);
     const uint32_t t = (uint32_t)(2 * (wave + 4 * j) + trow) * tld + tcol;
     aoff[j] = TRA ? t : (uint32_t)min(r, arows - 1) * (uint32_t)p.lda + chunk16 * 16;
+    if constexpr (AT) {  // (16 rows x 64 bytes, as in the kernel above)
+      const int ra = ((wave + 4 * j) & 15) * 16 + (lane >> 2);
+      aoff[j] = (uint32_t)min(ra, arows - 1) * (uint32_t)p.lda + achunk * 16;
+    }
     boff[j] = TRB ? t : (uint32_t)min(r, brows - 1) * (uint32_t)p.ldb + chunk16 * 16;
   }
   const int KF = p.K / 64;  // whole stages
@@ -635,6 +647,13 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
       for (int i = 0; i < NI; ++i) wf[q & 1][i].u = tr_read<TB>(smem + slot + q * 16 * TB + (tlane ^ i * 64));
       return;
     }
+    if constexpr (AT) {  // 16 codes: of this step and the next
+      if (q & 1) return;
+      const uint8_t* b = smem + slot + wpo / 2 + (((q + kh) ^ (rl >> 2)) & 3) * 16;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) wf[q / 2][i].u = *reinterpret_cast<const uint4*>(b + i * 2048);
+      return;
+    }
     const uint8_t* b = smem + slot + wpo + ((2 * q + kh) ^ vg_swz(rl)) * 16;
 #pragma unroll
     for (int i = 0; i < NI; ++i) wf[q & 1][i].u = *reinterpret_cast<const uint4*>(b + i * 4096);
@@ -645,7 +664,8 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
       for (int j = 0; j < MJ; ++j) xf[q & 1][j].u = tr_read<TB>(smem + slot + q * 16 * TB + (tlane ^ j * 128));
       return;
     }
-    const uint8_t* b = smem + slot + xpo + ((2 * q + kh) ^ vg_swz(rl)) * 16;
+    const int c = AT ? 4 * (q / 2) + 2 * kh + (q & 1) : 2 * q + kh;
+    const uint8_t* b = smem + slot + xpo + (c ^ vg_swz(rl)) * 16;
 #pragma unroll
     for (int j = 0; j < MJ; ++j) xf[q & 1][j].u = *reinterpret_cast<const uint4*>(b + j * 8192);
   };
@@ -657,9 +677,16 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
   auto mma_row = [&](int q, int i) {
+    bf16x8 a;
+    if constexpr (AT) {
+      const uint4 c = wf[q / 2][i].u;
+      a = q & 1 ? codes8_to_bf16<AT>(c.z, c.w) : codes8_to_bf16<AT>(c.x, c.y);
+    } else {
+      a = wf[q & 1][i].v;
+    }
 #pragma unroll
     for (int j = 0; j < MJ; ++j)
-      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[q & 1][i].v, xf[q & 1][j].v, acc[i][j], 0, 0, 0);
+      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, xf[q & 1][j].v, acc[i][j], 0, 0, 0);
   };
   if (KF > 0) {
     // (stages past the last one copy it again, into slots nobody reads)
@@ -675,14 +702,14 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
     auto dst = [&](uint32_t slot) { return (uint32_t)__builtin_amdgcn_readfirstlane(cw + slot); };
     auto wrap = [](uint32_t slot) { return slot >= RING ? slot - RING : slot; };
 #pragma unroll
-    for (int j = 0; j < 8; ++j) copy_a(asrc(0), j, end_of(0), dst(0) + j * 4096);
+    for (int j = 0; j < AI; ++j) copy_a(asrc(0), j, end_of(0), dst(0) + j * 4096);
 #pragma unroll
     for (int j = 0; j < BI; ++j) copy_b(bsrc(0), j, end_of(0), dst(SLOT) + j * 4096);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) copy_a(asrc(1), j, end_of(1), dst(2 * SLOT) + j * 4096);
+    for (int j = 0; j < AI; ++j) copy_a(asrc(1), j, end_of(1), dst(2 * SLOT) + j * 4096);
 #pragma unroll
     for (int j = 0; j < BI / 2; ++j) copy_b(bsrc(1), j, end_of(1), dst(3 * SLOT) + j * 4096);
-    wait_copies_upto<8 + BI / 2>();  // the first stage
+    wait_copies_upto<AI + BI / 2>();  // the first stage
     stage_barrier();
     read_w(0, 0);
     read_x(SLOT, 0);
@@ -695,14 +722,16 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if (q == 3) {
-          wait_copies_upto<8>();  // stage s + 1 has landed
+          wait_copies_upto<AI>();  // stage s + 1 has landed
           stage_barrier();        // and everybody holds this stage's last operands
         }
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
           if (i == 0) read_w(q < 3 ? sa : sa1, (q + 1) & 3);
           if (i == 1) read_x(q < 3 ? sb : sb1, (q + 1) & 3);
-          if (q == 1 || q == 2) copy_a(a2, 4 * (q - 1) + i, e2, da2 + (4 * (q - 1) + i) * 4096);
+          if (q == 1 || q == 2) {
+            if (4 * (q - 1) + i < AI) copy_a(a2, 4 * (q - 1) + i, e2, da2 + (4 * (q - 1) + i) * 4096);
+          }
           else if (i < BI / 2 && q == 0) copy_b(b1, BI / 2 + i, e1, db1 + i * 4096);
           else if (i < BI / 2) copy_b(b2, i, e2, db2 + i * 4096);
           mma_row(q, i);
@@ -715,12 +744,12 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
     __syncthreads();
   }
   if constexpr (TAIL) {  // the last, partial stage: zeros behind the rows' ends
-    const uint8_t *as = abase + (int64_t)KF * 128, *bs = bbase + (int64_t)KF * 128;
-    const bool in = KF * 64 + chunk16 * 8 < p.K;
+    const uint8_t *as = abase + (int64_t)KF * AB, *bs = bbase + (int64_t)KF * 128;
+    const bool ain = KF * 64 + (AT ? achunk * 16 : chunk16 * 8) < p.K, in = KF * 64 + chunk16 * 8 < p.K;
     const uint8_t* z = reinterpret_cast<const uint8_t*>(kVocabZero);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      lds_copy16(in ? as + aoff[j] : z, cw + j * 4096);
+      if (j < AI) lds_copy16(ain ? as + aoff[j] : z, cw + j * 4096);
       if (j < BI) lds_copy16(in ? bs + boff[j] : z, cw + SLOT + j * 4096);
     }
     wait_copies_upto<0>();
@@ -845,21 +874,32 @@ void launch_small(const VocabGemm& g, dim3 grid, hipStream_t st) {
   hipLaunchKernelGGL((vocab_gemm_kernel<EPI, BM, AT>), grid, dim3(kVThreads), 0, st, g);
 }
 
+template <int EPI, int BM, int AT>
+void launch_big_at(const VocabGemm& g, dim3 grid, hipStream_t st) {
+  constexpr bool kLogits = EPI == VE_LSE || EPI == VE_PROB;  // (the K of dx and dw is a multiple of 64)
+  if (kLogits && g.K % 64) hipLaunchKernelGGL((vocab_big_kernel<EPI, BM, AT, kLogits>), grid, dim3(kBThreads), 0, st, g);
+  else hipLaunchKernelGGL((vocab_big_kernel<EPI, BM, AT, false>), grid, dim3(kBThreads), 0, st, g);
+}
+template <int EPI, int BM>
+void launch_big(const VocabGemm& g, int at, dim3 grid, hipStream_t st) {
+  if constexpr (EPI == VE_LSE) {
+    if (at == 3) return launch_big_at<EPI, BM, 3>(g, grid, st);
+    if (at == 4) return launch_big_at<EPI, BM, 4>(g, grid, st);
+    if (at == 5) return launch_big_at<EPI, BM, 5>(g, grid, st);
+  }
+  launch_big_at<EPI, BM, 0>(g, grid, st);
+}
+
 // at: type of the A rows, 0 bf16 or the codes' table type (logits)
 template <int EPI>
 void launch_gemm(VocabGemm g, int at, int bm, int slices, hipStream_t st) {
-  constexpr bool kLogits = EPI == VE_LSE || EPI == VE_PROB;
   g.n_tiles = cdiv(g.na, kVN);
   g.m_tiles = cdiv(g.nb, bm);
   const dim3 grid((unsigned)(cdiv(g.n_tiles * g.m_tiles, kXcds) * kXcds), (unsigned)slices);
   if (bm == 256) {
-    // (the K of dx and dw is a multiple of 64)
-    if (kLogits && g.K % 64) hipLaunchKernelGGL((vocab_big_kernel<EPI, 256, kLogits>), grid, dim3(kBThreads), 0, st, g);
-    else hipLaunchKernelGGL((vocab_big_kernel<EPI, 256, false>), grid, dim3(kBThreads), 0, st, g);
-  } else if (!tr_b(EPI) && bm == 192) {
-    constexpr int E = tr_b(EPI) ? VE_SUM : EPI;
-    if (kLogits && g.K % 64) hipLaunchKernelGGL((vocab_big_kernel<E, 192, kLogits>), grid, dim3(kBThreads), 0, st, g);
-    else hipLaunchKernelGGL((vocab_big_kernel<E, 192, false>), grid, dim3(kBThreads), 0, st, g);
+    launch_big<EPI, 256>(g, at, grid, st);
+  } else if (bm == 192) {
+    if constexpr (!tr_b(EPI)) launch_big<EPI, 192>(g, at, grid, st);
   } else if (at == 0) {
     if constexpr (EPI == VE_SUM) launch_small<EPI, 64, 0>(g, grid, st);
     else if constexpr (EPI == VE_STORE) launch_small<EPI, 128, 0>(g, grid, st);
@@ -901,7 +941,6 @@ void launch_transpose(const LossArgs& a, uint16_t* out, int64_t ldo, const float
 // sizes whose tile counts, and the threads of their grids, fit 32 bits
 constexpr int64_t kMaxTokens = (int64_t)1 << 20, kMaxVocab = (int64_t)1 << 24, kMaxHidden = (int64_t)1 << 16;
 
-constexpr int64_t kDirectTokens = 1536;
 
 bool loss_sizes_ok(int64_t T, int64_t V, int64_t H) {
   return T >= 0 && T <= kMaxTokens && V > 0 && V <= kMaxVocab && H > 0 && H <= kMaxHidden && H % 8 == 0 &&
@@ -919,12 +958,13 @@ int loss_args_ok(const LossArgs& a) {
   return 1;
 }
 
-// Whether codes go to the tiles as they are stored: whole 16-byte chunks, and
-// not so many tokens that expanding a piece first, for the 256 x 256 tiles, is
-// the shorter way (e4m3, 131072 x 4096: 512 tokens 0.54 ms as they are, 0.86
-// expanded; 1024 1.07, 1.22; 1536 1.61, 1.78; 2048 2.15, 2.14)
-bool codes_direct(const void* w, int64_t ldw, int64_t H, int64_t T) {
-  return T <= kDirectTokens && H % 16 == 0 && ldw % 16 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+// Whether codes go to the tiles as they are stored: whole 16-byte chunks, and of
+// int8, whose expansion takes the most instructions, not so many tokens that
+// expanding a piece first is the shorter way (int8, 32003 x 2880: 1024 tokens 227
+// us as stored, 248 expanded; 4096 893, 785; e4m3, 131072 x 4096: 192 tokens 0.19
+// ms, 0.78; 1024 0.92, 1.23; 4096 3.61, 3.90)
+bool codes_direct(const void* w, int wtype, int64_t ldw, int64_t H, int64_t T) {
+  return (wtype != 4 || T <= 1536) && H % 16 == 0 && ldw % 16 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
 }
 
 // Table rows of a piece of the forward pass where codes are expanded first: 128
@@ -1024,7 +1064,7 @@ extern "C" int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void
   g.ignore = ignore_index;
   g.part = reinterpret_cast<float2*>(ws + off[0]);
   g.tgt = reinterpret_cast<float*>(ws + off[1]);
-  const bool direct = wtype && codes_direct(w, ldw, H, T);
+  const bool direct = wtype && codes_direct(w, wtype, ldw, H, T);
   const int64_t Vc = wtype && !direct ? loss_piece(V, H) : V;
   for (int64_t v0 = 0; v0 < V; v0 += Vc) {
     const uint8_t* rows = static_cast<const uint8_t*>(w) + v0 * ldw * (wtype ? 1 : 2);
@@ -1041,7 +1081,7 @@ extern "C" int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void
     g.v0 = v0;
     g.row_scale = row_scale ? row_scale + v0 : nullptr;
     g.part_tile = (int)(v0 / kVN);
-    launch_gemm<VE_LSE>(g, direct ? wtype : 0, direct ? std::min(vocab_bm(n, T), 128) : vocab_bm(n, T), 1, stream);
+    launch_gemm<VE_LSE>(g, direct ? wtype : 0, vocab_bm(n, T), 1, stream);
   }
   hipLaunchKernelGGL(vocab_loss_join_kernel, dim3((unsigned)cdiv(T, (int64_t)4)), dim3(256), 0, stream, g.part,
                      (int)cdiv(V, (int64_t)kVN), (int)T, g.tgt, targets, targets_i64, ignore_index, V, loss, lse);
