@@ -349,15 +349,11 @@ __device__ __forceinline__ bf16x8 codes8_to_bf16(uint32_t lo, uint32_t hi) {
     r.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8((int)hi, 1.0f, false);
     r.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8((int)hi, 1.0f, true);
   } else {
-    // n + 128 by the byte conversions, then - 128
-    const uint32_t u = lo ^ 0x80808080u, w = hi ^ 0x80808080u;
+    const uint32_t d[2] = {lo, hi};
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < 4; ++k)
       r.h[k] = __builtin_convertvector(
-          f32x2{(float)((u >> (16 * k)) & 0xffu) - 128.0f, (float)((u >> (16 * k + 8)) & 0xffu) - 128.0f}, bf16x2);
-      r.h[2 + k] = __builtin_convertvector(
-          f32x2{(float)((w >> (16 * k)) & 0xffu) - 128.0f, (float)((w >> (16 * k + 8)) & 0xffu) - 128.0f}, bf16x2);
-    }
+          f32x2{(float)(int8_t)(d[k / 2] >> (16 * (k & 1))), (float)(int8_t)(d[k / 2] >> (16 * (k & 1) + 8))}, bf16x2);
   }
   return r.v;
 }
@@ -784,18 +780,6 @@ __global__ __launch_bounds__(256) void vocab_loss_join_kernel(const float2* part
   loss[t] = tg == ignore ? 0.0f : (tg >= 0 && tg < V ? all - tgt[t] : __builtin_nanf(""));
 }
 
-// 4 e4m3 / int8 / e5m2 codes -> 4 bf16 (exact)
-template <int WT>
-__device__ __forceinline__ uint2 codes4_to_bf16(uint32_t c) {
-  float f[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t b = (c >> (8 * i)) & 0xffu;
-    f[i] = WT == 3 ? e4m3_to_f32(b) : (WT == 4 ? (float)(int8_t)b : e5m2_to_f32(b));
-  }
-  return make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
-}
-
 // Rows of codes -> bf16 rows; 8 codes per thread
 template <int WT>
 __global__ __launch_bounds__(256) void vocab_expand_kernel(const uint8_t* w, int64_t ldw, int64_t rows, int H8,
@@ -805,8 +789,7 @@ __global__ __launch_bounds__(256) void vocab_expand_kernel(const uint8_t* w, int
   const int64_t r = i / H8;
   const int c = (int)(i - r * H8) * 8;
   const uint2 d = *reinterpret_cast<const uint2*>(w + r * ldw + c);
-  const uint2 lo = codes4_to_bf16<WT>(d.x), hi = codes4_to_bf16<WT>(d.y);
-  *reinterpret_cast<uint4*>(out + r * ldo + c) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+  *reinterpret_cast<bf16x8*>(out + r * ldo + c) = codes8_to_bf16<WT>(d.x, d.y);
 }
 
 // x rows [R][C] -> out [C][ldo] bf16, columns R .. zero up to the next multiple of
@@ -958,13 +941,12 @@ int loss_args_ok(const LossArgs& a) {
   return 1;
 }
 
-// Whether codes go to the tiles as they are stored: whole 16-byte chunks, and of
-// int8, whose expansion takes the most instructions, not so many tokens that
-// expanding a piece first is the shorter way (int8, 32003 x 2880: 1024 tokens 227
-// us as stored, 248 expanded; 4096 893, 785; e4m3, 131072 x 4096: 192 tokens 0.19
-// ms, 0.78; 1024 0.92, 1.23; 4096 3.61, 3.90)
-bool codes_direct(const void* w, int wtype, int64_t ldw, int64_t H, int64_t T) {
-  return (wtype != 4 || T <= 1536) && H % 16 == 0 && ldw % 16 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+// Whether codes go to the tiles as they are stored: whole 16-byte chunks. (Else
+// pieces are expanded first. e4m3, 131072 x 4096: 192 tokens 0.19 ms as stored,
+// 0.78 expanded; 1024 0.92, 1.23; 4096 3.61, 3.90. int8, whose expansion takes
+// the most instructions, 32003 x 2880: 1024 tokens 200 us, 248; 4096 793, 785.)
+bool codes_direct(const void* w, int64_t ldw, int64_t H) {
+  return H % 16 == 0 && ldw % 16 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
 }
 
 // Table rows of a piece of the forward pass where codes are expanded first: 128
@@ -1064,7 +1046,7 @@ extern "C" int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void
   g.ignore = ignore_index;
   g.part = reinterpret_cast<float2*>(ws + off[0]);
   g.tgt = reinterpret_cast<float*>(ws + off[1]);
-  const bool direct = wtype && codes_direct(w, wtype, ldw, H, T);
+  const bool direct = wtype && codes_direct(w, ldw, H);
   const int64_t Vc = wtype && !direct ? loss_piece(V, H) : V;
   for (int64_t v0 = 0; v0 < V; v0 += Vc) {
     const uint8_t* rows = static_cast<const uint8_t*>(w) + v0 * ldw * (wtype ? 1 : 2);
