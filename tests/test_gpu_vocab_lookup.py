@@ -226,3 +226,23 @@ def test_lookup_compiles(dev):
     assert torch.equal(a, b)
     up = torch.randn_like(a)
     assert torch.equal(torch.autograd.grad(a, w, up)[0], torch.autograd.grad(b, w, up)[0])
+
+
+@pytest.mark.parametrize("shape", [(0,), (7,), (2, 3), (1, 0, 4)])
+def test_lookup_backward_takes_any_gradient(dev, shape):
+    """Contiguous, broadcast and strided gradients, ids of any shape and stride,
+    with and without a graph of the gradient (which ends there)."""
+    V, H = 19, 40
+    gen = torch.Generator(device=dev).manual_seed(3)
+    w = torch.randn((V, H), generator=gen, device=dev, requires_grad=True)
+    wide = torch.randint(0, V, (*shape, 2), generator=gen, device=dev)
+    for ids in (wide[..., 0], wide[..., 0].contiguous(), wide[..., 0].contiguous().to(torch.int32)):
+        up = torch.randn((*shape, H), generator=gen, device=dev)
+        for g in (up, up[..., :1].expand(up.shape), torch.stack((up, up), -1)[..., 0]):
+            for graph in (False, True):
+                out = embedding(ids, w, out_dtype=F32)
+                (dw,) = torch.autograd.grad(out, w, g, create_graph=graph)
+                _check_grad(dw.detach(), ids.reshape(-1).long(), g.reshape(-1, H), V, 1.0, None)
+        if graph and dw.requires_grad:
+            with pytest.raises(RuntimeError, match="once_differentiable"):
+                torch.autograd.grad(dw.sum(), w)

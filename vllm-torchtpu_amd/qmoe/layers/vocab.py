@@ -52,11 +52,27 @@ class _Embedding(torch.autograd.Function):
         return _lookup(ids, weight, None, scale, out_dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        # (autograd runs this with gradients off, and the node's device current;
+        # with create_graph the decorator puts the error for a second pass behind it)
+        if torch.is_grad_enabled():
+            return _Embedding._once(ctx, grad)
+        return _Embedding._grads(ctx, grad)
+
+    @staticmethod
+    def _grads(ctx, grad):
         (ids,) = ctx.saved_tensors
-        fn = ops.vocab_lookup_grad if ops.eager_call(grad, ids) else torch.ops.qmoe.vocab_lookup_grad
-        return None, fn(grad, ids, *ctx.args), None, None, None
+        vocab, scale, padding_idx, dtype = ctx.args
+        if torch.compiler.is_compiling() or type(grad) is not torch.Tensor or not grad.is_contiguous() or \
+                not ids.is_contiguous() or not grad.is_cuda:
+            fn = ops.vocab_lookup_grad if ops.eager_call(grad, ids) else torch.ops.qmoe.vocab_lookup_grad
+            return None, fn(grad, ids, vocab, scale, padding_idx, dtype), None, None, None
+        H = grad.shape[-1]
+        dw = ops.lookup_grad_run(grad, H, ids if ids.dim() == 1 else ids.view(-1), vocab, H, scale,
+                                 -1 if padding_idx is None else padding_idx, dtype)
+        return None, dw, None, None, None
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_grads.__func__))
 
 
 def _lookup(ids, weight, weight_scale, scale, out_dtype):

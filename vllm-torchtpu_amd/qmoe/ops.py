@@ -7,6 +7,7 @@ layouts on the host, and launches the HIP kernels on the current stream via
 
 import contextlib
 import ctypes
+import functools
 import math
 
 import torch
@@ -42,6 +43,15 @@ def _ptr(t):
 
 def _stream(dev):
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+
+
+# The current stream's handle without a Stream object around it, where torch has the call
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    def _raw_stream(dev):
+        return torch._C._cuda_getCurrentRawStream(dev.index)
+else:
+    def _raw_stream(dev):
+        return torch.cuda.current_stream(dev).cuda_stream
 
 
 _PLAIN = frozenset((type(None), torch.Tensor, torch.nn.Parameter))
@@ -764,7 +774,7 @@ def moe_few_tokens(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bia
         need = ctypes.c_int64(0)
         check(lib.qmoe_moe_few_workspace_size(ref, ctypes.byref(need)), "moe_few_tokens (shape)")
         ws, ws_n = _workspace(dev, need.value)
-        check(lib.qmoe_moe_few(ref, ws.data_ptr(), ws_n, torch.cuda.current_stream(dev).cuda_stream), "moe_few_tokens")
+        check(lib.qmoe_moe_few(ref, ws.data_ptr(), ws_n, _raw_stream(dev)), "moe_few_tokens")
     return out
 
 
@@ -844,8 +854,15 @@ def vocab_lookup(ids, weight, weight_scale=None, scale=1.0, out_dtype=torch.bflo
         check(lib.qmoe_vocab_lookup(flat.data_ptr(), flat.dtype is torch.int64, n, weight.data_ptr(),
                                     _TABLE_TYPES[weight.dtype], weight.stride(0), s.data_ptr() if s is not None else None,
                                     V, H, scale, out.data_ptr(), _TABLE_TYPES[out_dtype], H,
-                                    torch.cuda.current_stream(dev).cuda_stream), "vocab_lookup")
+                                    _raw_stream(dev)), "vocab_lookup")
     return out if ids.dim() == 1 else out.view(*ids.shape, H)
+
+
+@functools.lru_cache(maxsize=256)
+def _lookup_grad_bytes(n, vocab, H):
+    need = ctypes.c_int64(0)
+    check(lib.qmoe_vocab_lookup_grad_workspace_size(n, vocab, H, ctypes.byref(need)), "vocab_lookup_grad (shape)")
+    return need.value
 
 
 def vocab_lookup_grad(grad, ids, vocab, scale=1.0, padding_idx=None, dtype=torch.bfloat16, into=None):
@@ -871,16 +888,23 @@ def vocab_lookup_grad(grad, ids, vocab, scale=1.0, padding_idx=None, dtype=torch
     elif dtype not in _GRAD_TYPES:
         raise ValueError(f"vocab_lookup_grad: the table's gradient is bf16 or f32, not {dtype}")
     with _on_device(g, flat, into):
-        dev = g.device
-        dw = into if into is not None else torch.empty((vocab, H), dtype=dtype, device=dev)
-        need = ctypes.c_int64(0)
-        check(lib.qmoe_vocab_lookup_grad_workspace_size(n, vocab, H, ctypes.byref(need)), "vocab_lookup_grad (shape)")
-        ws, ws_n = _workspace(dev, need.value)
-        check(lib.qmoe_vocab_lookup_grad(flat.data_ptr(), flat.dtype is torch.int64, n, g.data_ptr(),
-                                         _TABLE_TYPES[g.dtype], g.stride(0) if n else H, vocab, H, scale,
-                                         -1 if padding_idx is None else padding_idx, dw.data_ptr(),
-                                         _TABLE_TYPES[dw.dtype], dw.stride(0), into is not None, ws.data_ptr(), ws_n,
-                                         torch.cuda.current_stream(dev).cuda_stream), "vocab_lookup_grad")
+        return lookup_grad_run(g, g.stride(0) if n else H, flat, vocab, H, scale, -1 if padding_idx is None else padding_idx,
+                               dtype, into)
+
+
+def lookup_grad_run(g, ldg, flat, vocab, H, scale, padding_idx, dtype, into=None):
+    """`vocab_lookup_grad` behind its checks, on the current device. A backward
+    pass calls it from autograd's own thread, where every Python object that the
+    forward pass has used comes from another core: it touches few."""
+    n = flat.shape[0]
+    need = _lookup_grad_bytes(n, vocab, H)
+    dw = into if into is not None else g.new_empty((vocab, H), dtype=dtype)
+    ws = g.new_empty(need, dtype=torch.uint8)
+    rc = lib.qmoe_vocab_lookup_grad(flat.data_ptr(), flat.dtype is torch.int64, n, g.data_ptr(), _TABLE_TYPES[g.dtype], ldg,
+                                    vocab, H, scale, padding_idx, dw.data_ptr(), _TABLE_TYPES[dw.dtype], dw.stride(0),
+                                    into is not None, ws.data_ptr(), need, _raw_stream(g.device))
+    if rc:
+        check(rc, "vocab_lookup_grad")
     return dw
 
 
@@ -931,7 +955,7 @@ def vocab_loss(x, weight, targets, weight_scale=None, ignore_index=-100):
         ws, ws_n = _workspace(dev, need.value)
         check(lib.qmoe_vocab_loss(_ptr(x2), x2.stride(0), T, _ptr(weight), wt, weight.stride(0), _ptr(s), V, H, _ptr(t),
                                   int(t.dtype == torch.int64), int(ignore_index), _ptr(loss), _ptr(lse), _ptr(ws), ws_n,
-                                  _stream(dev)), "vocab_loss")
+                                  _raw_stream(dev)), "vocab_loss")
     return loss, lse
 
 
@@ -964,5 +988,5 @@ def vocab_loss_grad(x, weight, targets, lse, g_loss, g_lse=None, weight_scale=No
             check(lib.qmoe_vocab_loss_grad(_ptr(x2), x2.stride(0), T, _ptr(weight), wt, weight.stride(0), _ptr(s), V, H,
                                            _ptr(t), int(t.dtype == torch.int64), int(ignore_index), _ptr(lse),
                                            _ptr(g_loss), _ptr(g_lse), _ptr(dx), H, _ptr(dw), H, _ptr(ws), ws_n,
-                                           _stream(dev)), "vocab_loss_grad")
+                                           _raw_stream(dev)), "vocab_loss_grad")
     return (dx.view(x.shape) if dx is not None else None), dw
