@@ -126,3 +126,27 @@ def test_which_steps_it_takes():
     assert ops.few_token_moe_takes(16, 8, "mxfp4") and ops.few_token_moe_takes(1, 64, "bf16")
     assert not ops.few_token_moe_takes(17, 1, "mxfp4") and not ops.few_token_moe_takes(16, 9, "mxfp4")
     assert not ops.few_token_moe_takes(1, 1, "fp8")
+
+
+def test_takes_only_sizes_that_it_has():
+    """What `moe_forward` asks before it leaves its other paths."""
+    z = lambda *s: torch.empty(s, dtype=torch.uint8, device="meta")  # noqa: E731
+    takes = ops.few_token_moe_takes
+    assert takes(4, 2, "mxfp4", z(8, 256, 64)) and takes(4, 2, "nvfp4", z(8, 96, 16))
+    assert not takes(4, 2, "mxfp4", z(8, 256, 24)) and not takes(4, 2, "bf16", z(8, 80, 64))
+    assert not takes(4, 2, "mxfp4", z(513, 256, 64)) and not takes(4, 2, "bf16", z(1, 65568, 32))
+    assert takes(4, 2, "fp8_w8a16", z(8, 256, 128)) and not takes(4, 2, "fp8_w8a16", z(8, 256, 64))
+    assert takes(4, 2, "int4", z(8, 128, 32), z(8, 128, 4)) and not takes(4, 2, "int4", z(8, 128, 18), z(8, 128, 3))
+    assert takes(4, 2, "int4", z(8, 128, 32), z(8, 128, 2)) and not takes(4, 2, "int4", z(8, 96, 32), z(8, 96, 2))
+    assert not takes(4, 2, "int4", z(8, 128, 32), z(8, 128, 16))
+
+
+def test_a_gradient_asked_of_it_is_an_error():
+    """It has no backward pass: the output says so instead of dropping the path."""
+    with FakeTensorMode():
+        a = _operands(device="cuda")
+        a[0].requires_grad_()
+        out = few_token_moe(*a, 2, "silu")
+        assert out.requires_grad
+        with torch.no_grad():
+            assert not few_token_moe(*a, 2, "silu").requires_grad

@@ -246,3 +246,22 @@ def test_lookup_backward_takes_any_gradient(dev, shape):
         if graph and dw.requires_grad:
             with pytest.raises(RuntimeError, match="once_differentiable"):
                 torch.autograd.grad(dw.sum(), w)
+
+
+def test_method_embeddings_of_other_tables(dev):
+    """Tables and scales that the kernel does not read as they are keep the
+    methods' results: strided codes, parameters that ask for gradients, float32."""
+    w, s = _table(dev, 60, 64, E4)
+    ids = torch.randint(0, 60, (11,), device=dev)
+    want = w.view(torch.uint8)[ids].view(E4).to(BF16) * s[ids].to(BF16).unsqueeze(-1)
+    layer = torch.nn.Module()
+    layer.params_dtype, layer.weight_scale = BF16, s
+    for table in (w, w.t().contiguous().t(), w.clone().requires_grad_()):
+        layer.weight = table
+        assert torch.equal(Fp8LinearMethod.embedding(None, layer, ids), want)
+    layer.weight, layer.weight_scale = w, s.clone().requires_grad_()
+    out = Fp8LinearMethod.embedding(None, layer, ids)
+    assert torch.equal(out, want) and out.requires_grad
+    plain = torch.nn.Module()
+    plain.weight = torch.randn((60, 64), device=dev)
+    assert torch.equal(UnquantizedLinearMethod().embedding(plain, ids), plain.weight[ids])

@@ -144,3 +144,14 @@ def test_loss_entry_points_check_their_arguments():
         a, 64, T, a, wt, 64, rs, 500, 64, a, 1, -100, a, a, None, dx, lddx, dw, 64, a, size, None)
     assert grad(dx=None, dw=None) == grad(wt=4, rs=a) == grad(lddx=62) == grad(T=0) == 1
     assert grad(size=need - 1) == 2
+
+
+def test_no_gradient_through_row_scales():
+    q, s = torch.zeros((8, 16), dtype=torch.int8), torch.ones(8, requires_grad=True)
+    ids, x = torch.zeros(3, dtype=torch.int64), torch.zeros((3, 16), dtype=torch.bfloat16)
+    with pytest.raises(NotImplementedError, match="or its scales"):
+        embedding(ids, q, s)
+    with pytest.raises(NotImplementedError, match="or its scales"):
+        vocab_cross_entropy(x, q, ids, s)
+    with torch.no_grad(), pytest.raises(ValueError, match="device tensors"):
+        embedding(ids, q, s)

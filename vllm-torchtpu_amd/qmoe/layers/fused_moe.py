@@ -278,8 +278,9 @@ def few_token_moe(hidden_states, router_logits, w1, w2, w1_scale, w2_scale, w1_b
     args = (hidden_states, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, int(topk), activation or "", fmt,
             scoring_func, bool(renormalize), e_score_correction_bias, float(routed_scaling_factor),
             int(num_expert_group or 1), int(topk_group or 1), bool(skip_padded_tokens))
-    if ops.eager_call(*args[:8], e_score_correction_bias):
-        return ops.moe_few_tokens(*args)
+    if ops.eager_call(*args[:8], e_score_correction_bias) and not (
+            torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:8])):
+        return ops.moe_few_tokens(*args)  # (the op's own error stands where a gradient would be asked of it)
     ops._check_few(*args[:12])
     return torch.ops.qmoe.few_token_moe(*args)
 
@@ -293,7 +294,7 @@ def moe_forward(layer, x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2
     launch; anything else (a model-supplied routing function, hash routing,
     larger batches) routes first and calls `fused_moe_gmm`. With
     ``QMOE_FEW_TOKEN_MOE`` set, such a batch of at most that many tokens runs
-    `few_token_moe` where it has the weight format."""
+    `few_token_moe` where it has the weight format and the sizes."""
     from qmoe import envs
     from qmoe.layers import moe_routing
 
@@ -310,7 +311,7 @@ def moe_forward(layer, x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2
         return fused_moe_gmm(x, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk_weights, topk_ids, None, topk,
                              act, skip_padded_tokens=skip_padded_tokens, weight_format=weight_format)
     ops.act_code(act)
-    if T <= envs.QMOE_FEW_TOKEN_MOE and act and ops.few_token_moe_takes(T, topk, weight_format):
+    if T <= envs.QMOE_FEW_TOKEN_MOE and act and ops.few_token_moe_takes(T, topk, weight_format, w2, w2_scale):
         bias, rsf, ng, tg = moe_routing.routing_params(layer)
         return few_token_moe(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk, act,
                              weight_format=weight_format, scoring_func=layer.scoring_func, renormalize=layer.renormalize,

@@ -30,9 +30,9 @@ class UnquantizedLinearMethod:
         return out
 
     def embedding(self, layer, input_):
-        """Rows of a bf16 ``[vocab, H]`` table (a `VocabParallelEmbedding` of an
-        unquantized checkpoint)."""
-        return embedding(input_, layer.weight)
+        """Rows of a bf16 or f32 ``[vocab, H]`` table (a `VocabParallelEmbedding`
+        of an unquantized checkpoint), in its type."""
+        return embedding(input_, layer.weight, out_dtype=layer.weight.dtype)
 
     def cross_entropy(self, layer, x, targets, ignore_index=-100):
         """(loss, lse) of the targets under softmax(apply(layer, x)), without

@@ -53,8 +53,7 @@ class _Embedding(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
-        # (autograd runs this with gradients off, and the node's device current;
-        # with create_graph the decorator puts the error for a second pass behind it)
+        # (autograd runs this with gradients off; with create_graph the decorator puts the error for a second pass behind it)
         if torch.is_grad_enabled():
             return _Embedding._once(ctx, grad)
         return _Embedding._grads(ctx, grad)
@@ -64,7 +63,7 @@ class _Embedding(torch.autograd.Function):
         (ids,) = ctx.saved_tensors
         vocab, scale, padding_idx, dtype = ctx.args
         if torch.compiler.is_compiling() or type(grad) is not torch.Tensor or not grad.is_contiguous() or \
-                not ids.is_contiguous() or not grad.is_cuda:
+                not ids.is_contiguous() or grad.get_device() != torch.cuda.current_device():
             fn = ops.vocab_lookup_grad if ops.eager_call(grad, ids) else torch.ops.qmoe.vocab_lookup_grad
             return None, fn(grad, ids, vocab, scale, padding_idx, dtype), None, None, None
         H = grad.shape[-1]
@@ -95,9 +94,9 @@ def embedding(ids, weight, weight_scale=None, scale=1.0, padding_idx=None, out_d
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"embedding: padding_idx {padding_idx} is outside the table of {weight.shape[0]} rows")
     scale = float(scale)
-    if weight.requires_grad and torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (weight.requires_grad or (weight_scale is not None and weight_scale.requires_grad)):
         if weight_scale is not None:
-            raise NotImplementedError("embedding: no gradient for a table of 1-byte codes")
+            raise NotImplementedError("embedding: no gradient for a table of 1-byte codes or its scales")
         if out_dtype == torch.float16:
             raise NotImplementedError("embedding: gradients flow through bf16 or f32 outputs, not f16")
         return _Embedding.apply(ids, weight, scale, padding_idx, out_dtype)
@@ -178,8 +177,9 @@ def vocab_cross_entropy(x, weight, targets, weight_scale=None, ignore_index=-100
     (gradients in bf16; a table of codes is frozen). The sums' order is fixed:
     the same bits on every call."""
     ignore_index = int(ignore_index)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        if weight.requires_grad and weight_scale is not None:
-            raise NotImplementedError("vocab_cross_entropy: no gradient for a table of 1-byte codes")
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                    (weight_scale is not None and weight_scale.requires_grad)):
+        if weight_scale is not None and (weight.requires_grad or weight_scale.requires_grad):
+            raise NotImplementedError("vocab_cross_entropy: no gradient for a table of 1-byte codes or its scales")
         return _VocabCrossEntropy.apply(x, weight, targets, weight_scale, ignore_index)
     return _loss(x, weight, targets, weight_scale, ignore_index)

@@ -677,9 +677,22 @@ _FEW_FORMATS = {
 }
 
 
-def few_token_moe_takes(T, topk, fmt):
-    """Whether `moe_few_tokens` has a form for this step."""
-    return fmt in _FEW_FORMATS and 1 <= T <= FEW_MAX_TOKENS and T * topk <= FEW_MAX_ROUTES
+def _few_multiple(fmt, group):
+    """H and I of a few-token MoE layer come in multiples of this."""
+    return 128 if fmt == "fp8_w8a16" else max(group, 32)
+
+
+def few_token_moe_takes(T, topk, fmt, w2=None, w2_scale=None):
+    """Whether `moe_few_tokens` has a form for this step (and, given them, for
+    these experts)."""
+    if fmt not in _FEW_FORMATS or not 1 <= T <= FEW_MAX_TOKENS or T * topk > FEW_MAX_ROUTES:
+        return False
+    if w2 is None:
+        return True
+    E, H, I = w2.shape[0], w2.shape[1], w2.shape[2] * _FEW_FORMATS[fmt][2]
+    group = I // w2_scale.shape[-1] if fmt == "int4" else 0
+    mult = _few_multiple(fmt, group)
+    return E <= 512 and max(H, I) <= 65536 and H % mult == 0 and I % mult == 0 and group in (0, 32, 64, 128)
 
 
 def _check_few(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk, activation, fmt, scoring_func):
@@ -727,7 +740,7 @@ def _check_few(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, t
     for b, n, name in ((w1_bias, n1, "w1_bias"), (w2_bias, H, "w2_bias")):
         if b is not None and b.numel() != E * n:
             raise ValueError(f"few-token MoE: {name} must hold [{E}, {n}] values, got {tuple(b.shape)}")
-    mult = 128 if fmt == "fp8_w8a16" else (group if group > 32 else 32)
+    mult = _few_multiple(fmt, group)
     if H % mult or I % mult:
         raise ValueError(f"few-token MoE: {fmt} needs H and I in multiples of {mult}, got {H}, {I}")
     return I, group
