@@ -309,3 +309,21 @@ def test_a_step_from_tokens_to_their_scores(dev):
     # logits' float32 sums, and the roundings of the loss
     lim = 264 * EPS * (y.double().abs() @ table.double().t().abs()).amax(1) + 300 * EPS * (1 + lg.abs().amax(1))
     assert ((loss.double() - ref).abs() <= 2 * lim).all()
+
+
+@pytest.mark.parametrize("T", [1, 5])
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4", "int4"])
+def test_a_scale_that_is_no_number_stays_in_its_row(dev, fmt, T):
+    """Rows that end inside a pair of 16-byte chunks: the scale behind their end
+    is the next row's first."""
+    c = _layer(dev, fmt, T, 8, 2, 96, 96, seed=14, group=32)
+    clean = _run(c)
+    if fmt == "mxfp4":
+        c.s2[:, 5, 0] = 255
+    else:
+        c.s2[:, 5, 0] = float("nan")
+        c.s2[:, 40, 0] = float("inf")
+    out, bad = _run(c), [5] if fmt == "mxfp4" else [5, 40]
+    assert not out[:, bad].isfinite().any()
+    kept = [n for n in range(96) if n not in bad]
+    assert torch.equal(out[:, kept], clean[:, kept])

@@ -184,13 +184,13 @@ __device__ __forceinline__ uint4 expand8(const uint4& c, int i, uint32_t s) {
 }
 
 // acc[t][i] += line t . tokens, MFMA i of each chunk; `first`: the line's first
-// chunk of the row, row_off: the lane's scale row. `tr`: this wavefront's LDS,
+// chunk of the row, `end`: the row's chunks, row_off: the lane's scale row. `tr`: this wavefront's LDS,
 // 2 KB per tile. Row r's chunk c lies at slot c ^ (r / 2), so that neither the
 // writes (the 8 chunks of a row by 8 adjacent lanes) nor the reads (one chunk of
 // 16 rows) meet in a bank.
 template <int F, int NT>
-__device__ __forceinline__ void consume(const Step<F, NT>& st, uint4* tr, uint32_t row_off, int first, int group_shift,
-                                        f32x4 (&acc)[NT][Fmt<F>::kMfma]) {
+__device__ __forceinline__ void consume(const Step<F, NT>& st, uint4* tr, uint32_t row_off, int first, int end,
+                                        int group_shift, f32x4 (&acc)[NT][Fmt<F>::kMfma]) {
   const int lane = threadIdx.x & 63, r = lane & 15, kg = lane >> 4;
   // the scale words are taken as loaded only here: their conversions, moved up
   // to the loads of the step before, would wait for every load in flight
@@ -214,7 +214,8 @@ __device__ __forceinline__ void consume(const Step<F, NT>& st, uint4* tr, uint32
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const uint4 c = tr[t * 128 + r * 8 + ((2 * kg + u) ^ (r >> 1))];
-      const uint32_t scale = scale_of<F>(sc[t], row_off, first + 2 * kg, u, group_shift);
+      // (behind a row's end lies the next row's scale: an infinity or NaN there, times the zero codes, is not this row's)
+      const uint32_t scale = first + 2 * kg + u < end ? scale_of<F>(sc[t], row_off, first + 2 * kg, u, group_shift) : 0u;
       Bf8 b;
       b.u = st.x[u];
 #pragma unroll
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(kUpWaves * 64, 3) void few_up_kernel(const FewParam
       if (!more && next) seek(item + 1);
 #pragma unroll
       for (int u = 0; u < A; ++u) {
-        consume<F, 2>(st[u], tr[wave], slane, (wave + kUpWaves * (c * A + u)) * 8, p.group_shift, acc);
+        consume<F, 2>(st[u], tr[wave], slane, (wave + kUpWaves * (c * A + u)) * 8, rb / 16, p.group_shift, acc);
         issue(st[u], (more ? (c + 1) * A : 0) + u, more || next);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -534,7 +535,7 @@ __global__ __launch_bounds__(kDownWaves * 64) void few_down_kernel(const FewPara
       if (now.slot < num) {
         if (now.slot != slot && slot >= 0) flush(slot);
         slot = now.slot;
-        consume<F, 1>(st[u], tr[wave], slane, now.line * 8, p.group_shift, acc);
+        consume<F, 1>(st[u], tr[wave], slane, now.line * 8, rb / 16, p.group_shift, acc);
       }
       issue(st[u], ahead);
       now.line += NW;
