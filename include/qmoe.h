@@ -489,8 +489,8 @@ int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void* w, int wt
  * counts) + g_lse[t]: P[t, v] = exp(l - lse[t]) c[t] - [v == target[t]]
  * g_loss[t], rounded to bf16; dx = P (s w) bf16 [T, lddx >= H], dw = P^T x bf16
  * [V, lddw >= H] (bf16 tables only). Either may be NULL. A token with neither
- * gradient leaves zeros in dx and nothing in dw, whatever its x holds. P and the
- * logits exist for one piece of the vocabulary at a time. lddx, lddw multiples
+ * gradient leaves zeros in dx and nothing in dw, whatever its x and its target
+ * are. P and the logits exist for one piece of the vocabulary at a time. lddx, lddw multiples
  * of 8, dx and dw 16-byte aligned. Every row of dx and dw is written; the sums'
  * order is fixed.
  */

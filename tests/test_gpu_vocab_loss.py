@@ -318,3 +318,18 @@ def test_tied_table_step(dev):
     ops.vocab_lookup_grad(full, ids, V, H ** 0.5, into=dw)
     # one rounding less than the sum of two rounded gradients
     assert ((dw.double() - both.double()).abs() <= 2 * HALF * (both.double().abs() + alone.double().abs())).all()
+
+
+@pytest.mark.parametrize("T", [5, 300])
+def test_a_loss_that_is_not_used_leaves_no_gradient(dev, T):
+    """Targets outside the table whose loss is dropped by a `where`: zero
+    gradient, as if the tokens were not there."""
+    x, w, _, t = _case(dev, T, 700, 64)
+    t[0], t[3] = 700, -5
+    good = torch.ones(T, dtype=torch.bool, device=dev)
+    good[0], good[3] = False, False
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss, _ = vocab_cross_entropy(xg, wg, t)
+    dx, dw = torch.autograd.grad(torch.where(good, loss, 0.0).sum(), (xg, wg))
+    assert not dx[~good].any()
+    _check_grads(dx, dw, x, w, None, torch.where(good, t, -100), good.float(), None)

@@ -240,7 +240,8 @@ __device__ __forceinline__ void vocab_epilogue(const VocabGemm& p, f32x16 (&acc)
       if (valid) {
         const int t = m0 + tb;
         const int64_t tg = load_target(p, t);
-        hot = tg == p.ignore ? 0.0f : (tg >= 0 && tg < p.V ? p.g_loss[t] : __builtin_nanf(""));
+        const float g = p.g_loss[t];  // (0 for a target outside the table: its NaN loss went nowhere)
+        hot = tg == p.ignore || g == 0.0f ? 0.0f : (tg >= 0 && tg < p.V ? g : __builtin_nanf(""));
         coef = hot + (p.g_lse ? p.g_lse[t] : 0.0f);
         lse2 = p.lse[t] * 1.4426950408889634f;
         const int64_t in = tg - p.v0 - n0;
