@@ -228,6 +228,34 @@ def test_lookup_compiles(dev):
     assert torch.equal(torch.autograd.grad(a, w, up)[0], torch.autograd.grad(b, w, up)[0])
 
 
+@pytest.mark.parametrize("kind", ["one", "half", "natural", "bad", "rows"])
+@pytest.mark.parametrize("N", [63, 1000, 1024, 1025])
+def test_lookup_grad_few_tokens(dev, kind, N):
+    """The same uneven tokens in short lists, around the sums' and the sort's
+    chunks, and many tokens of few neighbouring rows."""
+    V, H = 4099, 2120
+    gen = torch.Generator(device=dev).manual_seed(6)
+    ids = torch.randint(0, V, (N,), generator=gen, device=dev)
+    if kind == "one":
+        ids[:] = 77
+    elif kind == "half":
+        ids[torch.rand(N, generator=gen, device=dev) < 0.5] = V - 1
+    elif kind == "natural":
+        ids = (V ** torch.rand(N, generator=gen, device=dev, dtype=torch.float64)).long() - 1
+    elif kind == "bad":
+        ids[::3], ids[1::3] = -7, V + 12
+    else:
+        ids = ids % 16 + 48
+    g = torch.randn((N, H), generator=gen, device=dev).to(BF16)
+    for padding in (None, int(ids[0].clamp(0, V - 1))):
+        dw = ops.vocab_lookup_grad(g, ids, V, 0.5, padding, F32)
+        _check_grad(dw, ids, g, V, 0.5, padding)
+    into = torch.randn((V, H), generator=gen, device=dev)
+    before = into.clone()
+    ops.vocab_lookup_grad(g, ids.int(), V, into=into)
+    _check_grad(into, ids, g, V, 1.0, None, before)
+
+
 @pytest.mark.parametrize("shape", [(0,), (7,), (2, 3), (1, 0, 4)])
 def test_lookup_backward_takes_any_gradient(dev, shape):
     """Contiguous, broadcast and strided gradients, ids of any shape and stride,
