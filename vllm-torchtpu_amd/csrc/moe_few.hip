@@ -27,6 +27,15 @@
 //    (8-bit codes: two MFMAs, 8 tokens; bf16: one, 16.)
 //  * Sums are float32: per wavefront, then over the wavefronts in order; in
 //    launch 2 over the slots in ascending order per wavefront.
+//  * Rounded to bf16 are the matrix cores' operands: h, and code x scale of the
+//    4- and 8-bit formats (exact for MXFP4), as in the other bf16-activation
+//    paths; and out, once.
+//
+// Measured, launch 1 + 2: one token, MXFP4, 4 of 128 experts of 2880 x 2880 15.0 +
+// 8.7 us; 16 tokens 113 + 72 (442 and 236 MiB read: 4.1 and 3.4 TB/s; 17 us of
+// launch 1 are the routing of 16 tokens and latency, and launch 2 has 180
+// workgroups for 256 CUs); 8 tokens, NVFP4, 8 of 256 experts of 2048 x 7168 176 +
+// 92 (746 and 371 MiB, 4.4 and 4.2 TB/s).
 
 #include <algorithm>
 

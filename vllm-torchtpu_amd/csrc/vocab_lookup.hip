@@ -8,6 +8,10 @@
 // Both are bound by HBM: the lookup reads and writes N rows, the gradient reads
 // N rows and writes V (all of a fresh gradient; only the touched ones when it
 // is added into an existing one).
+// Measured: 16384 rows of 7168 bf16 67 us (168 MiB read, repeated rows come from
+// cache, 224 written: 6.1 TB/s), 8 rows of 4096 e4m3 3.5; gradient of 16384 rows
+// of 4096 bf16 into a fresh 131072-row one 11 (sort) + 211 (sums and zeros, 125
+// MiB read, 1035 written: 5.8 TB/s) + 19 (join).
 
 #include <algorithm>
 
