@@ -366,15 +366,17 @@ __device__ __forceinline__ bf16x8 codes8_to_bf16(uint32_t lo, uint32_t hi) {
 // TB/s): with codes (AT 3 e4m3, 4 int8, 5 e5m2) the table is read as it is stored
 // and expanded between LDS and the matrix cores. Stages of 64 k of every row in a ring of
 // as many as fit.
-template <int EPI, int BM, int AT>
-__global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGemm args) {
+// ONE: K is one stage (dw of up to 64 tokens): without a ring two workgroups
+// share a CU, and one's stores run under the other's copies.
+template <int EPI, int BM, int AT, bool ONE = false>
+__global__ __launch_bounds__(kVThreads, ONE ? 4 : 2) void vocab_gemm_kernel(const VocabGemm args) {
   constexpr int BN = kVN, NI = 2, MJ = BM / 64;
   constexpr bool TRA = tr_a(EPI), TRB = tr_b(EPI);
   constexpr int AB = AT ? 64 : 128;  // bytes of an A row per stage
   constexpr int WB = BN * AB, STG = WB + BM * 128;
-  constexpr int RING = 163840 / STG < 6 ? 163840 / STG : 6;
-  __shared__ __align__(1024) uint8_t smem[RING * STG];
-  static_assert(RING >= 3 && RING * STG >= 9216 + 65536, "ring, epilogue region");
+  constexpr int RING = ONE ? 1 : (163840 / STG < 6 ? 163840 / STG : 6), EPILOGUE = 9216 + 65536;
+  __shared__ __align__(1024) uint8_t smem[RING * STG > EPILOGUE ? RING * STG : EPILOGUE];
+  static_assert(ONE ? sizeof(smem) <= 81920 : RING >= 3 && sizeof(smem) <= 163840, "workgroups of a CU, ring");
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
   VocabGemm p = args;
   take_slice<EPI>(p);
@@ -494,7 +496,17 @@ __global__ __launch_bounds__(kVThreads, 2) void vocab_gemm_kernel(const VocabGem
   // read; then the next stage's copies have landed -> barrier: everybody holds
   // this stage's last operands, so that its slot takes the copies of stage s +
   // RING -> the last step, while the next stage's first operands are read.
-  if (KF > 0) {
+  if constexpr (ONE) {
+    copy_stage(0, 0);
+    wait_copies_upto<0>();
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      read_q(0, q);
+      mma(q);
+    }
+    __syncthreads();
+  } else if (KF > 0) {
 #pragma unroll
     for (int r = 0; r < RING; ++r) copy_stage(r, r);
     wait_copies_upto<(RING - 1) * (WI + XI)>();
@@ -886,7 +898,10 @@ void launch_gemm(VocabGemm g, int at, int bm, int slices, hipStream_t st) {
     if constexpr (!tr_b(EPI)) launch_big<EPI, 192>(g, at, grid, st);
   } else if (at == 0) {
     if constexpr (EPI == VE_SUM) launch_small<EPI, 64, 0>(g, grid, st);
-    else if constexpr (EPI == VE_STORE) launch_small<EPI, 128, 0>(g, grid, st);
+    else if constexpr (EPI == VE_STORE) {
+      if (g.K == 64) hipLaunchKernelGGL((vocab_gemm_kernel<EPI, 128, 0, true>), grid, dim3(kVThreads), 0, st, g);
+      else launch_small<EPI, 128, 0>(g, grid, st);
+    }
     else bm == 128 ? launch_small<EPI, 128, 0>(g, grid, st) : launch_small<EPI, 64, 0>(g, grid, st);
   } else if constexpr (EPI == VE_LSE) {
     if (at == 3) bm == 128 ? launch_small<EPI, 128, 3>(g, grid, st) : launch_small<EPI, 64, 3>(g, grid, st);
@@ -1163,7 +1178,7 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
       d.kr = (int)T;
       d.y = static_cast<uint16_t*>(dw) + v0 * lddw;
       d.ldy = lddw;
-      launch_gemm<VE_STORE>(d, 0, vocab_bm(H, n, true), 1, stream);
+      launch_gemm<VE_STORE>(d, 0, Tw == 64 ? 128 : vocab_bm(H, n, true), 1, stream);
     }
   }
   return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
