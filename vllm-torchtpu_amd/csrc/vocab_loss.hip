@@ -366,8 +366,8 @@ __device__ __forceinline__ bf16x8 codes8_to_bf16(uint32_t lo, uint32_t hi) {
 // TB/s): with codes (AT 3 e4m3, 4 int8, 5 e5m2) the table is read as it is stored
 // and expanded between LDS and the matrix cores. Stages of 64 k of every row in a ring of
 // as many as fit.
-// ONE: K is one stage (dw of up to 64 tokens): without a ring two workgroups
-// share a CU, and one's stores run under the other's copies.
+// ONE: a stage at a time, without a ring, so that two workgroups share a CU and
+// each one's copies and stores run under the other's products (kShortK).
 template <int EPI, int BM, int AT, bool ONE = false>
 __global__ __launch_bounds__(kVThreads, ONE ? 4 : 2) void vocab_gemm_kernel(const VocabGemm args) {
   constexpr int BN = kVN, NI = 2, MJ = BM / 64;
@@ -497,15 +497,17 @@ __global__ __launch_bounds__(kVThreads, ONE ? 4 : 2) void vocab_gemm_kernel(cons
   // this stage's last operands, so that its slot takes the copies of stage s +
   // RING -> the last step, while the next stage's first operands are read.
   if constexpr (ONE) {
-    copy_stage(0, 0);
-    wait_copies_upto<0>();
-    __syncthreads();
+    for (int s = 0; s < KF; ++s) {
+      copy_stage(s, 0);
+      wait_copies_upto<0>();
+      __syncthreads();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      read_q(0, q);
-      mma(q);
+      for (int q = 0; q < 4; ++q) {
+        read_q(0, q);
+        mma(q);
+      }
+      __syncthreads();
     }
-    __syncthreads();
   } else if (KF > 0) {
 #pragma unroll
     for (int r = 0; r < RING; ++r) copy_stage(r, r);
@@ -848,14 +850,21 @@ __global__ __launch_bounds__(256) void vocab_transpose_kernel(const uint8_t* src
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
+// K of a tile up to which two workgroups per CU without a ring, whose copies, products
+// and stores overlap each other's, beat the ring in tiles that store or reduce
+// much. dw of 50021 x 2880: 64 tokens 66 us, by 256 x 256 106; 128 90, 122; 333
+// 156, 178; 768 264, 272; 1024 333, 331. Probabilities of 333 tokens x 50021, H
+// 512, 1024, 2048: 37, 58, 103, by the ring 49, 65, 99; logits 31, 56, 100, by the
+// ring 36, 54, 90; of 2048 tokens 115, 204 (H 512, 1024), by the ring 138, 218.
+constexpr int64_t kShortK = 1024;
+
 // What a round of tiles over the 256 CUs costs: 256 x 256 and 256 x 192 by four
 // wavefronts, 256 x 128 by eight. (333 tokens x 50021 x 2880, 2, 2 and 3 rounds:
 // logits 142, 118, 136 us; probabilities 162, 128, 147.)
 int tile_cost(int bm) { return bm == 256 ? 160 : (bm == 192 ? 130 : 100); }
 
 // Tile of a problem of na A rows and nb B rows, by the rounds that it takes. (dw
-// has no 192 and no 64: K rows of P are copied by 256 or 512 bytes. 333 tokens,
-// H 2880: 178 us by 256 x 256, 195 by 256 x 128.)
+// has no 192 and no 64: K rows of P are copied by 256 or 512 bytes.)
 int vocab_bm(int64_t na, int64_t nb, bool dw = false) {
   const int64_t n = cdiv(na, (int64_t)kVN);
   if (nb <= 64 && !dw) return 64;
@@ -868,6 +877,11 @@ int vocab_bm(int64_t na, int64_t nb, bool dw = false) {
 template <int EPI, int BM, int AT>
 void launch_small(const VocabGemm& g, dim3 grid, hipStream_t st) {
   hipLaunchKernelGGL((vocab_gemm_kernel<EPI, BM, AT>), grid, dim3(kVThreads), 0, st, g);
+}
+
+template <int EPI>
+void launch_short(const VocabGemm& g, dim3 grid, hipStream_t st) {
+  hipLaunchKernelGGL((vocab_gemm_kernel<EPI, 128, 0, true>), grid, dim3(kVThreads), 0, st, g);
 }
 
 template <int EPI, int BM, int AT>
@@ -889,6 +903,9 @@ void launch_big(const VocabGemm& g, int at, dim3 grid, hipStream_t st) {
 // at: type of the A rows, 0 bf16 or the codes' table type (logits)
 template <int EPI>
 void launch_gemm(VocabGemm g, int at, int bm, int slices, hipStream_t st) {
+  const bool one = EPI == VE_STORE ? bm == 128 || g.K <= kShortK
+                                   : EPI != VE_SUM && at == 0 && g.nb > 128 && g.K <= kShortK;
+  if (one) bm = 128;
   g.n_tiles = cdiv(g.na, kVN);
   g.m_tiles = cdiv(g.nb, bm);
   const dim3 grid((unsigned)(cdiv(g.n_tiles * g.m_tiles, kXcds) * kXcds), (unsigned)slices);
@@ -898,11 +915,8 @@ void launch_gemm(VocabGemm g, int at, int bm, int slices, hipStream_t st) {
     if constexpr (!tr_b(EPI)) launch_big<EPI, 192>(g, at, grid, st);
   } else if (at == 0) {
     if constexpr (EPI == VE_SUM) launch_small<EPI, 64, 0>(g, grid, st);
-    else if constexpr (EPI == VE_STORE) {
-      if (g.K == 64) hipLaunchKernelGGL((vocab_gemm_kernel<EPI, 128, 0, true>), grid, dim3(kVThreads), 0, st, g);
-      else launch_small<EPI, 128, 0>(g, grid, st);
-    }
-    else bm == 128 ? launch_small<EPI, 128, 0>(g, grid, st) : launch_small<EPI, 64, 0>(g, grid, st);
+    else if (EPI == VE_STORE || one) launch_short<EPI>(g, grid, st);
+    else if constexpr (EPI != VE_STORE) bm == 128 ? launch_small<EPI, 128, 0>(g, grid, st) : launch_small<EPI, 64, 0>(g, grid, st);
   } else if constexpr (EPI == VE_LSE) {
     if (at == 3) bm == 128 ? launch_small<EPI, 128, 3>(g, grid, st) : launch_small<EPI, 64, 3>(g, grid, st);
     else if (at == 4) bm == 128 ? launch_small<EPI, 128, 4>(g, grid, st) : launch_small<EPI, 64, 4>(g, grid, st);
@@ -1178,7 +1192,7 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
       d.kr = (int)T;
       d.y = static_cast<uint16_t*>(dw) + v0 * lddw;
       d.ldy = lddw;
-      launch_gemm<VE_STORE>(d, 0, Tw == 64 ? 128 : vocab_bm(H, n, true), 1, stream);
+      launch_gemm<VE_STORE>(d, 0, vocab_bm(H, n, true), 1, stream);
     }
   }
   return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
