@@ -333,3 +333,49 @@ def test_a_loss_that_is_not_used_leaves_no_gradient(dev, T):
     dx, dw = torch.autograd.grad(torch.where(good, loss, 0.0).sum(), (xg, wg))
     assert not dx[~good].any()
     _check_grads(dx, dw, x, w, None, torch.where(good, t, -100), good.float(), None)
+
+
+def test_a_tied_step_the_ways_autograd_runs_it(dev):
+    """Lookup and loss on one table: traced without a break, on autograd's own
+    thread and on the caller's, twice from one graph, under checkpointing, on a
+    side stream and captured -- the same bits each time."""
+    from torch.utils.checkpoint import checkpoint
+    V, H = 1000, 128
+    gen = torch.Generator(device=dev).manual_seed(15)
+    table = (torch.randn((V, H), generator=gen, device=dev) * 0.1).to(BF16)
+    ids, nxt = (torch.randint(0, V, (6, 7), generator=gen, device=dev) for _ in range(2))
+
+    def step(w, ids, nxt):
+        loss, lse = vocab_cross_entropy(embedding(ids, w, scale=8.0, padding_idx=3), w, nxt)
+        return (loss + 1e-4 * lse * lse).sum()
+
+    def grad(fn):
+        w = table.clone().requires_grad_()
+        fn(w, ids, nxt).backward()
+        return w.grad
+
+    ref = grad(step)
+    torch._dynamo.reset()
+    assert torch.equal(grad(torch.compile(step, backend="aot_eager", fullgraph=True)), ref)
+    with torch.autograd.set_multithreading_enabled(False):
+        assert torch.equal(grad(step), ref)
+    for reentrant in (False, True):
+        assert torch.equal(grad(lambda *a: checkpoint(step, *a, use_reentrant=reentrant)), ref)
+    w = table.clone().requires_grad_()
+    out = step(w, ids, nxt)
+    once, again = (torch.autograd.grad(out, w, retain_graph=True)[0] for _ in range(2))
+    assert torch.equal(once, ref) and torch.equal(again, ref)
+    del out
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert torch.equal(torch.autograd.grad(step(w, ids, nxt), w)[0], ref)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (captured,) = torch.autograd.grad(step(w, ids, nxt), w)
+    for _ in range(3):
+        ids.copy_(torch.randint(0, V, (6, 7), generator=gen, device=dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, torch.autograd.grad(step(w, ids, nxt), w)[0])
