@@ -379,3 +379,22 @@ def test_a_tied_step_the_ways_autograd_runs_it(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(captured, torch.autograd.grad(step(w, ids, nxt), w)[0])
+
+
+@pytest.mark.parametrize("T,V,H", [(1, 300, 64), (70, 1031, 264), (333, 777, 128), (2500, 513, 64)])
+@pytest.mark.parametrize("kept", [0, 1, 0.1, 1.0])
+def test_gradients_of_few_kept_tokens(dev, T, V, H, kept):
+    """None, one, a tenth or all of the tokens scored, spread over the batch."""
+    x, w, _, t = _case(dev, T, V, H)
+    n = int(kept) if kept in (0, 1) and isinstance(kept, int) else max(1, int(T * kept))
+    gen = torch.Generator(device=dev).manual_seed(21)
+    keep = torch.zeros(T, dtype=torch.bool, device=dev)
+    keep[torch.randperm(T, generator=gen, device=dev)[:n]] = True
+    t = torch.where(keep, t, -100)
+    g = torch.randn(T, generator=gen, device=dev)
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    xg.data[~keep] = float("nan")
+    loss, lse = vocab_cross_entropy(xg, wg, t)
+    dx, dw = torch.autograd.grad(loss, (xg, wg), g)
+    assert not dx[~keep].any()
+    _check_grads(dx, dw, x, w, None, t, g, None)

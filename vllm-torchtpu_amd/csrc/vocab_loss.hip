@@ -21,12 +21,16 @@
 //   probs  : the same product again; P as [t][v]
 //   dx     : A = columns of the table piece, B = P rows; float32 sums added over
 //            the pieces
-//   dw     : A = columns of x (transposed once), B = columns of P
+//   dw     : A = columns of x (transposed once), B = columns of P; K = tokens
 // Rows run along K, the contiguous axis, or, of the table in dx and of P in dw,
 // across it: those are copied as they lie, 64 K rows of a stage, and transposed
 // on their way from LDS to registers by ds_read_b64_tr_b16. (With a transposed
 // copy of each table piece and P stored both ways instead: 892 us against 766 at
 // 333 tokens x 50021 x 2880, 14.26 ms against 14.15 at 4096 x 131072 x 4096.)
+// For the gradients the tokens that have one are gathered first, in order, so
+// that masked ones cost nothing and whatever they hold is not read: their number
+// stays on the device, and tiles behind it end at once (333 tokens x 50021 x 2880,
+// 101 of them not scored: 541 -> 488 us for loss and gradients).
 // Sums are float32; P is rounded to bf16 once, as the operand of the products.
 
 #include <algorithm>
@@ -61,6 +65,7 @@ struct VocabGemm {
   int part_tile;    // first tile of the piece
   float* tgt;       // [nb] the target's logit
   const float *lse, *g_loss, *g_lse;  // g_lse may be nullptr
+  const int32_t *live, *count;        // gradients: the tokens that have one, and how many (x, P and sums hold these)
   uint16_t* p;      // [nb][ldp] P
   int64_t ldp;
   // dx / dw: out[b row][a row]
@@ -238,7 +243,7 @@ __device__ __forceinline__ void vocab_epilogue(const VocabGemm& p, f32x16 (&acc)
       float hot = 0.0f, coef = 0.0f, lse2 = 0.0f;
       int at = -1;
       if (valid) {
-        const int t = m0 + tb;
+        const int t = p.live[m0 + tb];
         const int64_t tg = load_target(p, t);
         const float g = p.g_loss[t];  // (0 for a target outside the table: its NaN loss went nowhere)
         hot = tg == p.ignore || g == 0.0f ? 0.0f : (tg >= 0 && tg < p.V ? g : __builtin_nanf(""));
@@ -309,7 +314,7 @@ __device__ __forceinline__ void vocab_epilogue(const VocabGemm& p, f32x16 (&acc)
             continue;
           }
         }
-        *reinterpret_cast<uint4*>(p.y + row * p.ldy + n0 + c) = make_uint4(
+        *reinterpret_cast<uint4*>(p.y + (EPI == VE_SUM ? p.live[row] : row) * p.ldy + n0 + c) = make_uint4(
             pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
       }
     }
@@ -330,6 +335,19 @@ __device__ __forceinline__ void take_slice(VocabGemm& p) {
       p.first = 1, p.last = 0;
     }
   }
+}
+
+// B rows of the problem: tokens with a gradient of P and dx; of dw they are K
+template <int EPI>
+__device__ __forceinline__ int live_rows(VocabGemm& p) {
+  if constexpr (EPI == VE_LSE) return p.nb;
+  const int n = __builtin_amdgcn_readfirstlane(*p.count);
+  if constexpr (EPI == VE_STORE) {
+    p.kr = n;
+    p.K = (n + 63) / 64 * 64;
+    return p.nb;
+  }
+  return n;
 }
 
 // 8 codes of a chunk as bf16 (exact)
@@ -385,7 +403,8 @@ __global__ __launch_bounds__(kVThreads, ONE ? 4 : 2) void vocab_gemm_kernel(cons
   int mt, nt;
   if (!tile_dense(blockIdx.x, p.m_tiles, p.n_tiles, mt, nt)) return;
   const int n0 = nt * BN, m0 = mt * BM;
-  const int arows = min(BN, p.na - n0), brows = min(BM, p.nb - m0);
+  const int arows = min(BN, p.na - n0), brows = min(BM, live_rows<EPI>(p) - m0);
+  if ((EPI == VE_PROB || EPI == VE_SUM) && brows <= 0) return;
 
   // copies: one instruction = 8 rows x 128 bytes (lane -> row l >> 3, slot l & 7;
   // the slot of chunk c of row r is c ^ vg_swz(r)) or, of codes, 16 rows x 64
@@ -559,7 +578,7 @@ __global__ __launch_bounds__(kVThreads, ONE ? 4 : 2) void vocab_gemm_kernel(cons
 // the last piece, dx
 __global__ __launch_bounds__(256) void vocab_slices_kernel(const VocabGemm p, int slices) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, n = (int64_t)p.nb * p.ldsum;
-  if (i >= n) return;
+  if (i >= (int64_t)*p.count * p.ldsum) return;
   const int64_t row = i / p.ldsum;
   const int c = (int)(i - row * p.ldsum);
   float4 v = p.first ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *reinterpret_cast<const float4*>(p.sum + i);
@@ -568,7 +587,7 @@ __global__ __launch_bounds__(256) void vocab_slices_kernel(const VocabGemm p, in
     v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
   }
   if (!p.last) *reinterpret_cast<float4*>(p.sum + i) = v;
-  else *reinterpret_cast<uint2*>(p.y + row * p.ldy + c) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+  else *reinterpret_cast<uint2*>(p.y + p.live[row] * p.ldy + c) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
 
 // The same product in tiles of 256 x 256 (or 192: 4 x 3 blocks) by four wavefronts
@@ -613,7 +632,8 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
   int mt, nt;
   if (!tile_dense(blockIdx.x, p.m_tiles, p.n_tiles, mt, nt)) return;
   const int n0 = nt * BN, m0 = mt * BM;
-  const int arows = min(BN, p.na - n0), brows = min(BM, p.nb - m0);
+  const int arows = min(BN, p.na - n0), brows = min(BM, live_rows<EPI>(p) - m0);
+  if ((EPI == VE_PROB || EPI == VE_SUM) && brows <= 0) return;
 
   // copies: one instruction = 8 rows x 128 bytes (lane -> row l >> 3, slot l & 7;
   // the slot of chunk c of row r is c ^ vg_swz(r)); wavefront w moves the row
@@ -807,27 +827,63 @@ __global__ __launch_bounds__(256) void vocab_expand_kernel(const uint8_t* w, int
   *reinterpret_cast<bf16x8*>(out + r * ldo + c) = codes8_to_bf16<WT>(d.x, d.y);
 }
 
-// x rows [R][C] -> out [C][ldo] bf16, columns R .. zero up to the next multiple of
-// 64; a row whose token has no gradient becomes zeros (whatever it holds). 64 x
-// 64 tiles through LDS.
-__global__ __launch_bounds__(256) void vocab_transpose_kernel(const uint8_t* src, int64_t ld, int R, int C,
-                                                              uint16_t* out, int64_t ldo, const void* targets,
-                                                              int targets_i64, int64_t ignore, const float* g_loss,
-                                                              const float* g_lse) {
+// The tokens with a gradient, in order: live[k] = t, place[t] = k or -1, *count. One
+// workgroup, 1024 tokens at a time.
+__global__ __launch_bounds__(1024) void vocab_live_kernel(int T, const void* targets, int targets_i64, int64_t ignore,
+                                                          const float* g_loss, const float* g_lse, int32_t* live,
+                                                          int32_t* place, int32_t* count) {
+  __shared__ int part[2][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint64_t below = lane ? ~0ull >> (64 - lane) : 0ull;
+  int base = 0;
+  for (int t0 = 0, side = 0; t0 < T; t0 += 1024, side ^= 1) {
+    const int t = t0 + tid;
+    bool is = false;
+    if (t < T) {
+      const int64_t tg = targets_i64 ? static_cast<const int64_t*>(targets)[t]
+                                     : (int64_t) static_cast<const int32_t*>(targets)[t];
+      is = (tg != ignore && g_loss[t] != 0.0f) || (g_lse && g_lse[t] != 0.0f);
+    }
+    const uint64_t m = __ballot(is);
+    if (lane == 0) part[side][wave] = __popcll(m);
+    __syncthreads();  // (the other side is written next)
+    int before = base;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) before += part[side][w];
+      base += part[side][w];
+    }
+    const int k = before + __popcll(m & below);
+    if (is) live[k] = t;
+    if (t < T) place[t] = is ? k : -1;
+  }
+  if (tid == 0) *count = base;
+}
+
+// Rows of x of the tokens with a gradient, one after the other, and zeros in dx
+// (when not null) for the others. A workgroup per row.
+__global__ __launch_bounds__(256) void vocab_gather_kernel(const uint16_t* x, int64_t ldx, int H, const int32_t* place,
+                                                           uint16_t* out, uint16_t* dx, int64_t lddx) {
+  const int64_t t = blockIdx.x;
+  const int k = place[t];
+  const uint4* src = reinterpret_cast<const uint4*>(x + t * ldx);
+  uint4* dst = reinterpret_cast<uint4*>(k >= 0 ? out + (int64_t)k * H : dx + t * lddx);
+  if (k < 0 && !dx) return;
+  for (int c = threadIdx.x; c < H / 8; c += 256) dst[c] = k >= 0 ? src[c] : make_uint4(0, 0, 0, 0);
+}
+
+// Their rows [*count][C] -> out [C][ldo], columns from *count on zero. 64 x 64 tiles
+// through LDS.
+__global__ __launch_bounds__(256) void vocab_transpose_kernel(const uint8_t* src, int64_t ld, const int32_t* count, int C,
+                                                              uint16_t* out, int64_t ldo) {
   __shared__ uint16_t tile[64][66];
-  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, R = *count;
   const int tid = threadIdx.x;
   {
     const int c = (tid & 7) * 8;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int r = (tid >> 3) + 32 * k;
-      bool live = r0 + r < R && c0 + c < C;
-      if (live) {
-        const int64_t tg = targets_i64 ? static_cast<const int64_t*>(targets)[r0 + r]
-                                       : (int64_t) static_cast<const int32_t*>(targets)[r0 + r];
-        live = (tg != ignore && g_loss[r0 + r] != 0.0f) || (g_lse && g_lse[r0 + r] != 0.0f);
-      }
+      const bool live = r0 + r < R && c0 + c < C;
       uint4 v = make_uint4(0, 0, 0, 0);
       if (live) v = *reinterpret_cast<const uint4*>(src + (int64_t)(r0 + r) * ld + (int64_t)(c0 + c) * 2);
       const uint32_t u[4] = {v.x, v.y, v.z, v.w};
@@ -944,13 +1000,6 @@ struct LossArgs {
   int64_t ignore;
 };
 
-void launch_transpose(const LossArgs& a, uint16_t* out, int64_t ldo, const float* g_loss, const float* g_lse,
-                      hipStream_t st) {
-  hipLaunchKernelGGL(vocab_transpose_kernel, dim3((unsigned)cdiv(a.T, (int64_t)64), (unsigned)cdiv(a.H, (int64_t)64)),
-                     dim3(256), 0, st, static_cast<const uint8_t*>(a.x), a.ldx * 2, (int)a.T, (int)a.H, out, ldo,
-                     a.targets, a.targets_i64, a.ignore, g_loss, g_lse);
-}
-
 // sizes whose tile counts, and the threads of their grids, fit 32 bits
 constexpr int64_t kMaxTokens = (int64_t)1 << 20, kMaxVocab = (int64_t)1 << 24, kMaxHidden = (int64_t)1 << 16;
 
@@ -1023,8 +1072,8 @@ DxPlan dx_plan(int64_t T, int64_t H, int64_t K) {
   return d;
 }
 
-// P, x transposed, float32 sums, K slices, expanded rows
-int64_t grad_layout(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw, int64_t (&off)[5]) {
+// P, x transposed, float32 sums, K slices, expanded rows, x gathered, the tokens' list
+int64_t grad_layout(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw, int64_t (&off)[7]) {
   const int64_t Vc = grad_piece(T, V, H, wtype), Tw = up(T, 64);
   const bool pieces = Vc < V;
   int64_t at = 0;
@@ -1041,7 +1090,10 @@ int64_t grad_layout(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int
   }
   off[4] = at;
   if (wtype) at += up(Vc * H * 2, 256);
-  return at;
+  off[5] = at;
+  at += up(T * H * 2, 256);
+  off[6] = at;
+  return at + up((2 * T + 1) * 4, 256);
 }
 
 }  // namespace
@@ -1103,7 +1155,7 @@ extern "C" int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void
 extern "C" int qmoe_vocab_loss_grad_workspace_size(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw,
                                                    int64_t* bytes) {
   if (!loss_sizes_ok(T, V, H) || (wtype != 0 && (wtype < 3 || wtype > 5)) || !bytes) return QMOE_ERR_ARG;
-  int64_t off[5];
+  int64_t off[7];
   *bytes = grad_layout(T, V, H, wtype, need_dx, need_dw, off);
   return QMOE_OK;
 }
@@ -1118,13 +1170,21 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
   if (dw && wtype) return QMOE_ERR_ARG;  // codes have no gradient
   if (dx && (lddx < H || lddx % 8 || (reinterpret_cast<uintptr_t>(dx) & 15))) return QMOE_ERR_ARG;
   if (dw && (lddw < H || lddw % 8 || (reinterpret_cast<uintptr_t>(dw) & 15))) return QMOE_ERR_ARG;
-  int64_t off[5];
+  int64_t off[7];
   if (!workspace || ws_bytes < grad_layout(T, V, H, wtype, dx != nullptr, dw != nullptr, off)) return QMOE_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int64_t Vc = grad_piece(T, V, H, wtype), Tw = up(T, 64);
   uint16_t* P = reinterpret_cast<uint16_t*>(ws + off[0]);
   uint16_t* XT = reinterpret_cast<uint16_t*>(ws + off[1]);
-  if (dw) launch_transpose(a, XT, Tw, g_loss, g_lse, stream);
+  uint16_t* X = reinterpret_cast<uint16_t*>(ws + off[5]);
+  int32_t *live = reinterpret_cast<int32_t*>(ws + off[6]), *place = live + T, *count = place + T;
+  hipLaunchKernelGGL(vocab_live_kernel, dim3(1), dim3(1024), 0, stream, (int)T, targets, targets_i64, ignore_index, g_loss,
+                     g_lse, live, place, count);
+  hipLaunchKernelGGL(vocab_gather_kernel, dim3((unsigned)T), dim3(256), 0, stream, static_cast<const uint16_t*>(x), ldx, (int)H,
+                     place, X, static_cast<uint16_t*>(dx), lddx);
+  if (dw)
+    hipLaunchKernelGGL(vocab_transpose_kernel, dim3((unsigned)(Tw / 64), (unsigned)cdiv(H, (int64_t)64)), dim3(256), 0, stream,
+                       reinterpret_cast<const uint8_t*>(X), H * 2, count, (int)H, XT, Tw);
   for (int64_t v0 = 0; v0 < V; v0 += Vc) {
     const uint8_t* rows = static_cast<const uint8_t*>(w) + v0 * ldw * (wtype ? 1 : 2);
     const int64_t n = std::min(Vc, V - v0), np = up(n, 64);
@@ -1138,8 +1198,10 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
       g.lda = H * 2;
     }
     g.na = (int)n;
-    g.b = static_cast<const uint8_t*>(x);
-    g.ldb = ldx * 2;
+    g.b = reinterpret_cast<const uint8_t*>(X);
+    g.ldb = H * 2;
+    g.live = live;
+    g.count = count;
     g.nb = (int)T;
     g.K = (int)H;
     g.row_scale = row_scale ? row_scale + v0 : nullptr;
@@ -1156,6 +1218,8 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
     launch_gemm<VE_PROB>(g, 0, vocab_bm(n, T), 1, stream);
     if (dx) {
       VocabGemm d{};
+      d.live = live;
+      d.count = count;
       d.a = g.a;
       d.lda = g.lda;
       d.na = (int)H;
@@ -1182,6 +1246,8 @@ extern "C" int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const
     }
     if (dw) {
       VocabGemm d{};
+      d.live = live;
+      d.count = count;
       d.a = reinterpret_cast<const uint8_t*>(XT);
       d.lda = Tw * 2;
       d.na = (int)H;
