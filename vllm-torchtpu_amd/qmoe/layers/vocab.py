@@ -141,8 +141,13 @@ class _VocabCrossEntropy(torch.autograd.Function):
         return loss, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, g_lse):
+        if torch.is_grad_enabled():  # (as above)
+            return _VocabCrossEntropy._once(ctx, g_loss, g_lse)
+        return _VocabCrossEntropy._grads(ctx, g_loss, g_lse)
+
+    @staticmethod
+    def _grads(ctx, g_loss, g_lse):
         x, weight, targets, weight_scale, lse = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
         if g_loss is None and g_lse is None:
@@ -152,6 +157,8 @@ class _VocabCrossEntropy(torch.autograd.Function):
         fn = ops.vocab_loss_grad if ops.eager_call(x, weight, g_loss, g_lse) else torch.ops.qmoe.vocab_loss_grad
         dx, dw = fn(x, weight, targets, lse, g_loss, g_lse, weight_scale, ctx.ignore_index, need_x, need_w)
         return (dx if need_x else None), (dw if need_w else None), None, None, None
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_grads.__func__))
 
 
 def _loss(x, weight, targets, weight_scale, ignore_index):

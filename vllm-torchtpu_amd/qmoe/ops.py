@@ -952,6 +952,21 @@ def _loss_operands(x, weight, targets, weight_scale, what):
     return x2, t, s
 
 
+@functools.lru_cache(maxsize=256)
+def _loss_bytes(T, V, H, wtype):
+    need = ctypes.c_int64(0)
+    check(lib.qmoe_vocab_loss_workspace_size(T, V, H, wtype, ctypes.byref(need)), "vocab_loss (shape)")
+    return need.value
+
+
+@functools.lru_cache(maxsize=256)
+def _loss_grad_bytes(T, V, H, wtype, need_x, need_weight):
+    need = ctypes.c_int64(0)
+    check(lib.qmoe_vocab_loss_grad_workspace_size(T, V, H, wtype, need_x, need_weight, ctypes.byref(need)),
+          "vocab_loss_grad (shape)")
+    return need.value
+
+
 def vocab_loss(x, weight, targets, weight_scale=None, ignore_index=-100):
     """Softmax cross entropy of ``x`` [..., H] (bf16) projected onto the table
     [V, H]: float32 (loss, log of the sum of exponentials), both of the
@@ -963,12 +978,11 @@ def vocab_loss(x, weight, targets, weight_scale=None, ignore_index=-100):
         loss, lse = torch.empty(targets.shape, device=dev), torch.empty(targets.shape, device=dev)
         if T == 0:
             return loss, lse
-        need, wt = ctypes.c_int64(0), _TABLE_TYPES[weight.dtype]
-        check(lib.qmoe_vocab_loss_workspace_size(T, V, H, wt, ctypes.byref(need)), "vocab_loss (shape)")
-        ws, ws_n = _workspace(dev, need.value)
-        check(lib.qmoe_vocab_loss(_ptr(x2), x2.stride(0), T, _ptr(weight), wt, weight.stride(0), _ptr(s), V, H, _ptr(t),
-                                  int(t.dtype == torch.int64), int(ignore_index), _ptr(loss), _ptr(lse), _ptr(ws), ws_n,
-                                  _raw_stream(dev)), "vocab_loss")
+        wt = _TABLE_TYPES[weight.dtype]
+        ws, ws_n = _workspace(dev, _loss_bytes(T, V, H, wt))
+        check(lib.qmoe_vocab_loss(x2.data_ptr(), x2.stride(0), T, weight.data_ptr(), wt, weight.stride(0), _addr(s), V, H,
+                                  t.data_ptr(), t.dtype is torch.int64, int(ignore_index), loss.data_ptr(), lse.data_ptr(),
+                                  _addr(ws), ws_n, _raw_stream(dev)), "vocab_loss")
     return loss, lse
 
 
@@ -994,12 +1008,10 @@ def vocab_loss_grad(x, weight, targets, lse, g_loss, g_lse=None, weight_scale=No
         if T == 0 and dw is not None:
             dw.zero_()
         if T and (need_x or need_weight):
-            need, wt = ctypes.c_int64(0), _TABLE_TYPES[weight.dtype]
-            check(lib.qmoe_vocab_loss_grad_workspace_size(T, V, H, wt, int(need_x), int(need_weight), ctypes.byref(need)),
-                  "vocab_loss_grad (shape)")
-            ws, ws_n = _workspace(dev, need.value)
-            check(lib.qmoe_vocab_loss_grad(_ptr(x2), x2.stride(0), T, _ptr(weight), wt, weight.stride(0), _ptr(s), V, H,
-                                           _ptr(t), int(t.dtype == torch.int64), int(ignore_index), _ptr(lse),
-                                           _ptr(g_loss), _ptr(g_lse), _ptr(dx), H, _ptr(dw), H, _ptr(ws), ws_n,
-                                           _raw_stream(dev)), "vocab_loss_grad")
+            wt = _TABLE_TYPES[weight.dtype]
+            ws, ws_n = _workspace(dev, _loss_grad_bytes(T, V, H, wt, bool(need_x), bool(need_weight)))
+            check(lib.qmoe_vocab_loss_grad(x2.data_ptr(), x2.stride(0), T, weight.data_ptr(), wt, weight.stride(0),
+                                           _addr(s), V, H, t.data_ptr(), t.dtype is torch.int64, int(ignore_index),
+                                           lse.data_ptr(), g_loss.data_ptr(), _addr(g_lse), _addr(dx), H, _addr(dw), H,
+                                           _addr(ws), ws_n, _raw_stream(dev)), "vocab_loss_grad")
     return (dx.view(x.shape) if dx is not None else None), dw
