@@ -6,10 +6,11 @@ models put behind it, and its gradient for a bf16 or f32 table.
 ``vocab_cross_entropy`` scores tokens against the output projection (the tied
 table of `fp8.py:1679-1681`) without the [T, V] logits, and its gradients.
 
-Both run as torch custom ops (``torch.ops.qmoe.vocab_lookup`` ...) under
-`torch.compile` and fake tensors, and straight on the C ABI in eager mode: the
-op's dispatch takes longer than a decode step's lookup. Gradients come from
-`torch.autograd.Function`s around them.
+Both run as torch custom ops (``torch.ops.qmoe.vocab_lookup`` ...) under a
+trace, a dispatch mode, a functorch transform and fake tensors, and straight on
+the C ABI in eager mode: the op's dispatch takes longer than a decode step's
+lookup. Gradients come from `torch.autograd.Function`s around them; there is no
+forward-mode derivative, and a tangent is refused.
 """
 
 from typing import Optional, Tuple
@@ -62,10 +63,11 @@ class _Embedding(torch.autograd.Function):
     def _grads(ctx, grad):
         (ids,) = ctx.saved_tensors
         vocab, scale, padding_idx, dtype = ctx.args
-        if torch.compiler.is_compiling() or type(grad) is not torch.Tensor or not grad.is_contiguous() or \
-                not ids.is_contiguous() or grad.get_device() != torch.cuda.current_device():
-            fn = ops.vocab_lookup_grad if ops.eager_call(grad, ids) else torch.ops.qmoe.vocab_lookup_grad
-            return None, fn(grad, ids, vocab, scale, padding_idx, dtype), None, None, None
+        if not ops.eager_call(grad, ids):
+            dw = torch.ops.qmoe.vocab_lookup_grad(grad, ids, vocab, scale, padding_idx, dtype)
+            return None, dw, None, None, None
+        if not grad.is_contiguous() or not ids.is_contiguous() or grad.get_device() != torch.cuda.current_device():
+            return None, ops.vocab_lookup_grad(grad, ids, vocab, scale, padding_idx, dtype), None, None, None
         H = grad.shape[-1]
         dw = ops.lookup_grad_run(grad, H, ids if ids.dim() == 1 else ids.view(-1), vocab, H, scale,
                                  -1 if padding_idx is None else padding_idx, dtype)
@@ -94,6 +96,7 @@ def embedding(ids, weight, weight_scale=None, scale=1.0, padding_idx=None, out_d
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"embedding: padding_idx {padding_idx} is outside the table of {weight.shape[0]} rows")
     scale = float(scale)
+    ops.refuse_tangents("embedding", weight, weight_scale)
     if torch.is_grad_enabled() and (weight.requires_grad or (weight_scale is not None and weight_scale.requires_grad)):
         if weight_scale is not None:
             raise NotImplementedError("embedding: no gradient for a table of 1-byte codes or its scales")
@@ -184,6 +187,7 @@ def vocab_cross_entropy(x, weight, targets, weight_scale=None, ignore_index=-100
     (gradients in bf16; a table of codes is frozen). The sums' order is fixed:
     the same bits on every call."""
     ignore_index = int(ignore_index)
+    ops.refuse_tangents("vocab_cross_entropy", x, weight, weight_scale)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
                                     (weight_scale is not None and weight_scale.requires_grad)):
         if weight_scale is not None and (weight.requires_grad or weight_scale.requires_grad):

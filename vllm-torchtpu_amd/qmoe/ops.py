@@ -11,6 +11,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from qmoe import _capi
 from qmoe._capi import GemmDesc, check, lib
@@ -56,14 +57,36 @@ else:
 
 _PLAIN = frozenset((type(None), torch.Tensor, torch.nn.Parameter))
 
+# Dispatch keys that a thread includes without being asked to: a dispatch mode, the TorchScript tracer and a functorch
+# transform each add their own while they are active
+_WATCHING = ~(torch._C.DispatchKeySet(torch._C.DispatchKey.BackendSelect).raw_repr()
+              | torch._C.DispatchKeySet(torch._C.DispatchKey.ADInplaceOrView).raw_repr())
+_included_keys = torch._C._dispatch_tls_local_include_set
+
 
 def eager_call(*ts):
-    """Whether a call on these tensors runs at once (plain tensors outside of a
-    trace), so that no dispatcher has to see it."""
+    """Whether a call on these tensors runs at once, so that no dispatcher has to
+    see it: plain tensors, and neither a trace (torch.compile, make_fx,
+    torch.jit.trace), a dispatch mode nor a functorch transform on this thread."""
+    if torch.compiler.is_compiling():
+        return False
     for t in ts:
         if type(t) not in _PLAIN:
             return False
-    return not torch.compiler.is_compiling()
+    return not _included_keys().raw_repr() & _WATCHING
+
+
+def has_tangent(*ts):
+    """Whether one of these tensors (None aside) carries a forward-mode tangent."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
+
+
+def refuse_tangents(what, *ts):
+    """The operators have no forward-mode derivative: an operand that carries a
+    tangent is an error, where the result would come back without one."""
+    if has_tangent(*ts):
+        raise NotImplementedError(f"{what}: no forward-mode derivative")
 
 
 def _require_gpu(*ts):
