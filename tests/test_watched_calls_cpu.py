@@ -163,3 +163,15 @@ def test_method_embedding_traces_and_batches(dtype):
         layer.weight_scale = fw.make_dual(layer.weight_scale, torch.ones(10))
         tangent = fw.unpack_dual(fn(IDS)).tangent
         assert torch.equal(tangent, TABLE.to(dtype).to(BF16)[IDS])
+
+
+@pytest.mark.parametrize("which", ["x", "logits", "w1", "w2", "bias"])
+def test_a_gradient_asked_of_the_layer_is_an_error(which):
+    """Of any operand, the correction bias among them: the output says so when
+    the gradient is asked for."""
+    x, (lg, w1, w2), bias = torch.zeros(3, 32, dtype=BF16), _experts(), torch.zeros(4)
+    {"x": x, "logits": lg, "w1": w1, "w2": w2, "bias": bias}[which].requires_grad_()
+    out = few_token_moe(x, lg, w1, w2, None, None, None, None, 2, "silu", e_score_correction_bias=bias)
+    assert out.requires_grad
+    with pytest.raises(RuntimeError, match="autograd"):
+        out.sum().backward()
