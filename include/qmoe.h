@@ -380,8 +380,9 @@ int qmoe_moe_decode(const qmoe_moe_decode_desc* d, void* workspace, int64_t ws_b
  * (qmoe_moe_route's rule, float32 weights), then for every route j of token t
  *   h[t, j] = bf16(act(W13[e] x[t] + b13[e])),
  *   out[t] = bf16(sum over j of w[t, j] (W2[e] h[t, j] + b2[e])),
- * float32 sums in a fixed order, each weight bf16(code * scale) and bf16
- * activations (the dequantize-before-matmul regime of
+ * float32 sums in a fixed order, each weight bf16(code * scale) (FP8:
+ * bf16(code * bf16(scale)), as QMOE_W8A16_BLK) and bf16 activations (the
+ * dequantize-before-matmul regime of
  * `kernels/megablox/gmm_v2.py:452-462`). Replaces `layers/adapter/
  * moe_routing.py:232-323` followed by `layers/core/fused_moe_gmm.py:592-728`
  * for 1..16 tokens; against qmoe_moe_route_dispatch + qmoe_gemm (twice) +
@@ -392,7 +393,7 @@ enum {
   QMOE_FEW_MXFP4 = 0, /* e2m1 + e8m0 per 32 k */
   QMOE_FEW_NVFP4 = 1, /* e2m1 + bf16 per 16 k */
   QMOE_FEW_INT4 = 2,  /* offset-binary nibbles + bf16 per `group` k */
-  QMOE_FEW_FP8 = 3,   /* e4m3 + f32 per (row, 128 k) */
+  QMOE_FEW_FP8 = 3,   /* e4m3 + f32 per (row, 128 k), rounded to bf16 */
   QMOE_FEW_BF16 = 4
 };
 typedef struct qmoe_moe_few_desc {

@@ -327,3 +327,67 @@ def test_a_scale_that_is_no_number_stays_in_its_row(dev, fmt, T):
     assert not out[:, bad].isfinite().any()
     kept = [n for n in range(96) if n not in bad]
     assert torch.equal(out[:, kept], clean[:, kept])
+
+
+def _by_definition(c):
+    """The experts' values as the weight formats define them, in float64: fp8's
+    scales, too, are rounded to bf16 before they multiply the codes."""
+    if c.fmt != "fp8_w8a16":
+        return c.v1, c.v2
+    return tuple((q.float() * s.to(BF16).float().repeat_interleave(128, -1)).to(BF16).double()
+                 for q, s in ((c.w1, c.s1), (c.w2, c.s2)))
+
+
+def _check_both(c, after, before, tw, ids):
+    """Both paths' outputs against the layer with its bf16 intermediate values in
+    float64. A value of h that float32 sums may round either way moves by its
+    step (`flip`); the four-launch path (`before`) also rounds the routing
+    weights and the route outputs to bf16, half a step each."""
+    v1, v2 = _by_definition(c)
+    T, k, H, I = c.T, c.k, c.H, c.I
+    e, x = ids.long().flatten(), c.x.double().repeat_interleave(k, 0)
+    ref, bound, mag = (torch.zeros((T, H), dtype=torch.float64, device=x.device) for _ in range(3))
+    for r in range(T * k):
+        w, W1, W2 = float(tw.flatten()[r]), v1[e[r]], v2[e[r]]
+        gu, gue = W1 @ x[r], (H + 8) * EPS * (W1.abs() @ x[r].abs())
+        if c.b1 is not None:
+            gu = gu + c.b1[e[r]].double()
+            gue = gue + EPS * gu.abs()
+        h, dg, du, fac = _act("silu", gu[:I], gu[I:])
+        he = 1.01 * (dg * gue[:I] + du * gue[I:]) + 32 * EPS * fac
+        hr, lo, hi = (v.to(BF16).double() for v in (h, h - he, h + he))
+        flip = torch.maximum((lo - hr).abs(), (hi - hr).abs())
+        y, size = W2 @ hr, W2.abs() @ (hr.abs() + flip)
+        ye = W2.abs() @ flip + (I + 8) * EPS * size
+        if c.b2 is not None:
+            y = y + c.b2[e[r]].double()
+        ref[r // k] += w * y
+        bound[r // k] += abs(w) * (ye + (2 * k + 16) * EPS * (y.abs() + ye + size))
+        mag[r // k] += abs(w) * (y.abs() + ye)
+    for out, more in ((after, 0.0), (before, (2 * HALF + HALF * HALF) * mag)):
+        lim = bound + more
+        lim = lim + HALF * (ref.abs() + lim)
+        off = (out.double() - ref).abs()
+        assert out.shape == (T, H) and (off <= lim).all(), float((off / lim).max())
+
+
+def _method_outputs(c, monkeypatch, limit):
+    """The layer through `moe_forward`: by the two-launch layer, and without it."""
+    layer = SimpleNamespace(moe_config=SimpleNamespace(experts_per_token=c.k), _qmoe_activation="silu",
+                            scoring_func="softmax", renormalize=True)
+    outs = []
+    for switch in (limit, "0"):
+        monkeypatch.setenv("QMOE_FEW_TOKEN_MOE", switch)
+        outs.append(moe_forward(layer, c.x, c.logits, c.w1, c.w2, c.s1, c.s2, c.b1, c.b2, c.fmt))
+    return outs
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("T", [1, 6])
+def test_the_switch_keeps_the_weights(dev, fmt, T, monkeypatch):
+    """With and without the switch a layer multiplies by the same weights: the
+    results differ by the routing weights' and route outputs' roundings alone."""
+    c = _layer(dev, fmt, T, 32, 4, 256, 128, seed=16)
+    after, before = _method_outputs(c, monkeypatch, "16")
+    tw, ids = ops.moe_route(c.logits, 4, weights_f32=True)
+    _check_both(c, after, before, tw, ids)

@@ -28,8 +28,9 @@
 //  * Sums are float32: per wavefront, then over the wavefronts in order; in
 //    launch 2 over the slots in ascending order per wavefront.
 //  * Rounded to bf16 are the matrix cores' operands: h, and code x scale of the
-//    4- and 8-bit formats (exact for MXFP4), as in the other bf16-activation
-//    paths; and out, once.
+//    4- and 8-bit formats (exact for MXFP4; the float32 scales of FP8 are
+//    rounded to bf16 before the product), as in the other bf16-activation paths;
+//    and out, once.
 //
 // Measured, launch 1 + 2: one token, MXFP4, 4 of 128 experts of 2880 x 2880 15.0 +
 // 8.7 us; 16 tokens 113 + 72 (442 and 236 MiB read: 4.1 and 3.4 TB/s; 17 us of
@@ -165,7 +166,7 @@ __device__ __forceinline__ uint4 e2m1x8_to_bf16(uint32_t d, float scale) {
   return r.u;
 }
 
-// 8 e4m3 codes (two dwords) times a float32 scale, each rounded once to bf16
+// 8 e4m3 codes (two dwords) times a scale, each product rounded once to bf16
 __device__ __forceinline__ uint4 e4m3x8_to_bf16(uint32_t a, uint32_t b, float s) {
   typedef float v2f __attribute__((ext_vector_type(2)));
   const v2f f0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)a, false), f1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)a, true);
@@ -188,7 +189,7 @@ __device__ __forceinline__ uint4 expand8(const uint4& c, int i, uint32_t s) {
   if constexpr (F == FF_MX) return e2m1x8_to_bf16(d[i], e8m0_to_f32(s));
   else if constexpr (F == FF_NV) return nvfp4x8_to_bf16(d[i], bf16_to_f32((uint16_t)(i < 2 ? s : s >> 16)));
   else if constexpr (F == FF_I4) return int4x8_to_bf16(d[i], bf16_to_f32((uint16_t)s));
-  else if constexpr (F == FF_F8) return e4m3x8_to_bf16(d[2 * i], d[2 * i + 1], bits_f32(s));
+  else if constexpr (F == FF_F8) return e4m3x8_to_bf16(d[2 * i], d[2 * i + 1], bf16_round(bits_f32(s)));
   else return c;
 }
 
