@@ -150,3 +150,33 @@ def test_a_gradient_asked_of_it_is_an_error():
         assert out.requires_grad
         with torch.no_grad():
             assert not few_token_moe(*a, 2, "silu").requires_grad
+
+
+@pytest.mark.parametrize("T,topk,switch,takes", [(1, 4, 16, True), (8, 8, 16, True), (9, 8, 16, True), (16, 8, 16, True),
+                                                 (16, 9, 16, False), (9, 8, 8, False), (9, 8, 0, False), (17, 1, 64, False)])
+def test_which_steps_of_a_method_take_it(monkeypatch, T, topk, switch, takes):
+    """Every step that the layer has a form for, up to the switch's tokens,
+    whatever the route + dispatch launch of the other path holds."""
+    from types import SimpleNamespace
+
+    from qmoe.layers import fused_moe, moe_routing
+
+    called = []
+    monkeypatch.setenv("QMOE_FEW_TOKEN_MOE", str(switch))
+    monkeypatch.setattr(fused_moe, "few_token_moe", lambda *a, **k: called.append("few"))
+    monkeypatch.setattr(fused_moe, "fused_moe_gmm", lambda *a, **k: called.append("other"))
+    monkeypatch.setattr(moe_routing, "route", lambda *a, **k: (None, None))
+    layer = SimpleNamespace(moe_config=SimpleNamespace(experts_per_token=topk), _qmoe_activation="silu",
+                            scoring_func="softmax", renormalize=True)
+    a = _operands("bf16", T=T, E=16)
+    run = lambda ly, x: fused_moe.moe_forward(ly, x, *a[1:], "bf16")  # noqa: E731
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        run(layer, a[0])
+        assert (called == ["few"]) == takes
+        del called[:]
+        # a model's own routing function, other activations: never
+        layer.custom_routing_function = lambda *x, **k: None
+        run(layer, a[0])
+        del layer.custom_routing_function
+        run(layer, a[0].float())
+        assert called == ["other", "other"]

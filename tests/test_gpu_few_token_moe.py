@@ -391,3 +391,14 @@ def test_the_switch_keeps_the_weights(dev, fmt, T, monkeypatch):
     after, before = _method_outputs(c, monkeypatch, "16")
     tw, ids = ops.moe_route(c.logits, 4, weights_f32=True)
     _check_both(c, after, before, tw, ids)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("T,k", [(9, 8), (16, 8), (11, 10)])
+def test_methods_take_steps_of_up_to_128_routes(dev, fmt, T, k, monkeypatch):
+    """More routes than the other path's route + dispatch launch holds."""
+    c = _layer(dev, fmt, T, 32, k, 256, 128, seed=17)
+    after, before = _method_outputs(c, monkeypatch, "16")
+    assert torch.equal(after, _run(c))
+    tw, ids = ops.moe_route(c.logits, k, weights_f32=True)
+    _check_both(c, after, before, tw, ids)

@@ -295,8 +295,9 @@ def moe_forward(layer, x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2
     routes) with the layer's own scoring takes the fused route + dispatch
     launch; anything else (a model-supplied routing function, hash routing,
     larger batches) routes first and calls `fused_moe_gmm`. With
-    ``QMOE_FEW_TOKEN_MOE`` set, such a batch of at most that many tokens runs
-    `few_token_moe` where it has the weight format and the sizes."""
+    ``QMOE_FEW_TOKEN_MOE`` set, a batch of at most that many bf16 tokens with
+    the layer's own scoring runs `few_token_moe` where it has the weight format
+    and the sizes (at most 128 routes)."""
     from qmoe import envs
     from qmoe.layers import moe_routing
 
@@ -305,20 +306,20 @@ def moe_forward(layer, x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2
     custom = getattr(layer, "custom_routing_function", None)
     hashed = getattr(layer, "hash_indices_table", None) is not None and input_ids is not None
     act = layer._qmoe_activation
-    fusable = (custom is None and not hashed and x.dtype == torch.bfloat16
-               and 1 <= T <= ops.ROUTE_DISPATCH_MAX_TOKENS and T * topk <= ops.ROUTE_DISPATCH_MAX_ROUTES
-               and w1.shape[0] <= 512 and layer.scoring_func in ops._SCORING)
-    if not fusable:
-        topk_weights, topk_ids = moe_routing.route(layer, x, router_logits, input_ids=input_ids)
-        return fused_moe_gmm(x, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk_weights, topk_ids, None, topk,
-                             act, skip_padded_tokens=skip_padded_tokens, weight_format=weight_format)
-    ops.act_code(act)
-    if T <= envs.QMOE_FEW_TOKEN_MOE and act and ops.few_token_moe_takes(T, topk, weight_format, w2, w2_scale):
+    own = custom is None and not hashed and x.dtype == torch.bfloat16 and layer.scoring_func in ops._SCORING
+    if own and act and T <= envs.QMOE_FEW_TOKEN_MOE and ops.few_token_moe_takes(T, topk, weight_format, w2, w2_scale):
         bias, rsf, ng, tg = moe_routing.routing_params(layer)
         return few_token_moe(x, router_logits, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk, act,
                              weight_format=weight_format, scoring_func=layer.scoring_func, renormalize=layer.renormalize,
                              e_score_correction_bias=bias, routed_scaling_factor=rsf, num_expert_group=ng, topk_group=tg,
                              skip_padded_tokens=skip_padded_tokens)
+    fusable = (own and 1 <= T <= ops.ROUTE_DISPATCH_MAX_TOKENS and T * topk <= ops.ROUTE_DISPATCH_MAX_ROUTES
+               and w1.shape[0] <= 512)
+    if not fusable:
+        topk_weights, topk_ids = moe_routing.route(layer, x, router_logits, input_ids=input_ids)
+        return fused_moe_gmm(x, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, topk_weights, topk_ids, None, topk,
+                             act, skip_padded_tokens=skip_padded_tokens, weight_format=weight_format)
+    ops.act_code(act)
     if _dense_expert_admitted(x, w1, w2, w1_scale, w2_scale, w1_bias, w2_bias, act, weight_format):
         skip_padded_tokens = True  # the dense-expert branch's coefficient mask, as in fused_moe_gmm
     bias, rsf, ng, tg = moe_routing.routing_params(layer)
