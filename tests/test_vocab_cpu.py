@@ -155,3 +155,20 @@ def test_no_gradient_through_row_scales():
         vocab_cross_entropy(x, q, ids, s)
     with torch.no_grad(), pytest.raises(ValueError, match="device tensors"):
         embedding(ids, q, s)
+
+
+def test_which_tables_of_a_method_the_lookup_takes():
+    """The others keep the method's torch operations, and with them their results,
+    errors and gradients."""
+    z = lambda *s, dtype=torch.int8: torch.empty(s, dtype=dtype, device="meta")  # noqa: E731
+    w, s, ids = z(50, 64), z(50, 1, dtype=torch.float32), z(3, 4, dtype=torch.int64)
+    takes = lambda i=ids, t=w, r=s, o=torch.bfloat16: ops.vocab_lookup_takes(i, t, r, o)  # noqa: E731
+    assert takes() and takes(t=z(50, 64, dtype=torch.float8_e4m3fn)) and takes(t=z(50, 96)[:, :64]) and takes(i=ids[:0])
+    assert takes(i=z((1 << 24) - 1, dtype=torch.int32)) and not takes(i=z(1 << 24, dtype=torch.int32))
+    assert takes(t=z(1 << 27, 8), r=z(1 << 27, dtype=torch.float32))
+    assert not takes(t=z((1 << 27) + 1, 8), r=z((1 << 27) + 1, dtype=torch.float32))
+    assert takes(t=z(50, 1 << 20)) and not takes(t=z(50, (1 << 20) + 8))
+    assert not takes(t=z(0, 64), r=z(0, dtype=torch.float32)) and not takes(t=z(64, 50).t()) and not takes(r=s[:49])
+    assert not takes(t=z(50, 64, dtype=torch.uint8)) and not takes(r=s.double()) and not takes(o=torch.float64)
+    assert not takes(t=z(50, 64, dtype=torch.bfloat16))
+    assert not takes(r=s.clone().requires_grad_())

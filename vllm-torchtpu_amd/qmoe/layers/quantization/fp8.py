@@ -293,10 +293,7 @@ class Fp8LinearMethod:
         their per-row scales, dequantize in the layer's dtype."""
         out_dtype = getattr(layer, "params_dtype", None) or getattr(layer, "orig_dtype", None) or torch.bfloat16
         weight, scale = layer.weight, layer.weight_scale
-        if (weight.is_cuda and weight.dtype in (torch.float8_e4m3fn, torch.float8_e5m2, torch.int8) and weight.dim() == 2
-                and weight.stride(1) == 1 and weight.stride(0) >= weight.shape[1] and scale.dtype == torch.float32
-                and scale.numel() == weight.shape[0] and not scale.requires_grad
-                and not ops.has_tangent(weight, scale) and out_dtype in (torch.bfloat16, torch.float16, torch.float32)):
+        if weight.is_cuda and ops.vocab_lookup_takes(input_, weight, scale, out_dtype):
             return embedding(input_, weight.detach() if weight.requires_grad else weight, scale, out_dtype=out_dtype)
         flat = input_.reshape(-1)
         w = torch.index_select(layer.weight, 0, flat).to(out_dtype)

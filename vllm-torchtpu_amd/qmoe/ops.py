@@ -873,6 +873,21 @@ def _check_table(weight, weight_scale, what):
         weight_scale.reshape(-1).contiguous()
 
 
+# sizes that qmoe_vocab_lookup has: ids of a call, table rows, table width
+LOOKUP_MAX = ((1 << 24) - 1, 1 << 27, 1 << 20)
+
+
+def vocab_lookup_takes(ids, weight, weight_scale, out_dtype):
+    """Whether `vocab_lookup` has a form for these ids of a table of 1-byte codes,
+    with no derivative asked of it."""
+    if weight.dim() != 2 or weight.element_size() != 1 or weight.dtype not in _TABLE_TYPES or out_dtype not in _OUT_TYPES:
+        return False
+    V, H = weight.shape
+    return (ids.numel() <= LOOKUP_MAX[0] and 0 < V <= LOOKUP_MAX[1] and 0 < H <= LOOKUP_MAX[2] and weight.stride(1) == 1
+            and weight.stride(0) >= H and weight_scale.dtype is torch.float32 and weight_scale.numel() == V
+            and not weight_scale.requires_grad and not has_tangent(weight, weight_scale))
+
+
 def vocab_lookup(ids, weight, weight_scale=None, scale=1.0, out_dtype=torch.bfloat16):
     """Rows ``ids`` (any shape) of the table: round(scale * s * w) as
     ``out_dtype`` (bf16, f16 or f32) ``[*ids.shape, H]``; see
