@@ -172,3 +172,17 @@ def test_which_tables_of_a_method_the_lookup_takes():
     assert not takes(t=z(50, 64, dtype=torch.uint8)) and not takes(r=s.double()) and not takes(o=torch.float64)
     assert not takes(t=z(50, 64, dtype=torch.bfloat16))
     assert not takes(r=s.clone().requires_grad_())
+    trainable = z(50, 64, dtype=torch.float8_e4m3fn).requires_grad_()
+    assert not takes(t=trainable)  # (its output asks for a gradient, which torch then refuses)
+    with torch.no_grad():
+        assert takes(t=trainable) and takes(r=s.clone().requires_grad_())
+
+
+def test_method_embedding_of_a_trainable_code_table_asks_for_its_gradient():
+    from qmoe.layers.quantization.fp8 import Fp8LinearMethod
+
+    with FakeTensorMode():
+        layer = torch.nn.Module()
+        layer.weight = torch.empty((9, 16), dtype=torch.float8_e4m3fn, device="cuda").requires_grad_()
+        layer.weight_scale, layer.params_dtype = torch.empty(9, device="cuda"), torch.bfloat16
+        assert Fp8LinearMethod.embedding(None, layer, torch.empty(3, dtype=torch.int64, device="cuda")).requires_grad

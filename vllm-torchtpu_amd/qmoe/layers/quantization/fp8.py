@@ -294,7 +294,7 @@ class Fp8LinearMethod:
         out_dtype = getattr(layer, "params_dtype", None) or getattr(layer, "orig_dtype", None) or torch.bfloat16
         weight, scale = layer.weight, layer.weight_scale
         if weight.is_cuda and ops.vocab_lookup_takes(input_, weight, scale, out_dtype):
-            return embedding(input_, weight.detach() if weight.requires_grad else weight, scale, out_dtype=out_dtype)
+            return embedding(input_, weight, scale, out_dtype=out_dtype)
         flat = input_.reshape(-1)
         w = torch.index_select(layer.weight, 0, flat).to(out_dtype)
         s = torch.index_select(layer.weight_scale.reshape(-1), 0, flat).to(out_dtype).unsqueeze(-1)

@@ -885,7 +885,8 @@ def vocab_lookup_takes(ids, weight, weight_scale, out_dtype):
     V, H = weight.shape
     return (ids.numel() <= LOOKUP_MAX[0] and 0 < V <= LOOKUP_MAX[1] and 0 < H <= LOOKUP_MAX[2] and weight.stride(1) == 1
             and weight.stride(0) >= H and weight_scale.dtype is torch.float32 and weight_scale.numel() == V
-            and not weight_scale.requires_grad and not has_tangent(weight, weight_scale))
+            and not (torch.is_grad_enabled() and (weight.requires_grad or weight_scale.requires_grad))
+            and not has_tangent(weight, weight_scale))
 
 
 def vocab_lookup(ids, weight, weight_scale=None, scale=1.0, out_dtype=torch.bfloat16):
