@@ -485,6 +485,20 @@ int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void* w, int wt
                     qmoe_stream_t stream);
 
 /*
+ * The tiles of qmoe_vocab_loss and of the first vocabulary piece of
+ * qmoe_vocab_loss_grad for operands of these sizes with contiguous, 16-byte
+ * aligned rows: token rows of a tile (dw: table rows), 64 and 128 by eight
+ * wavefronts, 192 and 256 by four, 1 for 128 rows without a stage ring. Reads
+ * no memory.
+ */
+typedef struct qmoe_vocab_loss_tiles {
+  int32_t logits;      /* of the forward pass */
+  int32_t loss_pieces; /* vocabulary pieces of the forward pass (codes expanded first) */
+  int32_t probs, dx, dx_slices, dw, grad_pieces;
+} qmoe_vocab_loss_tiles;
+int qmoe_vocab_loss_plan(int64_t T, int64_t V, int64_t H, int wtype, qmoe_vocab_loss_tiles* plan);
+
+/*
  * Its gradients. g_loss, g_lse (optional): f32 [T] gradients of loss and lse;
  * lse as qmoe_vocab_loss wrote it. With c[t] = (g_loss[t] where the target
  * counts) + g_lse[t]: P[t, v] = exp(l - lse[t]) c[t] - [v == target[t]]

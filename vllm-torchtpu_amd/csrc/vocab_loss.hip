@@ -956,11 +956,16 @@ void launch_big(const VocabGemm& g, int at, dim3 grid, hipStream_t st) {
   launch_big_at<EPI, BM, 0>(g, grid, st);
 }
 
-// at: type of the A rows, 0 bf16 or the codes' table type (logits)
+// Whether a product whose tiles would be bm rows high takes the ones without a
+// ring. at: type of the A rows, 0 bf16 or the codes' table type (logits)
+template <int EPI>
+bool ringless(int at, int64_t nb, int64_t K, int bm) {
+  return EPI == VE_STORE ? bm == 128 || K <= kShortK : EPI != VE_SUM && at == 0 && nb > 128 && K <= kShortK;
+}
+
 template <int EPI>
 void launch_gemm(VocabGemm g, int at, int bm, int slices, hipStream_t st) {
-  const bool one = EPI == VE_STORE ? bm == 128 || g.K <= kShortK
-                                   : EPI != VE_SUM && at == 0 && g.nb > 128 && g.K <= kShortK;
+  const bool one = ringless<EPI>(at, g.nb, g.K, bm);
   if (one) bm = 128;
   g.n_tiles = cdiv(g.na, kVN);
   g.m_tiles = cdiv(g.nb, bm);
@@ -1150,6 +1155,26 @@ extern "C" int qmoe_vocab_loss(const void* x, int64_t ldx, int64_t T, const void
   hipLaunchKernelGGL(vocab_loss_join_kernel, dim3((unsigned)cdiv(T, (int64_t)4)), dim3(256), 0, stream, g.part,
                      (int)cdiv(V, (int64_t)kVN), (int)T, g.tgt, targets, targets_i64, ignore_index, V, loss, lse);
   return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
+}
+
+extern "C" int qmoe_vocab_loss_plan(int64_t T, int64_t V, int64_t H, int wtype, qmoe_vocab_loss_tiles* plan) {
+  if (!loss_sizes_ok(T, V, H) || T == 0 || (wtype != 0 && (wtype < 3 || wtype > 5)) || !plan) return QMOE_ERR_ARG;
+  const bool direct = wtype && H % 16 == 0;
+  const int at = direct ? wtype : 0;
+  auto pieces = [&](int64_t Vc) { return (int32_t)cdiv(V, Vc); };
+  auto tile = [](bool one, int bm) { return one ? 1 : bm; };
+  const int64_t lc = wtype && !direct ? loss_piece(V, H) : V, gc = grad_piece(T, V, H, wtype), ln = std::min(lc, V),
+                gn = std::min(gc, V), Tw = up(T, 64);
+  const int lbm = vocab_bm(ln, T), pbm = vocab_bm(gn, T), wbm = vocab_bm(H, gn, true);
+  const DxPlan dx = dx_plan(T, H, up(gn, 64));
+  plan->logits = tile(ringless<VE_LSE>(at, T, H, lbm), lbm);
+  plan->loss_pieces = pieces(lc);
+  plan->probs = tile(ringless<VE_PROB>(0, T, H, pbm), pbm);
+  plan->dx = dx.bm;
+  plan->dx_slices = dx.slices;
+  plan->dw = tile(ringless<VE_STORE>(0, gn, Tw, wbm), wbm);
+  plan->grad_pieces = pieces(gc);
+  return QMOE_OK;
 }
 
 extern "C" int qmoe_vocab_loss_grad_workspace_size(int64_t T, int64_t V, int64_t H, int wtype, int need_dx, int need_dw,

@@ -18,7 +18,7 @@ import torch  # noqa: F401  (its HIP runtime first; see above)
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libqmoe.so")
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 QMOE_OK = 0
 STATUS_TEXT = {
@@ -152,6 +152,12 @@ class FewDesc(ctypes.Structure):
     ]
 
 
+class VocabLossTiles(ctypes.Structure):
+    """Mirror of `qmoe_vocab_loss_tiles`."""
+
+    _fields_ = [(name, _i32) for name in ("logits", "loss_pieces", "probs", "dx", "dx_slices", "dw", "grad_pieces")]
+
+
 def _load():
     if not os.path.exists(_LIB_PATH):
         raise ImportError(
@@ -215,6 +221,8 @@ def _load():
     lib.qmoe_vocab_loss.restype = ctypes.c_int
     lib.qmoe_vocab_loss.argtypes = [_vp, _i64, _i64, _vp, ctypes.c_int, _i64, _vp, _i64, _i64, _vp, ctypes.c_int, _i64,
                                     _vp, _vp, _vp, _i64, _vp]
+    lib.qmoe_vocab_loss_plan.restype = ctypes.c_int
+    lib.qmoe_vocab_loss_plan.argtypes = [_i64, _i64, _i64, ctypes.c_int, ctypes.POINTER(VocabLossTiles)]
     lib.qmoe_vocab_loss_grad_workspace_size.restype = ctypes.c_int
     lib.qmoe_vocab_loss_grad_workspace_size.argtypes = [_i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                         ctypes.POINTER(_i64)]
@@ -255,6 +263,7 @@ EXPORTED = (
     "qmoe_vocab_lookup_grad",
     "qmoe_vocab_loss_workspace_size",
     "qmoe_vocab_loss",
+    "qmoe_vocab_loss_plan",
     "qmoe_vocab_loss_grad_workspace_size",
     "qmoe_vocab_loss_grad",
 )

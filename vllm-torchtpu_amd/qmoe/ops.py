@@ -1006,6 +1006,14 @@ def _loss_grad_bytes(T, V, H, wtype, need_x, need_weight):
     return need.value
 
 
+def vocab_loss_plan(T, V, H, dtype=torch.bfloat16):
+    """The tiles that `vocab_loss` and `vocab_loss_grad` take for contiguous
+    operands of these sizes (host-side `qmoe_vocab_loss_plan`), by name."""
+    tiles = _capi.VocabLossTiles()
+    check(lib.qmoe_vocab_loss_plan(T, V, H, _TABLE_TYPES[dtype], ctypes.byref(tiles)), "vocab_loss_plan")
+    return {name: getattr(tiles, name) for name, _ in tiles._fields_}
+
+
 def vocab_loss(x, weight, targets, weight_scale=None, ignore_index=-100):
     """Softmax cross entropy of ``x`` [..., H] (bf16) projected onto the table
     [V, H]: float32 (loss, log of the sum of exponentials), both of the
