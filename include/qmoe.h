@@ -449,8 +449,10 @@ int qmoe_vocab_lookup(const void* ids, int ids_i64, int64_t N, const void* w, in
 /*
  * Gradient of the lookup with respect to the table (no counterpart in the
  * reference, which serves only): dw[v] = round(scale * sum of grad[n] over
- * ids[n] == v), float32 sums in the order of n whatever the launch (the result
- * is bit-identical from call to call). Ids outside [0, V) and `padding_idx`
+ * ids[n] == v), in float32 and in a fixed order: the valid ids are sorted by
+ * (row, n), partial sums are taken per 16 of them (64 above N = 65536), and a
+ * row's are joined in order. The same ids and gradients give the same bits on
+ * every call; how a row's terms are grouped depends on the other ids. Ids outside [0, V) and `padding_idx`
  * (-1: none) add nothing. add = 0: every row of dw is written (zeros without a
  * token); add = 1: the sums are added to the rows that have a token, the
  * others are neither read nor written. grad [N, ldg >= H], dw [V, lddw >= H] of

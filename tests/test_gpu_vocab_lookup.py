@@ -293,3 +293,21 @@ def test_method_embeddings_of_other_tables(dev):
     plain = torch.nn.Module()
     plain.weight = torch.randn((60, 64), device=dev)
     assert torch.equal(UnquantizedLinearMethod().embedding(plain, ids), plain.weight[ids])
+
+
+@pytest.mark.parametrize("N", [65536, 65537, 70001])
+def test_lookup_grad_long_lists(dev, N):
+    """Around the token count from which a workgroup sums 64 entries instead of
+    16; one token runs over hundreds of chunks."""
+    V, H = 300, 40
+    gen = torch.Generator(device=dev).manual_seed(7)
+    ids = torch.randint(0, V, (N,), generator=gen, device=dev)
+    ids[torch.rand(N, generator=gen, device=dev) < 0.4] = 123
+    g = torch.randn((N, H), generator=gen, device=dev).to(BF16)
+    dw = ops.vocab_lookup_grad(g, ids, V, 0.5, 7, F32)
+    _check_grad(dw, ids, g, V, 0.5, 7)
+    assert torch.equal(dw, ops.vocab_lookup_grad(g, ids, V, 0.5, 7, F32))
+    # whole numbers: the sums are exact, so no entry is lost or taken twice
+    g = torch.randint(-8, 9, (N, H), generator=gen, device=dev).float()
+    want = torch.zeros((V, H), dtype=torch.float64, device=dev).index_add_(0, ids, g.double())
+    assert torch.equal(ops.vocab_lookup_grad(g, ids.int(), V, dtype=F32).double(), want)

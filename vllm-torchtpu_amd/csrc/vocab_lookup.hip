@@ -3,7 +3,8 @@
 //
 //   out[n]  = round(scale * s[id[n]] * w[id[n]])       (s: one scale per row of a 1-byte table,
 //                                                       rounded to the output type first)
-//   dw[v]   = round(scale * sum over n with id[n] == v of g[n]), sums in float32 in the order of n
+//   dw[v]   = round(scale * sum over n with id[n] == v of g[n]), sums in float32 in the order of n,
+//                                                       grouped by where the sorted ids are cut
 //
 // Both are bound by HBM: the lookup reads and writes N rows, the gradient reads
 // N rows and writes V (all of a fresh gradient; only the touched ones when it
@@ -184,7 +185,7 @@ void launch_lookup_out(const LookupParams& p, int ot, bool vec, hipStream_t st) 
 //    stretch of the sorted order begins, and places its own ones by (row, n):
 //    wavefront w scans the w-th part of the ids in order, so that the counts
 //    per (wavefront, row), summed in that order, make the placement stable and
-//    the order of the later sums fixed. No workgroup waits for another.
+//    the order of the later sums fixed for given ids. No workgroup waits for another.
 // 2. sum: workgroup c adds the gradient rows of the sorted entries
 //    [c * chunk, ...), whatever rows they belong to, so that a token that
 //    makes up a tenth of a batch costs as much per entry as a rare one. Runs

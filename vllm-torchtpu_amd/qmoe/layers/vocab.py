@@ -91,8 +91,9 @@ def embedding(ids, weight, weight_scale=None, scale=1.0, padding_idx=None, out_d
     The table is bf16 or f32, or 1-byte codes (e4m3, e5m2, int8) with one float32
     scale per row, which is rounded to ``out_dtype`` before the product. An id
     outside the table gives a row of NaN. A bf16 or f32 table that requires a
-    gradient gets one (in its own type, from float32 sums in token order, the
-    same bits on every call); ``padding_idx`` names the row that gets none."""
+    gradient gets one (in its own type, from float32 sums in a fixed order: the
+    same bits for the same ids and gradients); ``padding_idx`` names the row that
+    gets none."""
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"embedding: padding_idx {padding_idx} is outside the table of {weight.shape[0]} rows")
     scale = float(scale)
