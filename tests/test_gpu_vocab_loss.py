@@ -398,3 +398,29 @@ def test_gradients_of_few_kept_tokens(dev, T, V, H, kept):
     dx, dw = torch.autograd.grad(loss, (xg, wg), g)
     assert not dx[~keep].any()
     _check_grads(dx, dw, x, w, None, t, g, None)
+
+
+def test_methods_score_without_the_padding(dev):
+    """A table padded beyond its vocabulary: with the vocabulary's size the loss,
+    its log-sum and the gradients are those of the rows that count."""
+    class VocabParallelEmbedding(torch.nn.Module):
+        pass
+
+    V, rows = 450, 512
+    x, w, s, t = _case(dev, 33, V, 256, E4)
+    layer, bf = VocabParallelEmbedding(), torch.nn.Module()
+    layer.weight = torch.zeros((rows, 256), device=dev).to(E4)
+    layer.weight.view(torch.uint8)[:V] = w.view(torch.uint8)
+    layer.weight_scale = torch.cat((s, torch.ones(rows - V, device=dev)))[:, None]
+    m = Fp8LinearMethod.__new__(Fp8LinearMethod)
+    for got, want in zip(m.cross_entropy(layer, x, t, vocab_size=V), vocab_cross_entropy(x, w, t, s)):
+        assert torch.equal(got, want)
+    assert not torch.equal(m.cross_entropy(layer, x, t)[1], vocab_cross_entropy(x, w, t, s)[1])
+    bf.weight = torch.nn.Parameter(torch.zeros((rows, 256), dtype=BF16, device=dev))
+    bf.weight.data[:V] = (w.float() * s[:, None]).to(BF16)
+    loss, lse = UnquantizedLinearMethod().cross_entropy(bf, x, t, vocab_size=V)
+    short = bf.weight.detach()[:V].clone().requires_grad_()
+    want = vocab_cross_entropy(x, short, t)
+    assert torch.equal(loss, want[0]) and torch.equal(lse, want[1])
+    dw, ref = torch.autograd.grad(loss.sum(), bf.weight)[0], torch.autograd.grad(want[0].sum(), short)[0]
+    assert torch.equal(dw[:V], ref) and not dw[V:].any()

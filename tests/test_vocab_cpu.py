@@ -186,3 +186,22 @@ def test_method_embedding_of_a_trainable_code_table_asks_for_its_gradient():
         layer.weight = torch.empty((9, 16), dtype=torch.float8_e4m3fn, device="cuda").requires_grad_()
         layer.weight_scale, layer.params_dtype = torch.empty(9, device="cuda"), torch.bfloat16
         assert Fp8LinearMethod.embedding(None, layer, torch.empty(3, dtype=torch.int64, device="cuda")).requires_grad
+
+
+def test_methods_leave_the_padding_of_a_table_out():
+    from qmoe.layers.quantization.unquantized import UnquantizedLinearMethod
+    from qmoe.layers.vocab import unpadded_rows
+
+    w, s = torch.arange(24.0).view(8, 3), torch.arange(8.0)[:, None]
+    assert unpadded_rows(w, s, None) == (w, s)
+    rows, scales = unpadded_rows(w, s, 5)
+    assert torch.equal(rows, w[:5]) and torch.equal(scales, torch.arange(5.0))
+    assert unpadded_rows(w, None, 8)[1] is None
+    for bad in (0, -1, 9):
+        with pytest.raises(ValueError, match="vocab_size"):
+            unpadded_rows(w, s, bad)
+    with FakeTensorMode():
+        layer = torch.nn.Module()
+        layer.weight = torch.empty((64, 16), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+        x, t = torch.empty((3, 16), dtype=torch.bfloat16, device="cuda"), torch.empty(3, dtype=torch.int64, device="cuda")
+        assert UnquantizedLinearMethod().cross_entropy(layer, x, t, vocab_size=50)[0].requires_grad

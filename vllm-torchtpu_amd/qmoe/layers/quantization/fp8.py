@@ -37,7 +37,7 @@ import torch
 from qmoe import envs, ops
 from qmoe.layers.fused_moe import moe_forward
 from qmoe.layers.linear_common import KEEP_VLLM_LAYOUT_ATTR, quantized_matmul
-from qmoe.layers.vocab import embedding, vocab_cross_entropy
+from qmoe.layers.vocab import embedding, unpadded_rows, vocab_cross_entropy
 
 FP8 = torch.float8_e4m3fn
 # requantization targets (`fp8.py:122-127`); the short names are the ones
@@ -300,13 +300,15 @@ class Fp8LinearMethod:
         s = torch.index_select(layer.weight_scale.reshape(-1), 0, flat).to(out_dtype).unsqueeze(-1)
         return (w * s).reshape(*input_.shape, -1)
 
-    def cross_entropy(self, layer, x, targets, ignore_index=-100):
+    def cross_entropy(self, layer, x, targets, ignore_index=-100, vocab_size=None):
         """(loss, lse) of the targets under softmax(apply(layer, x)) of an
         embedding table used as the output projection, without the logits
-        (`qmoe.layers.vocab.vocab_cross_entropy`)."""
+        (`qmoe.layers.vocab.vocab_cross_entropy`); with ``vocab_size`` over its
+        first rows only (the rest pads the table)."""
         if not _is_embedding(layer):
             raise NotImplementedError("cross_entropy takes an embedding table (bf16 activations, one scale per row)")
-        return vocab_cross_entropy(x, layer.weight, targets, layer.weight_scale, ignore_index)
+        weight, scale = unpadded_rows(layer.weight, layer.weight_scale, vocab_size)
+        return vocab_cross_entropy(x, weight, targets, scale, ignore_index)
 
     def tie_weights(self, layer, embed_tokens):
         """`fp8.py:1700-1704`: share the embedding's codes and scales."""

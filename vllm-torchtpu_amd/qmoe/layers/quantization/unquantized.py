@@ -8,7 +8,7 @@ import torch
 from qmoe import _capi, envs, ops
 from qmoe.layers.fused_moe import moe_forward
 from qmoe.layers.quantization.fp8 import _activation, _device, _param
-from qmoe.layers.vocab import embedding, vocab_cross_entropy
+from qmoe.layers.vocab import embedding, unpadded_rows, vocab_cross_entropy
 
 
 class UnquantizedLinearMethod:
@@ -34,10 +34,11 @@ class UnquantizedLinearMethod:
         of an unquantized checkpoint), in its type."""
         return embedding(input_, layer.weight, out_dtype=layer.weight.dtype)
 
-    def cross_entropy(self, layer, x, targets, ignore_index=-100):
+    def cross_entropy(self, layer, x, targets, ignore_index=-100, vocab_size=None):
         """(loss, lse) of the targets under softmax(apply(layer, x)), without
-        the logits (`qmoe.layers.vocab.vocab_cross_entropy`)."""
-        return vocab_cross_entropy(x, layer.weight, targets, None, ignore_index)
+        the logits (`qmoe.layers.vocab.vocab_cross_entropy`); with
+        ``vocab_size`` over its first rows only (the rest pads the table)."""
+        return vocab_cross_entropy(x, unpadded_rows(layer.weight, None, vocab_size)[0], targets, None, ignore_index)
 
     def tie_weights(self, layer, embed_tokens):
         """Share the embedding's table, as `fp8.py:1700-1704`."""

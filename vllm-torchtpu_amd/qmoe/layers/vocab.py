@@ -172,6 +172,17 @@ def _loss(x, weight, targets, weight_scale, ignore_index):
     return torch.ops.qmoe.vocab_loss(x, weight, targets, weight_scale, ignore_index)
 
 
+def unpadded_rows(weight, weight_scale, vocab_size):
+    """The first ``vocab_size`` rows of a table and their scales (None: all); the
+    rows of a table padded beyond its vocabulary have logits too, which are not
+    the model's."""
+    if vocab_size is None:
+        return weight, weight_scale
+    if not 0 < vocab_size <= weight.shape[0]:
+        raise ValueError(f"cross_entropy: vocab_size {vocab_size} of a table of {weight.shape[0]} rows")
+    return weight[:vocab_size], None if weight_scale is None else weight_scale.reshape(-1)[:vocab_size]
+
+
 def vocab_cross_entropy(x, weight, targets, weight_scale=None, ignore_index=-100):
     """Cross entropy of the targets (int32 or int64 [...]) under softmax(x .
     w^T): (loss, lse), float32 of the targets' shape, without the logits in
