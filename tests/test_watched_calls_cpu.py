@@ -175,3 +175,14 @@ def test_a_gradient_asked_of_the_layer_is_an_error(which):
     assert out.requires_grad
     with pytest.raises(RuntimeError, match="autograd"):
         out.sum().backward()
+
+
+def test_tangents_of_a_gradient_are_refused():
+    """Forward over reverse: the operand has no tangent, what comes back has."""
+    w, x = TABLE.to(BF16).requires_grad_(), X.clone().requires_grad_()
+    for fn, leaf in ((lambda: embedding(IDS, w), w), (lambda: vocab_cross_entropy(x, w, IDS)[0], x)):
+        with fw.dual_level():
+            out = fn()
+            scaled = out * fw.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(scaled.sum(), leaf)

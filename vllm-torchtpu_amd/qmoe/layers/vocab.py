@@ -63,6 +63,7 @@ class _Embedding(torch.autograd.Function):
     def _grads(ctx, grad):
         (ids,) = ctx.saved_tensors
         vocab, scale, padding_idx, dtype = ctx.args
+        ops.refuse_tangents("embedding's gradient", grad)
         if not ops.eager_call(grad, ids):
             dw = torch.ops.qmoe.vocab_lookup_grad(grad, ids, vocab, scale, padding_idx, dtype)
             return None, dw, None, None, None
@@ -154,6 +155,7 @@ class _VocabCrossEntropy(torch.autograd.Function):
     def _grads(ctx, g_loss, g_lse):
         x, weight, targets, weight_scale, lse = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
+        ops.refuse_tangents("vocab_cross_entropy's gradients", g_loss, g_lse)
         if g_loss is None and g_lse is None:
             return None, None, None, None, None
         if g_loss is None:
