@@ -32,11 +32,12 @@
 //    rounded to bf16 before the product), as in the other bf16-activation paths;
 //    and out, once.
 //
-// Measured, launch 1 + 2: one token, MXFP4, 4 of 128 experts of 2880 x 2880 15.0 +
-// 8.7 us; 16 tokens 113 + 72 (442 and 236 MiB read: 4.1 and 3.4 TB/s; 17 us of
-// launch 1 are the routing of 16 tokens and latency, and launch 2 has 180
-// workgroups for 256 CUs); 8 tokens, NVFP4, 8 of 256 experts of 2048 x 7168 176 +
-// 92 (746 and 371 MiB, 4.4 and 4.2 TB/s).
+// Measured, launch 1 + 2, median (fastest) of 30: one token, MXFP4, 4 of 128 experts
+// of 2880 x 2880 15.7 (15.4) + 8.8 (8.6) us; 16 tokens 121 (114) + 81 (73), 443 and 232
+// MiB read, 3.8 and 3.0 TB/s (17 us of launch 1 are the routing of 16 tokens and
+// latency, and launch 2 has 180 workgroups for 256 CUs); 8 tokens, NVFP4, 8 of 256
+// experts of 2048 x 7168 211 (177) + 112 (93), 746 and 371 MiB, 3.7 and 3.5 TB/s, both
+// in 272 to 297 us a call without the profiler.
 
 #include <algorithm>
 
