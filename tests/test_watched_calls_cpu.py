@@ -186,3 +186,12 @@ def test_tangents_of_a_gradient_are_refused():
             scaled = out * fw.make_dual(torch.ones_like(out), torch.ones_like(out))
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 torch.autograd.grad(scaled.sum(), leaf)
+
+
+def test_tangents_of_trainable_operands_are_refused():
+    w, x = TABLE.to(BF16).requires_grad_(), X.clone().requires_grad_()
+    for fn, t in ((lambda t: embedding(IDS, t), w), (lambda t: vocab_cross_entropy(x, t, IDS)[0], w),
+                  (lambda t: vocab_cross_entropy(t, w, IDS)[0], x)):
+        with fw.dual_level():
+            with pytest.raises(NotImplementedError, match="forward"):
+                fn(fw.make_dual(t, torch.ones_like(t)))

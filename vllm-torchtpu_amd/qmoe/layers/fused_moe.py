@@ -279,10 +279,10 @@ def few_token_moe(hidden_states, router_logits, w1, w2, w1_scale, w2_scale, w1_b
             scoring_func, bool(renormalize), e_score_correction_bias, float(routed_scaling_factor),
             int(num_expert_group or 1), int(topk_group or 1), bool(skip_padded_tokens))
     tensors = (*args[:8], e_score_correction_bias)
-    ops.refuse_tangents("few-token MoE", *tensors)
     if ops.eager_call(*tensors) and not (
             torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)):
         return ops.moe_few_tokens(*args)  # (the op's own error stands where a gradient would be asked of it)
+    ops.refuse_tangents("few-token MoE", *tensors)
     ops._check_few(*args[:12])
     return torch.ops.qmoe.few_token_moe(*args)
 

@@ -63,12 +63,11 @@ class _Embedding(torch.autograd.Function):
     def _grads(ctx, grad):
         (ids,) = ctx.saved_tensors
         vocab, scale, padding_idx, dtype = ctx.args
-        ops.refuse_tangents("embedding's gradient", grad)
-        if not ops.eager_call(grad, ids):
-            dw = torch.ops.qmoe.vocab_lookup_grad(grad, ids, vocab, scale, padding_idx, dtype)
-            return None, dw, None, None, None
-        if not grad.is_contiguous() or not ids.is_contiguous() or grad.get_device() != torch.cuda.current_device():
-            return None, ops.vocab_lookup_grad(grad, ids, vocab, scale, padding_idx, dtype), None, None, None
+        if torch.compiler.is_compiling() or ops.watched() or type(grad) is not torch.Tensor or not grad.is_contiguous() or \
+                not ids.is_contiguous() or grad.get_device() != torch.cuda.current_device():
+            ops.refuse_tangents("embedding's gradient", grad)
+            fn = ops.vocab_lookup_grad if ops.eager_call(grad, ids) else torch.ops.qmoe.vocab_lookup_grad
+            return None, fn(grad, ids, vocab, scale, padding_idx, dtype), None, None, None
         H = grad.shape[-1]
         dw = ops.lookup_grad_run(grad, H, ids if ids.dim() == 1 else ids.view(-1), vocab, H, scale,
                                  -1 if padding_idx is None else padding_idx, dtype)
@@ -80,6 +79,7 @@ class _Embedding(torch.autograd.Function):
 def _lookup(ids, weight, weight_scale, scale, out_dtype):
     if ops.eager_call(ids, weight, weight_scale):
         return ops.vocab_lookup(ids, weight, weight_scale, scale, out_dtype)
+    ops.refuse_tangents("embedding", weight, weight_scale)
     ops._check_table(weight, weight_scale, "embedding")
     ops._check_ids(ids, "embedding: ids")
     return torch.ops.qmoe.vocab_lookup(ids, weight, weight_scale, scale, out_dtype)
@@ -98,7 +98,6 @@ def embedding(ids, weight, weight_scale=None, scale=1.0, padding_idx=None, out_d
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"embedding: padding_idx {padding_idx} is outside the table of {weight.shape[0]} rows")
     scale = float(scale)
-    ops.refuse_tangents("embedding", weight, weight_scale)
     if torch.is_grad_enabled() and (weight.requires_grad or (weight_scale is not None and weight_scale.requires_grad)):
         if weight_scale is not None:
             raise NotImplementedError("embedding: no gradient for a table of 1-byte codes or its scales")
@@ -155,12 +154,14 @@ class _VocabCrossEntropy(torch.autograd.Function):
     def _grads(ctx, g_loss, g_lse):
         x, weight, targets, weight_scale, lse = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
-        ops.refuse_tangents("vocab_cross_entropy's gradients", g_loss, g_lse)
         if g_loss is None and g_lse is None:
             return None, None, None, None, None
         if g_loss is None:
             g_loss = torch.zeros_like(g_lse)
-        fn = ops.vocab_loss_grad if ops.eager_call(x, weight, g_loss, g_lse) else torch.ops.qmoe.vocab_loss_grad
+        fn = ops.vocab_loss_grad
+        if not ops.eager_call(x, weight, g_loss, g_lse):
+            ops.refuse_tangents("vocab_cross_entropy's gradients", g_loss, g_lse)
+            fn = torch.ops.qmoe.vocab_loss_grad
         dx, dw = fn(x, weight, targets, lse, g_loss, g_lse, weight_scale, ctx.ignore_index, need_x, need_w)
         return (dx if need_x else None), (dw if need_w else None), None, None, None
 
@@ -170,6 +171,7 @@ class _VocabCrossEntropy(torch.autograd.Function):
 def _loss(x, weight, targets, weight_scale, ignore_index):
     if ops.eager_call(x, weight, targets, weight_scale):
         return ops.vocab_loss(x, weight, targets, weight_scale, ignore_index)
+    ops.refuse_tangents("vocab_cross_entropy", x, weight, weight_scale)
     ops._check_loss(x, weight, targets, weight_scale, "vocab_cross_entropy")
     return torch.ops.qmoe.vocab_loss(x, weight, targets, weight_scale, ignore_index)
 
@@ -201,7 +203,6 @@ def vocab_cross_entropy(x, weight, targets, weight_scale=None, ignore_index=-100
     (gradients in bf16; a table of codes is frozen). The sums' order is fixed:
     the same bits on every call."""
     ignore_index = int(ignore_index)
-    ops.refuse_tangents("vocab_cross_entropy", x, weight, weight_scale)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
                                     (weight_scale is not None and weight_scale.requires_grad)):
         if weight_scale is not None and (weight.requires_grad or weight_scale.requires_grad):

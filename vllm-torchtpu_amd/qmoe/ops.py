@@ -64,16 +64,21 @@ _WATCHING = ~(torch._C.DispatchKeySet(torch._C.DispatchKey.BackendSelect).raw_re
 _included_keys = torch._C._dispatch_tls_local_include_set
 
 
+def watched():
+    """Whether a trace (make_fx, torch.jit.trace), a dispatch mode, a functorch
+    transform or a forward-mode level is active on this thread."""
+    return _included_keys().raw_repr() & _WATCHING or forward_ad._current_level >= 0
+
+
 def eager_call(*ts):
     """Whether a call on these tensors runs at once, so that no dispatcher has to
-    see it: plain tensors, and neither a trace (torch.compile, make_fx,
-    torch.jit.trace), a dispatch mode nor a functorch transform on this thread."""
-    if torch.compiler.is_compiling():
+    see it: plain tensors, and nothing that `watched` names nor torch.compile."""
+    if torch.compiler.is_compiling() or _included_keys().raw_repr() & _WATCHING or forward_ad._current_level >= 0:
         return False
     for t in ts:
         if type(t) not in _PLAIN:
             return False
-    return not _included_keys().raw_repr() & _WATCHING
+    return True
 
 
 def has_tangent(*ts):
@@ -84,7 +89,8 @@ def has_tangent(*ts):
 
 def refuse_tangents(what, *ts):
     """The operators have no forward-mode derivative: an operand that carries a
-    tangent is an error, where the result would come back without one."""
+    tangent is an error, where the result would come back without one. (For a
+    call that `eager_call` declines; autograd refuses one of its functions'.)"""
     if has_tangent(*ts):
         raise NotImplementedError(f"{what}: no forward-mode derivative")
 
