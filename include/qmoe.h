@@ -520,6 +520,134 @@ int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const void* w, i
                          qmoe_stream_t stream);
 
 /*
+ * Routing with its balance loss and per-expert counts (no counterpart in the
+ * reference, which serves only): routes as qmoe_moe_route with float32 weights,
+ * then over the counted tokens (token_mask[t] != 0, or all without a mask), N of
+ * them, with p[t, e] = s[t, e] / sum over e of s[t, e] and counts[e] the counted
+ * tokens that chose e,
+ *   loss = E / (topk N^2) sum over e of counts[e] sum over t of p[t, e]    (0 for N = 0)
+ *   logits      : [T][E] bf16, or f32 with logits_f32; scoring 0..2, bias,
+ *                 renormalize, groups as qmoe_moe_route
+ *   token_mask  : one byte per token, or NULL. A token outside it is routed, with
+ *                 weights 0
+ *   topk_weights: f32 [T][topk]; topk_ids i32 [T][topk]; loss f32 [1]; counts i32 [E]
+ * 1 <= T <= 2^24, E <= 512. The sums' order is fixed. The workspace needs no
+ * initialisation.
+ */
+int qmoe_moe_balance_workspace_size(int64_t T, int E, int64_t* bytes);
+int qmoe_moe_balance(const void* logits, int logits_f32, int64_t T, int E, int topk, int scoring, const float* bias,
+                     int renormalize, float routed_scaling_factor, int num_group, int topk_group,
+                     const uint8_t* token_mask, float* topk_weights, int32_t* topk_ids, float* loss, int32_t* counts,
+                     void* workspace, int64_t ws_bytes, qmoe_stream_t stream);
+
+/*
+ * Its gradient: d_logits [T][E] (the logits' type) for the gradients of
+ * topk_weights (f32 [T][topk] or NULL) and of loss (f32 [1] or NULL); topk_ids and
+ * counts as qmoe_moe_balance wrote them. A token outside the mask gets zeros,
+ * whatever its logits are.
+ */
+int qmoe_moe_balance_grad(const void* logits, int logits_f32, int64_t T, int E, int topk, int scoring, int renormalize,
+                          float routed_scaling_factor, const uint8_t* token_mask, const int32_t* topk_ids,
+                          const int32_t* counts, const float* g_weights, const float* g_loss, void* d_logits,
+                          qmoe_stream_t stream);
+
+/*
+ * The norms before and after a block, its gate and the residual (no counterpart
+ * in the reference, whose models bring their own norms):
+ *   n(a; w) = a (mean a^2 + eps)^(-1/2) (weight_offset + w)
+ *   b = n(y; post_weight) or y,  h = residual_scale residual + scale gate b,  z = n(h; next_weight)
+ * y NULL: h is the residual itself (the norm before a block alone). Types: 0
+ * bf16, 1 f32, 2 f16; residual and h of y_type or f32; z and a gate per element
+ * of y_type. h is rounded as it is stored before its norm. Rows may be strided.
+ */
+typedef struct qmoe_block_desc {
+  int64_t T, H;            /* rows, 1..2^24; row length, 1..16384 */
+  const void* y;           /* [T][ldy] or NULL */
+  int64_t ldy;
+  const void* residual;    /* [T][ldr] (not read by the gradient) */
+  int64_t ldr;
+  const void* gate;        /* by gate_kind: NULL, [H], [T], [T][ldg] */
+  int64_t ldg;
+  const void* post_weight; /* [H] or NULL */
+  const void* next_weight; /* [H] or NULL */
+  void* h;                 /* [T][ldh]; the gradient reads it (without y: the residual) */
+  int64_t ldh;
+  void* z;                 /* [T][ldz], with next_weight */
+  int64_t ldz;
+  float* rstd_y;           /* [T] or NULL: the row factors of the two norms, for the gradient */
+  float* rstd_h;
+  int32_t y_type, residual_type, weight_type, gate_type;
+  int32_t gate_kind;       /* 0 none, 1 per channel, 2 per token, 3 per element */
+  float scale, residual_scale, weight_offset, eps;
+} qmoe_block_desc;
+int qmoe_block_residual(const qmoe_block_desc* d, qmoe_stream_t stream);
+
+/*
+ * Its gradients, for those of h and z (either may be NULL). Outputs that are NULL
+ * are not computed; d_y, d_residual and a per-element d_gate have contiguous rows,
+ * and each output its operand's type. The sums over tokens are float32 in a
+ * fixed order; the workspace (for weights and a gate per channel) needs no
+ * initialisation.
+ */
+typedef struct qmoe_block_grads {
+  const void* g_h; /* [T][ldgh] of residual_type */
+  int64_t ldgh;
+  const void* g_z; /* [T][ldgz] of y_type */
+  int64_t ldgz;
+  void* d_y;
+  void* d_residual;
+  void* d_gate;
+  void* d_post_weight;
+  void* d_next_weight;
+} qmoe_block_grads;
+int qmoe_block_residual_grad_workspace_size(int64_t T, int64_t H, int64_t* bytes);
+int qmoe_block_residual_grad(const qmoe_block_desc* d, const qmoe_block_grads* grads, void* workspace, int64_t ws_bytes,
+                             qmoe_stream_t stream);
+
+/*
+ * 8 bits of a row: for every 32 columns (the last ones may be fewer) e4m3fn codes
+ * and a byte s, the value being code * 2^(s - 127); s is the least byte with the
+ * finite values' absolute maximum <= 448 * 2^(s - 127). Infinities and NaN
+ * become NaN codes and count for no scale.
+ *
+ * Gated activation whose operands wait for the backward pass in 8 bits (no
+ * counterpart in the reference): gate = x[t][0..I), up = x[t][I..2I),
+ *   h[t] = act(gate, up)
+ * as the fused activations of qmoe_gemm; with codes also the 8 bits of gate and up.
+ *   x      : [T][ldx >= 2I] of `type`: 0 bf16, 2 f16; act QMOE_ACT_SILU ...
+ *   h      : [T][ldh >= I]
+ *   codes  : [T][2I] or NULL; scales [T][2][ceil(I / 32)]
+ * The gradient evaluates the derivatives at the 8-bit values: dx [T][2I]. A
+ * clamp passes the gradient at its limits.
+ */
+int qmoe_act_checkpoint(const void* x, int64_t ldx, int type, int64_t T, int64_t I, int act, float act_p0,
+                        float act_p1, void* h, int64_t ldh, uint8_t* codes, uint8_t* scales, qmoe_stream_t stream);
+int qmoe_act_checkpoint_grad(const uint8_t* codes, const uint8_t* scales, int64_t T, int64_t I, int act, float act_p0,
+                             float act_p1, const void* dh, int64_t lddh, int type, void* dx, qmoe_stream_t stream);
+
+/*
+ * The 8 bits of bf16 rows x [T][ldx >= K]: codes [T][K], scales [T][ceil(K / 32)].
+ */
+int qmoe_pack_8bit(const void* x, int64_t ldx, int64_t T, int64_t K, uint8_t* codes, uint8_t* scales,
+                   qmoe_stream_t stream);
+
+/*
+ * Gradients of a linear layer y = x w^T + bias whose input waited in 8 bits:
+ *   dx = dy w,  dw = dy^T x8,  dbias = sum over t of dy     (x8: the codes' values, K % 32 == 0, N % 8 == 0)
+ *   dy  : bf16 [T][lddy]; w bf16 [N][ldw] (for dx); codes / scales of qmoe_pack_8bit
+ *         (for dw); lddy and ldw multiples of 8, dy and w 16-byte aligned
+ *   dx  : bf16 [T][K]; dw bf16 [N][K]; dbias [N] bf16, or f32 with dbias_f32;
+ *         each may be NULL
+ * Sums are float32 in a fixed order. 1 <= T <= 2^20, N <= 2^18, K <= 2^16. The
+ * workspace needs no initialisation.
+ */
+int qmoe_linear_grad_workspace_size(int64_t T, int64_t N, int64_t K, int need_dx, int need_dw, int need_dbias,
+                                    int64_t* bytes);
+int qmoe_linear_grad(const void* dy, int64_t lddy, int64_t T, int64_t N, int64_t K, const void* w, int64_t ldw,
+                     const uint8_t* codes, const uint8_t* scales, void* dx, void* dw, void* dbias, int dbias_f32,
+                     void* workspace, int64_t ws_bytes, qmoe_stream_t stream);
+
+/*
  * Plain read of `bytes` (a multiple of 16, 16-byte aligned) at `src` by at
  * most `workgroups` 256-thread workgroups; `sink` receives at most one dword
  * per workgroup ([workgroups] uint32, normally untouched). No counterpart in

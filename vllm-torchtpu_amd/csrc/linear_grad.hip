@@ -1,0 +1,453 @@
+// Gradients of a linear layer y = x w^T + bias whose input waited in 8 bits:
+//
+//   dx[t, k] = sum_n dy[t, n] w[n, k],   dw[n, k] = sum_t dy[t, n] x8[t, k],   dbias[n] = sum_t dy[t, n]
+//
+// What bounds it: two products of 2 T N K operations on the bf16 matrix cores, or,
+// for few tokens, one read of w and one write of dw. The 8-bit values' scales
+// change along the summed axis, so the codes are multiplied as bf16 (exact: 4 of
+// its 8 significant bits), expanded and transposed once on the way to dw.
+//
+// Both products are the same tile: 256 "A" rows x BM "B" rows of a workgroup, a
+// ring of LDS stages of 64 k filled by direct copies, and one operand that lies
+// across K (gemm_across.h):
+//   dx : A = columns of w (across), B = rows of dy
+//   dw : A = columns of x8 (rows of its transpose, padded with zeros to 64 k), B = columns of dy (across)
+// The last stage copies zeros where K has ended. Sums are float32; a K axis that
+// is long for the number of tiles is cut into slices, added in order.
+
+#include <algorithm>
+
+#include "../../include/qmoe.h"
+#include "eight_bits.h"
+#include "gemm_across.h"
+
+namespace {
+
+constexpr int kAN = 256;  // A rows of a tile
+
+struct LinearGemm {
+  const uint8_t* a;  // rows along K [na][lda bytes], or across it [K][lda]
+  int64_t lda;
+  int na;
+  const uint8_t* b;
+  int64_t ldb;
+  int nb;
+  int K;
+  int n_tiles, m_tiles;
+  uint16_t* y;  // [nb][ldy]
+  int64_t ldy;
+  int kslice;   // K split: slice z takes the K range from z * kslice on and leaves float32 sums in [z][nb][na]
+  float* slices;
+};
+
+// B row t of the 64 that a round holds, A row n of it at n ^ vg_row_swz(t): 8
+// consecutive A rows per thread and store. 74 KB of LDS that no copy or read uses.
+template <int THREADS, int NI, int MJ>
+__device__ __forceinline__ void linear_epilogue(const LinearGemm& p, f32x16 (&acc)[NI][MJ], uint8_t* smem, int n0, int m0,
+                                                int arows, int brows, int wn, int wm) {
+  const int tid = threadIdx.x, lane = tid & 63, rl = lane & 31, kh = lane >> 5;
+  float* reg = reinterpret_cast<float*>(smem);  // [64][256]
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) {
+    const int tl = wm * 32 + rl;
+    if (64 * j >= brows) break;
+    if (j) __syncthreads();  // the rows before have been read
+    const int n1 = opaque_v(wn * NI * 32 + kh * 4);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = n1 + i * 32 + q * 8;
+        *reinterpret_cast<float4*>(reg + tl * kAN + (n ^ vg_row_swz(tl))) =
+            make_float4(acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]);
+      }
+    __syncthreads();
+    constexpr int CH = kAN / 8;
+    const int c = (tid % CH) * 8;
+#pragma unroll 2
+    for (int t = tid / CH; t < 64; t += THREADS / CH) {
+      const int64_t row = m0 + 64 * j + t;
+      if (64 * j + t >= brows) break;
+      if (c >= arows) continue;  // (A rows come in multiples of 8)
+      const float4 lo = *reinterpret_cast<const float4*>(reg + t * kAN + (c ^ vg_row_swz(t)));
+      const float4 hi = *reinterpret_cast<const float4*>(reg + t * kAN + ((c + 4) ^ vg_row_swz(t)));
+      if (p.kslice) {
+        float4* dst = reinterpret_cast<float4*>(p.slices + ((int64_t)blockIdx.y * p.nb + row) * p.na + n0 + c);
+        dst[0] = lo;
+        dst[1] = hi;
+      } else {
+        *reinterpret_cast<uint4*>(p.y + row * p.ldy + n0 + c) =
+            make_uint4(pack_bf16(lo.x, lo.y), pack_bf16(lo.z, lo.w), pack_bf16(hi.x, hi.y), pack_bf16(hi.z, hi.w));
+      }
+    }
+  }
+}
+
+// This workgroup's slice of K
+template <bool TRA>
+__device__ __forceinline__ void linear_slice(LinearGemm& p) {
+  if (!p.kslice) return;
+  const int64_t k0 = (int64_t)blockIdx.y * p.kslice;
+  p.a += TRA ? k0 * p.lda : k0 * 2;
+  p.b += TRA ? k0 * 2 : k0 * p.ldb;
+  p.K = (int)min((int64_t)p.kslice, p.K - k0);
+}
+
+// Tiles of 256 x BM (64 or 128) by eight wavefronts. ONE: a stage at a time,
+// without a ring, so that two workgroups share a CU.
+template <bool TRA, int BM, bool ONE>
+__global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const LinearGemm args) {
+  constexpr int NI = 2, MJ = BM / 64, WB = kAN * 128, STG = WB + BM * 128;
+  constexpr int RING = ONE ? 1 : (163840 / STG < 6 ? 163840 / STG : 6), EPILOGUE = 65536;
+  __shared__ __align__(1024) uint8_t smem[RING * STG > EPILOGUE ? RING * STG : EPILOGUE];
+  static_assert(ONE ? sizeof(smem) <= 81920 : RING >= 3 && sizeof(smem) <= 163840, "workgroups of a CU, ring");
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
+  LinearGemm p = args;
+  linear_slice<TRA>(p);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave & 3, wm = wave >> 2, rl = lane & 31, kh = lane >> 5;
+  int mt, nt;
+  if (!tile_dense(blockIdx.x, p.m_tiles, p.n_tiles, mt, nt)) return;
+  const int n0 = nt * kAN, m0 = mt * BM;
+  const int arows = min(kAN, p.na - n0), brows = min(BM, p.nb - m0);
+
+  // copies: one instruction = 8 rows x 128 bytes (lane -> row l >> 3, slot l & 7,
+  // chunk c of row r at c ^ vg_swz(r)), or 1 KB of K rows; wavefront w moves the
+  // groups w, w + 8, ...; rows and columns past the end repeat the last
+  constexpr int WI = WB / 8192, XI = BM / 64;
+  constexpr int TB = TRA ? kAN * 2 : BM * 2, TL = TB / 16;  // bytes, lanes of a K row
+  const int chunk = (lane & 7) ^ ((lane >> 3) ^ (wave & 1));
+  const int trow = lane / TL, tchunk = (lane % TL) ^ tr_swz<TB>(wave * (64 / TL) + trow);
+  const uint32_t tcol = (uint32_t)min(tchunk, (TRA ? arows : brows) / 8 - 1) * 16;
+  const uint8_t* abase = TRA ? p.a + n0 * 2 : p.a + (int64_t)n0 * p.lda;
+  const uint8_t* bbase = TRA ? p.b + (int64_t)m0 * p.ldb : p.b + m0 * 2;
+  const int64_t astep = TRA ? 64 * p.lda : 128, bstep = TRA ? 128 : 64 * p.ldb;
+  uint32_t aoff[WI], boff[XI];
+  int krow[TRA ? WI : XI];  // K row of a stage that copy j of the operand across K is in
+#pragma unroll
+  for (int j = 0; j < (TRA ? WI : XI); ++j) krow[j] = (wave + 8 * j) * (64 / TL) + trow;
+#pragma unroll
+  for (int j = 0; j < WI; ++j)
+    aoff[j] = TRA ? (uint32_t)krow[j] * (uint32_t)p.lda + tcol
+                  : (uint32_t)min((wave + 8 * j) * 8 + (lane >> 3), arows - 1) * (uint32_t)p.lda + chunk * 16;
+#pragma unroll
+  for (int j = 0; j < XI; ++j)
+    boff[j] = TRA ? (uint32_t)min((wave + 8 * j) * 8 + (lane >> 3), brows - 1) * (uint32_t)p.ldb + chunk * 16
+                  : (uint32_t)krow[j] * (uint32_t)p.ldb + tcol;
+  const int KF = p.K / 64, tail = p.K % 64;  // whole stages, k of the last
+  const uint32_t cw = lds0 + wave * 1024;
+  // stage s to slot `slot` (stages past the last whole one copy it again, into
+  // slots nobody reads)
+  auto copy_stage = [&](int s, int slot) {
+    const uint32_t d = __builtin_amdgcn_readfirstlane(cw + slot * STG);
+    const int k = min(s, KF - 1);
+    const uint8_t *as = uniform_ptr(abase + k * astep), *bs = uniform_ptr(bbase + k * bstep);
+#pragma unroll
+    for (int j = 0; j < WI; ++j) lds_copy16(as, aoff[j], d + j * 8192);
+#pragma unroll
+    for (int j = 0; j < XI; ++j) lds_copy16(bs, boff[j], d + WB + j * 8192);
+  };
+  // the last, partial stage, with zeros where K has ended
+  auto copy_tail = [&]() {
+    const uint8_t *as = abase + KF * astep, *bs = bbase + KF * bstep, *z = reinterpret_cast<const uint8_t*>(kZeroChunk);
+#pragma unroll
+    for (int j = 0; j < WI; ++j)
+      lds_copy16(!TRA || krow[TRA ? j : 0] < tail ? as + aoff[j] : z, __builtin_amdgcn_readfirstlane(cw + j * 8192));
+#pragma unroll
+    for (int j = 0; j < XI; ++j)
+      lds_copy16((TRA ? chunk * 8 : krow[TRA ? 0 : j]) < tail ? bs + boff[j] : z,
+                 __builtin_amdgcn_readfirstlane(cw + WB + j * 8192));
+  };
+
+  f32x16 acc[NI][MJ];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < MJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+  union B8 {
+    uint4 u;
+    bf16x8 v;
+  };
+  B8 wf[2][NI], xf[2][MJ];
+  const uint32_t tlane = tr_lane<TB>(lane);
+  // operands of step q (16 k) of a stage
+  auto read_q = [&](int slot, int q) {
+    const uint8_t* s = smem + slot * STG;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      if constexpr (TRA) wf[q & 1][i].u = tr_read<TB>(s + q * 16 * TB + (tlane ^ (wn * NI + i) * 64));
+      else wf[q & 1][i].u =
+          *reinterpret_cast<const uint4*>(s + (wn * 64 + i * 32 + rl) * 128 + ((2 * q + kh) ^ vg_swz(rl)) * 16);
+#pragma unroll
+    for (int j = 0; j < MJ; ++j)
+      if constexpr (!TRA) xf[q & 1][j].u = tr_read<TB>(s + WB + q * 16 * TB + (tlane ^ (2 * j + wm) * 64));
+      else xf[q & 1][j].u =
+          *reinterpret_cast<const uint4*>(s + WB + ((2 * j + wm) * 32 + rl) * 128 + ((2 * q + kh) ^ vg_swz(rl)) * 16);
+  };
+  auto mma = [&](int q) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < MJ; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[q & 1][i].v, xf[q & 1][j].v, acc[i][j], 0, 0, 0);
+  };
+  auto one_stage = [&]() {
+    wait_copies_upto<0>();
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      read_q(0, q);
+      mma(q);
+    }
+    __syncthreads();
+  };
+  // Ring: all but the last MFMA step run while the next step's operands are read;
+  // then the next stage's copies have landed -> barrier: everybody holds this
+  // stage's last operands, so that its slot takes the copies of stage s + RING ->
+  // the last step, while the next stage's first operands are read.
+  if constexpr (ONE) {
+    for (int s = 0; s < KF; ++s) {
+      copy_stage(s, 0);
+      one_stage();
+    }
+  } else if (KF > 0) {
+#pragma unroll
+    for (int r = 0; r < RING; ++r) copy_stage(r, r);
+    wait_copies_upto<(RING - 1) * (WI + XI)>();
+    stage_barrier();
+    read_q(0, 0);
+    int slot = 0;
+    for (int s = 0; s < KF; ++s) {
+      const int next = slot == RING - 1 ? 0 : slot + 1;
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        read_q(slot, q + 1);
+        mma(q);
+      }
+      wait_copies_upto<(RING - 2) * (WI + XI)>();
+      stage_barrier();
+      copy_stage(s + RING, slot);
+      asm volatile("" ::: "memory");
+      read_q(next, 0);
+      mma(3);
+      slot = next;
+    }
+    wait_copies_upto<0>();
+    __syncthreads();
+  }
+  if (tail) {
+    copy_tail();
+    one_stage();
+  }
+  linear_epilogue<512, NI, MJ>(p, acc, smem, n0, m0, arows, brows, wn, wm);
+}
+
+// The K slices -> bf16 rows
+__global__ __launch_bounds__(256) void linear_slices_kernel(const float* s, int slices, int64_t rows, int na,
+                                                            uint16_t* y, int64_t ldy) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, n = rows * na;
+  if (i >= n) return;
+  const int64_t row = i / na;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int z = 0; z < slices; ++z) {
+    const float4 a = *reinterpret_cast<const float4*>(s + z * n + i);
+    v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
+  }
+  *reinterpret_cast<uint2*>(y + row * ldy + (i - row * na)) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+}
+
+// Codes [T][K] -> bf16 [K][Tw], columns from T on zero. 64 x 64 tiles through LDS.
+__global__ __launch_bounds__(256) void linear_expand_kernel(const uint8_t* codes, const uint8_t* scales, int T, int K,
+                                                            uint16_t* out, int64_t Tw) {
+  __shared__ uint16_t tile[64][66];
+  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, tid = threadIdx.x;
+  {
+    const int c = (tid & 7) * 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = (tid >> 3) + 32 * h, t = r0 + r;
+      float v[8] = {};
+      if (t < T && c0 + c < K)
+        qmoe_row::decode8(*reinterpret_cast<const uint2*>(codes + (int64_t)t * K + c0 + c),
+                          scales[(int64_t)t * (K / 32) + (c0 + c) / 32], v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) tile[r][c + i] = f32_to_bf16(v[i]);
+    }
+  }
+  __syncthreads();
+  const int r = (tid & 7) * 8;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int c = (tid >> 3) + 32 * h;
+    if (c0 + c >= K) continue;
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = (uint32_t)tile[r + 2 * i][c] | (uint32_t)tile[r + 2 * i + 1][c] << 16;
+    *reinterpret_cast<uint4*>(out + (int64_t)(c0 + c) * Tw + r0 + r) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+
+// Column sums of dy: workgroup (x, y) adds the rows y, y + gridDim.y, ... of 64
+// columns, eight threads of 8 of them, 32 rows at a time -> parts [gridDim.y][N]
+__global__ __launch_bounds__(256) void linear_bias_kernel(const uint16_t* dy, int64_t lddy, int64_t T, int N,
+                                                          float* parts) {
+  __shared__ float s[32][65];
+  const int c = (threadIdx.x & 7) * 8, r = threadIdx.x >> 3, n = blockIdx.x * 64 + c;
+  float v[8] = {};
+  if (n < N)
+    for (int64_t t = (int64_t)blockIdx.y * 32 + r; t < T; t += (int64_t)gridDim.y * 32) {
+      float d[8];
+      qmoe_row::load8<qmoe_row::RT_BF16, true>(dy + t * lddy, n, N, d);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += d[k];
+    }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s[r][c + k] = v[k];
+  __syncthreads();
+  if (threadIdx.x >= 64 || (int)(blockIdx.x * 64 + threadIdx.x) >= N) return;
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int k = 0; k < 32; ++k) sum += s[k][threadIdx.x];
+  parts[(int64_t)blockIdx.y * N + blockIdx.x * 64 + threadIdx.x] = sum;
+}
+
+__global__ __launch_bounds__(256) void linear_bias_join_kernel(const float* parts, int n_parts, int N, void* out,
+                                                               int f32) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n >= N) return;
+  float v = 0.0f;
+  for (int k = 0; k < n_parts; ++k) v += parts[(int64_t)k * N + n];
+  if (f32) static_cast<float*>(out)[n] = v;
+  else static_cast<uint16_t*>(out)[n] = f32_to_bf16(v);
+}
+
+// ---------------------------------------------------------------- launches
+
+int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+// tile rows, K slices and their length of a product of na A rows, nb B rows and K
+struct LinearPlan {
+  int bm, slices, kslice;
+};
+LinearPlan linear_plan(int64_t na, int64_t nb, int64_t K) {
+  LinearPlan d{};
+  d.bm = nb <= 64 ? 64 : 128;
+  const int64_t tiles = cdiv(na, (int64_t)kAN) * cdiv(nb, (int64_t)d.bm);
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(256 / tiles, K / 512));
+  d.kslice = (int)up(cdiv(K, want), 64);
+  d.slices = (int)cdiv(K, (int64_t)d.kslice);
+  return d;
+}
+
+template <bool TRA>
+void launch_linear(LinearGemm g, uint8_t* ws, hipStream_t st) {
+  const LinearPlan d = linear_plan(g.na, g.nb, g.K);
+  if (d.slices > 1) {
+    g.kslice = d.kslice;
+    g.slices = reinterpret_cast<float*>(ws);
+  }
+  g.n_tiles = cdiv(g.na, kAN);
+  g.m_tiles = cdiv(g.nb, d.bm);
+  const dim3 grid((unsigned)up((int64_t)g.n_tiles * g.m_tiles, kXcds), (unsigned)d.slices);
+  if (d.bm == 64) hipLaunchKernelGGL((linear_small_kernel<TRA, 64, false>), grid, dim3(512), 0, st, g);
+  else hipLaunchKernelGGL((linear_small_kernel<TRA, 128, false>), grid, dim3(512), 0, st, g);
+  if (d.slices > 1)
+    hipLaunchKernelGGL(linear_slices_kernel, dim3((unsigned)cdiv((int64_t)g.nb * g.na / 4, (int64_t)256)), dim3(256), 0, st,
+                       g.slices, d.slices, (int64_t)g.nb, g.na, g.y, g.ldy);
+}
+
+int64_t slice_bytes(int64_t na, int64_t nb, int64_t K) {
+  const LinearPlan d = linear_plan(na, nb, K);
+  return d.slices > 1 ? up(4 * d.slices * na * nb, 256) : 0;
+}
+
+int bias_parts(int64_t T, int64_t N) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(T, (int64_t)128), cdiv((int64_t)2048, cdiv(N, (int64_t)64))));
+}
+
+// x8 transposed, K slices (dx's, then dw's), bias parts
+int64_t linear_layout(int64_t T, int64_t N, int64_t K, int need_dx, int need_dw, int need_dbias, int64_t (&off)[3]) {
+  int64_t at = 0;
+  off[0] = at;
+  if (need_dw) at += up(K * up(T, 64) * 2, 256);
+  off[1] = at;
+  int64_t s = need_dx ? slice_bytes(K, T, N) : 0;
+  if (need_dw) s = std::max(s, slice_bytes(K, N, T));
+  at += s;
+  off[2] = at;
+  if (need_dbias) at += up(4 * N * bias_parts(T, N), 256);
+  return at;
+}
+
+bool linear_sizes_ok(int64_t T, int64_t N, int64_t K) {
+  return T >= 1 && T <= ((int64_t)1 << 20) && N >= 8 && N <= ((int64_t)1 << 18) && K >= 32 && K <= ((int64_t)1 << 16) &&
+         N % 8 == 0 && K % 32 == 0;
+}
+
+bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+// See include/qmoe.h for the contract.
+extern "C" int qmoe_linear_grad_workspace_size(int64_t T, int64_t N, int64_t K, int need_dx, int need_dw, int need_dbias,
+                                               int64_t* bytes) {
+  if (!linear_sizes_ok(T, N, K) || !bytes) return QMOE_ERR_ARG;
+  int64_t off[3];
+  *bytes = linear_layout(T, N, K, need_dx, need_dw, need_dbias, off);
+  return QMOE_OK;
+}
+
+extern "C" int qmoe_linear_grad(const void* dy, int64_t lddy, int64_t T, int64_t N, int64_t K, const void* w, int64_t ldw,
+                                const uint8_t* codes, const uint8_t* scales, void* dx, void* dw, void* dbias,
+                                int dbias_f32, void* workspace, int64_t ws_bytes, hipStream_t stream) {
+  // (256 rows of a tile, or 64 of a stage, lie within 32-bit offsets)
+  constexpr int64_t kMaxPitch = (int64_t)1 << 22;
+  if (!linear_sizes_ok(T, N, K) || !dy || lddy < N || lddy % 8 || lddy >= kMaxPitch || !at16(dy)) return QMOE_ERR_ARG;
+  if (dx && (!w || ldw < K || ldw % 8 || ldw >= kMaxPitch || !at16(w) || !at16(dx))) return QMOE_ERR_ARG;
+  if (dw && (!codes || !scales || reinterpret_cast<uintptr_t>(codes) % 8 || !at16(dw))) return QMOE_ERR_ARG;
+  int64_t off[3];
+  const int64_t need = linear_layout(T, N, K, dx != nullptr, dw != nullptr, dbias != nullptr, off);
+  if (need && (!workspace || ws_bytes < need)) return QMOE_ERR_WORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (dx) {
+    LinearGemm g{};
+    g.a = static_cast<const uint8_t*>(w);
+    g.lda = ldw * 2;
+    g.na = (int)K;
+    g.b = static_cast<const uint8_t*>(dy);
+    g.ldb = lddy * 2;
+    g.nb = (int)T;
+    g.K = (int)N;
+    g.y = static_cast<uint16_t*>(dx);
+    g.ldy = K;
+    launch_linear<true>(g, ws + off[1], stream);
+  }
+  if (dw) {
+    const int64_t Tw = up(T, 64);
+    uint16_t* xt = reinterpret_cast<uint16_t*>(ws + off[0]);
+    hipLaunchKernelGGL(linear_expand_kernel, dim3((unsigned)(Tw / 64), (unsigned)cdiv(K, (int64_t)64)), dim3(256), 0,
+                       stream, codes, scales, (int)T, (int)K, xt, Tw);
+    LinearGemm g{};
+    g.a = reinterpret_cast<const uint8_t*>(xt);
+    g.lda = Tw * 2;
+    g.na = (int)K;
+    g.b = static_cast<const uint8_t*>(dy);
+    g.ldb = lddy * 2;
+    g.nb = (int)N;
+    g.K = (int)T;
+    g.y = static_cast<uint16_t*>(dw);
+    g.ldy = K;
+    launch_linear<false>(g, ws + off[1], stream);
+  }
+  if (dbias) {
+    float* parts = reinterpret_cast<float*>(ws + off[2]);
+    const int n_parts = bias_parts(T, N);
+    hipLaunchKernelGGL(linear_bias_kernel, dim3((unsigned)cdiv(N, (int64_t)64), (unsigned)n_parts), dim3(256), 0, stream,
+                       static_cast<const uint16_t*>(dy), lddy, T, (int)N, parts);
+    hipLaunchKernelGGL(linear_bias_join_kernel, dim3((unsigned)cdiv(N, (int64_t)256)), dim3(256), 0, stream, parts, n_parts,
+                       (int)N, dbias, dbias_f32);
+  }
+  return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
+}

@@ -209,32 +209,26 @@ __device__ __forceinline__ void row_scores(const void* __restrict__ logits, int 
 
 constexpr int kChoiceLds = kMaxSlots * 64 + 64;  // floats of LDS scratch per wavefront
 
-// Routes token t with the calling wavefront (all 64 lanes). `ch` is this
-// wavefront's LDS scratch of kChoiceLds floats (grouped selection: the
-// group scores, and the choice scores when groups are not a power of two).
-// When lds_ids is given, the token's ids and bf16 weights also go to
-// lds_ids / lds_w [t * topk + j]. The selection is branch-free per lane:
-// lane-dependent choices are selects, the remaining branches are uniform.
-template <int S, int SCORING, bool GROUPED>
-__device__ __forceinline__ void route_token(const void* __restrict__ logits, int logits_f32, int64_t t, int E,
+// Routes token t, whose scores are s and whose correction biases bv, with the
+// calling wavefront (all 64 lanes). `ch` is this wavefront's LDS scratch of
+// kChoiceLds floats (grouped selection: the group scores, and the choice scores
+// when groups are not a power of two). When lds_ids is given, the token's ids
+// and bf16 weights also go to lds_ids / lds_w [t * topk + j]. A token that is not
+// live gets zero weights. The selection is branch-free per lane: lane-dependent
+// choices are selects, the remaining branches are uniform. Returns the lane's
+// route (lane < topk).
+template <int S, bool GROUPED>
+__device__ __forceinline__ int route_scored(const float (&s)[kMaxSlots], const float (&bv)[kMaxSlots], int64_t t, int E,
                                             int topk, const float* __restrict__ bias, int renormalize, float rsf,
                                             int num_group, int topk_group, void* __restrict__ out_w, int w_f32,
                                             int32_t* __restrict__ out_ids, float* ch, int32_t* lds_ids,
-                                            uint16_t* lds_w) {
+                                            uint16_t* lds_w, bool live = true) {
   const int lane = threadIdx.x & 63;
   constexpr float kMin = -3.402823466e38f;  // -FLT_MAX
   const int neg_key = fkey(kNeg);
 
   uint64_t vm[kMaxSlots];
   expert_lanes<S>(E, vm);
-  // bias loads issued with the row's loads
-  float bv[kMaxSlots];
-  if (bias) {
-#pragma unroll
-    for (int j = 0; j < S; ++j) bv[j] = bias[j * 64 + lane < E ? j * 64 + lane : E - 1];
-  }
-  float s[kMaxSlots];
-  row_scores<S, SCORING>(logits, logits_f32, t, E, s);
 
   // keys of the choice scores, clamped to >= kNeg (NaN included)
   int cur[kMaxSlots];
@@ -343,6 +337,7 @@ __device__ __forceinline__ void route_token(const void* __restrict__ logits, int
     float v = myw;
     if (renormalize) v = v / (sum != sum ? sum : fmaxf(sum, 1e-20f));
     if (rsf != 1.0f) v = v * rsf;
+    if (!live) v = 0.0f;
     if (w_f32) {
       static_cast<float*>(out_w)[t * topk + lane] = v;
     } else {
@@ -352,6 +347,32 @@ __device__ __forceinline__ void route_token(const void* __restrict__ logits, int
     }
     if (lds_ids) lds_ids[t * topk + lane] = myid;
   }
+  return myid;
+}
+
+// The correction biases in the scores' layout
+template <int S>
+__device__ __forceinline__ void load_bias(const float* __restrict__ bias, int E, float (&bv)[kMaxSlots]) {
+  const int lane = threadIdx.x & 63;
+  if (bias) {
+#pragma unroll
+    for (int j = 0; j < S; ++j) bv[j] = bias[j * 64 + lane < E ? j * 64 + lane : E - 1];
+  }
+}
+
+// Scores of token t's row, then its routes
+template <int S, int SCORING, bool GROUPED>
+__device__ __forceinline__ void route_token(const void* __restrict__ logits, int logits_f32, int64_t t, int E,
+                                            int topk, const float* __restrict__ bias, int renormalize, float rsf,
+                                            int num_group, int topk_group, void* __restrict__ out_w, int w_f32,
+                                            int32_t* __restrict__ out_ids, float* ch, int32_t* lds_ids,
+                                            uint16_t* lds_w) {
+  // bias loads issued with the row's loads
+  float s[kMaxSlots], bv[kMaxSlots];
+  load_bias<S>(bias, E, bv);
+  row_scores<S, SCORING>(logits, logits_f32, t, E, s);
+  route_scored<S, GROUPED>(s, bv, t, E, topk, bias, renormalize, rsf, num_group, topk_group, out_w, w_f32, out_ids, ch,
+                           lds_ids, lds_w);
 }
 
 // route_token with the scoring rule and grouping chosen at run time (one

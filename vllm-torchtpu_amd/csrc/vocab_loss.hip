@@ -37,7 +37,7 @@
 #include <type_traits>
 
 #include "../../include/qmoe.h"
-#include "gemm_tile.h"
+#include "gemm_across.h"
 
 namespace {
 
@@ -79,51 +79,14 @@ struct VocabGemm {
   int64_t ldy;
 };
 
-__device__ __align__(16) const uint32_t kVocabZero[4] = {0, 0, 0, 0};
-
 __device__ __forceinline__ int64_t load_target(const VocabGemm& p, int t) {
   return p.targets_i64 ? static_cast<const int64_t*>(p.targets)[t]
                        : (int64_t) static_cast<const int32_t*>(p.targets)[t];
 }
 
-// Which operand lies across K, rows of 256 or BM columns, and how it passes
-// through LDS. ds_read_b64_tr_b16: lane 4 r + c of 16 gives the address of row r's
-// elements 4 c .. + 3, lane i receives column i of the 4 rows. An MFMA operand is
-// two of them (k + 4) per lane; the 4 rows of an access lie in different 64-byte
-// blocks, for which the 16-byte chunk c of row k is stored at c ^ tr_swz.
+// Which operand lies across K
 constexpr bool tr_a(int epi) { return epi == VE_SUM; }
 constexpr bool tr_b(int epi) { return epi == VE_STORE; }
-template <int RB>  // bytes of a row
-__device__ __forceinline__ int tr_swz(int k) {
-  return 4 * (RB == 128 ? (k >> 1) & 1 : k & 3);
-}
-// Byte of the lane's first 4 x 4 of k 0 .. 15 of columns 0 .. 31; those of columns
-// 32 f .. are at this ^ 64 f
-template <int RB>
-__device__ __forceinline__ uint32_t tr_lane(int lane) {
-  const int k = 8 * (lane >> 5) + ((lane & 15) >> 2);
-  return (uint32_t)(k * RB + ((32 * ((lane >> 4) & 1) + 8 * (lane & 3)) ^ (tr_swz<RB>(k) * 16)));
-}
-template <int RB>
-__device__ __forceinline__ uint4 tr_read(const uint8_t* at) {
-  typedef short s16x4 __attribute__((ext_vector_type(4)));
-  typedef __attribute__((address_space(3))) s16x4* Lds;
-  union {
-    s16x4 h[2];
-    uint4 u;
-  } r;
-  r.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(void*)at);
-  r.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(void*)(at + 4 * RB));
-  return r.u;
-}
-
-__device__ __forceinline__ int vg_swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
-
-__device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* q) {
-  const uint64_t b = reinterpret_cast<uint64_t>(q);
-  return reinterpret_cast<const uint8_t*>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 |
-                                          (uint32_t)__builtin_amdgcn_readfirstlane((int)b));
-}
 
 // (maximum, sum of exponentials below it) of two disjoint sets; the base of the
 // exponentials is 0 where the maximum is infinite, so that infinite logits give
@@ -137,33 +100,12 @@ __device__ __forceinline__ float2 lse_merge(float2 a, float2 b) {
   return make_float2(m, sa + sb);
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  union {
-    bf16x2 h;
-    uint32_t u;
-  } r;
-  r.h = __builtin_convertvector(f32x2{a, b}, bf16x2);
-  return r.u;
-}
-
 // The epilogues. A tile's wavefront (wn, wm), wn < WN, wm < 2, holds NI x MJ
 // blocks of 32 x 32: register quad q of block (i, j) is A rows (wn NI + i) 32 + 8
 // q + 4 kh .. + 3 and B row (2 j + wm) 32 + rl, rl = lane % 32, kh = lane / 32.
 // The logits are reduced in registers; the others pass 64 B rows at a time
 // through LDS (A row n of B row t at n ^ 4 f(t)), so that a thread stores 8
 // consecutive values. `smem`: 74 KB of LDS that no copy or read uses any more.
-// opaque_*: a value the compiler takes for a new one, so that what depends on
-// it (64 row scales, masks or addresses) is not kept for all MJ rounds at once.
-__device__ __forceinline__ int opaque_s(int v) {
-  asm volatile("" : "+s"(v));
-  return v;
-}
-__device__ __forceinline__ int opaque_v(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
-__device__ __forceinline__ int vg_row_swz(int t) { return 4 * ((t ^ (t >> 3)) & 15); }
-
 template <int EPI, int BM, int WN, int NI, int MJ>
 __device__ __forceinline__ void vocab_epilogue(const VocabGemm& p, f32x16 (&acc)[NI][MJ], uint8_t* smem, int nt, int m0,
                                                int arows, int brows, int wn, int wm) {
@@ -557,7 +499,7 @@ __global__ __launch_bounds__(kVThreads, ONE ? 4 : 2) void vocab_gemm_kernel(cons
   if ((EPI == VE_LSE || EPI == VE_PROB) && p.K % 64) {
     const uint8_t *as = abase + (int64_t)KF * AB, *bs = bbase + (int64_t)KF * 128;
     const bool ain = KF * 64 + achunk * (AT ? 16 : 8) < p.K, bin = KF * 64 + xchunk * 8 < p.K;
-    const uint8_t* z = reinterpret_cast<const uint8_t*>(kVocabZero);
+    const uint8_t* z = reinterpret_cast<const uint8_t*>(kZeroChunk);
 #pragma unroll
     for (int j = 0; j < WI; ++j) lds_copy16(ain ? as + aoff[j] : z, cw + j * 8192);
 #pragma unroll
@@ -777,7 +719,7 @@ __global__ __launch_bounds__(kBThreads, 1) void vocab_big_kernel(const VocabGemm
   if constexpr (TAIL) {  // the last, partial stage: zeros behind the rows' ends
     const uint8_t *as = abase + (int64_t)KF * AB, *bs = bbase + (int64_t)KF * 128;
     const bool ain = KF * 64 + (AT ? achunk * 16 : chunk16 * 8) < p.K, in = KF * 64 + chunk16 * 8 < p.K;
-    const uint8_t* z = reinterpret_cast<const uint8_t*>(kVocabZero);
+    const uint8_t* z = reinterpret_cast<const uint8_t*>(kZeroChunk);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if (j < AI) lds_copy16(ain ? as + aoff[j] : z, cw + j * 4096);

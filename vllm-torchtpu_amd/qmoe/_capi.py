@@ -18,7 +18,7 @@ import torch  # noqa: F401  (its HIP runtime first; see above)
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libqmoe.so")
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 QMOE_OK = 0
 STATUS_TEXT = {
@@ -158,6 +158,54 @@ class VocabLossTiles(ctypes.Structure):
     _fields_ = [(name, _i32) for name in ("logits", "loss_pieces", "probs", "dx", "dx_slices", "dw", "grad_pieces")]
 
 
+class BlockDesc(ctypes.Structure):
+    """Mirror of `qmoe_block_desc` (field order and types must match)."""
+
+    _fields_ = [
+        ("T", _i64),
+        ("H", _i64),
+        ("y", _vp),
+        ("ldy", _i64),
+        ("residual", _vp),
+        ("ldr", _i64),
+        ("gate", _vp),
+        ("ldg", _i64),
+        ("post_weight", _vp),
+        ("next_weight", _vp),
+        ("h", _vp),
+        ("ldh", _i64),
+        ("z", _vp),
+        ("ldz", _i64),
+        ("rstd_y", _vp),
+        ("rstd_h", _vp),
+        ("y_type", _i32),
+        ("residual_type", _i32),
+        ("weight_type", _i32),
+        ("gate_type", _i32),
+        ("gate_kind", _i32),
+        ("scale", _f32),
+        ("residual_scale", _f32),
+        ("weight_offset", _f32),
+        ("eps", _f32),
+    ]
+
+
+class BlockGrads(ctypes.Structure):
+    """Mirror of `qmoe_block_grads` (field order and types must match)."""
+
+    _fields_ = [
+        ("g_h", _vp),
+        ("ldgh", _i64),
+        ("g_z", _vp),
+        ("ldgz", _i64),
+        ("d_y", _vp),
+        ("d_residual", _vp),
+        ("d_gate", _vp),
+        ("d_post_weight", _vp),
+        ("d_next_weight", _vp),
+    ]
+
+
 def _load():
     if not os.path.exists(_LIB_PATH):
         raise ImportError(
@@ -229,6 +277,34 @@ def _load():
     lib.qmoe_vocab_loss_grad.restype = ctypes.c_int
     lib.qmoe_vocab_loss_grad.argtypes = [_vp, _i64, _i64, _vp, ctypes.c_int, _i64, _vp, _i64, _i64, _vp, ctypes.c_int,
                                          _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp]
+    lib.qmoe_moe_balance_workspace_size.restype = ctypes.c_int
+    lib.qmoe_moe_balance_workspace_size.argtypes = [_i64, ctypes.c_int, ctypes.POINTER(_i64)]
+    lib.qmoe_moe_balance.restype = ctypes.c_int
+    lib.qmoe_moe_balance.argtypes = [_vp, ctypes.c_int, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int,
+                                     _f32, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]
+    lib.qmoe_moe_balance_grad.restype = ctypes.c_int
+    lib.qmoe_moe_balance_grad.argtypes = [_vp, ctypes.c_int, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                          _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]
+    lib.qmoe_block_residual.restype = ctypes.c_int
+    lib.qmoe_block_residual.argtypes = [ctypes.POINTER(BlockDesc), _vp]
+    lib.qmoe_block_residual_grad_workspace_size.restype = ctypes.c_int
+    lib.qmoe_block_residual_grad_workspace_size.argtypes = [_i64, _i64, ctypes.POINTER(_i64)]
+    lib.qmoe_block_residual_grad.restype = ctypes.c_int
+    lib.qmoe_block_residual_grad.argtypes = [ctypes.POINTER(BlockDesc), ctypes.POINTER(BlockGrads), _vp, _i64, _vp]
+    lib.qmoe_act_checkpoint.restype = ctypes.c_int
+    lib.qmoe_act_checkpoint.argtypes = [_vp, _i64, ctypes.c_int, _i64, _i64, ctypes.c_int, _f32, _f32, _vp, _i64, _vp,
+                                        _vp, _vp]
+    lib.qmoe_act_checkpoint_grad.restype = ctypes.c_int
+    lib.qmoe_act_checkpoint_grad.argtypes = [_vp, _vp, _i64, _i64, ctypes.c_int, _f32, _f32, _vp, _i64, ctypes.c_int, _vp,
+                                             _vp]
+    lib.qmoe_pack_8bit.restype = ctypes.c_int
+    lib.qmoe_pack_8bit.argtypes = [_vp, _i64, _i64, _i64, _vp, _vp, _vp]
+    lib.qmoe_linear_grad_workspace_size.restype = ctypes.c_int
+    lib.qmoe_linear_grad_workspace_size.argtypes = [_i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                                    ctypes.POINTER(_i64)]
+    lib.qmoe_linear_grad.restype = ctypes.c_int
+    lib.qmoe_linear_grad.argtypes = [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, ctypes.c_int, _vp,
+                                     _i64, _vp]
     lib.qmoe_stream_read.restype = ctypes.c_int
     lib.qmoe_stream_read.argtypes = [_vp, _i64, _i32, _vp, _vp]
     v = lib.qmoe_abi_version()
@@ -266,6 +342,17 @@ EXPORTED = (
     "qmoe_vocab_loss_plan",
     "qmoe_vocab_loss_grad_workspace_size",
     "qmoe_vocab_loss_grad",
+    "qmoe_moe_balance_workspace_size",
+    "qmoe_moe_balance",
+    "qmoe_moe_balance_grad",
+    "qmoe_block_residual",
+    "qmoe_block_residual_grad_workspace_size",
+    "qmoe_block_residual_grad",
+    "qmoe_act_checkpoint",
+    "qmoe_act_checkpoint_grad",
+    "qmoe_pack_8bit",
+    "qmoe_linear_grad_workspace_size",
+    "qmoe_linear_grad",
 )
 
 

@@ -7,6 +7,10 @@ the lowest expert id), grouped selection, renormalization and scaling all run
 in one HIP kernel (`qmoe_moe_route`), registered as the torch custom op
 ``torch.ops.qmoe.moe_route`` with a fake implementation (the reference
 registers its router op the same way, `layers/adapter/router_topk.py:36-39`).
+
+``balanced_experts`` is the router in training: the same choice with the balance
+loss, per-expert counts and the logits' gradient (no reference counterpart, which
+serves only).
 """
 
 from typing import Optional, Tuple
@@ -118,3 +122,103 @@ def route(layer, hidden_states, router_logits, input_ids=None):
                       renormalize=layer.renormalize)
     return select_experts(hidden_states, router_logits, topk=topk, renormalize=layer.renormalize,
                           scoring_fn=layer.scoring_func, layer=layer, input_ids=input_ids)
+
+
+# ---------------------------------------------------------------- balanced routing
+
+
+@torch.library.custom_op("qmoe::moe_balance", mutates_args=())
+def _balance_op(logits: torch.Tensor, topk: int, scoring_func: str, renormalize: bool, bias: Optional[torch.Tensor],
+                routed_scaling_factor: float, num_expert_group: int, topk_group: int,
+                token_mask: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return ops.moe_balance(logits, topk, scoring_func, renormalize, bias, routed_scaling_factor, num_expert_group,
+                           topk_group, token_mask)
+
+
+@_balance_op.register_fake
+def _(logits, topk, scoring_func, renormalize, bias, routed_scaling_factor, num_expert_group, topk_group, token_mask):
+    T, E = logits.shape
+    return (logits.new_empty((T, topk), dtype=torch.float32), logits.new_empty((T, topk), dtype=torch.int32),
+            logits.new_empty((), dtype=torch.float32), logits.new_empty(E, dtype=torch.int32))
+
+
+@torch.library.custom_op("qmoe::moe_balance_grad", mutates_args=())
+def _balance_grad_op(logits: torch.Tensor, topk_ids: torch.Tensor, counts: torch.Tensor, g_weights: Optional[torch.Tensor],
+                     g_loss: Optional[torch.Tensor], scoring_func: str, renormalize: bool, routed_scaling_factor: float,
+                     token_mask: Optional[torch.Tensor]) -> torch.Tensor:
+    return ops.moe_balance_grad(logits, topk_ids, counts, g_weights, g_loss, scoring_func, renormalize,
+                                routed_scaling_factor, token_mask)
+
+
+@_balance_grad_op.register_fake
+def _(logits, topk_ids, counts, g_weights, g_loss, scoring_func, renormalize, routed_scaling_factor, token_mask):
+    return torch.empty_like(logits)
+
+
+class _Balance(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topk, args, bias, token_mask):
+        w, ids, loss, counts = _balance(logits, topk, args, bias, token_mask)
+        ctx.save_for_backward(logits, ids, counts, token_mask)
+        ctx.args = args[:3]
+        ctx.mark_non_differentiable(ids, counts)
+        ctx.set_materialize_grads(False)
+        return w, ids, loss, counts
+
+    @staticmethod
+    def backward(ctx, g_w, g_ids, g_loss, g_counts):
+        # (autograd runs this with gradients off; with create_graph the decorator puts the error for a second pass behind it)
+        if torch.is_grad_enabled():
+            return _Balance._once(ctx, g_w, g_ids, g_loss, g_counts)
+        return _Balance._grads(ctx, g_w, g_ids, g_loss, g_counts)
+
+    @staticmethod
+    def _grads(ctx, g_w, g_ids, g_loss, g_counts):
+        if g_w is None and g_loss is None:
+            return (None,) * 5
+        logits, ids, counts, mask = ctx.saved_tensors
+        fn = ops.moe_balance_grad
+        if not ops.eager_call(logits, ids, counts, g_w, g_loss, mask):
+            ops.refuse_tangents("balanced_experts' gradient", g_w, g_loss)
+            fn = torch.ops.qmoe.moe_balance_grad
+        return fn(logits, ids, counts, g_w, g_loss, *ctx.args, mask), None, None, None, None
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_grads.__func__))
+
+
+def _balance(logits, topk, args, bias, token_mask):
+    scoring_func, renormalize, rsf, ng, tg = args
+    if ops.eager_call(logits, bias, token_mask):
+        return ops.moe_balance(logits, topk, scoring_func, renormalize, bias, rsf, ng, tg, token_mask)
+    ops.refuse_tangents("balanced_experts", logits, bias)
+    ops._check_balance(logits, topk, scoring_func, bias, ng, tg, token_mask, "balanced_experts")
+    return torch.ops.qmoe.moe_balance(logits, topk, scoring_func, renormalize, bias, rsf, ng, tg, token_mask)
+
+
+def balanced_experts(router_logits, topk, scoring_func="softmax", renormalize=True, e_score_correction_bias=None,
+                     routed_scaling_factor=1.0, num_expert_group=1, topk_group=1, token_mask=None):
+    """Routing for training, and for watching a server's load: (topk_weights f32
+    [T, k], topk_ids int32 [T, k], balance_loss f32 [], expert_counts int32 [E]) of
+    router logits [T, E] (bf16, f32, or another float type taken as f32).
+
+    Experts and weights as `select_experts` chooses them (scoring "softmax",
+    "sigmoid" or "sqrtsoftplus"), the weights not rounded. Over the N tokens of
+    ``token_mask`` (bool [T]; None: all), with f[e] the share of their k N routes that
+    expert e has and P[e] the mean of their scores' share of e (softmax: the score):
+
+        balance_loss = E sum_e f[e] P[e]          (1 for an even load; 0 for N = 0)
+
+    ``expert_counts`` are those routes. A token outside the mask gets weights 0, and no
+    gradient whatever its logits are. Differentiable in the logits through the
+    weights and the loss (through P; the choice and f are constants), in their type;
+    the correction bias only chooses and has no gradient. The sums' order is fixed."""
+    if torch.is_grad_enabled() and e_score_correction_bias is not None and e_score_correction_bias.requires_grad:
+        raise NotImplementedError("balanced_experts: no gradient for the correction bias, which only chooses")
+    if router_logits.dtype not in (torch.bfloat16, torch.float32) and router_logits.is_floating_point():
+        router_logits = router_logits.float()
+    args = (scoring_func, bool(renormalize), float(routed_scaling_factor), int(num_expert_group or 1),
+            int(topk_group or 1))
+    topk = int(topk)
+    if torch.is_grad_enabled() and router_logits.requires_grad:
+        return _Balance.apply(router_logits, topk, args, e_score_correction_bias, token_mask)
+    return _balance(router_logits, topk, args, e_score_correction_bias, token_mask)

@@ -6,6 +6,7 @@ the qmoe grouped GEMM (bf16 MFMA, f32 accumulation)."""
 import torch
 
 from qmoe import _capi, envs, ops
+from qmoe.layers.block import checkpointed_linear
 from qmoe.layers.fused_moe import moe_forward
 from qmoe.layers.quantization.fp8 import _activation, _device, _param
 from qmoe.layers.vocab import embedding, unpadded_rows, vocab_cross_entropy
@@ -28,6 +29,11 @@ class UnquantizedLinearMethod:
         if bias is not None:
             out = out + bias
         return out
+
+    def apply_checkpointed(self, layer, x, bias=None):
+        """`apply` with gradients: ``x`` waits for the weight's in 8 bits
+        (`qmoe.layers.block.checkpointed_linear`)."""
+        return checkpointed_linear(x.to(torch.bfloat16), layer.weight, bias)
 
     def embedding(self, layer, input_):
         """Rows of a bf16 or f32 ``[vocab, H]`` table (a `VocabParallelEmbedding`

@@ -1068,3 +1068,399 @@ def vocab_loss_grad(x, weight, targets, lse, g_loss, g_lse=None, weight_scale=No
                                            lse.data_ptr(), g_loss.data_ptr(), _addr(g_lse), _addr(dx), H, _addr(dw), H,
                                            _addr(ws), ws_n, _raw_stream(dev)), "vocab_loss_grad")
     return (dx.view(x.shape) if dx is not None else None), dw
+
+
+# ---------------------------------------------------------------- balanced routing
+
+_BALANCE_SCORING = frozenset(("softmax", "sigmoid", "sqrtsoftplus"))
+BALANCE_MAX = ((1 << 24), 512)  # tokens, experts
+
+
+def _check_balance(logits, topk, scoring_func, bias, num_expert_group, topk_group, token_mask, what):
+    if scoring_func not in _BALANCE_SCORING:
+        raise NotImplementedError(f"{what}: the scores are {sorted(_BALANCE_SCORING)}, not {scoring_func!r}")
+    if logits.dim() != 2 or logits.dtype not in _GRAD_TYPES:
+        raise ValueError(f"{what}: router logits must be bf16 or f32 [T, E], got {logits.dtype} {tuple(logits.shape)}")
+    T, E = logits.shape
+    if not 1 <= topk <= min(E, 64) or E > BALANCE_MAX[1] or T > BALANCE_MAX[0]:
+        raise ValueError(f"{what}: takes 1 <= topk <= experts (64 at most), {BALANCE_MAX[1]} experts and {BALANCE_MAX[0]} "
+                         f"tokens at most, got topk={topk}, {T} tokens, {E} experts")
+    ng, tg = num_expert_group or 1, topk_group or 1
+    if ng > 1 and tg < ng and (E % ng or ng > 64 or tg < 1 or topk > tg * (E // ng)):
+        raise ValueError(f"{what}: {topk} of {E} experts from {tg} of {ng} groups")
+    if bias is not None and (bias.numel() != E or not bias.is_floating_point()):
+        raise ValueError(f"{what}: the correction bias must hold {E} values, got {bias.dtype} {tuple(bias.shape)}")
+    if token_mask is not None and (token_mask.dtype is not torch.bool or token_mask.shape != (T,)):
+        raise ValueError(f"{what}: the token mask must be bool [{T}], got {token_mask.dtype} {tuple(token_mask.shape)}")
+
+
+@functools.lru_cache(maxsize=256)
+def _balance_bytes(T, E):
+    need = ctypes.c_int64(0)
+    check(lib.qmoe_moe_balance_workspace_size(T, E, ctypes.byref(need)), "moe_balance (shape)")
+    return need.value
+
+
+def moe_balance(router_logits, topk, scoring_func="softmax", renormalize=True, bias=None, routed_scaling_factor=1.0,
+                num_expert_group=1, topk_group=1, token_mask=None):
+    """Routing with its balance loss: (weights f32 [T, k], ids int32 [T, k],
+    loss f32 [], counts int32 [E]); see include/qmoe.h `qmoe_moe_balance`."""
+    _check_balance(router_logits, topk, scoring_func, bias, num_expert_group, topk_group, token_mask, "moe_balance")
+    with _on_device(router_logits, bias, token_mask):
+        dev = router_logits.device
+        T, E = router_logits.shape
+        w = torch.empty((T, topk), dtype=torch.float32, device=dev)
+        ids = torch.empty((T, topk), dtype=torch.int32, device=dev)
+        if T == 0:
+            return w, ids, torch.zeros((), device=dev), torch.zeros(E, dtype=torch.int32, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        counts = torch.empty(E, dtype=torch.int32, device=dev)
+        x, b = router_logits.contiguous(), _f32_flat(bias)
+        m = None if token_mask is None else token_mask.contiguous()
+        ws, ws_n = _workspace(dev, _balance_bytes(T, E))
+        check(lib.qmoe_moe_balance(x.data_ptr(), x.dtype is torch.float32, T, E, topk, _SCORING[scoring_func], _addr(b),
+                                   bool(renormalize), routed_scaling_factor, num_expert_group or 1, topk_group or 1,
+                                   _addr(m), w.data_ptr(), ids.data_ptr(), loss.data_ptr(), counts.data_ptr(), _addr(ws),
+                                   ws_n, _raw_stream(dev)), "moe_balance")
+    return w, ids, loss, counts
+
+
+def moe_balance_grad(router_logits, topk_ids, counts, g_weights, g_loss, scoring_func="softmax", renormalize=True,
+                     routed_scaling_factor=1.0, token_mask=None):
+    """Gradient of `moe_balance` with respect to the logits (in their type), for
+    those of its weights and loss (either may be None)."""
+    k = topk_ids.shape[-1]
+    _check_balance(router_logits, k, scoring_func, None, 1, 1, token_mask, "moe_balance_grad")
+    T, E = router_logits.shape
+    for v, shape, dtype, name in ((topk_ids, (T, k), torch.int32, "topk_ids"), (counts, (E,), torch.int32, "counts"),
+                                  (g_weights, (T, k), torch.float32, "g_weights"), (g_loss, (), torch.float32, "g_loss")):
+        if v is not None and (v.dtype is not dtype or tuple(v.shape) != shape):
+            raise ValueError(f"moe_balance_grad: {name} must be {dtype} {shape}, got {v.dtype} {tuple(v.shape)}")
+    with _on_device(router_logits, topk_ids, counts, g_weights, g_loss, token_mask):
+        dev = router_logits.device
+        d = torch.empty((T, E), dtype=router_logits.dtype, device=dev)
+        if T == 0:
+            return d
+        x, ids, c = router_logits.contiguous(), topk_ids.contiguous(), counts.contiguous()
+        gw = None if g_weights is None else g_weights.contiguous()
+        m = None if token_mask is None else token_mask.contiguous()
+        check(lib.qmoe_moe_balance_grad(x.data_ptr(), x.dtype is torch.float32, T, E, k, _SCORING[scoring_func],
+                                        bool(renormalize), routed_scaling_factor, _addr(m), ids.data_ptr(), c.data_ptr(),
+                                        _addr(gw), _addr(g_loss), d.data_ptr(), _raw_stream(dev)), "moe_balance_grad")
+    return d
+
+
+# ---------------------------------------------------------------- norms around a block
+
+_ROW_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+BLOCK_MAX = (1 << 24, 16384)  # rows, row length
+
+
+def _rows(t, H):
+    """(rows [T, H] with contiguous elements, their pitch) of ``t`` [..., H]."""
+    r = t if t.dim() == 2 else t.reshape(-1, H)
+    T = r.shape[0]
+    if (H > 1 and r.stride(1) != 1) or (T > 1 and r.stride(0) < H):
+        r = r.clone(memory_format=torch.contiguous_format)
+    return r, (r.stride(0) if T > 1 else H)
+
+
+def _gate_kind(gate, shape, what):
+    """0 none, 1 per channel, 2 per token, 3 per element of a block's output of ``shape``."""
+    if gate is None:
+        return 0
+    g = tuple(gate.shape)
+    if gate.dtype in _ROW_TYPES:
+        if g == shape[-1:]:
+            return 1
+        if g == (*shape[:-1], 1):
+            return 2
+        if g == shape:
+            return 3
+    raise ValueError(f"{what}: the gate of a block of {shape} is bf16, f16 or f32 {shape[-1:]}, {(*shape[:-1], 1)} or {shape}, "
+                     f"got {gate.dtype} {g}")
+
+
+def _check_block(y, residual, gate, post_weight, next_weight, z_dtype, what):
+    shape = tuple(residual.shape)
+    if residual.dim() < 1 or residual.dtype not in _ROW_TYPES:
+        raise ValueError(f"{what}: rows must be bf16, f16 or f32 [..., H], got {residual.dtype} {shape}")
+    H = shape[-1]
+    if not 1 <= H <= BLOCK_MAX[1] or residual.numel() // H > BLOCK_MAX[0]:
+        raise ValueError(f"{what}: takes rows of 1 to {BLOCK_MAX[1]} values, {BLOCK_MAX[0]} of them at most, got {shape}")
+    yt = z_dtype if y is None else y.dtype
+    if yt not in _ROW_TYPES or (residual.dtype is not yt and residual.dtype is not torch.float32):
+        raise ValueError(f"{what}: a residual of {residual.dtype} for a block in {yt} (its own type, or float32)")
+    if y is not None and tuple(y.shape) != shape:
+        raise ValueError(f"{what}: a residual of {shape} for a block of {tuple(y.shape)}")
+    kind = _gate_kind(gate, shape, what)
+    if kind == 3 and gate.dtype is not yt:
+        raise ValueError(f"{what}: a gate per element has the block's type {yt}, not {gate.dtype}")
+    wt = None
+    for w, name in ((post_weight, "norm_weight"), (next_weight, "next_weight")):
+        if w is None:
+            continue
+        if w.dtype not in _ROW_TYPES or tuple(w.shape) != (H,):
+            raise ValueError(f"{what}: {name} must be bf16, f16 or f32 [{H}], got {w.dtype} {tuple(w.shape)}")
+        if wt is not None and w.dtype is not wt:
+            raise ValueError(f"{what}: the two norm weights must have one type, got {wt} and {w.dtype}")
+        wt = w.dtype
+    return kind, yt, wt
+
+
+def _block_desc(T, H, y, residual, gate, kind, post, nxt, yt, rt, wt, scale, residual_scale, eps, offset):
+    """(`qmoe_block_desc` without its outputs, the tensors whose addresses it holds)"""
+    d = _capi.BlockDesc()
+    d.T, d.H = T, H
+    keep = []
+    for name, pitch, t in (("y", "ldy", y), ("residual", "ldr", residual)):
+        if t is not None:
+            r, ld = _rows(t, H)
+            keep.append(r)
+            setattr(d, name, r.data_ptr())
+            setattr(d, pitch, ld)
+    if kind:
+        if kind == 3:
+            g, d.ldg = _rows(gate, H)
+        else:
+            g = gate.reshape(-1).contiguous()
+        keep.append(g)
+        d.gate, d.gate_type = g.data_ptr(), _ROW_TYPES[gate.dtype]
+    for name, w in (("post_weight", post), ("next_weight", nxt)):
+        if w is not None:
+            w = w.contiguous()
+            keep.append(w)
+            setattr(d, name, w.data_ptr())
+    d.y_type, d.residual_type, d.weight_type, d.gate_kind = _ROW_TYPES[yt], _ROW_TYPES[rt], _ROW_TYPES.get(wt, 0), kind
+    d.scale, d.residual_scale, d.weight_offset, d.eps = scale, residual_scale, offset, eps
+    return d, keep
+
+
+def block_residual(y, residual, gate=None, post_weight=None, next_weight=None, scale=1.0, residual_scale=1.0, eps=1e-6,
+                   weight_offset=0.0, z_dtype=None, keep=False):
+    """(h, z, rstd_y, rstd_h) of a block's output ``y``, see include/qmoe.h
+    `qmoe_block_residual`; None for what the call has not (h without y, the norm
+    of the residual alone, whose z is of ``z_dtype``; z without ``next_weight``;
+    the rows' factors without ``keep``)."""
+    what = "block_residual"
+    if y is None and (next_weight is None or gate is not None or post_weight is not None):
+        raise ValueError(f"{what}: without a block's output there is only the next norm")
+    kind, yt, wt = _check_block(y, residual, gate, post_weight, next_weight, z_dtype, what)
+    shape, H = residual.shape, residual.shape[-1]
+    T = residual.numel() // H
+    with _on_device(residual, y, gate, post_weight, next_weight):
+        dev, f32 = residual.device, torch.float32
+        h = None if y is None else torch.empty(shape, dtype=residual.dtype, device=dev)
+        z = None if next_weight is None else torch.empty(shape, dtype=yt, device=dev)
+        ry = torch.empty(T, dtype=f32, device=dev) if keep and post_weight is not None else None
+        rh = torch.empty(T, dtype=f32, device=dev) if keep and next_weight is not None else None
+        if T == 0:
+            return h, z, ry, rh
+        d, held = _block_desc(T, H, y, residual, gate, kind, post_weight, next_weight, yt, residual.dtype, wt, scale,
+                              residual_scale, eps, weight_offset)
+        d.h, d.ldh, d.z, d.ldz, d.rstd_y, d.rstd_h = _addr(h), H, _addr(z), H, _addr(ry), _addr(rh)
+        check(lib.qmoe_block_residual(ctypes.byref(d), _raw_stream(dev)), what)
+    return h, z, ry, rh
+
+
+@functools.lru_cache(maxsize=256)
+def _block_grad_bytes(T, H):
+    need = ctypes.c_int64(0)
+    check(lib.qmoe_block_residual_grad_workspace_size(T, H, ctypes.byref(need)), "block_residual_grad (shape)")
+    return need.value
+
+
+def block_residual_grad(g_h, g_z, y, h, gate, post_weight, next_weight, rstd_y, rstd_h, scale=1.0, residual_scale=1.0,
+                        eps=1e-6, weight_offset=0.0, z_dtype=None, need=(True,) * 5):
+    """Gradients of `block_residual` for those of h and z (one may be None): of
+    (y, residual, gate, post_weight, next_weight), None for operands that the
+    call has not, that ``need`` leaves out or that no gradient reaches. ``h`` is
+    its first result (without y: the residual)."""
+    what = "block_residual_grad"
+    kind, yt, wt = _check_block(y, h, gate, post_weight, next_weight, z_dtype, what)
+    shape, H, rt = h.shape, h.shape[-1], h.dtype
+    T = h.numel() // H
+    for g, dtype, name in ((g_h, rt, "g_h"), (g_z, yt, "g_z")):
+        if g is not None and (g.dtype is not dtype or g.shape != shape):
+            raise ValueError(f"{what}: {name} must be {dtype} {tuple(shape)}, got {g.dtype} {tuple(g.shape)}")
+    if (g_h is None and g_z is None) or (g_z is not None and next_weight is None):
+        raise ValueError(f"{what}: needs the gradient of h or of z")
+    for r, w, name in ((rstd_y, post_weight, "rstd_y"), (rstd_h, next_weight if g_z is not None else None, "rstd_h")):
+        if w is not None and (r is None or r.dtype is not torch.float32 or r.numel() != T or not r.is_contiguous()):
+            raise ValueError(f"{what}: {name} must hold the {T} row factors that block_residual kept")
+    with _on_device(h, y, gate, post_weight, next_weight, g_h, g_z, rstd_y, rstd_h):
+        dev = h.device
+
+        def like(wanted, t):
+            return torch.empty(t.shape, dtype=t.dtype, device=dev) if wanted and t is not None else None
+
+        dy, dr, dg = like(need[0], y), like(need[1], h), like(need[2], gate)
+        dp, dn = like(need[3], post_weight), like(need[4] and g_z is not None, next_weight)
+        if T == 0:
+            return tuple(None if t is None else t.zero_() for t in (dy, dr, dg, dp, dn))
+        d, held = _block_desc(T, H, y, None, gate, kind, post_weight, next_weight, yt, rt, wt, scale, residual_scale, eps,
+                              weight_offset)
+        hr, d.ldh = _rows(h, H)
+        d.h, d.rstd_y, d.rstd_h = hr.data_ptr(), _addr(rstd_y), _addr(rstd_h)
+        g = _capi.BlockGrads()
+        for name, pitch, t in (("g_h", "ldgh", g_h), ("g_z", "ldgz", g_z)):
+            if t is not None:
+                r, ld = _rows(t, H)
+                held.append(r)
+                setattr(g, name, r.data_ptr())
+                setattr(g, pitch, ld)
+        g.d_y, g.d_residual, g.d_gate, g.d_post_weight, g.d_next_weight = (_addr(t) for t in (dy, dr, dg, dp, dn))
+        sums = dp is not None or dn is not None or (kind == 1 and dg is not None)
+        ws, ws_n = _workspace(dev, _block_grad_bytes(T, H) if sums else 0)
+        check(lib.qmoe_block_residual_grad(ctypes.byref(d), ctypes.byref(g), _addr(ws), ws_n, _raw_stream(dev)), what)
+    return dy, dr, dg, dp, dn
+
+
+# ---------------------------------------------------------------- 8-bit checkpoints
+
+ACT_MAX = (1 << 24, 1 << 20)     # rows, gate columns
+LINEAR_MAX = (1 << 20, 1 << 18, 1 << 16)  # tokens, outputs, inputs
+
+
+def _check_act(x, activation, what):
+    act = act_code(activation)
+    if act[0] == _capi.ACT_NONE:
+        raise ValueError(f"{what}: a gate / up activation is required")
+    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
+        raise ValueError(f"{what}: gate and up must be bf16 or f16, got {x.dtype}")
+    n = x.shape[-1] if x.dim() else 0
+    if n == 0 or n % 2 or n // 2 > ACT_MAX[1] or x.numel() // n > ACT_MAX[0]:
+        raise ValueError(f"{what}: takes [..., 2 I] of I up to {ACT_MAX[1]}, {ACT_MAX[0]} rows at most, got {tuple(x.shape)}")
+    return act
+
+
+def act_checkpoint(x, activation, keep=True):
+    """Gated activation of ``x`` [..., 2 I] ([gate | up], bf16 or f16): (h [..., I],
+    codes uint8 [T, 2 I], scales uint8 [T, 2, ceil(I / 32)]), the 8 bits of gate and
+    up for `act_checkpoint_grad` (None without ``keep``)."""
+    act, p0, p1 = _check_act(x, activation, "act_checkpoint")
+    n = x.shape[-1]
+    I, T = n // 2, x.numel() // n
+    with _on_device(x):
+        dev = x.device
+        h = torch.empty((*x.shape[:-1], I), dtype=x.dtype, device=dev)
+        codes = torch.empty((T, n), dtype=torch.uint8, device=dev) if keep else None
+        scales = torch.empty((T, 2, (I + 31) // 32), dtype=torch.uint8, device=dev) if keep else None
+        if T:
+            r, ld = _rows(x, n)
+            check(lib.qmoe_act_checkpoint(r.data_ptr(), ld, _ROW_TYPES[x.dtype], T, I, act, p0, p1, h.data_ptr(), I,
+                                          _addr(codes), _addr(scales), _raw_stream(dev)), "act_checkpoint")
+    return h, codes, scales
+
+
+def act_checkpoint_grad(codes, scales, dh, activation):
+    """Gradient [..., 2 I] of `act_checkpoint` for that of h, at its 8-bit values."""
+    act, p0, p1 = act_code(activation)
+    I = dh.shape[-1] if dh.dim() else 0
+    T = dh.numel() // I if I else 0
+    if act == _capi.ACT_NONE or (dh.dtype is not torch.bfloat16 and dh.dtype is not torch.float16) or I == 0:
+        raise ValueError(f"act_checkpoint_grad: {activation!r} of a gradient of {dh.dtype} {tuple(dh.shape)}")
+    for t, shape, name in ((codes, (T, 2 * I), "codes"), (scales, (T, 2, (I + 31) // 32), "scales")):
+        if t.dtype is not torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"act_checkpoint_grad: {name} must be contiguous uint8 {shape}, got {t.dtype} {tuple(t.shape)}")
+    with _on_device(codes, scales, dh):
+        dx = torch.empty((*dh.shape[:-1], 2 * I), dtype=dh.dtype, device=dh.device)
+        if T:
+            r, ld = _rows(dh, I)
+            check(lib.qmoe_act_checkpoint_grad(codes.data_ptr(), scales.data_ptr(), T, I, act, p0, p1, r.data_ptr(), ld,
+                                               _ROW_TYPES[dh.dtype], dx.data_ptr(), _raw_stream(dh.device)),
+                  "act_checkpoint_grad")
+    return dx
+
+
+def _gemm_rows(t, n):
+    """Rows of ``t`` [..., n] that the tiles copy 16 bytes at a time, and their pitch."""
+    r, ld = _rows(t, n)
+    if ld % 8 or ld >= 1 << 22 or r.data_ptr() % 16:
+        r, ld = r.clone(memory_format=torch.contiguous_format), n
+    return r, ld
+
+
+def _check_linear(x, weight, bias, what):
+    if x.dtype is not torch.bfloat16 or weight.dtype is not torch.bfloat16 or weight.dim() != 2 or x.dim() < 1 or \
+            x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{what}: takes bf16 [..., K] and [N, K], got {x.dtype} {tuple(x.shape)} and {weight.dtype} "
+                         f"{tuple(weight.shape)}")
+    N, K = weight.shape
+    if N == 0 or K == 0 or K % 32 or N % 8 or N > LINEAR_MAX[1] or K > LINEAR_MAX[2] or x.numel() // K > LINEAR_MAX[0]:
+        raise ValueError(f"{what}: takes K in multiples of 32 up to {LINEAR_MAX[2]}, N in multiples of 8 up to "
+                         f"{LINEAR_MAX[1]} and {LINEAR_MAX[0]} rows at most, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if weight.stride(1) != 1 or weight.stride(0) < K or weight.stride(0) % 8 or weight.stride(0) >= 1 << 22:
+        raise ValueError(f"{what}: the weight's rows must be contiguous and apart by a multiple of 8, got strides "
+                         f"{weight.stride()}")
+    if bias is not None and (bias.dtype not in _GRAD_TYPES or tuple(bias.shape) != (N,)):
+        raise ValueError(f"{what}: the bias must be bf16 or f32 [{N}], got {bias.dtype} {tuple(bias.shape)}")
+
+
+def _check_aligned(weight, what):
+    if weight.data_ptr() % 16:
+        raise ValueError(f"{what}: the weight must be 16-byte aligned")
+
+
+def linear_checkpoint(x, weight, bias=None, keep=True):
+    """y = x w^T + bias (bf16 [..., N]) and the 8 bits of x: (y, codes uint8 [T, K],
+    scales uint8 [T, K / 32]) for `linear_grad` (None without ``keep``)."""
+    _check_linear(x, weight, bias, "linear_checkpoint")
+    _check_aligned(weight, "linear_checkpoint")
+    N, K = weight.shape
+    with _on_device(x, weight, bias):
+        dev = x.device
+        T = x.numel() // K
+        codes = torch.empty((T, K), dtype=torch.uint8, device=dev) if keep else None
+        scales = torch.empty((T, K // 32), dtype=torch.uint8, device=dev) if keep else None
+        if T == 0:
+            return torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev), codes, scales
+        r, ld = _gemm_rows(x, K)
+        if keep:
+            check(lib.qmoe_pack_8bit(r.data_ptr(), ld, T, K, codes.data_ptr(), scales.data_ptr(), _raw_stream(dev)),
+                  "linear_checkpoint (8 bits)")
+        y = gemm(_capi.W16A16, r, weight, bias=None if bias is None else _f32_flat(bias))
+    return y.view(*x.shape[:-1], N), codes, scales
+
+
+@functools.lru_cache(maxsize=256)
+def _linear_grad_bytes(T, N, K, need_x, need_weight, need_bias):
+    need = ctypes.c_int64(0)
+    check(lib.qmoe_linear_grad_workspace_size(T, N, K, need_x, need_weight, need_bias, ctypes.byref(need)),
+          "linear_grad (shape)")
+    return need.value
+
+
+def linear_grad(dy, weight, codes=None, scales=None, need_x=True, need_weight=True, bias_dtype=None):
+    """Gradients (dx bf16 [..., K], dw bf16 [N, K], dbias of ``bias_dtype``) of
+    `linear_checkpoint` for that of y; None for what is not asked for. ``codes`` and
+    ``scales`` are needed for dw."""
+    if weight.dim() != 2 or dy.dtype is not torch.bfloat16 or dy.dim() < 1 or dy.shape[-1] != weight.shape[0]:
+        raise ValueError(f"linear_grad: a gradient of {dy.dtype} {tuple(dy.shape)} for a weight of {tuple(weight.shape)}")
+    N, K = weight.shape
+    _check_linear(dy.new_empty((0, K)), weight, None, "linear_grad")
+    _check_aligned(weight, "linear_grad")
+    T = dy.numel() // N
+    if T > LINEAR_MAX[0]:
+        raise ValueError(f"linear_grad: takes {LINEAR_MAX[0]} rows at most, got {T}")
+    if need_weight:
+        for t, shape, name in ((codes, (T, K), "codes"), (scales, (T, K // 32), "scales")):
+            if t is None or t.dtype is not torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous():
+                raise ValueError(f"linear_grad: {name} must be contiguous uint8 {shape}")
+    if bias_dtype is not None and bias_dtype not in _GRAD_TYPES:
+        raise ValueError(f"linear_grad: the bias is bf16 or f32, not {bias_dtype}")
+    with _on_device(dy, weight, codes, scales):
+        dev, bf16 = dy.device, torch.bfloat16
+        dx = torch.empty((*dy.shape[:-1], K), dtype=bf16, device=dev) if need_x else None
+        dw = torch.empty((N, K), dtype=bf16, device=dev) if need_weight else None
+        db = torch.empty(N, dtype=bias_dtype, device=dev) if bias_dtype is not None else None
+        if T == 0:
+            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
+        if need_x or need_weight or db is not None:
+            r, ld = _gemm_rows(dy, N)
+            ws, ws_n = _workspace(dev, _linear_grad_bytes(T, N, K, bool(need_x), bool(need_weight), db is not None))
+            check(lib.qmoe_linear_grad(r.data_ptr(), ld, T, N, K, weight.data_ptr(), weight.stride(0),
+                                       _addr(codes) if need_weight else None, _addr(scales) if need_weight else None,
+                                       _addr(dx), _addr(dw), _addr(db), bias_dtype is torch.float32, _addr(ws), ws_n,
+                                       _raw_stream(dev)), "linear_grad")
+    return dx, dw, db
