@@ -288,7 +288,10 @@ def test_linear_layouts_and_method(dev):
     method = UnquantizedLinearMethod()
     x = wide[..., :96].contiguous()
     y = method.apply_checkpointed(layer, x)
-    assert torch.equal(y, method.apply(layer, x)) and y.requires_grad
+    # (the same product by other kernels: both within half a step of the exact sum)
+    apart = (y - method.apply(layer, x)).abs().to(D)
+    mag = x.to(D).abs() @ w.to(D).abs().t()
+    assert (apart <= torch.finfo(BF16).eps * y.abs().to(D) + 4 * 96 * EPS * mag).all() and y.requires_grad
     y.sum().backward()
     assert layer.weight.grad.shape == layer.weight.shape
 

@@ -90,7 +90,7 @@ struct ActParams {
 
 // codes / scale bytes of columns i .. i + 7 of row half r2 (2 t: g, 2 t + 1: u)
 template <bool AL>
-__device__ __forceinline__ void put_codes(const ActParams& p, int64_t r2, int64_t i, const float (&v)[8]) {
+__device__ __forceinline__ void put_codes(const ActParams& p, int64_t r2, uint32_t i, const float (&v)[8]) {
   uint32_t byte;
   const uint2 c = encode8(v, byte);
   if (i >= p.I) return;
@@ -105,7 +105,7 @@ __device__ __forceinline__ void put_codes(const ActParams& p, int64_t r2, int64_
   if ((i & 31) == 0) p.scales[r2 * p.nb + i / 32] = (uint8_t)byte;
 }
 template <bool AL>
-__device__ __forceinline__ void get_codes(const ActParams& p, int64_t r2, int64_t i, uint2& c, uint32_t& byte) {
+__device__ __forceinline__ void get_codes(const ActParams& p, int64_t r2, uint32_t i, uint2& c, uint32_t& byte) {
   const uint8_t* at = p.codes + r2 * p.I + i;
   if constexpr (AL) {
     c = *reinterpret_cast<const uint2*>(at);
@@ -121,7 +121,8 @@ __device__ __forceinline__ void get_codes(const ActParams& p, int64_t r2, int64_
 // Workgroup (t, y): row t, threads y * blockDim.x .. of 8 columns each
 template <int T, int ACT, bool AL>
 __global__ __launch_bounds__(512) void act_kernel(const ActParams p) {
-  const int64_t t = blockIdx.x, i = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * 8, I = p.I;
+  const int64_t t = blockIdx.x, I = p.I;
+  const uint32_t i = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
   const uint8_t* x = p.x + t * p.ldx;
   float g[8] = {}, u[8] = {}, h[8];
   if (i < I) {
@@ -141,7 +142,8 @@ __global__ __launch_bounds__(512) void act_kernel(const ActParams p) {
 
 template <int T, int ACT, bool AL>
 __global__ __launch_bounds__(512) void act_grad_kernel(const ActParams p) {
-  const int64_t t = blockIdx.x, i = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * 8, I = p.I;
+  const int64_t t = blockIdx.x, I = p.I;
+  const uint32_t i = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
   if (i >= I) return;
   uint2 cg, cu;
   uint32_t bg, bu;
@@ -164,7 +166,8 @@ __global__ __launch_bounds__(512) void act_grad_kernel(const ActParams p) {
 
 // Rows of bf16 -> 8 bits
 __global__ __launch_bounds__(512) void pack_kernel(const ActParams p) {
-  const int64_t t = blockIdx.x, i = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * 8;
+  const int64_t t = blockIdx.x;
+  const uint32_t i = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
   float v[8] = {};
   if (i < p.I) load8<RT_BF16, true>(p.x + t * p.ldx, i, p.I, v);
   put_codes<true>(p, t, i, v);

@@ -27,6 +27,7 @@ namespace {
 using namespace qmoe_row;
 
 constexpr int kMaxThreads = 1024;
+constexpr int64_t kMaxLdsRow = 8192;  // two float32 vectors of a row in 64 KB of LDS
 constexpr int64_t kMaxRow = kMaxThreads * 16, kMaxRows = 1 << 24;
 
 enum { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_TOKEN = 2, GATE_FULL = 3 };
@@ -51,13 +52,17 @@ __device__ __forceinline__ void row_sums(float (&v)[K], float (*red)[16][K], int
 }
 
 // Piece c of this thread starts at this column
-__device__ __forceinline__ int64_t piece(int c) { return ((int64_t)c * blockDim.x + threadIdx.x) * 8; }
+__device__ __forceinline__ uint32_t piece(int c) { return (c * blockDim.x + threadIdx.x) * 8; }
+
+// This wavefront's row of the workgroup
+__device__ __forceinline__ int own_row() { return __builtin_amdgcn_readfirstlane(threadIdx.y); }
 
 template <int YT, int RT, int C, int THREADS, bool AL>
 __global__ __launch_bounds__(THREADS) void block_residual_kernel(const qmoe_block_desc p) {
   __shared__ float red[2][8][16][1];
   const int W = blockDim.x >> 6;
-  const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, H = p.H;
+  const int64_t t = (int64_t)blockIdx.x * blockDim.y + own_row();
+  const uint32_t H = (uint32_t)p.H;
   const bool row = t < p.T;
   Raw8<YT> yr[C], gr[C];
   Raw8<RT> rr[C];
@@ -66,7 +71,7 @@ __global__ __launch_bounds__(THREADS) void block_residual_kernel(const qmoe_bloc
   const uint8_t* full = static_cast<const uint8_t*>(p.gate) + t * p.ldg * rt_size(YT);
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int64_t i = piece(c);
+    const uint32_t i = piece(c);
     if (!row || i >= H) continue;
     if (p.y) yr[c] = load_raw8<YT, AL>(y, i, H);
     if (p.gate_kind == GATE_FULL) gr[c] = load_raw8<YT, AL>(full, i, H);
@@ -92,7 +97,7 @@ __global__ __launch_bounds__(THREADS) void block_residual_kernel(const qmoe_bloc
   float s[1] = {0.0f};
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int64_t i = piece(c);
+    const uint32_t i = piece(c);
     if (!row || i >= H) continue;
     raw8_values<RT>(rr[c], h[c]);
     if (p.y) {
@@ -121,7 +126,7 @@ __global__ __launch_bounds__(THREADS) void block_residual_kernel(const qmoe_bloc
   if (row && p.rstd_h && threadIdx.x == 0) p.rstd_h[t] = rh;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int64_t i = piece(c);
+    const uint32_t i = piece(c);
     if (!row || i >= H) continue;
     float m[8];
     load8_any<AL>(p.next_weight, p.weight_type, i, H, m);
@@ -131,74 +136,119 @@ __global__ __launch_bounds__(THREADS) void block_residual_kernel(const qmoe_bloc
   }
 }
 
-// Sums over tokens leave in parts [workgroups][3][H] (next weight, post weight,
-// channel gate; those not asked for are not written)
-template <int YT, int RT, int C, int THREADS, bool AL>
-__global__ __launch_bounds__(THREADS) void block_residual_grad_kernel(const qmoe_block_desc p, const qmoe_block_grads d,
-                                                                   float* parts) {
+// The gradients. What rows share are two vectors, c1 = off + wn and c2 = (off + wp)
+// gate (a gate per channel; else without it), and what is summed over tokens are two
+// as well: dz nh, and H' ny (times a gate per token or element), of which the
+// gradients of wp and of a gate per channel are the multiples by sc gate and sc
+// (off + wp). c1 and c2 lie in LDS (LDSC; rows of up to 8192), the sums in
+// registers; they leave in parts [workgroups][2][H].
+// PARTS: 1 both norms are there, 2 the second alone (no y), 0 asked at run time, at
+// the cost of registers.
+template <int YT, int RT, int C, int THREADS, bool AL, int PARTS, bool LDSC>
+__global__ __launch_bounds__(THREADS, THREADS == 512 && AL ? 4 : 1) void block_residual_grad_kernel(
+    const qmoe_block_desc p, const qmoe_block_grads d, float* parts) {
   __shared__ float red1[2][8][16][1], red2[2][8][16][2];
-  extern __shared__ float rowbuf[];  // [H] where several rows share the workgroup
+  extern __shared__ float dyn[];  // LDSC: c1 [H8], c2 [H8]; afterwards rows' sums
   const int W = blockDim.x >> 6, R = blockDim.y;
-  const int64_t H = p.H;
+  const uint32_t H = (uint32_t)p.H, H8 = (H + 7) / 8 * 8;
   const float invH = 1.0f / (float)H;
-  const bool post = p.y && p.post_weight, next = p.next_weight && d.g_z;
-  float an[C][8], ap[C][8], ag[C][8];
+  const bool has_y = PARTS ? PARTS == 1 : p.y != nullptr, post = PARTS ? PARTS == 1 : p.y && p.post_weight,
+             next = PARTS || (p.next_weight && d.g_z);
+  const int kind = p.gate_kind;
+  auto make_c1 = [&](uint32_t i, float (&c)[8]) {
+    load8_any<AL>(p.next_weight, p.weight_type, i, H, c);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) c[k] += p.weight_offset;
+  };
+  auto make_c2 = [&](uint32_t i, float (&c)[8]) {
+    float g[8];
+    if (post) load8_any<AL>(p.post_weight, p.weight_type, i, H, c);
+    if (kind == GATE_CHANNEL) load8_any<AL>(p.gate, p.gate_type, i, H, g);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) c[k] = (post ? c[k] + p.weight_offset : 1.0f) * (kind == GATE_CHANNEL ? g[k] : 1.0f);
+  };
+  if constexpr (LDSC) {
+    for (uint32_t i = (threadIdx.y * blockDim.x + threadIdx.x) * 8; i < H; i += blockDim.x * R * 8) {
+      float c[8];
+      if (next) {
+        make_c1(i, c);
+        store8<RT_F32, true>(dyn, i, H8, c);
+      }
+      if (has_y) {
+        make_c2(i, c);
+        store8<RT_F32, true>(dyn + H8, i, H8, c);
+      }
+    }
+    __syncthreads();
+  }
+  auto c1_at = [&](uint32_t i, float (&c)[8]) {
+    if constexpr (LDSC) load8<RT_F32, true>(dyn, i, H8, c);
+    else make_c1(i, c);
+  };
+  auto c2_at = [&](uint32_t i, float (&c)[8]) {
+    if constexpr (LDSC) load8<RT_F32, true>(dyn + H8, i, H8, c);
+    else make_c2(i, c);
+  };
+  float an[C][8], ap[C][8];
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) an[c][k] = ap[c][k] = ag[c][k] = 0.0f;
+    for (int k = 0; k < 8; ++k) an[c][k] = ap[c][k] = 0.0f;
   int side = 0;
   for (int64_t t0 = (int64_t)blockIdx.x * R; t0 < p.T; t0 += (int64_t)gridDim.x * R, side ^= 1) {
-    const int64_t t = t0 + threadIdx.y;
+    const int64_t t = t0 + own_row();
     const bool row = t < p.T;
     Raw8<YT> yr[C], gr[C], zr[C];
     Raw8<RT> hr[C], dr[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int64_t i = piece(c);
+      const uint32_t i = piece(c);
       if (!row || i >= H) continue;
       if (next) {
         zr[c] = load_raw8<YT, AL>(static_cast<const uint8_t*>(d.g_z) + t * d.ldgz * rt_size(YT), i, H);
         hr[c] = load_raw8<RT, AL>(static_cast<const uint8_t*>(p.h) + t * p.ldh * rt_size(RT), i, H);
       }
       if (d.g_h) dr[c] = load_raw8<RT, AL>(static_cast<const uint8_t*>(d.g_h) + t * d.ldgh * rt_size(RT), i, H);
-      if (p.y) yr[c] = load_raw8<YT, AL>(static_cast<const uint8_t*>(p.y) + t * p.ldy * rt_size(YT), i, H);
-      if (p.gate_kind == GATE_FULL)
+      if (has_y) yr[c] = load_raw8<YT, AL>(static_cast<const uint8_t*>(p.y) + t * p.ldy * rt_size(YT), i, H);
+      if (kind == GATE_FULL)
         gr[c] = load_raw8<YT, AL>(static_cast<const uint8_t*>(p.gate) + t * p.ldg * rt_size(YT), i, H);
     }
     const float rh = next && row ? p.rstd_h[t] : 0.0f, ry = post && row ? p.rstd_y[t] : 1.0f;
-    const float gt = p.gate_kind == GATE_TOKEN && row ? one_any(p.gate, p.gate_type, t) : 1.0f;
-    float g[C][8];  // the gradient of h, then of b
+    const float gt = kind == GATE_TOKEN && row ? one_any(p.gate, p.gate_type, t) : 1.0f;
     float s1[1] = {0.0f};
+    if (next) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int64_t i = piece(c);
-      if (!row || i >= H) continue;
-      if (!next) continue;
-      float n[8], w[8];
-      raw8_values<YT>(zr[c], g[c]);
-      raw8_values<RT>(hr[c], n);
-      load8_any<AL>(p.next_weight, p.weight_type, i, H, w);
+      for (int c = 0; c < C; ++c) {
+        const uint32_t i = piece(c);
+        if (!row || i >= H) continue;
+        float q[8], n[8], w[8];
+        raw8_values<YT>(zr[c], q);
+        raw8_values<RT>(hr[c], n);
+        c1_at(i, w);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        n[k] *= rh;
-        an[c][k] += g[c][k] * n[k];
-        g[c][k] *= p.weight_offset + w[k];
-        s1[0] += g[c][k] * n[k];
+        for (int k = 0; k < 8; ++k) {
+          const float m = q[k] * (n[k] * rh);
+          an[c][k] += m;
+          s1[0] += m * w[k];
+        }
       }
+      row_sums<1>(s1, red1[side], W);
+      s1[0] *= invH;
     }
-    if (next) row_sums<1>(s1, red1[side], W);
+    float g[C][8];  // H'
     float s2[2] = {0.0f, 0.0f};
-    float b[C][8];  // y r(y), for the post-norm
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int64_t i = piece(c);
+      const uint32_t i = piece(c);
       if (!row || i >= H) continue;
-      float v[8];
+      float v[8], w[8];
       if (next) {
+        float q[8];
+        raw8_values<YT>(zr[c], q);
         raw8_values<RT>(hr[c], v);
+        c1_at(i, w);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) g[c][k] = rh * (g[c][k] - v[k] * rh * (s1[0] * invH));
+        for (int k = 0; k < 8; ++k) g[c][k] = rh * (q[k] * w[k] - v[k] * rh * s1[0]);
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) g[c][k] = 0.0f;
@@ -213,48 +263,26 @@ __global__ __launch_bounds__(THREADS) void block_residual_grad_kernel(const qmoe
         for (int k = 0; k < 8; ++k) v[k] = p.residual_scale * g[c][k];
         store8<RT, AL>(static_cast<uint8_t*>(d.d_residual) + t * H * rt_size(RT), i, H, v);
       }
-      if (!p.y) continue;
-      float m[8], w[8];
-      raw8_values<YT>(yr[c], b[c]);
-      if (post) {
-        load8_any<AL>(p.post_weight, p.weight_type, i, H, w);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          w[k] += p.weight_offset;
-          b[c][k] *= ry;
-          v[k] = b[c][k] * w[k];
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = b[c][k];
-      }
-      if (p.gate_kind == GATE_CHANNEL) load8_any<AL>(p.gate, p.gate_type, i, H, m);
-      if (p.gate_kind == GATE_FULL) raw8_values<YT>(gr[c], m);
+      if (!has_y) continue;
+      float b[8];
+      raw8_values<YT>(yr[c], b);
+      c2_at(i, w);
+      if (kind == GATE_FULL) raw8_values<YT>(gr[c], v);
       float dg[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float gate = p.gate_kind == GATE_CHANNEL || p.gate_kind == GATE_FULL ? m[k] : gt;
-        dg[k] = p.scale * g[c][k] * v[k];
+        const float u = g[c][k] * (b[k] * ry);
+        const float gate = kind == GATE_FULL ? v[k] : gt;  // (a gate per channel is in w)
+        ap[c][k] += gate * u;
+        dg[k] = p.scale * u * w[k];
+        s2[0] += gate * u * w[k];
         s2[1] += dg[k];
-        g[c][k] = p.scale * (gate * g[c][k]);
       }
-      if (p.gate_kind == GATE_CHANNEL) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) ag[c][k] += dg[k];
-      }
-      if (p.gate_kind == GATE_FULL && d.d_gate)
+      if (kind == GATE_FULL && d.d_gate)
         store8<YT, AL>(static_cast<uint8_t*>(d.d_gate) + t * H * rt_size(YT), i, H, dg);
-      if (post) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          ap[c][k] += g[c][k] * b[c][k];
-          g[c][k] *= w[k];
-          s2[0] += g[c][k] * b[c][k];
-        }
-      }
     }
-    if (!p.y) continue;
-    const bool token = p.gate_kind == GATE_TOKEN && d.d_gate;
+    if (!has_y) continue;
+    const bool token = kind == GATE_TOKEN && d.d_gate;
     if (post || token) row_sums<2>(s2, red2[side], W);
     if (token && row && threadIdx.x == 0) {
       if (p.gate_type == RT_BF16) static_cast<uint16_t*>(d.d_gate)[t] = f32_to_bf16(s2[1]);
@@ -262,67 +290,82 @@ __global__ __launch_bounds__(THREADS) void block_residual_grad_kernel(const qmoe
       else static_cast<_Float16*>(d.d_gate)[t] = (_Float16)s2[1];
     }
     if (!d.d_y) continue;
+    const float off = post ? s2[0] * invH : 0.0f, by = p.scale * ry;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int64_t i = piece(c);
+      const uint32_t i = piece(c);
       if (!row || i >= H) continue;
-      if (post) {
+      float b[8], w[8], v[8];
+      raw8_values<YT>(yr[c], b);
+      c2_at(i, w);
+      if (kind == GATE_FULL) raw8_values<YT>(gr[c], v);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) g[c][k] = ry * (g[c][k] - b[c][k] * (s2[0] * invH));
+      for (int k = 0; k < 8; ++k) {
+        const float gate = kind == GATE_FULL ? v[k] : gt;
+        const float q = gate * (g[c][k] * w[k]);
+        g[c][k] = by * (post ? q - b[k] * ry * off : q);
       }
       store8<YT, AL>(static_cast<uint8_t*>(d.d_y) + t * H * rt_size(YT), i, H, g[c]);
     }
   }
   if (!parts) return;
-  float* out = parts + (int64_t)blockIdx.x * 3 * H;
+  float* out = parts + (int64_t)blockIdx.x * 2 * H;
 #pragma unroll
-  for (int kind = 0; kind < 3; ++kind) {
-    const bool want = kind == 0 ? next && d.d_next_weight : kind == 1 ? post && d.d_post_weight
-                                                                       : p.gate_kind == GATE_CHANNEL && d.d_gate;
-    if (!want) continue;
-    float (&a)[C][8] = kind == 0 ? an : kind == 1 ? ap : ag;
+  for (int k2 = 0; k2 < 2; ++k2) {
+    if (k2 == 0 ? !(next && d.d_next_weight) : !has_y) continue;
+    float (&a)[C][8] = k2 == 0 ? an : ap;
     for (int r = 1; r < R; ++r) {  // the other rows' sums, one row after the other
       __syncthreads();
       if ((int)threadIdx.y == r)
 #pragma unroll
         for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (piece(c) + k < H) rowbuf[piece(c) + k] = a[c][k];
+          if (piece(c) < H) store8<RT_F32, true>(dyn, piece(c), H8, a[c]);
       __syncthreads();
       if (threadIdx.y == 0)
 #pragma unroll
         for (int c = 0; c < C; ++c)
+          if (piece(c) < H) {
+            float v[8];
+            load8<RT_F32, true>(dyn, piece(c), H8, v);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (piece(c) + k < H) a[c][k] += rowbuf[piece(c) + k];
+            for (int k = 0; k < 8; ++k) a[c][k] += v[k];
+          }
     }
     if (threadIdx.y == 0)
 #pragma unroll
       for (int c = 0; c < C; ++c)
-        if (piece(c) < H) store8<RT_F32, AL>(out + kind * H, piece(c), H, a[c]);
+        if (piece(c) < H) store8<RT_F32, AL>(out + k2 * H, piece(c), H, a[c]);
   }
 }
 
-// Columns 64 x .. of kind y: parts of all workgroups, 16 at a time, then across them
-__global__ __launch_bounds__(1024) void block_join_kernel(const float* parts, int groups, int64_t H, void* d_next,
-                                                          void* d_post, int weight_type, void* d_gate, int gate_type) {
+// Columns 64 x .. of sum y: parts of all workgroups, 16 at a time, then across
+// them, and the factors of the two gradients that the second is for
+__global__ __launch_bounds__(1024) void block_join_kernel(const float* parts, int groups, const qmoe_block_desc p,
+                                                          const qmoe_block_grads d) {
   __shared__ float s[16][64];
-  const int kind = blockIdx.y, c = threadIdx.x & 63, r = threadIdx.x >> 6;
-  void* out = kind == 0 ? d_next : kind == 1 ? d_post : d_gate;
-  if (!out) return;
+  const int k2 = blockIdx.y, c = threadIdx.x & 63, r = threadIdx.x >> 6;
+  const bool post = p.y && p.post_weight, channel = p.gate_kind == GATE_CHANNEL;
+  if (k2 == 0 ? !d.d_next_weight : !((post && d.d_post_weight) || (channel && d.d_gate))) return;
   const int64_t i = (int64_t)blockIdx.x * 64 + c;
   float v = 0.0f;
-  if (i < H)
-    for (int g = r; g < groups; g += 16) v += parts[((int64_t)g * 3 + kind) * H + i];
+  if (i < p.H) {
+#pragma unroll 8
+    for (int g = r; g < groups; g += 16) v += parts[((int64_t)g * 2 + k2) * p.H + i];
+  }
   s[r][c] = v;
   __syncthreads();
-  if (r || i >= H) return;
+  if (r || i >= p.H) return;
   for (int k = 1; k < 16; ++k) v += s[k][c];
-  const int type = kind == 2 ? gate_type : weight_type;
-  if (type == RT_BF16) static_cast<uint16_t*>(out)[i] = f32_to_bf16(v);
-  else if (type == RT_F32) static_cast<float*>(out)[i] = v;
-  else static_cast<_Float16*>(out)[i] = (_Float16)v;
+  auto put = [&](void* out, int type, float x) {
+    if (type == RT_BF16) static_cast<uint16_t*>(out)[i] = f32_to_bf16(x);
+    else if (type == RT_F32) static_cast<float*>(out)[i] = x;
+    else static_cast<_Float16*>(out)[i] = (_Float16)x;
+  };
+  if (k2 == 0) return put(d.d_next_weight, p.weight_type, v);
+  v *= p.scale;
+  if (post && d.d_post_weight) put(d.d_post_weight, p.weight_type, v * (channel ? one_any(p.gate, p.gate_type, i) : 1.0f));
+  if (channel && d.d_gate)
+    put(d.d_gate, p.gate_type, v * (post ? p.weight_offset + one_any(p.post_weight, p.weight_type, i) : 1.0f));
 }
 
 // ---------------------------------------------------------------- launches
@@ -331,19 +374,21 @@ struct BlockShape {
   int pieces, waves, rows;
 };
 
-// pieces of 8 per lane, wavefronts of a row, rows of a workgroup: rows of up to
-// 8 wavefronts, then more values per lane
-BlockShape block_shape(int64_t H) {
+// pieces of 8 per lane, wavefronts of a row, rows of a workgroup. Rows of up to 8
+// wavefronts, then (forward) two pieces per lane, or (gradient, whose sums take
+// registers) up to 16 wavefronts. 8192 rows of 7168 bf16, one / two pieces: forward
+// 115 / 98 us, gradient 160 / 167.
+BlockShape block_shape(int64_t H, bool grad) {
   const int64_t chunks = cdiv<int64_t>(H, 8);
-  const int C = chunks <= 512 ? 1 : 2;
+  const int C = chunks <= (grad ? 1024 : 512) ? 1 : 2;
   const int W = (int)cdiv<int64_t>(chunks, 64 * C);
-  const int R = W > 8 ? 1 : 8 / W;
-  return {C, W, R};
+  return {C, W, W > 8 ? 1 : 8 / W};
 }
 
-int grad_groups(int64_t T, int R) {
-  const int64_t g = cdiv<int64_t>(T, R);
-  return (int)(g < 512 ? g : 512);
+// workgroups of the gradient: two per CU, one of more than 8 wavefronts
+int grad_groups(int64_t T, BlockShape s) {
+  const int64_t g = cdiv<int64_t>(T, s.rows), most = s.waves > 8 ? 256 : 512;
+  return (int)(g < most ? g : most);
 }
 
 bool aligned16(const void* p, int64_t ld, int size) {
@@ -383,7 +428,8 @@ void with_pieces(BlockShape s, bool al, F&& f) {
             std::integral_constant<int, TH>(), std::true_type());                                                  \
   else f(std::integral_constant<int, YT>(), std::integral_constant<int, RT>(), std::integral_constant<int, CC>(),   \
          std::integral_constant<int, TH>(), std::false_type())
-  if (s.pieces == 1) QMOE_BLOCK(1, 512);
+  if (s.pieces == 1 && s.waves <= 8) QMOE_BLOCK(1, 512);
+  else if (s.pieces == 1) QMOE_BLOCK(1, 1024);
   else if (s.waves <= 8) QMOE_BLOCK(2, 512);
   else QMOE_BLOCK(2, 1024);
 #undef QMOE_BLOCK
@@ -405,17 +451,18 @@ extern "C" int qmoe_block_residual(const qmoe_block_desc* p, hipStream_t stream)
   if (!p->residual || p->ldr < p->H || (p->y && (!p->h || p->ldh < p->H)) ||
       (p->next_weight && (!p->z || p->ldz < p->H)))
     return QMOE_ERR_ARG;
-  const BlockShape s = block_shape(p->H);
+  const BlockShape s = block_shape(p->H, false);
   const dim3 grid((unsigned)cdiv<int64_t>(p->T, s.rows)), block(64 * s.waves, s.rows);
   with_types(p->y_type, p->residual_type, s, wide(p), [&](auto yt, auto rt, auto c, auto th, auto al) {
-    hipLaunchKernelGGL((block_residual_kernel<yt(), rt(), c(), th(), al()>), grid, block, 0, stream, *p);
+    if constexpr (th() == 512 || c() == 2)  // (one piece and more than 8 wavefronts: the gradient's)
+      hipLaunchKernelGGL((block_residual_kernel<yt(), rt(), c(), th(), al()>), grid, block, 0, stream, *p);
   });
   return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
 }
 
 extern "C" int qmoe_block_residual_grad_workspace_size(int64_t T, int64_t H, int64_t* bytes) {
   if (T < 1 || T > kMaxRows || H < 1 || H > kMaxRow || !bytes) return QMOE_ERR_ARG;
-  *bytes = (int64_t)grad_groups(T, block_shape(H).rows) * 3 * H * 4;
+  *bytes = (int64_t)grad_groups(T, block_shape(H, true)) * 2 * H * 4;
   return QMOE_OK;
 }
 
@@ -429,22 +476,35 @@ extern "C" int qmoe_block_residual_grad(const qmoe_block_desc* p, const qmoe_blo
   if (d->g_h && d->ldgh < p->H) return QMOE_ERR_ARG;
   const bool sums = (next && d->d_next_weight) || (post && d->d_post_weight) ||
                     (p->gate_kind == GATE_CHANNEL && d->d_gate);
-  const BlockShape s = block_shape(p->H);
-  const int groups = grad_groups(p->T, s.rows);
-  if (sums && (!workspace || ws_bytes < (int64_t)groups * 3 * p->H * 4)) return QMOE_ERR_WORKSPACE;
+  const BlockShape s = block_shape(p->H, true);
+  const int groups = grad_groups(p->T, s);
+  if (sums && (!workspace || ws_bytes < (int64_t)groups * 2 * p->H * 4)) return QMOE_ERR_WORKSPACE;
   const int ys = rt_size(p->y_type), rs = rt_size(p->residual_type);
   const bool al = wide(p) && aligned16(d->g_h, d->ldgh, rs) && aligned16(d->g_z, d->ldgz, ys) &&
                   aligned16(d->d_y, p->H, ys) && aligned16(d->d_residual, p->H, rs) && aligned16(workspace, 0, 1) &&
                   (p->gate_kind != GATE_FULL || aligned16(d->d_gate, p->H, ys));
   const dim3 block(64 * s.waves, s.rows);
   float* parts = sums ? static_cast<float*>(workspace) : nullptr;
+  const bool lds = p->H <= kMaxLdsRow;
+  const size_t dyn = (lds ? 8 : s.rows > 1 ? 4 : 0) * (size_t)(cdiv<int64_t>(p->H, 8) * 8);
   with_types(p->y_type, p->residual_type, s, al, [&](auto yt, auto rt, auto c, auto th, auto a) {
-    hipLaunchKernelGGL((block_residual_grad_kernel<yt(), rt(), c(), th(), a()>), dim3(groups), block,
-                       s.rows > 1 ? (size_t)p->H * 4 : 0, stream, *p, *d, parts);
+    constexpr bool kLds = c() == 1;  // (rows of up to 8192)
+    if constexpr (th() == 512 && c() == 2) {
+      return;  // (the forward's)
+    } else {
+      if (a() && next && post)
+        hipLaunchKernelGGL((block_residual_grad_kernel<yt(), rt(), c(), th(), a(), a() ? 1 : 0, kLds>), dim3(groups), block,
+                           dyn, stream, *p, *d, parts);
+      else if (a() && next && !p->y)
+        hipLaunchKernelGGL((block_residual_grad_kernel<yt(), rt(), c(), th(), a(), a() ? 2 : 0, kLds>), dim3(groups), block,
+                           dyn, stream, *p, *d, parts);
+      else
+        hipLaunchKernelGGL((block_residual_grad_kernel<yt(), rt(), c(), th(), a(), 0, kLds>), dim3(groups), block, dyn,
+                           stream, *p, *d, parts);
+    }
   });
   if (sums)
-    hipLaunchKernelGGL(block_join_kernel, dim3((unsigned)cdiv<int64_t>(p->H, 64), 3), dim3(1024), 0, stream, parts,
-                       groups, p->H, next ? d->d_next_weight : nullptr, post ? d->d_post_weight : nullptr, p->weight_type,
-                       p->gate_kind == GATE_CHANNEL ? d->d_gate : nullptr, p->gate_type);
+    hipLaunchKernelGGL(block_join_kernel, dim3((unsigned)cdiv<int64_t>(p->H, 64), 2), dim3(1024), 0, stream, parts, groups,
+                       *p, *d);
   return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
 }

@@ -38,6 +38,7 @@ struct LinearGemm {
   int64_t ldy;
   int kslice;   // K split: slice z takes the K range from z * kslice on and leaves float32 sums in [z][nb][na]
   float* slices;
+  const float* bias;  // of the A rows, or nullptr
 };
 
 // B row t of the 64 that a round holds, A row n of it at n ^ vg_row_swz(t): 8
@@ -76,26 +77,31 @@ __device__ __forceinline__ void linear_epilogue(const LinearGemm& p, f32x16 (&ac
         dst[0] = lo;
         dst[1] = hi;
       } else {
+        float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        if (p.bias) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] += p.bias[n0 + c + k];
+        }
         *reinterpret_cast<uint4*>(p.y + row * p.ldy + n0 + c) =
-            make_uint4(pack_bf16(lo.x, lo.y), pack_bf16(lo.z, lo.w), pack_bf16(hi.x, hi.y), pack_bf16(hi.z, hi.w));
+            make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
       }
     }
   }
 }
 
 // This workgroup's slice of K
-template <bool TRA>
+template <bool TRA, bool TRB>
 __device__ __forceinline__ void linear_slice(LinearGemm& p) {
   if (!p.kslice) return;
   const int64_t k0 = (int64_t)blockIdx.y * p.kslice;
   p.a += TRA ? k0 * p.lda : k0 * 2;
-  p.b += TRA ? k0 * 2 : k0 * p.ldb;
+  p.b += TRB ? k0 * p.ldb : k0 * 2;
   p.K = (int)min((int64_t)p.kslice, p.K - k0);
 }
 
 // Tiles of 256 x BM (64 or 128) by eight wavefronts. ONE: a stage at a time,
 // without a ring, so that two workgroups share a CU.
-template <bool TRA, int BM, bool ONE>
+template <bool TRA, bool TRB, int BM, bool ONE>
 __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const LinearGemm args) {
   constexpr int NI = 2, MJ = BM / 64, WB = kAN * 128, STG = WB + BM * 128;
   constexpr int RING = ONE ? 1 : (163840 / STG < 6 ? 163840 / STG : 6), EPILOGUE = 65536;
@@ -103,7 +109,7 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
   static_assert(ONE ? sizeof(smem) <= 81920 : RING >= 3 && sizeof(smem) <= 163840, "workgroups of a CU, ring");
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
   LinearGemm p = args;
-  linear_slice<TRA>(p);
+  linear_slice<TRA, TRB>(p);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave & 3, wm = wave >> 2, rl = lane & 31, kh = lane >> 5;
   int mt, nt;
@@ -115,25 +121,24 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
   // chunk c of row r at c ^ vg_swz(r)), or 1 KB of K rows; wavefront w moves the
   // groups w, w + 8, ...; rows and columns past the end repeat the last
   constexpr int WI = WB / 8192, XI = BM / 64;
-  constexpr int TB = TRA ? kAN * 2 : BM * 2, TL = TB / 16;  // bytes, lanes of a K row
+  constexpr int TB = TRA ? kAN * 2 : BM * 2, TL = TB / 16;  // bytes, lanes of a K row (of the one operand across)
+  static_assert(!TRA || !TRB, "one operand across K");
   const int chunk = (lane & 7) ^ ((lane >> 3) ^ (wave & 1));
   const int trow = lane / TL, tchunk = (lane % TL) ^ tr_swz<TB>(wave * (64 / TL) + trow);
   const uint32_t tcol = (uint32_t)min(tchunk, (TRA ? arows : brows) / 8 - 1) * 16;
   const uint8_t* abase = TRA ? p.a + n0 * 2 : p.a + (int64_t)n0 * p.lda;
-  const uint8_t* bbase = TRA ? p.b + (int64_t)m0 * p.ldb : p.b + m0 * 2;
-  const int64_t astep = TRA ? 64 * p.lda : 128, bstep = TRA ? 128 : 64 * p.ldb;
+  const uint8_t* bbase = TRB ? p.b + m0 * 2 : p.b + (int64_t)m0 * p.ldb;
+  const int64_t astep = TRA ? 64 * p.lda : 128, bstep = TRB ? 64 * p.ldb : 128;
   uint32_t aoff[WI], boff[XI];
-  int krow[TRA ? WI : XI];  // K row of a stage that copy j of the operand across K is in
-#pragma unroll
-  for (int j = 0; j < (TRA ? WI : XI); ++j) krow[j] = (wave + 8 * j) * (64 / TL) + trow;
+  auto krow = [&](int j) { return (wave + 8 * j) * (64 / TL) + trow; };  // of a stage, of copy j of the operand across K
 #pragma unroll
   for (int j = 0; j < WI; ++j)
-    aoff[j] = TRA ? (uint32_t)krow[j] * (uint32_t)p.lda + tcol
+    aoff[j] = TRA ? (uint32_t)krow(j) * (uint32_t)p.lda + tcol
                   : (uint32_t)min((wave + 8 * j) * 8 + (lane >> 3), arows - 1) * (uint32_t)p.lda + chunk * 16;
 #pragma unroll
   for (int j = 0; j < XI; ++j)
-    boff[j] = TRA ? (uint32_t)min((wave + 8 * j) * 8 + (lane >> 3), brows - 1) * (uint32_t)p.ldb + chunk * 16
-                  : (uint32_t)krow[j] * (uint32_t)p.ldb + tcol;
+    boff[j] = TRB ? (uint32_t)krow(j) * (uint32_t)p.ldb + tcol
+                  : (uint32_t)min((wave + 8 * j) * 8 + (lane >> 3), brows - 1) * (uint32_t)p.ldb + chunk * 16;
   const int KF = p.K / 64, tail = p.K % 64;  // whole stages, k of the last
   const uint32_t cw = lds0 + wave * 1024;
   // stage s to slot `slot` (stages past the last whole one copy it again, into
@@ -152,10 +157,10 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
     const uint8_t *as = abase + KF * astep, *bs = bbase + KF * bstep, *z = reinterpret_cast<const uint8_t*>(kZeroChunk);
 #pragma unroll
     for (int j = 0; j < WI; ++j)
-      lds_copy16(!TRA || krow[TRA ? j : 0] < tail ? as + aoff[j] : z, __builtin_amdgcn_readfirstlane(cw + j * 8192));
+      lds_copy16((TRA ? krow(j) : chunk * 8) < tail ? as + aoff[j] : z, __builtin_amdgcn_readfirstlane(cw + j * 8192));
 #pragma unroll
     for (int j = 0; j < XI; ++j)
-      lds_copy16((TRA ? chunk * 8 : krow[TRA ? 0 : j]) < tail ? bs + boff[j] : z,
+      lds_copy16((TRB ? krow(j) : chunk * 8) < tail ? bs + boff[j] : z,
                  __builtin_amdgcn_readfirstlane(cw + WB + j * 8192));
   };
 
@@ -182,7 +187,7 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
           *reinterpret_cast<const uint4*>(s + (wn * 64 + i * 32 + rl) * 128 + ((2 * q + kh) ^ vg_swz(rl)) * 16);
 #pragma unroll
     for (int j = 0; j < MJ; ++j)
-      if constexpr (!TRA) xf[q & 1][j].u = tr_read<TB>(s + WB + q * 16 * TB + (tlane ^ (2 * j + wm) * 64));
+      if constexpr (TRB) xf[q & 1][j].u = tr_read<TB>(s + WB + q * 16 * TB + (tlane ^ (2 * j + wm) * 64));
       else xf[q & 1][j].u =
           *reinterpret_cast<const uint4*>(s + WB + ((2 * j + wm) * 32 + rl) * 128 + ((2 * q + kh) ^ vg_swz(rl)) * 16);
   };
@@ -208,8 +213,9 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
   // stage's last operands, so that its slot takes the copies of stage s + RING ->
   // the last step, while the next stage's first operands are read.
   if constexpr (ONE) {
-    for (int s = 0; s < KF; ++s) {
-      copy_stage(s, 0);
+    for (int s = 0; s < KF + (tail != 0); ++s) {
+      if (s < KF) copy_stage(s, 0);
+      else copy_tail();
       one_stage();
     }
   } else if (KF > 0) {
@@ -237,25 +243,178 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
     wait_copies_upto<0>();
     __syncthreads();
   }
-  if (tail) {
+  if (!ONE && tail) {
     copy_tail();
     one_stage();
   }
   linear_epilogue<512, NI, MJ>(p, acc, smem, n0, m0, arows, brows, wn, wm);
 }
 
+// The same products in tiles of 256 x BM (256 or 192) by four wavefronts of 4 x
+// BM / 64 blocks, one per SIMD, the sums in accumulation registers: a wavefront of
+// 128 x 128 reads 32 KB of operands from LDS per 64 MFMAs where one of 64 x 64
+// reads 32 per 32, and eight of those fill LDS's 128 bytes per cycle.
+//
+// Stages of 64 k: 32 KB of A rows and up to 32 KB of B rows, in a ring of five such
+// slots (all of LDS): A(s), B(s), A(s + 1), B(s + 1), A(s + 2). At the barrier of
+// stage s every wavefront holds its last operands, and the stage's two slots
+// take B(s + 2) and A(s + 3). The copies go out four per MFMA step, one at a time
+// between the MFMAs.
+// TAIL: K is not a multiple of 64 (an instance of its own: the extra stage costs
+// the others registers).
+template <bool TRA, bool TRB, int BM, bool TAIL>
+__global__ __launch_bounds__(256, 1) void linear_big_kernel(const LinearGemm args) {
+  constexpr int NI = 4, MJ = BM / 64, AI = 8, BI = 2 * MJ;  // a wavefront's copies of A and B per stage
+  constexpr uint32_t SLOT = kAN * 128, RING = 5 * SLOT;
+  constexpr int TB = 512, TL = 32;  // bytes, lanes of a K row of the operand across K
+  static_assert(!TRB || BM == 256, "K rows of 512 bytes");
+  static_assert(!TRA || !TRB, "one operand across K");
+  __shared__ __align__(1024) uint8_t smem[RING];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
+  LinearGemm p = args;
+  linear_slice<TRA, TRB>(p);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave & 1, wm = wave >> 1, rl = lane & 31, kh = lane >> 5;
+  int mt, nt;
+  if (!tile_dense(blockIdx.x, p.m_tiles, p.n_tiles, mt, nt)) return;
+  const int n0 = nt * kAN, m0 = mt * BM;
+  const int arows = min(kAN, p.na - n0), brows = min(BM, p.nb - m0);
+
+  // copies as in the kernel above; wavefront w moves the groups w, w + 4, ...
+  const int chunk = (lane & 7) ^ ((lane >> 3) ^ (wave & 1));
+  const int trow = lane / TL, tchunk = (lane % TL) ^ tr_swz<TB>(2 * wave + trow);
+  const uint32_t tcol = (uint32_t)min(tchunk, (TRA ? arows : brows) / 8 - 1) * 16;
+  const uint8_t* abase = TRA ? p.a + n0 * 2 : p.a + (int64_t)n0 * p.lda;
+  const uint8_t* bbase = TRB ? p.b + m0 * 2 : p.b + (int64_t)m0 * p.ldb;
+  const int64_t astep = TRA ? 64 * p.lda : 128, bstep = TRB ? 64 * p.ldb : 128;
+  uint32_t aoff[AI], boff[BI];
+#pragma unroll
+  for (int j = 0; j < AI; ++j)
+    aoff[j] = TRA ? (uint32_t)(2 * (wave + 4 * j) + trow) * (uint32_t)p.lda + tcol
+                  : (uint32_t)min((wave + 4 * j) * 8 + (lane >> 3), arows - 1) * (uint32_t)p.lda + chunk * 16;
+#pragma unroll
+  for (int j = 0; j < BI; ++j)
+    boff[j] = TRB ? (uint32_t)(2 * (wave + 4 * j) + trow) * (uint32_t)p.ldb + tcol
+                  : (uint32_t)min((wave + 4 * j) * 8 + (lane >> 3), brows - 1) * (uint32_t)p.ldb + chunk * 16;
+  const int KF = p.K / 64, tail = p.K % 64;
+  const uint32_t cw = lds0 + wave * 1024;
+  union B8 {
+    uint4 u;
+    bf16x8 v;
+  };
+  B8 wf[2][NI], xf[2][MJ];
+  const uint32_t wpo = (uint32_t)(wn * NI * 4096 + rl * 128), xpo = (uint32_t)(wm * 4096 + rl * 128);
+  const uint32_t tlane = tr_lane<TB>(lane) ^ (TRA ? wn * NI * 64 : wm * 64);
+  auto read_w = [&](uint32_t slot, int q) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      if constexpr (TRA) wf[q & 1][i].u = tr_read<TB>(smem + slot + q * 16 * TB + (tlane ^ i * 64));
+      else wf[q & 1][i].u =
+          *reinterpret_cast<const uint4*>(smem + slot + wpo + i * 4096 + ((2 * q + kh) ^ vg_swz(rl)) * 16);
+  };
+  auto read_x = [&](uint32_t slot, int q) {
+#pragma unroll
+    for (int j = 0; j < MJ; ++j)
+      if constexpr (TRB) xf[q & 1][j].u = tr_read<TB>(smem + slot + q * 16 * TB + (tlane ^ j * 128));
+      else xf[q & 1][j].u =
+          *reinterpret_cast<const uint4*>(smem + slot + xpo + j * 8192 + ((2 * q + kh) ^ vg_swz(rl)) * 16);
+  };
+  f32x16 acc[NI][MJ];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < MJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+  auto mma_row = [&](int q, int i) {
+#pragma unroll
+    for (int j = 0; j < MJ; ++j)
+      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[q & 1][i].v, xf[q & 1][j].v, acc[i][j], 0, 0, 0);
+  };
+  if (KF > 0) {
+    // (stages past the last whole one copy it again, into slots nobody reads)
+    auto asrc = [&](int s) { return uniform_ptr(abase + min(s, KF - 1) * astep); };
+    auto bsrc = [&](int s) { return uniform_ptr(bbase + min(s, KF - 1) * bstep); };
+    auto dst = [&](uint32_t slot) { return (uint32_t)__builtin_amdgcn_readfirstlane(cw + slot); };
+    auto wrap = [](uint32_t slot) { return slot >= RING ? slot - RING : slot; };
+#pragma unroll
+    for (int j = 0; j < AI; ++j) lds_copy16(asrc(0), aoff[j], dst(0) + j * 4096);
+#pragma unroll
+    for (int j = 0; j < BI; ++j) lds_copy16(bsrc(0), boff[j], dst(SLOT) + j * 4096);
+#pragma unroll
+    for (int j = 0; j < AI; ++j) lds_copy16(asrc(1), aoff[j], dst(2 * SLOT) + j * 4096);
+#pragma unroll
+    for (int j = 0; j < BI / 2; ++j) lds_copy16(bsrc(1), boff[j], dst(3 * SLOT) + j * 4096);
+    wait_copies_upto<AI + BI / 2>();  // the first stage
+    stage_barrier();
+    read_w(0, 0);
+    read_x(SLOT, 0);
+    uint32_t sa = 0;  // slot of A(s); B(s), A(s + 1), ... follow
+    for (int s = 0; s < KF; ++s) {
+      const uint32_t sb = wrap(sa + SLOT), sa1 = wrap(sa + 2 * SLOT), sb1 = wrap(sa + 3 * SLOT), sa2 = wrap(sa + 4 * SLOT);
+      const uint8_t *b1 = bsrc(s + 1), *a2 = asrc(s + 2), *b2 = bsrc(s + 2);
+      const uint32_t db1 = dst(sb1) + BI / 2 * 4096, da2 = dst(sa2), db2 = dst(sa);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (q == 3) {
+          wait_copies_upto<AI>();  // stage s + 1 has landed
+          stage_barrier();         // and everybody holds this stage's last operands
+        }
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          if (i == 0) read_w(q < 3 ? sa : sa1, (q + 1) & 3);
+          if (i == 1) read_x(q < 3 ? sb : sb1, (q + 1) & 3);
+          if (q == 1 || q == 2) lds_copy16(a2, aoff[4 * (q - 1) + i], da2 + (4 * (q - 1) + i) * 4096);
+          else if (i < BI / 2 && q == 0) lds_copy16(b1, boff[BI / 2 + i], db1 + i * 4096);
+          else if (i < BI / 2) lds_copy16(b2, boff[i], db2 + i * 4096);
+          mma_row(q, i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      sa = sa1;
+    }
+    wait_copies_upto<0>();
+    __syncthreads();
+  }
+  if constexpr (TAIL) {  // the last, partial stage, with zeros where K has ended
+    const uint8_t *as = abase + KF * astep, *bs = bbase + KF * bstep, *z = reinterpret_cast<const uint8_t*>(kZeroChunk);
+#pragma unroll
+    for (int j = 0; j < AI; ++j)
+      lds_copy16((TRA ? 2 * (wave + 4 * j) + trow : chunk * 8) < tail ? as + aoff[j] : z,
+                 __builtin_amdgcn_readfirstlane(cw + j * 4096));
+#pragma unroll
+    for (int j = 0; j < BI; ++j)
+      lds_copy16((TRB ? 2 * (wave + 4 * j) + trow : chunk * 8) < tail ? bs + boff[j] : z,
+                 __builtin_amdgcn_readfirstlane(cw + SLOT + j * 4096));
+    wait_copies_upto<0>();
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      read_w(0, q);
+      read_x(SLOT, q);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) mma_row(q, i);
+    }
+    __syncthreads();
+  }
+  linear_epilogue<256, NI, MJ>(p, acc, smem, n0, m0, arows, brows, wn, wm);
+}
+
 // The K slices -> bf16 rows
 __global__ __launch_bounds__(256) void linear_slices_kernel(const float* s, int slices, int64_t rows, int na,
-                                                            uint16_t* y, int64_t ldy) {
+                                                            const float* bias, uint16_t* y, int64_t ldy) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, n = rows * na;
   if (i >= n) return;
   const int64_t row = i / na;
+  const int c = (int)(i - row * na);
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
   for (int z = 0; z < slices; ++z) {
     const float4 a = *reinterpret_cast<const float4*>(s + z * n + i);
     v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
   }
-  *reinterpret_cast<uint2*>(y + row * ldy + (i - row * na)) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+  if (bias) v.x += bias[c], v.y += bias[c + 1], v.z += bias[c + 2], v.w += bias[c + 3];
+  *reinterpret_cast<uint2*>(y + row * ldy + c) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
 
 // Codes [T][K] -> bf16 [K][Tw], columns from T on zero. 64 x 64 tiles through LDS.
@@ -327,39 +486,79 @@ __global__ __launch_bounds__(256) void linear_bias_join_kernel(const float* part
 
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
-// tile rows, K slices and their length of a product of na A rows, nb B rows and K
+// Which operand of a product lies across K
+enum LinearMode { LM_FORWARD = 0, LM_DX = 1, LM_DW = 2 };
+
+// Tile rows (1: of 128, without a ring), K slices and their length of a product of
+// na A rows, nb B rows and K
 struct LinearPlan {
   int bm, slices, kslice;
 };
-LinearPlan linear_plan(int64_t na, int64_t nb, int64_t K) {
-  LinearPlan d{};
-  d.bm = nb <= 64 ? 64 : 128;
-  const int64_t tiles = cdiv(na, (int64_t)kAN) * cdiv(nb, (int64_t)d.bm);
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(256 / tiles, K / 512));
-  d.kslice = (int)up(cdiv(K, want), 64);
-  d.slices = (int)cdiv(K, (int64_t)d.kslice);
-  return d;
+// The least time of a model: rounds of the tiles on the chip times (stages times
+// a stage's time + the rest of a tile), and for K slices their sums' way to memory
+// and back. Times from sweeps of every tile and 1 to 16 slices over 16 sizes (1 to
+// 8192 tokens, 256 x 1024 to 4096 x 28672); the plan's own time was within 5 % of
+// the best of the sweep for most, 14 % at most. Both sides, us: 4096 tokens x 4096 x
+// 28672 forward / dx / dw tiles of 256 723 / 676 / 734, of 128 887 / 816 / 875;
+// 777 x 4096 x 4096 dx 64 rows 38.5, 128 rows in 2 slices 42; dw without a ring 36.9,
+// 256 rows 39.3; 333 x 2880 x 5760 dx 128 rows in 6 slices 28.8, 64 in 3 39.
+LinearPlan linear_plan(int mode, int64_t na, int64_t nb, int64_t K) {
+  struct Tile {
+    int bm, cus, stage, fixed;  // workgroups of a round, ns of a stage and of the rest of a tile
+  };
+  // (dw: few stages and the most to write; without a ring one workgroup's stores run under the other's products)
+  constexpr Tile kAlong[] = {{256, 256, 1680, 6000}, {192, 256, 1290, 5000}, {128, 256, 1050, 4000}, {1, 512, 2000, 5000},
+                             {64, 256, 700, 2000}};
+  constexpr Tile kDw[] = {{256, 256, 1680, 11000}, {128, 256, 1050, 8000}, {1, 512, 1900, 5000}, {64, 256, 700, 4000}};
+  LinearPlan best{};
+  int64_t least = INT64_MAX;
+  const int64_t stages = cdiv(K, (int64_t)64), n = cdiv(na, (int64_t)kAN);
+  for (int i = 0; i < (mode == LM_DW ? 4 : 5); ++i) {
+    const Tile& t = mode == LM_DW ? kDw[i] : kAlong[i];
+    const int64_t tiles = n * cdiv(nb, (int64_t)(t.bm == 1 ? 128 : t.bm));
+    for (int64_t want = 1; want <= 16 && want <= stages; ++want) {
+      const int64_t per = cdiv(stages, want), slices = cdiv(stages, per);
+      // (each XCD takes an eighth of the tiles, of every slice)
+      int64_t ns = cdiv(cdiv(tiles, (int64_t)kXcds) * slices, (int64_t)t.cus / kXcds) * (per * t.stage + t.fixed);
+      if (slices > 1) ns += 3000 + slices * 300 + slices * na * nb * 8 / 7000;
+      if (ns < least) {
+        least = ns;
+        best = LinearPlan{t.bm, (int)slices, (int)(per * 64)};
+      }
+    }
+  }
+  return best;
 }
 
-template <bool TRA>
+template <bool TRA, bool TRB, int BM>
+void launch_big(const LinearGemm& g, dim3 grid, hipStream_t st) {
+  if (g.K % 64) hipLaunchKernelGGL((linear_big_kernel<TRA, TRB, BM, true>), grid, dim3(256), 0, st, g);
+  else hipLaunchKernelGGL((linear_big_kernel<TRA, TRB, BM, false>), grid, dim3(256), 0, st, g);
+}
+
+template <int MODE>
 void launch_linear(LinearGemm g, uint8_t* ws, hipStream_t st) {
-  const LinearPlan d = linear_plan(g.na, g.nb, g.K);
+  constexpr bool TRA = MODE == LM_DX, TRB = MODE == LM_DW;
+  const LinearPlan d = linear_plan(MODE, g.na, g.nb, g.K);
   if (d.slices > 1) {
     g.kslice = d.kslice;
     g.slices = reinterpret_cast<float*>(ws);
   }
   g.n_tiles = cdiv(g.na, kAN);
-  g.m_tiles = cdiv(g.nb, d.bm);
+  g.m_tiles = cdiv(g.nb, d.bm == 1 ? 128 : d.bm);
   const dim3 grid((unsigned)up((int64_t)g.n_tiles * g.m_tiles, kXcds), (unsigned)d.slices);
-  if (d.bm == 64) hipLaunchKernelGGL((linear_small_kernel<TRA, 64, false>), grid, dim3(512), 0, st, g);
-  else hipLaunchKernelGGL((linear_small_kernel<TRA, 128, false>), grid, dim3(512), 0, st, g);
+  if (d.bm == 256) launch_big<TRA, TRB, 256>(g, grid, st);
+  else if (d.bm == 192) { if constexpr (!TRB) launch_big<TRA, TRB, 192>(g, grid, st); }
+  else if (d.bm == 64) hipLaunchKernelGGL((linear_small_kernel<TRA, TRB, 64, false>), grid, dim3(512), 0, st, g);
+  else if (d.bm == 128) hipLaunchKernelGGL((linear_small_kernel<TRA, TRB, 128, false>), grid, dim3(512), 0, st, g);
+  else hipLaunchKernelGGL((linear_small_kernel<TRA, TRB, 128, true>), grid, dim3(512), 0, st, g);
   if (d.slices > 1)
     hipLaunchKernelGGL(linear_slices_kernel, dim3((unsigned)cdiv((int64_t)g.nb * g.na / 4, (int64_t)256)), dim3(256), 0, st,
-                       g.slices, d.slices, (int64_t)g.nb, g.na, g.y, g.ldy);
+                       g.slices, d.slices, (int64_t)g.nb, g.na, g.bias, g.y, g.ldy);
 }
 
-int64_t slice_bytes(int64_t na, int64_t nb, int64_t K) {
-  const LinearPlan d = linear_plan(na, nb, K);
+int64_t slice_bytes(int mode, int64_t na, int64_t nb, int64_t K) {
+  const LinearPlan d = linear_plan(mode, na, nb, K);
   return d.slices > 1 ? up(4 * d.slices * na * nb, 256) : 0;
 }
 
@@ -373,8 +572,8 @@ int64_t linear_layout(int64_t T, int64_t N, int64_t K, int need_dx, int need_dw,
   off[0] = at;
   if (need_dw) at += up(K * up(T, 64) * 2, 256);
   off[1] = at;
-  int64_t s = need_dx ? slice_bytes(K, T, N) : 0;
-  if (need_dw) s = std::max(s, slice_bytes(K, N, T));
+  int64_t s = need_dx ? slice_bytes(LM_DX, K, T, N) : 0;
+  if (need_dw) s = std::max(s, slice_bytes(LM_DW, K, N, T));
   at += s;
   off[2] = at;
   if (need_dbias) at += up(4 * N * bias_parts(T, N), 256);
@@ -386,11 +585,42 @@ bool linear_sizes_ok(int64_t T, int64_t N, int64_t K) {
          N % 8 == 0 && K % 32 == 0;
 }
 
+// (256 rows of a tile, or 64 of a stage, lie within 32-bit offsets)
+constexpr int64_t kMaxPitch = (int64_t)1 << 22;
+
 bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
 
 // See include/qmoe.h for the contract.
+extern "C" int qmoe_linear_workspace_size(int64_t T, int64_t N, int64_t K, int64_t* bytes) {
+  if (!linear_sizes_ok(T, N, K) || !bytes) return QMOE_ERR_ARG;
+  *bytes = slice_bytes(LM_FORWARD, N, T, K);
+  return QMOE_OK;
+}
+
+extern "C" int qmoe_linear(const void* x, int64_t ldx, int64_t T, int64_t N, int64_t K, const void* w, int64_t ldw,
+                           const float* bias, void* y, void* workspace, int64_t ws_bytes, hipStream_t stream) {
+  if (!linear_sizes_ok(T, N, K) || !x || !w || !y || ldx < K || ldx % 8 || ldx >= kMaxPitch || ldw < K || ldw % 8 ||
+      ldw >= kMaxPitch || !at16(x) || !at16(w) || !at16(y))
+    return QMOE_ERR_ARG;
+  const int64_t need = slice_bytes(LM_FORWARD, N, T, K);
+  if (need && (!workspace || ws_bytes < need)) return QMOE_ERR_WORKSPACE;
+  LinearGemm g{};
+  g.a = static_cast<const uint8_t*>(w);
+  g.lda = ldw * 2;
+  g.na = (int)N;
+  g.b = static_cast<const uint8_t*>(x);
+  g.ldb = ldx * 2;
+  g.nb = (int)T;
+  g.K = (int)K;
+  g.y = static_cast<uint16_t*>(y);
+  g.ldy = N;
+  g.bias = bias;
+  launch_linear<LM_FORWARD>(g, static_cast<uint8_t*>(workspace), stream);
+  return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
+}
+
 extern "C" int qmoe_linear_grad_workspace_size(int64_t T, int64_t N, int64_t K, int need_dx, int need_dw, int need_dbias,
                                                int64_t* bytes) {
   if (!linear_sizes_ok(T, N, K) || !bytes) return QMOE_ERR_ARG;
@@ -402,8 +632,6 @@ extern "C" int qmoe_linear_grad_workspace_size(int64_t T, int64_t N, int64_t K, 
 extern "C" int qmoe_linear_grad(const void* dy, int64_t lddy, int64_t T, int64_t N, int64_t K, const void* w, int64_t ldw,
                                 const uint8_t* codes, const uint8_t* scales, void* dx, void* dw, void* dbias,
                                 int dbias_f32, void* workspace, int64_t ws_bytes, hipStream_t stream) {
-  // (256 rows of a tile, or 64 of a stage, lie within 32-bit offsets)
-  constexpr int64_t kMaxPitch = (int64_t)1 << 22;
   if (!linear_sizes_ok(T, N, K) || !dy || lddy < N || lddy % 8 || lddy >= kMaxPitch || !at16(dy)) return QMOE_ERR_ARG;
   if (dx && (!w || ldw < K || ldw % 8 || ldw >= kMaxPitch || !at16(w) || !at16(dx))) return QMOE_ERR_ARG;
   if (dw && (!codes || !scales || reinterpret_cast<uintptr_t>(codes) % 8 || !at16(dw))) return QMOE_ERR_ARG;
@@ -422,7 +650,7 @@ extern "C" int qmoe_linear_grad(const void* dy, int64_t lddy, int64_t T, int64_t
     g.K = (int)N;
     g.y = static_cast<uint16_t*>(dx);
     g.ldy = K;
-    launch_linear<true>(g, ws + off[1], stream);
+    launch_linear<LM_DX>(g, ws + off[1], stream);
   }
   if (dw) {
     const int64_t Tw = up(T, 64);
@@ -439,7 +667,7 @@ extern "C" int qmoe_linear_grad(const void* dy, int64_t lddy, int64_t T, int64_t
     g.K = (int)T;
     g.y = static_cast<uint16_t*>(dw);
     g.ldy = K;
-    launch_linear<false>(g, ws + off[1], stream);
+    launch_linear<LM_DW>(g, ws + off[1], stream);
   }
   if (dbias) {
     float* parts = reinterpret_cast<float*>(ws + off[2]);

@@ -1,5 +1,7 @@
 // Eight consecutive values of a row as float32, of the row types that the
-// block's elementwise kernels take (bf16, f32, f16), and sums over wavefronts.
+// block's elementwise kernels take (bf16, f32, f16), and sums over wavefronts. A
+// row's address is uniform and places in it are 32-bit offsets, so that accesses
+// take a scalar base and one register.
 #pragma once
 
 #include "qmoe_common.h"
@@ -26,10 +28,10 @@ __device__ __forceinline__ float one_value(const void* p, int64_t i) {
 // Values i .. i + 7 of the row at p; AL: 16-byte aligned, and all there; else
 // those from n on are zeros
 template <int T, bool AL>
-__device__ __forceinline__ Raw8<T> load_raw8(const void* p, int64_t i, int64_t n) {
+__device__ __forceinline__ Raw8<T> load_raw8(const void* p, uint32_t i, uint32_t n) {
   Raw8<T> r;
   if constexpr (AL) {
-    const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * (T == RT_F32 ? 4 : 2));
+    const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * (T == RT_F32 ? 4u : 2u));
     r.q[0] = s[0];
     if constexpr (T == RT_F32) r.q[1] = s[1];
   } else if constexpr (T == RT_F32) {
@@ -72,13 +74,13 @@ __device__ __forceinline__ void raw8_values(const Raw8<T>& r, float (&v)[8]) {
 }
 
 template <int T, bool AL>
-__device__ __forceinline__ void load8(const void* p, int64_t i, int64_t n, float (&v)[8]) {
+__device__ __forceinline__ void load8(const void* p, uint32_t i, uint32_t n, float (&v)[8]) {
   raw8_values<T>(load_raw8<T, AL>(p, i, n), v);
 }
 
 // ... of a type known at run time (uniform)
 template <bool AL>
-__device__ __forceinline__ void load8_any(const void* p, int type, int64_t i, int64_t n, float (&v)[8]) {
+__device__ __forceinline__ void load8_any(const void* p, int type, uint32_t i, uint32_t n, float (&v)[8]) {
   if (type == RT_BF16) load8<RT_BF16, AL>(p, i, n, v);
   else if (type == RT_F32) load8<RT_F32, AL>(p, i, n, v);
   else load8<RT_F16, AL>(p, i, n, v);
@@ -106,7 +108,7 @@ __device__ __forceinline__ uint32_t two_bf16(float a, float b) {
 }
 
 template <int T, bool AL>
-__device__ __forceinline__ void store8(void* p, int64_t i, int64_t n, const float (&v)[8]) {
+__device__ __forceinline__ void store8(void* p, uint32_t i, uint32_t n, const float (&v)[8]) {
   if constexpr (!AL) {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
@@ -116,7 +118,7 @@ __device__ __forceinline__ void store8(void* p, int64_t i, int64_t n, const floa
         else static_cast<uint16_t*>(p)[i + k] = f32_to_bf16(v[k]);
       }
   } else {
-    uint4* d = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p) + i * (T == RT_F32 ? 4 : 2));
+    uint4* d = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p) + i * (T == RT_F32 ? 4u : 2u));
     if constexpr (T == RT_F32) {
       d[0] = make_uint4(f32_bits(v[0]), f32_bits(v[1]), f32_bits(v[2]), f32_bits(v[3]));
       d[1] = make_uint4(f32_bits(v[4]), f32_bits(v[5]), f32_bits(v[6]), f32_bits(v[7]));

@@ -299,6 +299,10 @@ def _load():
                                              _vp]
     lib.qmoe_pack_8bit.restype = ctypes.c_int
     lib.qmoe_pack_8bit.argtypes = [_vp, _i64, _i64, _i64, _vp, _vp, _vp]
+    lib.qmoe_linear_workspace_size.restype = ctypes.c_int
+    lib.qmoe_linear_workspace_size.argtypes = [_i64, _i64, _i64, ctypes.POINTER(_i64)]
+    lib.qmoe_linear.restype = ctypes.c_int
+    lib.qmoe_linear.argtypes = [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp]
     lib.qmoe_linear_grad_workspace_size.restype = ctypes.c_int
     lib.qmoe_linear_grad_workspace_size.argtypes = [_i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                     ctypes.POINTER(_i64)]
@@ -351,6 +355,8 @@ EXPORTED = (
     "qmoe_act_checkpoint",
     "qmoe_act_checkpoint_grad",
     "qmoe_pack_8bit",
+    "qmoe_linear_workspace_size",
+    "qmoe_linear",
     "qmoe_linear_grad_workspace_size",
     "qmoe_linear_grad",
 )

@@ -303,8 +303,8 @@ def _linear(x, weight, bias, keep):
 
 def checkpointed_linear(x, weight, bias=None):
     """x weight^T + bias: bf16 ``x`` [..., K] and ``weight`` [N, K] (K a multiple of 32, N
-    of 8), bias [N] bf16 or f32 -> bf16 [..., N], the product of
-    `UnquantizedLinearMethod.apply` with the bias added before its one rounding.
+    of 8), bias [N] bf16 or f32 -> bf16 [..., N]: float32 sums, the bias added before
+    the one rounding.
 
     When the weight's gradient is asked for, the 8 bits of ``x`` are kept instead of
     its 16 (33/32 bytes a value), and that gradient is dy^T x8; those of ``x`` and the

@@ -1402,6 +1402,13 @@ def _check_aligned(weight, what):
         raise ValueError(f"{what}: the weight must be 16-byte aligned")
 
 
+@functools.lru_cache(maxsize=256)
+def _linear_bytes(T, N, K):
+    need = ctypes.c_int64(0)
+    check(lib.qmoe_linear_workspace_size(T, N, K, ctypes.byref(need)), "linear_checkpoint (shape)")
+    return need.value
+
+
 def linear_checkpoint(x, weight, bias=None, keep=True):
     """y = x w^T + bias (bf16 [..., N]) and the 8 bits of x: (y, codes uint8 [T, K],
     scales uint8 [T, K / 32]) for `linear_grad` (None without ``keep``)."""
@@ -1419,8 +1426,12 @@ def linear_checkpoint(x, weight, bias=None, keep=True):
         if keep:
             check(lib.qmoe_pack_8bit(r.data_ptr(), ld, T, K, codes.data_ptr(), scales.data_ptr(), _raw_stream(dev)),
                   "linear_checkpoint (8 bits)")
-        y = gemm(_capi.W16A16, r, weight, bias=None if bias is None else _f32_flat(bias))
-    return y.view(*x.shape[:-1], N), codes, scales
+        y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
+        b = _f32_flat(bias)
+        ws, ws_n = _workspace(dev, _linear_bytes(T, N, K))
+        check(lib.qmoe_linear(r.data_ptr(), ld, T, N, K, weight.data_ptr(), weight.stride(0), _addr(b), y.data_ptr(),
+                              _addr(ws), ws_n, _raw_stream(dev)), "linear_checkpoint")
+    return y, codes, scales
 
 
 @functools.lru_cache(maxsize=256)
