@@ -284,13 +284,13 @@ def test_captured_and_on_two_streams(dev):
 
 def test_kept_factors_and_refusals(dev):
     ts = _operands(dev, 4, 64, BF16, BF16, BF16, "token", True, True, 4)
-    h, z, ry, rh = ops.block_residual(*ts[:5], keep=True)
-    assert ry.shape == rh.shape == (4,)
+    h, z, rstd = ops.block_residual(*ts[:5], keep=True)
+    assert rstd.shape == (2, 4)
     ref = (ts[0].double().square().mean(-1) + E).rsqrt()
-    assert ((ry.double() - ref).abs() <= 32 * EPS * ref).all()
+    assert ((rstd[0].double() - ref).abs() <= 32 * EPS * ref).all()
     with pytest.raises(ValueError):
-        ops.block_residual_grad(ts[5], ts[6], ts[0], h, *ts[2:5], None, rh)
+        ops.block_residual_grad(ts[5], ts[6], ts[0], h, *ts[2:5], None)
     with pytest.raises(ValueError):
-        ops.block_residual_grad(None, None, ts[0], h, *ts[2:5], ry, rh)
+        ops.block_residual_grad(None, None, ts[0], h, *ts[2:5], rstd)
     with pytest.raises(ValueError):
         block_residual(ts[0].cpu(), ts[1])

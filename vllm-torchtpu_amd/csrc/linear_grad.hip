@@ -449,9 +449,14 @@ __global__ __launch_bounds__(256) void linear_expand_kernel(const uint8_t* codes
 }
 
 // Column sums of dy: workgroup (x, y) adds the rows y, y + gridDim.y, ... of 64
-// columns, eight threads of 8 of them, 32 rows at a time -> parts [gridDim.y][N]
+// columns, eight threads of 8 of them, 32 rows at a time -> parts [gridDim.y][N], or,
+// alone, the sums themselves
+__device__ __forceinline__ void put_bias(void* out, int f32, int n, float v) {
+  if (f32) static_cast<float*>(out)[n] = v;
+  else static_cast<uint16_t*>(out)[n] = f32_to_bf16(v);
+}
 __global__ __launch_bounds__(256) void linear_bias_kernel(const uint16_t* dy, int64_t lddy, int64_t T, int N,
-                                                          float* parts) {
+                                                          float* parts, void* out, int f32) {
   __shared__ float s[32][65];
   const int c = (threadIdx.x & 7) * 8, r = threadIdx.x >> 3, n = blockIdx.x * 64 + c;
   float v[8] = {};
@@ -469,7 +474,9 @@ __global__ __launch_bounds__(256) void linear_bias_kernel(const uint16_t* dy, in
   float sum = 0.0f;
 #pragma unroll 8
   for (int k = 0; k < 32; ++k) sum += s[k][threadIdx.x];
-  parts[(int64_t)blockIdx.y * N + blockIdx.x * 64 + threadIdx.x] = sum;
+  const int at = blockIdx.x * 64 + threadIdx.x;
+  if (gridDim.y == 1) put_bias(out, f32, at, sum);
+  else parts[(int64_t)blockIdx.y * N + at] = sum;
 }
 
 __global__ __launch_bounds__(256) void linear_bias_join_kernel(const float* parts, int n_parts, int N, void* out,
@@ -477,9 +484,9 @@ __global__ __launch_bounds__(256) void linear_bias_join_kernel(const float* part
   const int n = blockIdx.x * 256 + threadIdx.x;
   if (n >= N) return;
   float v = 0.0f;
+#pragma unroll 8
   for (int k = 0; k < n_parts; ++k) v += parts[(int64_t)k * N + n];
-  if (f32) static_cast<float*>(out)[n] = v;
-  else static_cast<uint16_t*>(out)[n] = f32_to_bf16(v);
+  put_bias(out, f32, n, v);
 }
 
 // ---------------------------------------------------------------- launches
@@ -563,7 +570,7 @@ int64_t slice_bytes(int mode, int64_t na, int64_t nb, int64_t K) {
 }
 
 int bias_parts(int64_t T, int64_t N) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(T, (int64_t)128), cdiv((int64_t)2048, cdiv(N, (int64_t)64))));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(T / 128, cdiv((int64_t)2048, cdiv(N, (int64_t)64))));
 }
 
 // x8 transposed, K slices (dx's, then dw's), bias parts
@@ -673,9 +680,10 @@ extern "C" int qmoe_linear_grad(const void* dy, int64_t lddy, int64_t T, int64_t
     float* parts = reinterpret_cast<float*>(ws + off[2]);
     const int n_parts = bias_parts(T, N);
     hipLaunchKernelGGL(linear_bias_kernel, dim3((unsigned)cdiv(N, (int64_t)64), (unsigned)n_parts), dim3(256), 0, stream,
-                       static_cast<const uint16_t*>(dy), lddy, T, (int)N, parts);
-    hipLaunchKernelGGL(linear_bias_join_kernel, dim3((unsigned)cdiv(N, (int64_t)256)), dim3(256), 0, stream, parts, n_parts,
-                       (int)N, dbias, dbias_f32);
+                       static_cast<const uint16_t*>(dy), lddy, T, (int)N, parts, dbias, dbias_f32);
+    if (n_parts > 1)
+      hipLaunchKernelGGL(linear_bias_join_kernel, dim3((unsigned)cdiv(N, (int64_t)256)), dim3(256), 0, stream, parts, n_parts,
+                         (int)N, dbias, dbias_f32);
   }
   return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
 }

@@ -119,25 +119,28 @@ __global__ __launch_bounds__(1024) void balance_route_kernel(const BalanceParams
   if (wave == 0) balance_loss(scratch[0], cnt, E, p.topk, p.loss);
 }
 
-// Workgroup x adds the parts of experts 16 x .. + 15 (16 rows of parts at a
-// time, then across them), and the last to finish the loss.
+// Workgroup x adds the parts of experts 8 x .. + 7 (32 workgroups' parts at a time,
+// then across them), and the last to finish the loss.
 __global__ __launch_bounds__(256) void balance_join_kernel(const BalanceParams p, int groups) {
-  __shared__ float sp[16][17];
-  __shared__ int32_t sc[16][17];
+  __shared__ float sp[32][9];
+  __shared__ int32_t sc[32][9];
   __shared__ bool last;
-  const int tid = threadIdx.x, c = tid & 15, r = tid >> 4, e = blockIdx.x * 16 + c;
+  const int tid = threadIdx.x, c = tid & 7, r = tid >> 3, e = blockIdx.x * 8 + c;
   float v = 0.0f;
   int32_t n = 0;
-  if (e < p.E)
-    for (int g = r; g < groups; g += 16) {
+  if (e < p.E) {
+#pragma unroll 8
+    for (int g = r; g < groups; g += 32) {
       v += p.part_p[(int64_t)g * p.E + e];
       n += p.part_c[(int64_t)g * p.E + e];
     }
+  }
   sp[r][c] = v;
   sc[r][c] = n;
   __syncthreads();
   if (r == 0 && e < p.E) {
-    for (int i = 1; i < 16; ++i) {
+#pragma unroll
+    for (int i = 1; i < 32; ++i) {
       v += sp[i][c];
       n += sc[i][c];
     }
@@ -384,7 +387,7 @@ extern "C" int qmoe_moe_balance(const void* logits, int logits_f32, int64_t T, i
     case 4: launch_balance<4>(scoring, grouped, groups, waves, p, stream); break;
     default: launch_balance<8>(scoring, grouped, groups, waves, p, stream); break;
   }
-  if (groups > 1) hipLaunchKernelGGL(balance_join_kernel, dim3(cdiv(E, 16)), dim3(256), 0, stream, p, groups);
+  if (groups > 1) hipLaunchKernelGGL(balance_join_kernel, dim3(cdiv(E, 8)), dim3(256), 0, stream, p, groups);
   return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
 }
 

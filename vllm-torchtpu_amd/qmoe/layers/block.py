@@ -34,7 +34,7 @@ def _wants(*ts):
 def _block_op(y: Optional[torch.Tensor], residual: torch.Tensor, gate: Optional[torch.Tensor],
               norm_weight: Optional[torch.Tensor], next_weight: Optional[torch.Tensor], scale: float,
               residual_scale: float, eps: float, weight_offset: float, z_dtype: torch.dtype,
-              keep: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+              keep: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(a result that the call has not comes back empty)"""
     out = ops.block_residual(y, residual, gate, norm_weight, next_weight, scale, residual_scale, eps, weight_offset, z_dtype,
                              keep)
@@ -43,30 +43,26 @@ def _block_op(y: Optional[torch.Tensor], residual: torch.Tensor, gate: Optional[
 
 @_block_op.register_fake
 def _(y, residual, gate, norm_weight, next_weight, scale, residual_scale, eps, weight_offset, z_dtype, keep):
-    T = residual.numel() // residual.shape[-1]
-
-    def rows(there):
-        return residual.new_empty(T if there else 0, dtype=torch.float32)
-
     return (residual.new_empty(0 if y is None else residual.shape),
             residual.new_empty(0) if next_weight is None else residual.new_empty(residual.shape, dtype=z_dtype),
-            rows(keep and norm_weight is not None), rows(keep and next_weight is not None))
+            residual.new_empty((2, residual.numel() // residual.shape[-1]), dtype=torch.float32) if keep else
+            residual.new_empty(0))
 
 
 @torch.library.custom_op("qmoe::block_residual_grad", mutates_args=())
 def _block_grad_op(g_h: Optional[torch.Tensor], g_z: Optional[torch.Tensor], y: Optional[torch.Tensor], h: torch.Tensor,
                    gate: Optional[torch.Tensor], norm_weight: Optional[torch.Tensor], next_weight: Optional[torch.Tensor],
-                   rstd_y: Optional[torch.Tensor], rstd_h: Optional[torch.Tensor], scale: float, residual_scale: float,
-                   eps: float, weight_offset: float, z_dtype: torch.dtype, need_y: bool, need_residual: bool,
-                   need_gate: bool, need_norm: bool, need_next: bool
+                   rstd: torch.Tensor, scale: float, residual_scale: float, eps: float, weight_offset: float,
+                   z_dtype: torch.dtype, need_y: bool, need_residual: bool, need_gate: bool, need_norm: bool,
+                   need_next: bool
                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    out = ops.block_residual_grad(g_h, g_z, y, h, gate, norm_weight, next_weight, rstd_y, rstd_h, scale, residual_scale, eps,
+    out = ops.block_residual_grad(g_h, g_z, y, h, gate, norm_weight, next_weight, rstd, scale, residual_scale, eps,
                                   weight_offset, z_dtype, (need_y, need_residual, need_gate, need_norm, need_next))
     return tuple(h.new_empty(0) if t is None else t for t in out)
 
 
 @_block_grad_op.register_fake
-def _(g_h, g_z, y, h, gate, norm_weight, next_weight, rstd_y, rstd_h, scale, residual_scale, eps, weight_offset, z_dtype,
+def _(g_h, g_z, y, h, gate, norm_weight, next_weight, rstd, scale, residual_scale, eps, weight_offset, z_dtype,
       need_y, need_residual, need_gate, need_norm, need_next):
     wanted = ((y, need_y), (h, need_residual), (gate, need_gate), (norm_weight, need_norm),
               (next_weight, need_next and g_z is not None))
@@ -76,8 +72,8 @@ def _(g_h, g_z, y, h, gate, norm_weight, next_weight, rstd_y, rstd_h, scale, res
 class _Block(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, residual, gate, norm_weight, next_weight, args):
-        h, z, rstd_y, rstd_h = _block(y, residual, gate, norm_weight, next_weight, args, True)
-        ctx.save_for_backward(y, residual if y is None else h, gate, norm_weight, next_weight, rstd_y, rstd_h)
+        h, z, rstd, ctx.desc = _block(y, residual, gate, norm_weight, next_weight, args, True)
+        ctx.save_for_backward(y, residual if y is None else h, gate, norm_weight, next_weight, rstd)
         ctx.args = args
         ctx.set_materialize_grads(False)
         return h, z
@@ -95,6 +91,10 @@ class _Block(torch.autograd.Function):
             return (None,) * 6
         saved, need = ctx.saved_tensors, ctx.needs_input_grad[:5]
         if ops.eager_call(g_h, g_z, *saved):
+            if ctx.desc is not None and ops.plain_here(g_h, g_z, *saved):
+                grads = ops.block_grad_plain(ctx.desc, g_h, g_z, *saved, need)
+                if grads is not None:
+                    return (*grads, None)
             return (*ops.block_residual_grad(g_h, g_z, *saved, *ctx.args, need), None)
         ops.refuse_tangents("block_residual's gradients", g_h, g_z)
         grads = torch.ops.qmoe.block_residual_grad(g_h, g_z, *saved, *ctx.args, *need)
@@ -107,12 +107,11 @@ class _Block(torch.autograd.Function):
 def _block(y, residual, gate, norm_weight, next_weight, args, keep):
     ts = (y, residual, gate, norm_weight, next_weight)
     if ops.eager_call(*ts):
-        return ops.block_residual(*ts, *args, keep)
+        return ops.block_residual_desc(*ts, *args, keep)
     ops.refuse_tangents("block_residual", *ts)
     ops._check_block(*ts, args[-1], "block_residual")
-    h, z, rstd_y, rstd_h = torch.ops.qmoe.block_residual(*ts, *args, keep)
-    return (None if y is None else h, None if next_weight is None else z,
-            rstd_y if keep and norm_weight is not None else None, rstd_h if keep and next_weight is not None else None)
+    h, z, rstd = torch.ops.qmoe.block_residual(*ts, *args, keep)
+    return None if y is None else h, None if next_weight is None else z, rstd if keep else None, None
 
 
 def block_norm(x, weight, eps=1e-6, weight_offset=0.0, out_dtype=None):
@@ -187,6 +186,7 @@ class _Activation(torch.autograd.Function):
         h, codes, scales = _act(gate_up, activation, True)
         ctx.save_for_backward(codes, scales)
         ctx.activation = activation
+        ctx.act = ops.act_code(activation)
         return h
 
     @staticmethod
@@ -199,7 +199,12 @@ class _Activation(torch.autograd.Function):
     def _grads(ctx, grad):
         codes, scales = ctx.saved_tensors
         fn = ops.act_checkpoint_grad
-        if not ops.eager_call(grad, codes, scales):
+        if ops.eager_call(grad, codes, scales):
+            I = grad.shape[-1]
+            T = grad.numel() // I
+            if T and codes.numel() == 2 * T * I and ops.plain_here(grad, codes, scales):
+                return ops.act_grad_run(codes, scales, grad, I, grad.shape, T, I, *ctx.act), None
+        else:
             ops.refuse_tangents("checkpointed_activation's gradient", grad)
             fn = torch.ops.qmoe.act_checkpoint_grad
         return fn(codes, scales, grad, ctx.activation), None
@@ -270,6 +275,9 @@ class _Linear(torch.autograd.Function):
         keep = ctx.needs_input_grad[1]
         y, codes, scales = _linear(x, weight, bias, keep)
         ctx.save_for_backward(weight, *((codes, scales) if keep else (None, None)))
+        ctx.sizes = weight.shape
+        # (the checks of the weight hold for the one that they have seen)
+        ctx.weight_at = weight.data_ptr() if ops.eager_call(weight) else None
         ctx.bias_dtype = bias.dtype if bias is not None and ctx.needs_input_grad[2] else None
         return y
 
@@ -284,7 +292,14 @@ class _Linear(torch.autograd.Function):
         weight, codes, scales = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
         fn = ops.linear_grad
-        if not ops.eager_call(grad, weight, codes, scales):
+        if ops.eager_call(grad, weight, codes, scales):
+            N, K = ctx.sizes
+            T = grad.numel() // N
+            if T and grad.data_ptr() % 16 == 0 and weight.data_ptr() == ctx.weight_at and \
+                    (codes is None or codes.numel() == T * K) and ops.plain_here(grad, codes, scales):
+                return ops.linear_grad_run(grad, N, grad.shape, T, N, K, weight, codes, scales, need_x, need_w,
+                                           ctx.bias_dtype)
+        else:
             ops.refuse_tangents("checkpointed_linear's gradients", grad)
             fn = torch.ops.qmoe.linear_grad
         dx, dw, db = fn(grad, weight, codes, scales, need_x, need_w, ctx.bias_dtype)

@@ -178,7 +178,13 @@ class _Balance(torch.autograd.Function):
             return (None,) * 5
         logits, ids, counts, mask = ctx.saved_tensors
         fn = ops.moe_balance_grad
-        if not ops.eager_call(logits, ids, counts, g_w, g_loss, mask):
+        if ops.eager_call(logits, ids, counts, g_w, g_loss, mask):
+            T, E = logits.shape
+            if T and ops.plain_here(logits, ids, counts, g_w, g_loss, mask):
+                scoring, renormalize, rsf = ctx.args
+                return (ops.balance_grad_run(logits, ids, counts, g_w, g_loss, T, E, ids.shape[1], ops._SCORING[scoring],
+                                             renormalize, rsf, mask), None, None, None, None)
+        else:
             ops.refuse_tangents("balanced_experts' gradient", g_w, g_loss)
             fn = torch.ops.qmoe.moe_balance_grad
         return fn(logits, ids, counts, g_w, g_loss, *ctx.args, mask), None, None, None, None

@@ -81,6 +81,20 @@ def eager_call(*ts):
     return True
 
 
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+def plain_here(*ts):
+    """Whether these tensors (None aside) are contiguous and on the current device, as
+    what a backward pass gets nearly always is: a call on them that also is an
+    `eager_call` needs no checks but the forward pass's."""
+    dev = _current_device()
+    for t in ts:
+        if t is not None and (t.get_device() != dev or not t.is_contiguous()):
+            return False
+    return True
+
+
 def has_tangent(*ts):
     """Whether one of these tensors (None aside) carries a forward-mode tangent."""
     return forward_ad._current_level >= 0 and any(
@@ -1137,16 +1151,24 @@ def moe_balance_grad(router_logits, topk_ids, counts, g_weights, g_loss, scoring
         if v is not None and (v.dtype is not dtype or tuple(v.shape) != shape):
             raise ValueError(f"moe_balance_grad: {name} must be {dtype} {shape}, got {v.dtype} {tuple(v.shape)}")
     with _on_device(router_logits, topk_ids, counts, g_weights, g_loss, token_mask):
-        dev = router_logits.device
-        d = torch.empty((T, E), dtype=router_logits.dtype, device=dev)
         if T == 0:
-            return d
-        x, ids, c = router_logits.contiguous(), topk_ids.contiguous(), counts.contiguous()
+            return router_logits.new_empty((T, E))
         gw = None if g_weights is None else g_weights.contiguous()
         m = None if token_mask is None else token_mask.contiguous()
-        check(lib.qmoe_moe_balance_grad(x.data_ptr(), x.dtype is torch.float32, T, E, k, _SCORING[scoring_func],
-                                        bool(renormalize), routed_scaling_factor, _addr(m), ids.data_ptr(), c.data_ptr(),
-                                        _addr(gw), _addr(g_loss), d.data_ptr(), _raw_stream(dev)), "moe_balance_grad")
+        return balance_grad_run(router_logits.contiguous(), topk_ids.contiguous(), counts.contiguous(), gw, g_loss, T, E, k,
+                                _SCORING[scoring_func], bool(renormalize), routed_scaling_factor, m)
+
+
+def balance_grad_run(logits, ids, counts, g_weights, g_loss, T, E, k, scoring, renormalize, rsf, mask):
+    """`moe_balance_grad` behind its checks, on the current device (few Python objects,
+    see `block_grad_run`)."""
+    d = logits.new_empty((T, E))
+    rc = lib.qmoe_moe_balance_grad(logits.data_ptr(), logits.dtype is torch.float32, T, E, k, scoring, renormalize, rsf,
+                                   None if mask is None else mask.data_ptr(), ids.data_ptr(), counts.data_ptr(),
+                                   None if g_weights is None else g_weights.data_ptr(),
+                                   None if g_loss is None else g_loss.data_ptr(), d.data_ptr(), _raw_stream(logits.device))
+    if rc:
+        check(rc, "moe_balance_grad")
     return d
 
 
@@ -1208,40 +1230,36 @@ def _check_block(y, residual, gate, post_weight, next_weight, z_dtype, what):
     return kind, yt, wt
 
 
-def _block_desc(T, H, y, residual, gate, kind, post, nxt, yt, rt, wt, scale, residual_scale, eps, offset):
-    """(`qmoe_block_desc` without its outputs, the tensors whose addresses it holds)"""
-    d = _capi.BlockDesc()
-    d.T, d.H = T, H
-    keep = []
-    for name, pitch, t in (("y", "ldy", y), ("residual", "ldr", residual)):
-        if t is not None:
-            r, ld = _rows(t, H)
-            keep.append(r)
-            setattr(d, name, r.data_ptr())
-            setattr(d, pitch, ld)
-    if kind:
-        if kind == 3:
-            g, d.ldg = _rows(gate, H)
-        else:
-            g = gate.reshape(-1).contiguous()
-        keep.append(g)
-        d.gate, d.gate_type = g.data_ptr(), _ROW_TYPES[gate.dtype]
-    for name, w in (("post_weight", post), ("next_weight", nxt)):
-        if w is not None:
-            w = w.contiguous()
-            keep.append(w)
-            setattr(d, name, w.data_ptr())
-    d.y_type, d.residual_type, d.weight_type, d.gate_kind = _ROW_TYPES[yt], _ROW_TYPES[rt], _ROW_TYPES.get(wt, 0), kind
-    d.scale, d.residual_scale, d.weight_offset, d.eps = scale, residual_scale, offset, eps
-    return d, keep
+def _block_gate(gate, kind, H):
+    """(tensor, pitch) of the gate as the kernels read it"""
+    if kind == 3:
+        return _rows(gate, H)
+    return (gate if gate.dim() == 1 else gate.reshape(-1)).contiguous(), 0
+
+
+def _block_desc(T, H, y, ldy, residual, ldr, gate, ldg, kind, post, nxt, h, ldh, z, ry, rh, yt, rt, wt, scale,
+                residual_scale, eps, offset):
+    """`qmoe_block_desc` of rows, gate and weights as the kernels read them (None where
+    the call has none)"""
+    return _capi.BlockDesc(T, H, _addr(y), ldy, _addr(residual), ldr, _addr(gate), ldg, _addr(post), _addr(nxt), _addr(h),
+                           ldh, _addr(z), H, ry, rh, _ROW_TYPES[yt], _ROW_TYPES[rt], 0 if wt is None else _ROW_TYPES[wt],
+                           _ROW_TYPES[gate.dtype] if kind else 0, kind, scale, residual_scale, offset, eps)
 
 
 def block_residual(y, residual, gate=None, post_weight=None, next_weight=None, scale=1.0, residual_scale=1.0, eps=1e-6,
                    weight_offset=0.0, z_dtype=None, keep=False):
-    """(h, z, rstd_y, rstd_h) of a block's output ``y``, see include/qmoe.h
+    """(h, z, rstd) of a block's output ``y``, see include/qmoe.h
     `qmoe_block_residual`; None for what the call has not (h without y, the norm
     of the residual alone, whose z is of ``z_dtype``; z without ``next_weight``;
-    the rows' factors without ``keep``)."""
+    without ``keep`` the row factors of the two norms, f32 [2, T])."""
+    return block_residual_desc(y, residual, gate, post_weight, next_weight, scale, residual_scale, eps, weight_offset, z_dtype,
+                               keep)[:3]
+
+
+def block_residual_desc(y, residual, gate, post_weight, next_weight, scale, residual_scale, eps, weight_offset, z_dtype,
+                        keep):
+    """`block_residual`, and the descriptor of the call (None without rows), for
+    `block_grad_plain`"""
     what = "block_residual"
     if y is None and (next_weight is None or gate is not None or post_weight is not None):
         raise ValueError(f"{what}: without a block's output there is only the next norm")
@@ -1249,18 +1267,22 @@ def block_residual(y, residual, gate=None, post_weight=None, next_weight=None, s
     shape, H = residual.shape, residual.shape[-1]
     T = residual.numel() // H
     with _on_device(residual, y, gate, post_weight, next_weight):
-        dev, f32 = residual.device, torch.float32
-        h = None if y is None else torch.empty(shape, dtype=residual.dtype, device=dev)
-        z = None if next_weight is None else torch.empty(shape, dtype=yt, device=dev)
-        ry = torch.empty(T, dtype=f32, device=dev) if keep and post_weight is not None else None
-        rh = torch.empty(T, dtype=f32, device=dev) if keep and next_weight is not None else None
+        rt = residual.dtype
+        h = None if y is None else residual.new_empty(shape)
+        z = None if next_weight is None else residual.new_empty(shape, dtype=yt)
+        rstd = residual.new_empty((2, T), dtype=torch.float32) if keep else None
         if T == 0:
-            return h, z, ry, rh
-        d, held = _block_desc(T, H, y, residual, gate, kind, post_weight, next_weight, yt, residual.dtype, wt, scale,
-                              residual_scale, eps, weight_offset)
-        d.h, d.ldh, d.z, d.ldz, d.rstd_y, d.rstd_h = _addr(h), H, _addr(z), H, _addr(ry), _addr(rh)
-        check(lib.qmoe_block_residual(ctypes.byref(d), _raw_stream(dev)), what)
-    return h, z, ry, rh
+            return h, z, rstd, None
+        r, ldr = _rows(residual, H)
+        yr, ldy = (None, 0) if y is None else _rows(y, H)
+        g, ldg = _block_gate(gate, kind, H) if kind else (None, 0)
+        wp = None if post_weight is None else post_weight.contiguous()
+        wn = None if next_weight is None else next_weight.contiguous()
+        ry = rstd.data_ptr() if keep else None
+        d = _block_desc(T, H, yr, ldy, r, ldr, g, ldg, kind, wp, wn, h, H, z, ry, ry + 4 * T if keep else None, yt, rt, wt,
+                        scale, residual_scale, eps, weight_offset)
+        check(lib.qmoe_block_residual(ctypes.byref(d), _raw_stream(residual.device)), what)
+    return h, z, rstd, d
 
 
 @functools.lru_cache(maxsize=256)
@@ -1270,12 +1292,12 @@ def _block_grad_bytes(T, H):
     return need.value
 
 
-def block_residual_grad(g_h, g_z, y, h, gate, post_weight, next_weight, rstd_y, rstd_h, scale=1.0, residual_scale=1.0,
-                        eps=1e-6, weight_offset=0.0, z_dtype=None, need=(True,) * 5):
+def block_residual_grad(g_h, g_z, y, h, gate, post_weight, next_weight, rstd, scale=1.0, residual_scale=1.0, eps=1e-6,
+                        weight_offset=0.0, z_dtype=None, need=(True,) * 5):
     """Gradients of `block_residual` for those of h and z (one may be None): of
     (y, residual, gate, post_weight, next_weight), None for operands that the
     call has not, that ``need`` leaves out or that no gradient reaches. ``h`` is
-    its first result (without y: the residual)."""
+    its first result (without y: the residual), ``rstd`` its row factors."""
     what = "block_residual_grad"
     kind, yt, wt = _check_block(y, h, gate, post_weight, next_weight, z_dtype, what)
     shape, H, rt = h.shape, h.shape[-1], h.dtype
@@ -1285,34 +1307,61 @@ def block_residual_grad(g_h, g_z, y, h, gate, post_weight, next_weight, rstd_y, 
             raise ValueError(f"{what}: {name} must be {dtype} {tuple(shape)}, got {g.dtype} {tuple(g.shape)}")
     if (g_h is None and g_z is None) or (g_z is not None and next_weight is None):
         raise ValueError(f"{what}: needs the gradient of h or of z")
-    for r, w, name in ((rstd_y, post_weight, "rstd_y"), (rstd_h, next_weight if g_z is not None else None, "rstd_h")):
-        if w is not None and (r is None or r.dtype is not torch.float32 or r.numel() != T or not r.is_contiguous()):
-            raise ValueError(f"{what}: {name} must hold the {T} row factors that block_residual kept")
-    with _on_device(h, y, gate, post_weight, next_weight, g_h, g_z, rstd_y, rstd_h):
-        dev = h.device
-
-        def like(wanted, t):
-            return torch.empty(t.shape, dtype=t.dtype, device=dev) if wanted and t is not None else None
-
-        dy, dr, dg = like(need[0], y), like(need[1], h), like(need[2], gate)
-        dp, dn = like(need[3], post_weight), like(need[4] and g_z is not None, next_weight)
+    if rstd is None or rstd.dtype is not torch.float32 or rstd.shape != (2, T) or not rstd.is_contiguous():
+        raise ValueError(f"{what}: rstd must hold the row factors [2, {T}] that block_residual kept")
+    with _on_device(h, y, gate, post_weight, next_weight, g_h, g_z, rstd):
         if T == 0:
-            return tuple(None if t is None else t.zero_() for t in (dy, dr, dg, dp, dn))
-        d, held = _block_desc(T, H, y, None, gate, kind, post_weight, next_weight, yt, rt, wt, scale, residual_scale, eps,
-                              weight_offset)
-        hr, d.ldh = _rows(h, H)
-        d.h, d.rstd_y, d.rstd_h = hr.data_ptr(), _addr(rstd_y), _addr(rstd_h)
-        g = _capi.BlockGrads()
-        for name, pitch, t in (("g_h", "ldgh", g_h), ("g_z", "ldgz", g_z)):
-            if t is not None:
-                r, ld = _rows(t, H)
-                held.append(r)
-                setattr(g, name, r.data_ptr())
-                setattr(g, pitch, ld)
-        g.d_y, g.d_residual, g.d_gate, g.d_post_weight, g.d_next_weight = (_addr(t) for t in (dy, dr, dg, dp, dn))
-        sums = dp is not None or dn is not None or (kind == 1 and dg is not None)
-        ws, ws_n = _workspace(dev, _block_grad_bytes(T, H) if sums else 0)
-        check(lib.qmoe_block_residual_grad(ctypes.byref(d), ctypes.byref(g), _addr(ws), ws_n, _raw_stream(dev)), what)
+            return tuple(t.new_zeros(t.shape) if n and t is not None else None
+                         for t, n in zip((y, h, gate, post_weight, next_weight if g_z is not None else None), need))
+        hr, ldh = _rows(h, H)
+        yr, ldy = (None, 0) if y is None else _rows(y, H)
+        g, ldg = _block_gate(gate, kind, H) if kind else (None, 0)
+        ghr, ldgh = (None, 0) if g_h is None else _rows(g_h, H)
+        gzr, ldgz = (None, 0) if g_z is None else _rows(g_z, H)
+        wp = None if post_weight is None else post_weight.contiguous()
+        wn = None if next_weight is None else next_weight.contiguous()
+        ry = rstd.data_ptr()
+        d = _block_desc(T, H, yr, ldy, None, 0, g, ldg, kind, wp, wn, hr, ldh, None, ry, ry + 4 * T, yt, rt, wt, scale,
+                        residual_scale, eps, weight_offset)
+        return block_grad_run(d, ghr, ldgh, gzr, ldgz, y, h, gate, post_weight, next_weight, need)
+
+
+def block_grad_plain(d, g_h, g_z, y, h, gate, post, nxt, rstd, need):
+    """`block_grad_run` with the forward call's descriptor, for tensors that are
+    `plain_here`; None where one of them does not lie where that call read it (an
+    operand that it had to copy, a saved tensor that a hook has moved)"""
+    if h.data_ptr() != (d.residual if y is None else d.h) or rstd.data_ptr() != d.rstd_y or \
+            (y is not None and y.data_ptr() != d.y) or (gate is not None and gate.data_ptr() != d.gate) or \
+            (post is not None and post.data_ptr() != d.post_weight) or \
+            (nxt is not None and nxt.data_ptr() != d.next_weight):
+        return None
+    if y is None:
+        d.h, d.ldh = d.residual, d.H
+    return block_grad_run(d, g_h, d.H, g_z, d.H, y, h, gate, post, nxt, need)
+
+
+def block_grad_run(d, g_h, ldgh, g_z, ldgz, y, h, gate, post, nxt, need):
+    """`block_residual_grad` behind its checks, on the current device (``d`` holds the
+    operands' addresses). A backward pass calls it from autograd's own thread, where
+    every Python object that the forward pass has used comes from another core: it
+    touches few."""
+    dy = y.new_empty(y.shape) if need[0] and y is not None else None
+    dr = h.new_empty(h.shape) if need[1] else None
+    dg = gate.new_empty(gate.shape) if need[2] and gate is not None else None
+    dp = post.new_empty(post.shape) if need[3] and post is not None else None
+    dn = nxt.new_empty(nxt.shape) if need[4] and g_z is not None else None
+    ws, n = None, 0
+    if dp is not None or dn is not None or dg is not None:
+        n = _block_grad_bytes(d.T, d.H)
+        ws = h.new_empty(n, dtype=torch.uint8)
+    g = _capi.BlockGrads(None if g_h is None else g_h.data_ptr(), ldgh, None if g_z is None else g_z.data_ptr(), ldgz,
+                         None if dy is None else dy.data_ptr(), None if dr is None else dr.data_ptr(),
+                         None if dg is None else dg.data_ptr(), None if dp is None else dp.data_ptr(),
+                         None if dn is None else dn.data_ptr())
+    rc = lib.qmoe_block_residual_grad(ctypes.byref(d), ctypes.byref(g), None if ws is None else ws.data_ptr(), n,
+                                      _raw_stream(h.device))
+    if rc:
+        check(rc, "block_residual_grad")
     return dy, dr, dg, dp, dn
 
 
@@ -1364,12 +1413,20 @@ def act_checkpoint_grad(codes, scales, dh, activation):
         if t.dtype is not torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous():
             raise ValueError(f"act_checkpoint_grad: {name} must be contiguous uint8 {shape}, got {t.dtype} {tuple(t.shape)}")
     with _on_device(codes, scales, dh):
-        dx = torch.empty((*dh.shape[:-1], 2 * I), dtype=dh.dtype, device=dh.device)
-        if T:
-            r, ld = _rows(dh, I)
-            check(lib.qmoe_act_checkpoint_grad(codes.data_ptr(), scales.data_ptr(), T, I, act, p0, p1, r.data_ptr(), ld,
-                                               _ROW_TYPES[dh.dtype], dx.data_ptr(), _raw_stream(dh.device)),
-                  "act_checkpoint_grad")
+        if T == 0:
+            return dh.new_empty((*dh.shape[:-1], 2 * I))
+        r, ld = _rows(dh, I)
+        return act_grad_run(codes, scales, r, ld, dh.shape, T, I, act, p0, p1)
+
+
+def act_grad_run(codes, scales, dh, ld, shape, T, I, act, p0, p1):
+    """`act_checkpoint_grad` behind its checks, on the current device (few Python
+    objects, see `block_grad_run`)."""
+    dx = dh.new_empty((*shape[:-1], 2 * I))
+    rc = lib.qmoe_act_checkpoint_grad(codes.data_ptr(), scales.data_ptr(), T, I, act, p0, p1, dh.data_ptr(), ld,
+                                      _ROW_TYPES[dh.dtype], dx.data_ptr(), _raw_stream(dh.device))
+    if rc:
+        check(rc, "act_checkpoint_grad")
     return dx
 
 
@@ -1386,15 +1443,22 @@ def _check_linear(x, weight, bias, what):
             x.shape[-1] != weight.shape[1]:
         raise ValueError(f"{what}: takes bf16 [..., K] and [N, K], got {x.dtype} {tuple(x.shape)} and {weight.dtype} "
                          f"{tuple(weight.shape)}")
+    _check_weight(weight, what)
     N, K = weight.shape
-    if N == 0 or K == 0 or K % 32 or N % 8 or N > LINEAR_MAX[1] or K > LINEAR_MAX[2] or x.numel() // K > LINEAR_MAX[0]:
-        raise ValueError(f"{what}: takes K in multiples of 32 up to {LINEAR_MAX[2]}, N in multiples of 8 up to "
-                         f"{LINEAR_MAX[1]} and {LINEAR_MAX[0]} rows at most, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if x.numel() // K > LINEAR_MAX[0]:
+        raise ValueError(f"{what}: takes {LINEAR_MAX[0]} rows at most, got {tuple(x.shape)}")
+    if bias is not None and (bias.dtype not in _GRAD_TYPES or tuple(bias.shape) != (N,)):
+        raise ValueError(f"{what}: the bias must be bf16 or f32 [{N}], got {bias.dtype} {tuple(bias.shape)}")
+
+
+def _check_weight(weight, what):
+    N, K = weight.shape
+    if weight.dtype is not torch.bfloat16 or N == 0 or K == 0 or K % 32 or N % 8 or N > LINEAR_MAX[1] or K > LINEAR_MAX[2]:
+        raise ValueError(f"{what}: takes bf16 weights of K in multiples of 32 up to {LINEAR_MAX[2]} and N in multiples of 8 "
+                         f"up to {LINEAR_MAX[1]}, got {weight.dtype} {tuple(weight.shape)}")
     if weight.stride(1) != 1 or weight.stride(0) < K or weight.stride(0) % 8 or weight.stride(0) >= 1 << 22:
         raise ValueError(f"{what}: the weight's rows must be contiguous and apart by a multiple of 8, got strides "
                          f"{weight.stride()}")
-    if bias is not None and (bias.dtype not in _GRAD_TYPES or tuple(bias.shape) != (N,)):
-        raise ValueError(f"{what}: the bias must be bf16 or f32 [{N}], got {bias.dtype} {tuple(bias.shape)}")
 
 
 def _check_aligned(weight, what):
@@ -1449,7 +1513,7 @@ def linear_grad(dy, weight, codes=None, scales=None, need_x=True, need_weight=Tr
     if weight.dim() != 2 or dy.dtype is not torch.bfloat16 or dy.dim() < 1 or dy.shape[-1] != weight.shape[0]:
         raise ValueError(f"linear_grad: a gradient of {dy.dtype} {tuple(dy.shape)} for a weight of {tuple(weight.shape)}")
     N, K = weight.shape
-    _check_linear(dy.new_empty((0, K)), weight, None, "linear_grad")
+    _check_weight(weight, "linear_grad")
     _check_aligned(weight, "linear_grad")
     T = dy.numel() // N
     if T > LINEAR_MAX[0]:
@@ -1461,17 +1525,26 @@ def linear_grad(dy, weight, codes=None, scales=None, need_x=True, need_weight=Tr
     if bias_dtype is not None and bias_dtype not in _GRAD_TYPES:
         raise ValueError(f"linear_grad: the bias is bf16 or f32, not {bias_dtype}")
     with _on_device(dy, weight, codes, scales):
-        dev, bf16 = dy.device, torch.bfloat16
-        dx = torch.empty((*dy.shape[:-1], K), dtype=bf16, device=dev) if need_x else None
-        dw = torch.empty((N, K), dtype=bf16, device=dev) if need_weight else None
-        db = torch.empty(N, dtype=bias_dtype, device=dev) if bias_dtype is not None else None
         if T == 0:
-            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
-        if need_x or need_weight or db is not None:
-            r, ld = _gemm_rows(dy, N)
-            ws, ws_n = _workspace(dev, _linear_grad_bytes(T, N, K, bool(need_x), bool(need_weight), db is not None))
-            check(lib.qmoe_linear_grad(r.data_ptr(), ld, T, N, K, weight.data_ptr(), weight.stride(0),
-                                       _addr(codes) if need_weight else None, _addr(scales) if need_weight else None,
-                                       _addr(dx), _addr(dw), _addr(db), bias_dtype is torch.float32, _addr(ws), ws_n,
-                                       _raw_stream(dev)), "linear_grad")
+            return (dy.new_empty((*dy.shape[:-1], K)) if need_x else None, dy.new_zeros((N, K)) if need_weight else None,
+                    None if bias_dtype is None else dy.new_zeros(N, dtype=bias_dtype))
+        r, ld = _gemm_rows(dy, N)
+        return linear_grad_run(r, ld, dy.shape, T, N, K, weight, codes, scales, need_x, need_weight, bias_dtype)
+
+
+def linear_grad_run(dy, ld, shape, T, N, K, weight, codes, scales, need_x, need_weight, bias_dtype):
+    """`linear_grad` behind its checks, on the current device (few Python objects, see
+    `block_grad_run`)."""
+    dx = dy.new_empty((*shape[:-1], K)) if need_x else None
+    dw = dy.new_empty((N, K)) if need_weight else None
+    db = None if bias_dtype is None else dy.new_empty(N, dtype=bias_dtype)
+    n = _linear_grad_bytes(T, N, K, need_x, need_weight, db is not None)
+    ws = dy.new_empty(n, dtype=torch.uint8) if n else None
+    rc = lib.qmoe_linear_grad(dy.data_ptr(), ld, T, N, K, weight.data_ptr(), weight.stride(0),
+                              codes.data_ptr() if need_weight else None, scales.data_ptr() if need_weight else None,
+                              None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+                              None if db is None else db.data_ptr(), bias_dtype is torch.float32,
+                              None if ws is None else ws.data_ptr(), n, _raw_stream(dy.device))
+    if rc:
+        check(rc, "linear_grad")
     return dx, dw, db
