@@ -80,9 +80,8 @@ class _Block(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_h, g_z):
-        # (autograd runs this with gradients off; with create_graph the decorator puts the error for a second pass behind it)
-        if torch.is_grad_enabled():
-            return _Block._once(ctx, g_h, g_z)
+        if torch.is_grad_enabled():  # (a backward pass that records itself)
+            return ops.once("block_residual", _Block._grads, ctx, g_h, g_z)
         return _Block._grads(ctx, g_h, g_z)
 
     @staticmethod
@@ -100,8 +99,6 @@ class _Block(torch.autograd.Function):
         grads = torch.ops.qmoe.block_residual_grad(g_h, g_z, *saved, *ctx.args, *need)
         there = (saved[0], saved[1], saved[2], saved[3], saved[4] if g_z is not None else None)
         return (*(g if n and t is not None else None for g, n, t in zip(grads, need, there)), None)
-
-    _once = staticmethod(torch.autograd.function.once_differentiable(_grads.__func__))
 
 
 def _block(y, residual, gate, norm_weight, next_weight, args, keep):
@@ -192,7 +189,7 @@ class _Activation(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         if torch.is_grad_enabled():  # (as above)
-            return _Activation._once(ctx, grad)
+            return ops.once("checkpointed_activation", _Activation._grads, ctx, grad)
         return _Activation._grads(ctx, grad)
 
     @staticmethod
@@ -208,8 +205,6 @@ class _Activation(torch.autograd.Function):
             ops.refuse_tangents("checkpointed_activation's gradient", grad)
             fn = torch.ops.qmoe.act_checkpoint_grad
         return fn(codes, scales, grad, ctx.activation), None
-
-    _once = staticmethod(torch.autograd.function.once_differentiable(_grads.__func__))
 
 
 def _act(gate_up, activation, keep):
@@ -284,7 +279,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         if torch.is_grad_enabled():  # (as above)
-            return _Linear._once(ctx, grad)
+            return ops.once("checkpointed_linear", _Linear._grads, ctx, grad)
         return _Linear._grads(ctx, grad)
 
     @staticmethod
@@ -304,8 +299,6 @@ class _Linear(torch.autograd.Function):
             fn = torch.ops.qmoe.linear_grad
         dx, dw, db = fn(grad, weight, codes, scales, need_x, need_w, ctx.bias_dtype)
         return (dx if need_x else None), (dw if need_w else None), (db if ctx.bias_dtype is not None else None)
-
-    _once = staticmethod(torch.autograd.function.once_differentiable(_grads.__func__))
 
 
 def _linear(x, weight, bias, keep):

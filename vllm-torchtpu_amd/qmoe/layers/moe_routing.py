@@ -167,9 +167,8 @@ class _Balance(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_w, g_ids, g_loss, g_counts):
-        # (autograd runs this with gradients off; with create_graph the decorator puts the error for a second pass behind it)
-        if torch.is_grad_enabled():
-            return _Balance._once(ctx, g_w, g_ids, g_loss, g_counts)
+        if torch.is_grad_enabled():  # (a backward pass that records itself)
+            return ops.once("balanced_experts", _Balance._grads, ctx, g_w, g_ids, g_loss, g_counts)
         return _Balance._grads(ctx, g_w, g_ids, g_loss, g_counts)
 
     @staticmethod
@@ -188,8 +187,6 @@ class _Balance(torch.autograd.Function):
             ops.refuse_tangents("balanced_experts' gradient", g_w, g_loss)
             fn = torch.ops.qmoe.moe_balance_grad
         return fn(logits, ids, counts, g_w, g_loss, *ctx.args, mask), None, None, None, None
-
-    _once = staticmethod(torch.autograd.function.once_differentiable(_grads.__func__))
 
 
 def _balance(logits, topk, args, bias, token_mask):

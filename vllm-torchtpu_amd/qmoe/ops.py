@@ -109,6 +109,26 @@ def refuse_tangents(what, *ts):
         raise NotImplementedError(f"{what}: no forward-mode derivative")
 
 
+class _NoSecond(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, *grads):
+        ctx.what = what
+        return tuple(None if g is None else g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what}: no second derivative")
+
+
+def once(what, fn, *args):
+    """``fn(*args)``, the gradients of a backward pass that records itself
+    (create_graph), with an error behind them for whoever differentiates them: without
+    one they would count as constants, and a penalty on them as zero."""
+    with torch.no_grad():
+        grads = fn(*args)
+    return _NoSecond.apply(what, *(g.detach().requires_grad_() if torch.is_tensor(g) else None for g in grads))
+
+
 def _require_gpu(*ts):
     for t in ts:
         if t is not None and t.device.type != "cuda":
