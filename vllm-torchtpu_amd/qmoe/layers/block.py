@@ -72,9 +72,11 @@ def _(g_h, g_z, y, h, gate, norm_weight, next_weight, rstd, scale, residual_scal
 class _Block(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, residual, gate, norm_weight, next_weight, args):
-        h, z, rstd, ctx.desc = _block(y, residual, gate, norm_weight, next_weight, args, True)
-        ctx.save_for_backward(y, residual if y is None else h, gate, norm_weight, next_weight, rstd)
+        h, z, rstd, desc = _block(y, residual, gate, norm_weight, next_weight, args, True)
+        saved = (y, residual if y is None else h, gate, norm_weight, next_weight, rstd)
+        ctx.save_for_backward(*saved)
         ctx.args = args
+        ctx.desc = None if desc is None else ops.block_saved(desc, *saved)
         ctx.set_materialize_grads(False)
         return h, z
 
@@ -89,11 +91,11 @@ class _Block(torch.autograd.Function):
         if g_h is None and g_z is None:
             return (None,) * 6
         saved, need = ctx.saved_tensors, ctx.needs_input_grad[:5]
+        if ctx.desc is not None and (g_h is None or ops.plain_grad(g_h)) and (g_z is None or ops.plain_grad(g_z)):
+            grads = ops.block_grad_plain(ctx.desc, g_h, g_z, *saved, need)
+            if grads is not None:
+                return (*grads, None)
         if ops.eager_call(g_h, g_z, *saved):
-            if ctx.desc is not None and ops.plain_here(g_h, g_z, *saved):
-                grads = ops.block_grad_plain(ctx.desc, g_h, g_z, *saved, need)
-                if grads is not None:
-                    return (*grads, None)
             return (*ops.block_residual_grad(g_h, g_z, *saved, *ctx.args, need), None)
         ops.refuse_tangents("block_residual's gradients", g_h, g_z)
         grads = torch.ops.qmoe.block_residual_grad(g_h, g_z, *saved, *ctx.args, *need)
@@ -183,7 +185,10 @@ class _Activation(torch.autograd.Function):
         h, codes, scales = _act(gate_up, activation, True)
         ctx.save_for_backward(codes, scales)
         ctx.activation = activation
-        ctx.act = ops.act_code(activation)
+        ctx.run = None
+        if ops.eager_call(gate_up) and h.numel():
+            I = h.shape[-1]
+            ctx.run = (codes.data_ptr(), scales.data_ptr(), h.shape, h.numel() // I, I, *ops.act_code(activation))
         return h
 
     @staticmethod
@@ -195,13 +200,11 @@ class _Activation(torch.autograd.Function):
     @staticmethod
     def _grads(ctx, grad):
         codes, scales = ctx.saved_tensors
+        run = ctx.run
+        if run is not None and ops.plain_grad(grad) and codes.data_ptr() == run[0] and scales.data_ptr() == run[1]:
+            return ops.act_grad_run(codes, scales, grad, run[4], *run[2:]), None
         fn = ops.act_checkpoint_grad
-        if ops.eager_call(grad, codes, scales):
-            I = grad.shape[-1]
-            T = grad.numel() // I
-            if T and codes.numel() == 2 * T * I and ops.plain_here(grad, codes, scales):
-                return ops.act_grad_run(codes, scales, grad, I, grad.shape, T, I, *ctx.act), None
-        else:
+        if not ops.eager_call(grad, codes, scales):
             ops.refuse_tangents("checkpointed_activation's gradient", grad)
             fn = torch.ops.qmoe.act_checkpoint_grad
         return fn(codes, scales, grad, ctx.activation), None
@@ -270,10 +273,12 @@ class _Linear(torch.autograd.Function):
         keep = ctx.needs_input_grad[1]
         y, codes, scales = _linear(x, weight, bias, keep)
         ctx.save_for_backward(weight, *((codes, scales) if keep else (None, None)))
-        ctx.sizes = weight.shape
-        # (the checks of the weight hold for the one that they have seen)
-        ctx.weight_at = weight.data_ptr() if ops.eager_call(weight) else None
         ctx.bias_dtype = bias.dtype if bias is not None and ctx.needs_input_grad[2] else None
+        ctx.run = None
+        if ops.eager_call(x, weight, bias) and y.numel():
+            N, K = weight.shape
+            at = (codes.data_ptr(), scales.data_ptr()) if keep else (0, 0)
+            ctx.run = (weight.data_ptr(), *at, N, y.shape, y.numel() // N, N, K)
         return y
 
     @staticmethod
@@ -286,15 +291,12 @@ class _Linear(torch.autograd.Function):
     def _grads(ctx, grad):
         weight, codes, scales = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
+        run = ctx.run
+        if run is not None and ops.plain_grad(grad) and grad.data_ptr() % 16 == 0 and weight.data_ptr() == run[0] and \
+                (codes is None or (codes.data_ptr() == run[1] and scales.data_ptr() == run[2])):
+            return ops.linear_grad_run(grad, *run[3:], weight, codes, scales, need_x, need_w, ctx.bias_dtype)
         fn = ops.linear_grad
-        if ops.eager_call(grad, weight, codes, scales):
-            N, K = ctx.sizes
-            T = grad.numel() // N
-            if T and grad.data_ptr() % 16 == 0 and weight.data_ptr() == ctx.weight_at and \
-                    (codes is None or codes.numel() == T * K) and ops.plain_here(grad, codes, scales):
-                return ops.linear_grad_run(grad, N, grad.shape, T, N, K, weight, codes, scales, need_x, need_w,
-                                           ctx.bias_dtype)
-        else:
+        if not ops.eager_call(grad, weight, codes, scales):
             ops.refuse_tangents("checkpointed_linear's gradients", grad)
             fn = torch.ops.qmoe.linear_grad
         dx, dw, db = fn(grad, weight, codes, scales, need_x, need_w, ctx.bias_dtype)

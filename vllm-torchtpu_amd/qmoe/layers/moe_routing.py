@@ -161,6 +161,11 @@ class _Balance(torch.autograd.Function):
         w, ids, loss, counts = _balance(logits, topk, args, bias, token_mask)
         ctx.save_for_backward(logits, ids, counts, token_mask)
         ctx.args = args[:3]
+        ctx.run = None
+        if ops.eager_call(logits, bias, token_mask) and logits.numel() and logits.is_contiguous() and \
+                (token_mask is None or token_mask.is_contiguous()):
+            at = (logits.data_ptr(), ids.data_ptr(), counts.data_ptr(), 0 if token_mask is None else token_mask.data_ptr())
+            ctx.run = (at, *logits.shape, topk, ops._SCORING[args[0]], *args[1:3])
         ctx.mark_non_differentiable(ids, counts)
         ctx.set_materialize_grads(False)
         return w, ids, loss, counts
@@ -176,14 +181,12 @@ class _Balance(torch.autograd.Function):
         if g_w is None and g_loss is None:
             return (None,) * 5
         logits, ids, counts, mask = ctx.saved_tensors
+        run = ctx.run
+        if run is not None and (g_w is None or ops.plain_grad(g_w)) and (g_loss is None or ops.plain_grad(g_loss)) and \
+                (logits.data_ptr(), ids.data_ptr(), counts.data_ptr(), 0 if mask is None else mask.data_ptr()) == run[0]:
+            return ops.balance_grad_run(logits, ids, counts, g_w, g_loss, *run[1:], mask), None, None, None, None
         fn = ops.moe_balance_grad
-        if ops.eager_call(logits, ids, counts, g_w, g_loss, mask):
-            T, E = logits.shape
-            if T and ops.plain_here(logits, ids, counts, g_w, g_loss, mask):
-                scoring, renormalize, rsf = ctx.args
-                return (ops.balance_grad_run(logits, ids, counts, g_w, g_loss, T, E, ids.shape[1], ops._SCORING[scoring],
-                                             renormalize, rsf, mask), None, None, None, None)
-        else:
+        if not ops.eager_call(logits, ids, counts, g_w, g_loss, mask):
             ops.refuse_tangents("balanced_experts' gradient", g_w, g_loss)
             fn = torch.ops.qmoe.moe_balance_grad
         return fn(logits, ids, counts, g_w, g_loss, *ctx.args, mask), None, None, None, None

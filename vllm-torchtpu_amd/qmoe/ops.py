@@ -84,15 +84,14 @@ def eager_call(*ts):
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
-def plain_here(*ts):
-    """Whether these tensors (None aside) are contiguous and on the current device, as
-    what a backward pass gets nearly always is: a call on them that also is an
-    `eager_call` needs no checks but the forward pass's."""
-    dev = _current_device()
-    for t in ts:
-        if t is not None and (t.get_device() != dev or not t.is_contiguous()):
-            return False
-    return True
+def plain_grad(grad):
+    """Whether a gradient that autograd hands to a backward pass is an ordinary
+    contiguous tensor on the current device, and the pass itself runs at once (see
+    `eager_call`). With saved tensors that lie where the forward pass had them, such a
+    call needs no checks but the forward pass's."""
+    return (type(grad) is torch.Tensor and grad.is_contiguous() and grad.get_device() == _current_device()
+            and not _included_keys().raw_repr() & _WATCHING and forward_ad._current_level < 0
+            and not torch.compiler.is_compiling())
 
 
 def has_tangent(*ts):
@@ -1346,17 +1345,26 @@ def block_residual_grad(g_h, g_z, y, h, gate, post_weight, next_weight, rstd, sc
         return block_grad_run(d, ghr, ldgh, gzr, ldgz, y, h, gate, post_weight, next_weight, need)
 
 
-def block_grad_plain(d, g_h, g_z, y, h, gate, post, nxt, rstd, need):
-    """`block_grad_run` with the forward call's descriptor, for tensors that are
-    `plain_here`; None where one of them does not lie where that call read it (an
-    operand that it had to copy, a saved tensor that a hook has moved)"""
-    if h.data_ptr() != (d.residual if y is None else d.h) or rstd.data_ptr() != d.rstd_y or \
-            (y is not None and y.data_ptr() != d.y) or (gate is not None and gate.data_ptr() != d.gate) or \
-            (post is not None and post.data_ptr() != d.post_weight) or \
-            (nxt is not None and nxt.data_ptr() != d.next_weight):
-        return None
+def block_saved(d, y, h, gate, post, nxt, rstd):
+    """The descriptor of a forward call where its operands are contiguous and lie where
+    it has read them (not copies that it had to make): its backward pass may take the
+    addresses from there. Else None."""
+    for t, at in ((y, d.y), (h, d.residual if y is None else d.h), (gate, d.gate), (post, d.post_weight),
+                  (nxt, d.next_weight)):
+        if t is not None and (t.data_ptr() != at or not t.is_contiguous()):
+            return None
     if y is None:
         d.h, d.ldh = d.residual, d.H
+    return d
+
+
+def block_grad_plain(d, g_h, g_z, y, h, gate, post, nxt, rstd, need):
+    """`block_grad_run` with the descriptor that `block_saved` passed, for contiguous
+    gradients; None where a hook has moved a saved tensor"""
+    if h.data_ptr() != d.h or rstd.data_ptr() != d.rstd_y or (y is not None and y.data_ptr() != d.y) or \
+            (gate is not None and gate.data_ptr() != d.gate) or (post is not None and post.data_ptr() != d.post_weight) or \
+            (nxt is not None and nxt.data_ptr() != d.next_weight):
+        return None
     return block_grad_run(d, g_h, d.H, g_z, d.H, y, h, gate, post, nxt, need)
 
 
