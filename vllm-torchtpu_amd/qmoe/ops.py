@@ -867,18 +867,18 @@ def _on_device(*ts):
     """One device for every tensor given (None aside), made the current one
     for the launches of a ``with`` block: the runtime launches on the current
     device, whatever device the stream and the pointers belong to."""
-    dev = None
+    dev, first = None, None
     for t in ts:
         if t is None:
             continue
-        d = t.device
-        if dev is None:
-            dev = d
-            if d.type != "cuda":
-                raise ValueError(f"qmoe kernels need device tensors, got a {d} tensor")
+        d = t.get_device()  # (the device's number, without a device object; -1 is the CPU)
+        if first is None:
+            dev, first = d, t
+            if d < 0 or not t.is_cuda:
+                raise ValueError(f"qmoe kernels need device tensors, got a {t.device} tensor")
         elif d != dev:
-            raise ValueError(f"qmoe kernels need device tensors, all on one device, got {dev} and {d}")
-    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+            raise ValueError(f"qmoe kernels need device tensors, all on one device, got {first.device} and {t.device}")
+    return _HERE if dev == _current_device() else torch.cuda.device(dev)
 
 
 def _check_ids(ids, what):
