@@ -645,7 +645,8 @@ int qmoe_linear(const void* x, int64_t ldx, int64_t T, int64_t N, int64_t K, con
  * Gradients of a linear layer y = x w^T + bias whose input waited in 8 bits:
  *   dx = dy w,  dw = dy^T x8,  dbias = sum over t of dy     (x8: the codes' values, K % 32 == 0, N % 8 == 0)
  *   dy  : bf16 [T][lddy]; w bf16 [N][ldw] (for dx); codes / scales of qmoe_pack_8bit
- *         (for dw); lddy and ldw multiples of 8, dy and w 16-byte aligned
+ *         (for dw); lddy and ldw multiples of 8, dy, w and codes
+ *         16-byte aligned
  *   dx  : bf16 [T][K]; dw bf16 [N][K]; dbias [N] bf16, or f32 with dbias_f32;
  *         each may be NULL
  * Sums are float32 in a fixed order. 1 <= T <= 2^20, N <= 2^18, K <= 2^16. The

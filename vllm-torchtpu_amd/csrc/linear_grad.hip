@@ -39,6 +39,7 @@ struct LinearGemm {
   int kslice;   // K split: slice z takes the K range from z * kslice on and leaves float32 sums in [z][nb][na]
   float* slices;
   const float* bias;  // of the A rows, or nullptr
+  const uint8_t* scales;  // of A where it is codes [K][na], bytes [K][na / 32]
 };
 
 // B row t of the 64 that a round holds, A row n of it at n ^ vg_row_swz(t): 8
@@ -90,18 +91,22 @@ __device__ __forceinline__ void linear_epilogue(const LinearGemm& p, f32x16 (&ac
 }
 
 // This workgroup's slice of K
-template <bool TRA, bool TRB>
+template <bool TRA, bool TRB, bool CODES = false>
 __device__ __forceinline__ void linear_slice(LinearGemm& p) {
   if (!p.kslice) return;
   const int64_t k0 = (int64_t)blockIdx.y * p.kslice;
   p.a += TRA ? k0 * p.lda : k0 * 2;
+  if constexpr (CODES) p.scales += k0 * (p.na / 32);
   p.b += TRB ? k0 * p.ldb : k0 * 2;
   p.K = (int)min((int64_t)p.kslice, p.K - k0);
 }
 
 // Tiles of 256 x BM (64 or 128) by eight wavefronts. ONE: a stage at a time,
-// without a ring, so that two workgroups share a CU.
-template <bool TRA, bool TRB, int BM, bool ONE>
+// without a ring, so that two workgroups share a CU. CODES: the A operand is x8
+// itself, codes and scale bytes across K, expanded on the way to LDS (a thread 32
+// columns of a row): no transposed copy of x8 before the product, whose launch and
+// bytes count where the sums are short.
+template <bool TRA, bool TRB, int BM, bool ONE, bool CODES>
 __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const LinearGemm args) {
   constexpr int NI = 2, MJ = BM / 64, WB = kAN * 128, STG = WB + BM * 128;
   constexpr int RING = ONE ? 1 : (163840 / STG < 6 ? 163840 / STG : 6), EPILOGUE = 65536;
@@ -109,7 +114,7 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
   static_assert(ONE ? sizeof(smem) <= 81920 : RING >= 3 && sizeof(smem) <= 163840, "workgroups of a CU, ring");
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
   LinearGemm p = args;
-  linear_slice<TRA, TRB>(p);
+  linear_slice<TRA, TRB, CODES>(p);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave & 3, wm = wave >> 2, rl = lane & 31, kh = lane >> 5;
   int mt, nt;
@@ -121,11 +126,13 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
   // chunk c of row r at c ^ vg_swz(r)), or 1 KB of K rows; wavefront w moves the
   // groups w, w + 8, ...; rows and columns past the end repeat the last
   constexpr int WI = WB / 8192, XI = BM / 64;
-  constexpr int TB = TRA ? kAN * 2 : BM * 2, TL = TB / 16;  // bytes, lanes of a K row (of the one operand across)
-  static_assert(!TRA || !TRB, "one operand across K");
+  constexpr bool COPY_A = TRA && !CODES;               // the operand across K that is copied
+  constexpr int TB = COPY_A ? kAN * 2 : BM * 2, TL = TB / 16;  // bytes, lanes of its K row
+  static_assert(!COPY_A || !TRB, "one copied operand across K");
+  static_assert(!CODES || (ONE && TRA && TRB), "codes");
   const int chunk = (lane & 7) ^ ((lane >> 3) ^ (wave & 1));
   const int trow = lane / TL, tchunk = (lane % TL) ^ tr_swz<TB>(wave * (64 / TL) + trow);
-  const uint32_t tcol = (uint32_t)min(tchunk, (TRA ? arows : brows) / 8 - 1) * 16;
+  const uint32_t tcol = (uint32_t)min(tchunk, (COPY_A ? arows : brows) / 8 - 1) * 16;
   const uint8_t* abase = TRA ? p.a + n0 * 2 : p.a + (int64_t)n0 * p.lda;
   const uint8_t* bbase = TRB ? p.b + m0 * 2 : p.b + (int64_t)m0 * p.ldb;
   const int64_t astep = TRA ? 64 * p.lda : 128, bstep = TRB ? 64 * p.ldb : 128;
@@ -133,7 +140,7 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
   auto krow = [&](int j) { return (wave + 8 * j) * (64 / TL) + trow; };  // of a stage, of copy j of the operand across K
 #pragma unroll
   for (int j = 0; j < WI; ++j)
-    aoff[j] = TRA ? (uint32_t)krow(j) * (uint32_t)p.lda + tcol
+    aoff[j] = CODES ? 0u : TRA ? (uint32_t)krow(j) * (uint32_t)p.lda + tcol
                   : (uint32_t)min((wave + 8 * j) * 8 + (lane >> 3), arows - 1) * (uint32_t)p.lda + chunk * 16;
 #pragma unroll
   for (int j = 0; j < XI; ++j)
@@ -147,17 +154,21 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
     const uint32_t d = __builtin_amdgcn_readfirstlane(cw + slot * STG);
     const int k = min(s, KF - 1);
     const uint8_t *as = uniform_ptr(abase + k * astep), *bs = uniform_ptr(bbase + k * bstep);
+    if constexpr (!CODES) {
 #pragma unroll
-    for (int j = 0; j < WI; ++j) lds_copy16(as, aoff[j], d + j * 8192);
+      for (int j = 0; j < WI; ++j) lds_copy16(as, aoff[j], d + j * 8192);
+    }
 #pragma unroll
     for (int j = 0; j < XI; ++j) lds_copy16(bs, boff[j], d + WB + j * 8192);
   };
   // the last, partial stage, with zeros where K has ended
   auto copy_tail = [&]() {
     const uint8_t *as = abase + KF * astep, *bs = bbase + KF * bstep, *z = reinterpret_cast<const uint8_t*>(kZeroChunk);
+    if constexpr (!CODES) {
 #pragma unroll
-    for (int j = 0; j < WI; ++j)
-      lds_copy16((TRA ? krow(j) : chunk * 8) < tail ? as + aoff[j] : z, __builtin_amdgcn_readfirstlane(cw + j * 8192));
+      for (int j = 0; j < WI; ++j)
+        lds_copy16((TRA ? krow(j) : chunk * 8) < tail ? as + aoff[j] : z, __builtin_amdgcn_readfirstlane(cw + j * 8192));
+    }
 #pragma unroll
     for (int j = 0; j < XI; ++j)
       lds_copy16((TRB ? krow(j) : chunk * 8) < tail ? bs + boff[j] : z,
@@ -176,18 +187,18 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
     bf16x8 v;
   };
   B8 wf[2][NI], xf[2][MJ];
-  const uint32_t tlane = tr_lane<TB>(lane);
+  const uint32_t alane = tr_lane<kAN * 2>(lane), blane = tr_lane<BM * 2>(lane);
   // operands of step q (16 k) of a stage
   auto read_q = [&](int slot, int q) {
     const uint8_t* s = smem + slot * STG;
 #pragma unroll
     for (int i = 0; i < NI; ++i)
-      if constexpr (TRA) wf[q & 1][i].u = tr_read<TB>(s + q * 16 * TB + (tlane ^ (wn * NI + i) * 64));
+      if constexpr (TRA) wf[q & 1][i].u = tr_read<kAN * 2>(s + q * 32 * kAN + (alane ^ (wn * NI + i) * 64));
       else wf[q & 1][i].u =
           *reinterpret_cast<const uint4*>(s + (wn * 64 + i * 32 + rl) * 128 + ((2 * q + kh) ^ vg_swz(rl)) * 16);
 #pragma unroll
     for (int j = 0; j < MJ; ++j)
-      if constexpr (TRB) xf[q & 1][j].u = tr_read<TB>(s + WB + q * 16 * TB + (tlane ^ (2 * j + wm) * 64));
+      if constexpr (TRB) xf[q & 1][j].u = tr_read<BM * 2>(s + WB + q * 32 * BM + (blane ^ (2 * j + wm) * 64));
       else xf[q & 1][j].u =
           *reinterpret_cast<const uint4*>(s + WB + ((2 * j + wm) * 32 + rl) * 128 + ((2 * q + kh) ^ vg_swz(rl)) * 16);
   };
@@ -213,9 +224,40 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
   // stage's last operands, so that its slot takes the copies of stage s + RING ->
   // the last step, while the next stage's first operands are read.
   if constexpr (ONE) {
+    // codes: row k of the stage, 32 columns from 32 g on; zeros behind the ends
+    const int k = tid >> 3, g = tid & 7;
+    const bool col = 32 * g < arows;
+    const uint8_t *cp = p.a + (int64_t)k * p.lda + n0 + 32 * g, *sp = p.scales + (int64_t)k * (p.na / 32) + n0 / 32 + g;
+    uint8_t* to = smem + k * kAN * 2 + ((g * 64) ^ (tr_swz<kAN * 2>(k) * 16));
     for (int s = 0; s < KF + (tail != 0); ++s) {
+      uint4 c[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+      uint32_t scale = 0;
+      if constexpr (CODES) {
+        if (col && 64 * s + k < p.K) {
+          const uint4* at = reinterpret_cast<const uint4*>(cp + (int64_t)s * 64 * p.lda);
+          c[0] = at[0];
+          c[1] = at[1];
+          scale = sp[(int64_t)s * 64 * (p.na / 32)];
+        }
+      }
       if (s < KF) copy_stage(s, 0);
       else copy_tail();
+      if constexpr (CODES) {
+        const uint32_t* d = reinterpret_cast<const uint32_t*>(c);
+        const float f = bits_f32(scale << 23);  // (the conversion takes the exponent alone, 0 as 2^-127)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          union {
+            bf16x2 h[4];
+            uint4 u;
+          } v;
+          v.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)d[2 * j], f, false);
+          v.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)d[2 * j], f, true);
+          v.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)d[2 * j + 1], f, false);
+          v.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)d[2 * j + 1], f, true);
+          *reinterpret_cast<uint4*>(to + j * 16) = v.u;
+        }
+      }
       one_stage();
     }
   } else if (KF > 0) {
@@ -537,6 +579,12 @@ LinearPlan linear_plan(int mode, int64_t na, int64_t nb, int64_t K) {
   return best;
 }
 
+// Whether dw takes the codes as they are: tiles without a ring of up to 512 tokens.
+// Every tile of N expands them again: 19 tokens x 2880 x 2880 10.4 us (13.4 with the
+// transposed copy), 200 x 7168 x 2048 19.6 (22.1), 512 x 4096 x 4096 29.7 (30.0), but 777
+// x 4096 x 4096 42.7 (38.9), 1500 x 14336 x 4096 235 (180).
+bool linear_codes(int64_t N, int64_t K, int64_t T) { return T <= 512 && linear_plan(LM_DW, K, N, T).bm == 1; }
+
 template <bool TRA, bool TRB, int BM>
 void launch_big(const LinearGemm& g, dim3 grid, hipStream_t st) {
   if (g.K % 64) hipLaunchKernelGGL((linear_big_kernel<TRA, TRB, BM, true>), grid, dim3(256), 0, st, g);
@@ -556,9 +604,11 @@ void launch_linear(LinearGemm g, uint8_t* ws, hipStream_t st) {
   const dim3 grid((unsigned)up((int64_t)g.n_tiles * g.m_tiles, kXcds), (unsigned)d.slices);
   if (d.bm == 256) launch_big<TRA, TRB, 256>(g, grid, st);
   else if (d.bm == 192) { if constexpr (!TRB) launch_big<TRA, TRB, 192>(g, grid, st); }
-  else if (d.bm == 64) hipLaunchKernelGGL((linear_small_kernel<TRA, TRB, 64, false>), grid, dim3(512), 0, st, g);
-  else if (d.bm == 128) hipLaunchKernelGGL((linear_small_kernel<TRA, TRB, 128, false>), grid, dim3(512), 0, st, g);
-  else hipLaunchKernelGGL((linear_small_kernel<TRA, TRB, 128, true>), grid, dim3(512), 0, st, g);
+  else if (d.bm == 64) hipLaunchKernelGGL((linear_small_kernel<TRA, TRB, 64, false, false>), grid, dim3(512), 0, st, g);
+  else if (d.bm == 128) hipLaunchKernelGGL((linear_small_kernel<TRA, TRB, 128, false, false>), grid, dim3(512), 0, st, g);
+  else if (MODE == LM_DW && g.scales)
+    hipLaunchKernelGGL((linear_small_kernel<TRA || MODE == LM_DW, TRB, 128, true, MODE == LM_DW>), grid, dim3(512), 0, st, g);
+  else hipLaunchKernelGGL((linear_small_kernel<TRA, TRB, 128, true, false>), grid, dim3(512), 0, st, g);
   if (d.slices > 1)
     hipLaunchKernelGGL(linear_slices_kernel, dim3((unsigned)cdiv((int64_t)g.nb * g.na / 4, (int64_t)256)), dim3(256), 0, st,
                        g.slices, d.slices, (int64_t)g.nb, g.na, g.bias, g.y, g.ldy);
@@ -577,7 +627,7 @@ int bias_parts(int64_t T, int64_t N) {
 int64_t linear_layout(int64_t T, int64_t N, int64_t K, int need_dx, int need_dw, int need_dbias, int64_t (&off)[3]) {
   int64_t at = 0;
   off[0] = at;
-  if (need_dw) at += up(K * up(T, 64) * 2, 256);
+  if (need_dw && !linear_codes(N, K, T)) at += up(K * up(T, 64) * 2, 256);
   off[1] = at;
   int64_t s = need_dx ? slice_bytes(LM_DX, K, T, N) : 0;
   if (need_dw) s = std::max(s, slice_bytes(LM_DW, K, N, T));
@@ -641,7 +691,7 @@ extern "C" int qmoe_linear_grad(const void* dy, int64_t lddy, int64_t T, int64_t
                                 int dbias_f32, void* workspace, int64_t ws_bytes, hipStream_t stream) {
   if (!linear_sizes_ok(T, N, K) || !dy || lddy < N || lddy % 8 || lddy >= kMaxPitch || !at16(dy)) return QMOE_ERR_ARG;
   if (dx && (!w || ldw < K || ldw % 8 || ldw >= kMaxPitch || !at16(w) || !at16(dx))) return QMOE_ERR_ARG;
-  if (dw && (!codes || !scales || reinterpret_cast<uintptr_t>(codes) % 8 || !at16(dw))) return QMOE_ERR_ARG;
+  if (dw && (!codes || !scales || !at16(codes) || !at16(dw))) return QMOE_ERR_ARG;
   int64_t off[3];
   const int64_t need = linear_layout(T, N, K, dx != nullptr, dw != nullptr, dbias != nullptr, off);
   if (need && (!workspace || ws_bytes < need)) return QMOE_ERR_WORKSPACE;
@@ -660,13 +710,19 @@ extern "C" int qmoe_linear_grad(const void* dy, int64_t lddy, int64_t T, int64_t
     launch_linear<LM_DX>(g, ws + off[1], stream);
   }
   if (dw) {
-    const int64_t Tw = up(T, 64);
-    uint16_t* xt = reinterpret_cast<uint16_t*>(ws + off[0]);
-    hipLaunchKernelGGL(linear_expand_kernel, dim3((unsigned)(Tw / 64), (unsigned)cdiv(K, (int64_t)64)), dim3(256), 0,
-                       stream, codes, scales, (int)T, (int)K, xt, Tw);
     LinearGemm g{};
-    g.a = reinterpret_cast<const uint8_t*>(xt);
-    g.lda = Tw * 2;
+    if (linear_codes(N, K, T)) {
+      g.a = codes;
+      g.lda = K;
+      g.scales = scales;
+    } else {
+      const int64_t Tw = up(T, 64);
+      uint16_t* xt = reinterpret_cast<uint16_t*>(ws + off[0]);
+      hipLaunchKernelGGL(linear_expand_kernel, dim3((unsigned)(Tw / 64), (unsigned)cdiv(K, (int64_t)64)), dim3(256), 0,
+                         stream, codes, scales, (int)T, (int)K, xt, Tw);
+      g.a = reinterpret_cast<const uint8_t*>(xt);
+      g.lda = Tw * 2;
+    }
     g.na = (int)K;
     g.b = static_cast<const uint8_t*>(dy);
     g.ldb = lddy * 2;
