@@ -634,12 +634,13 @@ int qmoe_pack_8bit(const void* x, int64_t ldx, int64_t T, int64_t K, uint8_t* co
 /*
  * A linear layer: y = x w^T + bias, bf16 [T][N], float32 sums and one rounding. x bf16
  * [T][ldx], w bf16 [N][ldw], bias f32 [N] or NULL; sizes and alignment as
- * qmoe_linear_grad. For many tokens; qmoe_gemm (QMOE_W16A16) has the streaming
- * kernels for few.
+ * qmoe_linear_grad. With codes (NULL: without) also the 8 bits of x, as
+ * qmoe_pack_8bit.
  */
 int qmoe_linear_workspace_size(int64_t T, int64_t N, int64_t K, int64_t* bytes);
 int qmoe_linear(const void* x, int64_t ldx, int64_t T, int64_t N, int64_t K, const void* w, int64_t ldw,
-                const float* bias, void* y, void* workspace, int64_t ws_bytes, qmoe_stream_t stream);
+                const float* bias, void* y, uint8_t* codes, uint8_t* scales, void* workspace, int64_t ws_bytes,
+                qmoe_stream_t stream);
 
 /*
  * Gradients of a linear layer y = x w^T + bias whose input waited in 8 bits:

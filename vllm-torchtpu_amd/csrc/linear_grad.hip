@@ -657,12 +657,16 @@ extern "C" int qmoe_linear_workspace_size(int64_t T, int64_t N, int64_t K, int64
 }
 
 extern "C" int qmoe_linear(const void* x, int64_t ldx, int64_t T, int64_t N, int64_t K, const void* w, int64_t ldw,
-                           const float* bias, void* y, void* workspace, int64_t ws_bytes, hipStream_t stream) {
+                           const float* bias, void* y, uint8_t* codes, uint8_t* scales, void* workspace,
+                           int64_t ws_bytes, hipStream_t stream) {
   if (!linear_sizes_ok(T, N, K) || !x || !w || !y || ldx < K || ldx % 8 || ldx >= kMaxPitch || ldw < K || ldw % 8 ||
       ldw >= kMaxPitch || !at16(x) || !at16(w) || !at16(y))
     return QMOE_ERR_ARG;
+  if (codes && (!scales || !at16(codes))) return QMOE_ERR_ARG;
   const int64_t need = slice_bytes(LM_FORWARD, N, T, K);
   if (need && (!workspace || ws_bytes < need)) return QMOE_ERR_WORKSPACE;
+  if (codes)
+    if (const int st = qmoe_pack_8bit(x, ldx, T, K, codes, scales, stream)) return st;
   LinearGemm g{};
   g.a = static_cast<const uint8_t*>(w);
   g.lda = ldw * 2;

@@ -302,7 +302,7 @@ def _load():
     lib.qmoe_linear_workspace_size.restype = ctypes.c_int
     lib.qmoe_linear_workspace_size.argtypes = [_i64, _i64, _i64, ctypes.POINTER(_i64)]
     lib.qmoe_linear.restype = ctypes.c_int
-    lib.qmoe_linear.argtypes = [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp]
+    lib.qmoe_linear.argtypes = [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp]
     lib.qmoe_linear_grad_workspace_size.restype = ctypes.c_int
     lib.qmoe_linear_grad_workspace_size.argtypes = [_i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                     ctypes.POINTER(_i64)]

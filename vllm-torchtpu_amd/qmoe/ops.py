@@ -1515,14 +1515,11 @@ def linear_checkpoint(x, weight, bias=None, keep=True):
         if T == 0:
             return torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev), codes, scales
         r, ld = _gemm_rows(x, K)
-        if keep:
-            check(lib.qmoe_pack_8bit(r.data_ptr(), ld, T, K, codes.data_ptr(), scales.data_ptr(), _raw_stream(dev)),
-                  "linear_checkpoint (8 bits)")
         y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
         b = _f32_flat(bias)
         ws, ws_n = _workspace(dev, _linear_bytes(T, N, K))
         check(lib.qmoe_linear(r.data_ptr(), ld, T, N, K, weight.data_ptr(), weight.stride(0), _addr(b), y.data_ptr(),
-                              _addr(ws), ws_n, _raw_stream(dev)), "linear_checkpoint")
+                              _addr(codes), _addr(scales), _addr(ws), ws_n, _raw_stream(dev)), "linear_checkpoint")
     return y, codes, scales
 
 
