@@ -83,7 +83,7 @@ struct ActParams {
   int64_t ldy;       // bytes
   uint8_t* codes;
   uint8_t* scales;
-  int64_t I;
+  int64_t T, I;
   int nb;  // blocks of 32 columns of g
   float p0, p1;
 };
@@ -118,10 +118,11 @@ __device__ __forceinline__ void get_codes(const ActParams& p, int64_t r2, uint32
   byte = p.scales[r2 * p.nb + i / 32];
 }
 
-// Workgroup (t, y): row t, threads y * blockDim.x .. of 8 columns each
+// Workgroup (t, y): row t (row_group), threads y * blockDim.x .. of 8 columns each
 template <int T, int ACT, bool AL>
 __global__ __launch_bounds__(512) void act_kernel(const ActParams p) {
-  const int64_t t = blockIdx.x, I = p.I;
+  const int64_t t = row_group(), I = p.I;
+  if (t >= p.T) return;
   const uint32_t i = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
   const uint8_t* x = p.x + t * p.ldx;
   float g[8] = {}, u[8] = {}, h[8];
@@ -142,7 +143,8 @@ __global__ __launch_bounds__(512) void act_kernel(const ActParams p) {
 
 template <int T, int ACT, bool AL>
 __global__ __launch_bounds__(512) void act_grad_kernel(const ActParams p) {
-  const int64_t t = blockIdx.x, I = p.I;
+  const int64_t t = row_group(), I = p.I;
+  if (t >= p.T) return;
   const uint32_t i = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
   if (i >= I) return;
   uint2 cg, cu;
@@ -166,7 +168,8 @@ __global__ __launch_bounds__(512) void act_grad_kernel(const ActParams p) {
 
 // Rows of bf16 -> 8 bits
 __global__ __launch_bounds__(512) void pack_kernel(const ActParams p) {
-  const int64_t t = blockIdx.x;
+  const int64_t t = row_group();
+  if (t >= p.T) return;
   const uint32_t i = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
   float v[8] = {};
   if (i < p.I) load8<RT_BF16, true>(p.x + t * p.ldx, i, p.I, v);
@@ -179,7 +182,7 @@ dim3 row_grid(int64_t T, int64_t I, dim3* block) {
   const int64_t n = cdiv<int64_t>(I, 32) * 4;
   const int64_t parts = cdiv<int64_t>(n, 512);
   block->x = (unsigned)(cdiv<int64_t>(cdiv<int64_t>(n, parts), 64) * 64);
-  return dim3((unsigned)T, (unsigned)cdiv<int64_t>(n, block->x));
+  return row_groups(T, (unsigned)cdiv<int64_t>(n, block->x));
 }
 
 template <typename F>
@@ -215,7 +218,7 @@ extern "C" int qmoe_act_checkpoint(const void* x, int64_t ldx, int type, int64_t
   if (!x || !h || T < 1 || T > kMaxRows || I < 1 || I > kMaxCols || (type != RT_BF16 && type != RT_F16) ||
       ldx < 2 * I || ldh < I || (codes && !scales))
     return QMOE_ERR_ARG;
-  const ActParams p{static_cast<const uint8_t*>(x), ldx * 2, static_cast<uint8_t*>(h), ldh * 2, codes, scales, I,
+  const ActParams p{static_cast<const uint8_t*>(x), ldx * 2, static_cast<uint8_t*>(h), ldh * 2, codes, scales, T, I,
                     (int)cdiv<int64_t>(I, 32), act_p0, act_p1};
   const bool al = I % 8 == 0 && al16(x, ldx * 2) && al16(h, ldh * 2) && reinterpret_cast<uintptr_t>(codes) % 8 == 0;
   dim3 block;
@@ -234,7 +237,7 @@ extern "C" int qmoe_act_checkpoint_grad(const uint8_t* codes, const uint8_t* sca
       (type != RT_BF16 && type != RT_F16) || lddh < I)
     return QMOE_ERR_ARG;
   const ActParams p{static_cast<const uint8_t*>(dh), lddh * 2, static_cast<uint8_t*>(dx), 4 * I,
-                    const_cast<uint8_t*>(codes), const_cast<uint8_t*>(scales), I, (int)cdiv<int64_t>(I, 32), act_p0,
+                    const_cast<uint8_t*>(codes), const_cast<uint8_t*>(scales), T, I, (int)cdiv<int64_t>(I, 32), act_p0,
                     act_p1};
   const bool al = I % 8 == 0 && al16(dh, lddh * 2) && al16(dx, 4 * I) && reinterpret_cast<uintptr_t>(codes) % 8 == 0;
   dim3 block;
@@ -251,7 +254,7 @@ extern "C" int qmoe_pack_8bit(const void* x, int64_t ldx, int64_t T, int64_t K, 
   if (!x || !codes || !scales || T < 1 || T > kMaxRows || K < 1 || K > kMaxCols || K % 8 || ldx < K ||
       !al16(x, ldx * 2) || reinterpret_cast<uintptr_t>(codes) % 8)
     return QMOE_ERR_ARG;
-  const ActParams p{static_cast<const uint8_t*>(x), ldx * 2, nullptr, 0, codes, scales, K, (int)cdiv<int64_t>(K, 32),
+  const ActParams p{static_cast<const uint8_t*>(x), ldx * 2, nullptr, 0, codes, scales, T, K, (int)cdiv<int64_t>(K, 32),
                     0.0f, 0.0f};
   dim3 block;
   const dim3 grid = row_grid(T, K, &block);

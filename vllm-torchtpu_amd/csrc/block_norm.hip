@@ -68,7 +68,7 @@ template <int YT, int RT, int C, int THREADS, bool AL>
 __global__ __launch_bounds__(THREADS) void block_residual_kernel(const qmoe_block_desc p) {
   __shared__ float red[2][8][16][1];
   const int W = blockDim.x >> 6;
-  const int64_t t = (int64_t)blockIdx.x * blockDim.y + own_row();
+  const int64_t t = row_group() * blockDim.y + own_row();
   const uint32_t H = (uint32_t)p.H;
   const double inv = 1.0 / (double)H;
   const bool row = t < p.T;
@@ -460,7 +460,7 @@ extern "C" int qmoe_block_residual(const qmoe_block_desc* p, hipStream_t stream)
       (p->next_weight && (!p->z || p->ldz < p->H)))
     return QMOE_ERR_ARG;
   const BlockShape s = block_shape(p->H, false);
-  const dim3 grid((unsigned)cdiv<int64_t>(p->T, s.rows)), block(64 * s.waves, s.rows);
+  const dim3 grid = row_groups(cdiv<int64_t>(p->T, s.rows)), block(64 * s.waves, s.rows);
   with_types(p->y_type, p->residual_type, s, wide(p), [&](auto yt, auto rt, auto c, auto th, auto al) {
     if constexpr (th() == 512 || c() == 2)  // (one piece and more than 8 wavefronts: the gradient's)
       hipLaunchKernelGGL((block_residual_kernel<yt(), rt(), c(), th(), al()>), grid, block, 0, stream, *p);

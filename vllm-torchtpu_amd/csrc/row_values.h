@@ -12,6 +12,15 @@ enum { RT_BF16 = 0, RT_F32 = 1, RT_F16 = 2 };
 
 QMOE_HD int rt_size(int t) { return t == RT_F32 ? 4 : 2; }
 
+// Workgroups of a launch with one for every (few) rows: blockIdx.x, and above 2^16 of
+// them blockIdx.z, since a launch takes less than 2^32 threads along an axis. The last
+// of z may lie behind the end.
+constexpr int64_t kRowGroups = 1 << 16;
+inline dim3 row_groups(int64_t n, unsigned y = 1) {
+  return dim3((unsigned)(n < kRowGroups ? n : kRowGroups), y, (unsigned)cdiv(n, kRowGroups));
+}
+__device__ __forceinline__ int64_t row_group() { return (int64_t)blockIdx.z * kRowGroups + blockIdx.x; }
+
 // The values as they lie in memory, to be loaded long before they are used
 template <int T>
 struct Raw8 {
