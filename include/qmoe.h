@@ -531,8 +531,8 @@ int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const void* w, i
  *   token_mask  : one byte per token, or NULL. A token outside it is routed, with
  *                 weights 0
  *   topk_weights: f32 [T][topk]; topk_ids i32 [T][topk]; loss f32 [1]; counts i32 [E]
- * 1 <= T <= 2^24, E <= 512. The sums' order is fixed. The workspace needs no
- * initialisation.
+ * 1 <= T <= 2^24, E <= 512. The sums' order is fixed. The workspace is 16-byte
+ * aligned and needs no initialisation.
  */
 int qmoe_moe_balance_workspace_size(int64_t T, int E, int64_t* bytes);
 int qmoe_moe_balance(const void* logits, int logits_f32, int64_t T, int E, int topk, int scoring, const float* bias,
@@ -584,10 +584,11 @@ int qmoe_block_residual(const qmoe_block_desc* d, qmoe_stream_t stream);
 
 /*
  * Its gradients, for those of h and z (either may be NULL). Outputs that are NULL
- * are not computed; d_y, d_residual and a per-element d_gate have contiguous rows,
+ * are not computed, and one whose operand is not there (d_next_weight: without
+ * g_z) is refused; d_y, d_residual and a per-element d_gate have contiguous rows,
  * and each output its operand's type. The sums over tokens are float32 in a
- * fixed order; the workspace (for weights and a gate per channel) needs no
- * initialisation.
+ * fixed order; the workspace (for weights and a gate per channel) is 16-byte
+ * aligned and needs no initialisation.
  */
 typedef struct qmoe_block_grads {
   const void* g_h; /* [T][ldgh] of residual_type */
@@ -627,6 +628,7 @@ int qmoe_act_checkpoint_grad(const uint8_t* codes, const uint8_t* scales, int64_
 
 /*
  * The 8 bits of bf16 rows x [T][ldx >= K]: codes [T][K], scales [T][ceil(K / 32)].
+ * K and ldx multiples of 8, x 16-byte aligned, codes 8-byte aligned.
  */
 int qmoe_pack_8bit(const void* x, int64_t ldx, int64_t T, int64_t K, uint8_t* codes, uint8_t* scales,
                    qmoe_stream_t stream);
@@ -646,12 +648,11 @@ int qmoe_linear(const void* x, int64_t ldx, int64_t T, int64_t N, int64_t K, con
  * Gradients of a linear layer y = x w^T + bias whose input waited in 8 bits:
  *   dx = dy w,  dw = dy^T x8,  dbias = sum over t of dy     (x8: the codes' values, K % 32 == 0, N % 8 == 0)
  *   dy  : bf16 [T][lddy]; w bf16 [N][ldw] (for dx); codes / scales of qmoe_pack_8bit
- *         (for dw); lddy and ldw multiples of 8, dy, w and codes
- *         16-byte aligned
+ *         (for dw); lddy and ldw multiples of 8 below 2^22
  *   dx  : bf16 [T][K]; dw bf16 [N][K]; dbias [N] bf16, or f32 with dbias_f32;
  *         each may be NULL
- * Sums are float32 in a fixed order. 1 <= T <= 2^20, N <= 2^18, K <= 2^16. The
- * workspace needs no initialisation.
+ * Matrices, codes and workspace are 16-byte aligned. Sums are float32 in a fixed
+ * order. 1 <= T <= 2^20, N <= 2^18, K <= 2^16. The workspace needs no initialisation.
  */
 int qmoe_linear_grad_workspace_size(int64_t T, int64_t N, int64_t K, int need_dx, int need_dw, int need_dbias,
                                     int64_t* bytes);

@@ -2,8 +2,10 @@
 the balanced router, without a GPU: nothing here launches a kernel."""
 
 import ctypes
-import re
 import os
+import re
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -179,3 +181,45 @@ def test_c_arguments():
         bad = list(lin)
         bad[i] = v
         assert lib.qmoe_linear_grad(*bad, at, n.value, None) == 1, i
+
+
+def test_c_outputs_without_operands_and_workspaces():
+    """outputs whose operand the call has not, and workspaces that the kernels' 16-byte
+    accesses do not take"""
+    lib, n = _capi.lib, ctypes.c_int64(0)
+    at = 0x1000
+
+    def grads(desc, **kw):
+        d, g = _capi.BlockDesc(), _capi.BlockGrads()
+        for k, v in dict(T=4, H=64, y=at, ldy=64, h=at, ldh=64, rstd_y=at, rstd_h=at, residual_scale=1.0, scale=1.0,
+                         eps=1e-6, **desc).items():
+            setattr(d, k, v)
+        for k, v in dict(g_h=at, ldgh=64, **kw).items():
+            setattr(g, k, v)
+        return ctypes.byref(d), ctypes.byref(g)
+
+    for desc, out in ((dict(next_weight=at, post_weight=at), dict(d_next_weight=at, d_post_weight=at)),
+                      (dict(next_weight=at), dict(d_post_weight=at)), (dict(post_weight=at), dict(d_gate=at))):
+        assert lib.qmoe_block_residual_grad(*grads(desc, **out), at, 1 << 20, None) == 1
+    d, g = grads(dict(next_weight=at), g_z=at, ldgz=64, d_y=at)
+    d._obj.y = None
+    assert lib.qmoe_block_residual_grad(d, g, at, 1 << 20, None) == 1
+    d, g = grads(dict(post_weight=at), d_post_weight=at)
+    assert lib.qmoe_block_residual_grad(d, g, at + 8, 1 << 20, None) == 2
+    assert lib.qmoe_moe_balance_workspace_size(5000, 64, ctypes.byref(n)) == 0
+    assert lib.qmoe_moe_balance(at, 1, 5000, 64, 4, 0, None, 1, 1.0, 1, 1, None, at, at, at, at, at + 4, n.value, None) == 2
+    assert lib.qmoe_linear_grad_workspace_size(1000, 256, 64, 1, 1, 1, ctypes.byref(n)) == 0 and n.value > 0
+    assert lib.qmoe_linear_grad(at, 256, 1000, 256, 64, at, 64, at, at, at, at, at, 0, at + 8, n.value, None) == 2
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not available")
+@pytest.mark.parametrize("cname,cls", [("qmoe_block_desc", _capi.BlockDesc), ("qmoe_block_grads", _capi.BlockGrads)])
+def test_structures_have_the_c_layout(tmp_path, cname, cls):
+    names = [f for f, *_ in cls._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "qmoe.h"\nint main(void) {\n'
+                   + f'printf("%zu", sizeof({cname}));\n'
+                   + "".join(f'printf(" %zu", offsetof({cname}, {f}));\n' for f in names) + "return 0;\n}\n")
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "layout")], check=True)
+    out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()
+    assert [int(v) for v in out] == [ctypes.sizeof(cls)] + [getattr(cls, f).offset for f in names]

@@ -478,6 +478,10 @@ extern "C" int qmoe_block_residual_grad(const qmoe_block_desc* p, const qmoe_blo
                                         int64_t ws_bytes, hipStream_t stream) {
   if (const int st = check(p)) return st;
   if (!d || (!d->g_h && !d->g_z) || (d->g_z && !p->next_weight)) return QMOE_ERR_ARG;
+  // (outputs of operands that are not there, or that no gradient reaches)
+  if ((d->d_next_weight && !d->g_z) || (d->d_y && !p->y) || (d->d_gate && !p->gate_kind) ||
+      (d->d_post_weight && !p->post_weight))
+    return QMOE_ERR_ARG;
   const bool next = d->g_z != nullptr, post = p->y && p->post_weight;
   if (next && (!p->h || p->ldh < p->H || !p->rstd_h || d->ldgz < p->H)) return QMOE_ERR_ARG;
   if (post && !p->rstd_y) return QMOE_ERR_ARG;
@@ -486,10 +490,10 @@ extern "C" int qmoe_block_residual_grad(const qmoe_block_desc* p, const qmoe_blo
                     (p->gate_kind == GATE_CHANNEL && d->d_gate);
   const BlockShape s = block_shape(p->H, true);
   const int groups = grad_groups(p->T, s);
-  if (sums && (!workspace || ws_bytes < (int64_t)groups * 2 * p->H * 4)) return QMOE_ERR_WORKSPACE;
+  if (sums && (!aligned16(workspace, 0, 1) || !workspace || ws_bytes < (int64_t)groups * 2 * p->H * 4)) return QMOE_ERR_WORKSPACE;
   const int ys = rt_size(p->y_type), rs = rt_size(p->residual_type);
   const bool al = wide(p) && aligned16(d->g_h, d->ldgh, rs) && aligned16(d->g_z, d->ldgz, ys) &&
-                  aligned16(d->d_y, p->H, ys) && aligned16(d->d_residual, p->H, rs) && aligned16(workspace, 0, 1) &&
+                  aligned16(d->d_y, p->H, ys) && aligned16(d->d_residual, p->H, rs) &&
                   (p->gate_kind != GATE_FULL || aligned16(d->d_gate, p->H, ys));
   const dim3 block(64 * s.waves, s.rows);
   float* parts = sums ? static_cast<float*>(workspace) : nullptr;

@@ -10,8 +10,8 @@ namespace {
 
 __device__ __align__(16) const uint32_t kZeroChunk[4] = {0, 0, 0, 0};
 
-// How an operand across K, rows of 256 or BM columns, passes
-// through LDS. ds_read_b64_tr_b16: lane 4 r + c of 16 gives the address of row r's
+// How an operand across K, rows of 256 or BM columns, passes through LDS.
+// ds_read_b64_tr_b16: lane 4 r + c of 16 gives the address of row r's
 // elements 4 c .. + 3, lane i receives column i of the 4 rows. An MFMA operand is
 // two of them (k + 4) per lane; the 4 rows of an access lie in different 64-byte
 // blocks, for which the 16-byte chunk c of row k is stored at c ^ tr_swz.

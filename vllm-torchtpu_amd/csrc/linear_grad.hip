@@ -43,7 +43,7 @@ struct LinearGemm {
 };
 
 // B row t of the 64 that a round holds, A row n of it at n ^ vg_row_swz(t): 8
-// consecutive A rows per thread and store. 74 KB of LDS that no copy or read uses.
+// consecutive A rows per thread and store. 64 KB of LDS, once no copy or read uses it.
 template <int THREADS, int NI, int MJ>
 __device__ __forceinline__ void linear_epilogue(const LinearGemm& p, f32x16 (&acc)[NI][MJ], uint8_t* smem, int n0, int m0,
                                                 int arows, int brows, int wn, int wm) {
@@ -664,7 +664,7 @@ extern "C" int qmoe_linear(const void* x, int64_t ldx, int64_t T, int64_t N, int
     return QMOE_ERR_ARG;
   if (codes && (!scales || !at16(codes))) return QMOE_ERR_ARG;
   const int64_t need = slice_bytes(LM_FORWARD, N, T, K);
-  if (need && (!workspace || ws_bytes < need)) return QMOE_ERR_WORKSPACE;
+  if (need && (!workspace || !at16(workspace) || ws_bytes < need)) return QMOE_ERR_WORKSPACE;
   if (codes)
     if (const int st = qmoe_pack_8bit(x, ldx, T, K, codes, scales, stream)) return st;
   LinearGemm g{};
@@ -698,7 +698,7 @@ extern "C" int qmoe_linear_grad(const void* dy, int64_t lddy, int64_t T, int64_t
   if (dw && (!codes || !scales || !at16(codes) || !at16(dw))) return QMOE_ERR_ARG;
   int64_t off[3];
   const int64_t need = linear_layout(T, N, K, dx != nullptr, dw != nullptr, dbias != nullptr, off);
-  if (need && (!workspace || ws_bytes < need)) return QMOE_ERR_WORKSPACE;
+  if (need && (!workspace || !at16(workspace) || ws_bytes < need)) return QMOE_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   if (dx) {
     LinearGemm g{};

@@ -385,7 +385,7 @@ extern "C" int qmoe_moe_balance(const void* logits, int logits_f32, int64_t T, i
   BalanceParams p{logits, logits_f32, T, E, topk, bias, renormalize, routed_scaling_factor, num_group, topk_group,
                   token_mask, topk_weights, topk_ids, loss, counts, nullptr, nullptr, nullptr, nullptr};
   if (groups > 1) {
-    if (!workspace || ws_bytes < balance_bytes(T, E)) return QMOE_ERR_WORKSPACE;
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || ws_bytes < balance_bytes(T, E)) return QMOE_ERR_WORKSPACE;
     p.ticket = static_cast<uint32_t*>(workspace);
     p.sum_p = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 256);
     p.part_p = p.sum_p + E;

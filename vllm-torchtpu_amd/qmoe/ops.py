@@ -1379,7 +1379,7 @@ def block_grad_run(d, g_h, ldgh, g_z, ldgz, y, h, gate, post, nxt, need):
     dp = post.new_empty(post.shape) if need[3] and post is not None else None
     dn = nxt.new_empty(nxt.shape) if need[4] and g_z is not None else None
     ws, n = None, 0
-    if dp is not None or dn is not None or dg is not None:
+    if dp is not None or dn is not None or (dg is not None and d.gate_kind == 1):
         n = _block_grad_bytes(d.T, d.H)
         ws = h.new_empty(n, dtype=torch.uint8)
     g = _capi.BlockGrads(None if g_h is None else g_h.data_ptr(), ldgh, None if g_z is None else g_z.data_ptr(), ldgz,
