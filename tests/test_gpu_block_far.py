@@ -76,6 +76,32 @@ def test_linear(dev):
     assert not dx[:-LAST].any()
 
 
+# tiles of more than one for every CU, with ragged ends: of 256 and of 192 rows along K,
+# across it in the input's gradient, and in the weight's
+@pytest.mark.parametrize("T,K,N,bias", [(4072, 512, 4104, True), (3000, 512, 8200, False), (3000, 512, 8200, True),
+                                        (4072, 4128, 512, False), (3000, 8224, 512, True), (2048, 5152, 5128, False)])
+def test_linear_of_many_tiles(dev, T, K, N, bias):
+    """sums of K, N and T products in float32, one rounding to bf16; what is read behind
+    each matrix is its own, so that a wrong place shows"""
+    g = torch.Generator(device=dev).manual_seed(T + K + N)
+    x, dy = (torch.randn((T, n), generator=g, device=dev).to(BF16) for n in (K, N))
+    w = (0.05 * torch.randn((N, K), generator=g, device=dev)).to(BF16)
+    b = torch.randn(N, generator=g, device=dev) if bias else None
+    leaves = [t.detach().requires_grad_() for t in ((x, w, b) if bias else (x, w))]
+    y = checkpointed_linear(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy)
+    _, codes, scales = ops.linear_checkpoint(x, w)
+    x8 = (codes.view(torch.float8_e4m3fn).to(F64).view(T, K // 32, 32) * torch.exp2(scales.to(F64) - 127)[..., None]).view(T, K)
+    gd, xd, wd = dy.to(F64), x.to(F64), w.to(F64)
+    for got, p, q, n, plus in ((y.detach(), xd, wd.t(), K, b), (grads[0], gd, wd, N, None), (grads[1], gd.t(), x8, T, None)):
+        ref, mag = p @ q, p.abs() @ q.abs()
+        if plus is not None:
+            ref, mag = ref + plus, mag + plus.abs()
+        assert ((got.to(F64) - ref).abs() <= 2.0 ** -8 * ref.abs() + (n + 8) * 2.0 ** -24 * mag).all()
+    for g1, g2 in zip(grads, torch.autograd.grad(checkpointed_linear(*leaves), leaves, dy)):
+        assert torch.equal(g1, g2)
+
+
 def test_balance(dev):
     T, E, k = (1 << 23) + LAST, 264, 4
     assert T * E > 1 << 31

@@ -5,13 +5,16 @@
 // What bounds it: two products of 2 T N K operations on the bf16 matrix cores, or,
 // for few tokens, one read of w and one write of dw. The 8-bit values' scales
 // change along the summed axis, so the codes are multiplied as bf16 (exact: 4 of
-// its 8 significant bits), expanded and transposed once on the way to dw.
+// its 8 significant bits): of up to 512 tokens by the tiles themselves, of more expanded
+// and transposed once on the way to dw (4096 x 4096: 14 us).
 //
-// Both products are the same tile: 256 "A" rows x BM "B" rows of a workgroup, a
+// The products (the layer's own among them) are the same tile: 256 "A" rows x BM "B" rows of a workgroup, a
 // ring of LDS stages of 64 k filled by direct copies, and one operand that lies
 // across K (gemm_across.h):
 //   dx : A = columns of w (across), B = rows of dy
-//   dw : A = columns of x8 (rows of its transpose, padded with zeros to 64 k), B = columns of dy (across)
+//   dw : A = columns of x8 (rows of its transpose, padded with zeros to 64 k, or codes across K), B = columns
+//        of dy (across)
+//   y  : A = rows of w, B = rows of x (neither across)
 // The last stage copies zeros where K has ended. Sums are float32; a K axis that
 // is long for the number of tiles is cut into slices, added in order.
 
@@ -24,6 +27,8 @@
 namespace {
 
 constexpr int kAN = 256;  // A rows of a tile
+
+QMOE_HD int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 struct LinearGemm {
   const uint8_t* a;  // rows along K [na][lda bytes], or across it [K][lda]
@@ -102,7 +107,9 @@ __device__ __forceinline__ void linear_slice(LinearGemm& p) {
 }
 
 // Tiles of 256 x BM (64 or 128) by eight wavefronts. ONE: a stage at a time,
-// without a ring, so that two workgroups share a CU. CODES: the A operand is x8
+// without a ring, so that two workgroups share a CU. 777 tokens, 4096 x 4096: 64 rows,
+// forward / dx 40.2 / 43.9 us (26 and 24 % of the matrix cores' cycles: 208 tiles of 256
+// CUs, and LDS feeds a wavefront of 64 x 32), dw without a ring 30. CODES: the A operand is x8
 // itself, codes and scale bytes across K, expanded on the way to LDS (a thread 32
 // columns of a row): no transposed copy of x8 before the product, whose launch and
 // bytes count where the sums are short.
@@ -292,6 +299,58 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
   linear_epilogue<512, NI, MJ>(p, acc, smem, n0, m0, arows, brows, wn, wm);
 }
 
+// The same without slices in 32 KB of LDS (at `region`), waiting for none of the copies
+// that are in flight to the rest of it: a round takes 64 B rows of two of a wavefront's
+// four blocks, row t's float n at n ^ 4 (t & 31), and leaves 128 bytes of each row.
+template <int NI, int MJ>
+__device__ __forceinline__ void linear_rows(const LinearGemm& p, f32x16 (&acc)[NI][MJ], uint8_t* region, int n0, int m0,
+                                            int arows, int brows, int wn, int wm) {
+  static_assert(NI == 4, "two halves");
+  const int tid = threadIdx.x, lane = tid & 63, rl = lane & 31, kh = lane >> 5;
+  float* reg = reinterpret_cast<float*>(region);  // [64][128]
+  float* to = reg + (wm * 32 + rl) * 128;
+  const int c = (tid & 15) * 8, t0 = tid >> 4, n = (c >> 6) * 128 + (c & 63);
+  uint16_t* y = p.y + (int64_t)(m0 + t0) * p.ldy + n0 + n;
+  float bias[2][8] = {};
+  if (p.bias) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (n + 64 * h < arows)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) bias[h][k] = p.bias[n0 + n + 64 * h + k];
+  }
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) {
+    if (64 * j >= brows) break;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (j || h) stage_barrier();  // the rows before have been read
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x16& v = acc[2 * h + i][j];
+          *reinterpret_cast<float4*>(to + ((wn * 64 + i * 32 + q * 8 + kh * 4) ^ (4 * rl))) =
+              make_float4(v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]);
+        }
+      stage_barrier();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = t0 + 16 * k;
+        if (64 * j + t < brows && n + 64 * h < arows) {  // (A rows come in multiples of 8)
+          const float4 lo = *reinterpret_cast<const float4*>(reg + t * 128 + (c ^ (4 * (t & 31))));
+          const float4 hi = *reinterpret_cast<const float4*>(reg + t * 128 + ((c + 4) ^ (4 * (t & 31))));
+          const float* b = bias[h];
+          *reinterpret_cast<uint4*>(y + (int64_t)(64 * j + 16 * k) * p.ldy + 64 * h) =
+              make_uint4(pack_bf16(lo.x + b[0], lo.y + b[1]), pack_bf16(lo.z + b[2], lo.w + b[3]),
+                         pack_bf16(hi.x + b[4], hi.y + b[5]), pack_bf16(hi.z + b[6], hi.w + b[7]));
+        }
+      }
+    }
+  }
+  stage_barrier();  // the last rows have been read
+}
+
 // The same products in tiles of 256 x BM (256 or 192) by four wavefronts of 4 x
 // BM / 64 blocks, one per SIMD, the sums in accumulation registers: a wavefront of
 // 128 x 128 reads 32 KB of operands from LDS per 64 MFMAs where one of 64 x 64
@@ -302,8 +361,16 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
 // stage s every wavefront holds its last operands, and the stage's two slots
 // take B(s + 2) and A(s + 3). The copies go out four per MFMA step, one at a time
 // between the MFMAs.
+// A workgroup goes on to the tile gridDim.x further: its first stages follow the
+// last of the tile before in the ring, so that they are there when that tile's results
+// have been stored (of two stages and more; one of a single stage has a tile only).
+// 4096 tokens, 4096 x 28672, seven tiles each: forward 727 us (755 with a workgroup per
+// tile) = 1323 TFLOP/s, dw 729 (740); one tile each, dx 709 = 1357 TFLOP/s. The matrix
+// cores are busy for 70 to 75 % of the cycles, and the clock falls with more. Results
+// stored straight from the registers, 64 bytes of a row at a time, cost 838 where rows
+// lie a multiple of 4 KB apart.
 // TAIL: K is not a multiple of 64 (an instance of its own: the extra stage costs
-// the others registers).
+// the others registers), a tile per workgroup.
 template <bool TRA, bool TRB, int BM, bool TAIL>
 __global__ __launch_bounds__(256, 1) void linear_big_kernel(const LinearGemm args) {
   constexpr int NI = 4, MJ = BM / 64, AI = 8, BI = 2 * MJ;  // a wavefront's copies of A and B per stage
@@ -317,27 +384,39 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(const LinearGemm arg
   linear_slice<TRA, TRB>(p);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave & 1, wm = wave >> 1, rl = lane & 31, kh = lane >> 5;
-  int mt, nt;
-  if (!tile_dense(blockIdx.x, p.m_tiles, p.n_tiles, mt, nt)) return;
-  const int n0 = nt * kAN, m0 = mt * BM;
-  const int arows = min(kAN, p.na - n0), brows = min(BM, p.nb - m0);
+  struct Tile {
+    int n0, m0, arows, brows;
+    const uint8_t *a, *b;
+  };
+  const int tiles = (int)up(p.m_tiles * p.n_tiles, kXcds);
+  auto tile_of = [&](int b, Tile& t) {
+    int mt, nt;
+    if (b >= tiles || !tile_dense(b, p.m_tiles, p.n_tiles, mt, nt)) return false;
+    t.n0 = nt * kAN;
+    t.m0 = mt * BM;
+    t.arows = min(kAN, p.na - t.n0);
+    t.brows = min(BM, p.nb - t.m0);
+    t.a = TRA ? p.a + t.n0 * 2 : p.a + (int64_t)t.n0 * p.lda;
+    t.b = TRB ? p.b + t.m0 * 2 : p.b + (int64_t)t.m0 * p.ldb;
+    return true;
+  };
+  int block = blockIdx.x;
+  Tile cur, nxt;
+  if (!tile_of(block, cur)) return;
 
   // copies as in the kernel above; wavefront w moves the groups w, w + 4, ...
   const int chunk = (lane & 7) ^ ((lane >> 3) ^ (wave & 1));
   const int trow = lane / TL, tchunk = (lane % TL) ^ tr_swz<TB>(2 * wave + trow);
-  const uint32_t tcol = (uint32_t)min(tchunk, (TRA ? arows : brows) / 8 - 1) * 16;
-  const uint8_t* abase = TRA ? p.a + n0 * 2 : p.a + (int64_t)n0 * p.lda;
-  const uint8_t* bbase = TRB ? p.b + m0 * 2 : p.b + (int64_t)m0 * p.ldb;
   const int64_t astep = TRA ? 64 * p.lda : 128, bstep = TRB ? 64 * p.ldb : 128;
   uint32_t aoff[AI], boff[BI];
+  auto place = [&](bool across, int j, int rows, int64_t ld) {
+    if (across) return (uint32_t)(2 * (wave + 4 * j) + trow) * (uint32_t)ld + (uint32_t)min(tchunk, rows / 8 - 1) * 16;
+    return (uint32_t)min((wave + 4 * j) * 8 + (lane >> 3), rows - 1) * (uint32_t)ld + chunk * 16;
+  };
 #pragma unroll
-  for (int j = 0; j < AI; ++j)
-    aoff[j] = TRA ? (uint32_t)(2 * (wave + 4 * j) + trow) * (uint32_t)p.lda + tcol
-                  : (uint32_t)min((wave + 4 * j) * 8 + (lane >> 3), arows - 1) * (uint32_t)p.lda + chunk * 16;
+  for (int j = 0; j < AI; ++j) aoff[j] = place(TRA, j, cur.arows, p.lda);
 #pragma unroll
-  for (int j = 0; j < BI; ++j)
-    boff[j] = TRB ? (uint32_t)(2 * (wave + 4 * j) + trow) * (uint32_t)p.ldb + tcol
-                  : (uint32_t)min((wave + 4 * j) * 8 + (lane >> 3), brows - 1) * (uint32_t)p.ldb + chunk * 16;
+  for (int j = 0; j < BI; ++j) boff[j] = place(TRB, j, cur.brows, p.ldb);
   const int KF = p.K / 64, tail = p.K % 64;
   const uint32_t cw = lds0 + wave * 1024;
   union B8 {
@@ -362,64 +441,102 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(const LinearGemm arg
           *reinterpret_cast<const uint4*>(smem + slot + xpo + j * 8192 + ((2 * q + kh) ^ vg_swz(rl)) * 16);
   };
   f32x16 acc[NI][MJ];
+  // (by a product of zeros: sums set to zero one register at a time pass through others)
+  auto clear = [&]() {
+    bf16x8 no = {};
+    const f32x16 zero = {};
 #pragma unroll
-  for (int i = 0; i < NI; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-    for (int j = 0; j < MJ; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+      for (int j = 0; j < MJ; ++j) {
+        asm volatile("" : "+v"(no));  // (one product each: one for all would be copied)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(no, no, zero, 0, 0, 0);
+      }
+  };
   auto mma_row = [&](int q, int i) {
 #pragma unroll
     for (int j = 0; j < MJ; ++j)
       acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[q & 1][i].v, xf[q & 1][j].v, acc[i][j], 0, 0, 0);
   };
-  if (KF > 0) {
-    // (stages past the last whole one copy it again, into slots nobody reads)
-    auto asrc = [&](int s) { return uniform_ptr(abase + min(s, KF - 1) * astep); };
-    auto bsrc = [&](int s) { return uniform_ptr(bbase + min(s, KF - 1) * bstep); };
+  if constexpr (TAIL) clear();
+  if (!TAIL || KF > 0) {
+    bool more = !TAIL && KF > 1 && tile_of(block + gridDim.x, nxt);
     auto dst = [&](uint32_t slot) { return (uint32_t)__builtin_amdgcn_readfirstlane(cw + slot); };
-    auto wrap = [](uint32_t slot) { return slot >= RING ? slot - RING : slot; };
+    const uint8_t *a2 = uniform_ptr(cur.a), *b1 = uniform_ptr(cur.b), *b2;
 #pragma unroll
-    for (int j = 0; j < AI; ++j) lds_copy16(asrc(0), aoff[j], dst(0) + j * 4096);
+    for (int j = 0; j < AI; ++j) lds_copy16(a2, aoff[j], dst(0) + j * 4096);
 #pragma unroll
-    for (int j = 0; j < BI; ++j) lds_copy16(bsrc(0), boff[j], dst(SLOT) + j * 4096);
+    for (int j = 0; j < BI; ++j) lds_copy16(b1, boff[j], dst(SLOT) + j * 4096);
+    if (KF > 1) {
+      a2 += astep;
+      b1 += bstep;
+    }
 #pragma unroll
-    for (int j = 0; j < AI; ++j) lds_copy16(asrc(1), aoff[j], dst(2 * SLOT) + j * 4096);
+    for (int j = 0; j < AI; ++j) lds_copy16(a2, aoff[j], dst(2 * SLOT) + j * 4096);
 #pragma unroll
-    for (int j = 0; j < BI / 2; ++j) lds_copy16(bsrc(1), boff[j], dst(3 * SLOT) + j * 4096);
+    for (int j = 0; j < BI / 2; ++j) lds_copy16(b1, boff[j], dst(3 * SLOT) + j * 4096);
+    a2 += astep;
+    b2 = b1 + bstep;
     wait_copies_upto<AI + BI / 2>();  // the first stage
     stage_barrier();
     read_w(0, 0);
     read_x(SLOT, 0);
-    uint32_t sa = 0;  // slot of A(s); B(s), A(s + 1), ... follow
-    for (int s = 0; s < KF; ++s) {
-      const uint32_t sb = wrap(sa + SLOT), sa1 = wrap(sa + 2 * SLOT), sb1 = wrap(sa + 3 * SLOT), sa2 = wrap(sa + 4 * SLOT);
-      const uint8_t *b1 = bsrc(s + 1), *a2 = asrc(s + 2), *b2 = bsrc(s + 2);
-      const uint32_t db1 = dst(sb1) + BI / 2 * 4096, da2 = dst(sa2), db2 = dst(sa);
+    uint32_t sa = 0, sb = SLOT, sa1 = 2 * SLOT, sb1 = 3 * SLOT, sa2 = 4 * SLOT;  // slots of A(s), B(s), A(s + 1), ...
+    for (;;) {
+      if constexpr (!TAIL) clear();
+      for (int s = 0; s < KF; ++s) {
+        if (s + 2 >= KF) {  // the next tile's stages; without one the last again, into slots nobody reads
+          if (!more) {
+            a2 -= astep;
+            b2 -= bstep;
+          } else if (s + 2 == KF) {
+            a2 = uniform_ptr(nxt.a);
+            b2 = uniform_ptr(nxt.b);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (q == 3) {
-          wait_copies_upto<AI>();  // stage s + 1 has landed
-          stage_barrier();         // and everybody holds this stage's last operands
-        }
+            for (int j = 0; j < AI; ++j) aoff[j] = place(TRA, j, nxt.arows, p.lda);
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          if (i == 0) read_w(q < 3 ? sa : sa1, (q + 1) & 3);
-          if (i == 1) read_x(q < 3 ? sb : sb1, (q + 1) & 3);
-          if (q == 1 || q == 2) lds_copy16(a2, aoff[4 * (q - 1) + i], da2 + (4 * (q - 1) + i) * 4096);
-          else if (i < BI / 2 && q == 0) lds_copy16(b1, boff[BI / 2 + i], db1 + i * 4096);
-          else if (i < BI / 2) lds_copy16(b2, boff[i], db2 + i * 4096);
-          mma_row(q, i);
-          __builtin_amdgcn_sched_barrier(0);
+            for (int j = 0; j < BI / 2; ++j) boff[j] = place(TRB, j, nxt.brows, p.ldb);
+          } else {
+#pragma unroll
+            for (int j = BI / 2; j < BI; ++j) boff[j] = place(TRB, j, nxt.brows, p.ldb);
+          }
         }
+        const uint32_t db1 = dst(sb1) + BI / 2 * 4096, da2 = dst(sa2), db2 = dst(sa);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (q == 3) {
+            wait_copies_upto<AI>();  // stage s + 1 has landed
+            stage_barrier();         // and everybody holds this stage's last operands
+          }
+#pragma unroll
+          for (int i = 0; i < NI; ++i) {
+            if (i == 0) read_w(q < 3 ? sa : sa1, (q + 1) & 3);
+            if (i == 1) read_x(q < 3 ? sb : sb1, (q + 1) & 3);
+            if (q == 1 || q == 2) lds_copy16(a2, aoff[4 * (q - 1) + i], da2 + (4 * (q - 1) + i) * 4096);
+            else if (i < BI / 2 && q == 0) lds_copy16(b1, boff[BI / 2 + i], db1 + i * 4096);
+            else if (i < BI / 2) lds_copy16(b2, boff[i], db2 + i * 4096);
+            mma_row(q, i);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        a2 += astep;
+        b1 = b2;
+        b2 += bstep;
+        const uint32_t s0 = sa, s1 = sb;
+        sa = sa1, sb = sb1, sa1 = sa2, sb1 = s0, sa2 = s1;
       }
-      sa = sa1;
+      if (TAIL || !more) wait_copies_upto<0>();
+      if (TAIL || p.kslice) break;
+      linear_rows<NI, MJ>(p, acc, smem + sa2, cur.n0, cur.m0, cur.arows, cur.brows, wn, wm);  // (A(s + 2)'s slot is free)
+      if (!more) return;
+      cur = nxt;
+      block += gridDim.x;
+      more = tile_of(block + gridDim.x, nxt);
     }
-    wait_copies_upto<0>();
     __syncthreads();
   }
   if constexpr (TAIL) {  // the last, partial stage, with zeros where K has ended
-    const uint8_t *as = abase + KF * astep, *bs = bbase + KF * bstep, *z = reinterpret_cast<const uint8_t*>(kZeroChunk);
+    const uint8_t *as = cur.a + KF * astep, *bs = cur.b + KF * bstep, *z = reinterpret_cast<const uint8_t*>(kZeroChunk);
 #pragma unroll
     for (int j = 0; j < AI; ++j)
       lds_copy16((TRA ? 2 * (wave + 4 * j) + trow : chunk * 8) < tail ? as + aoff[j] : z,
@@ -439,7 +556,7 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(const LinearGemm arg
     }
     __syncthreads();
   }
-  linear_epilogue<256, NI, MJ>(p, acc, smem, n0, m0, arows, brows, wn, wm);
+  linear_epilogue<256, NI, MJ>(p, acc, smem, cur.n0, cur.m0, cur.arows, cur.brows, wn, wm);
 }
 
 // The K slices -> bf16 rows
@@ -533,8 +650,6 @@ __global__ __launch_bounds__(256) void linear_bias_join_kernel(const float* part
 
 // ---------------------------------------------------------------- launches
 
-int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
-
 // Which operand of a product lies across K
 enum LinearMode { LM_FORWARD = 0, LM_DX = 1, LM_DW = 2 };
 
@@ -546,9 +661,9 @@ struct LinearPlan {
 // The least time of a model: rounds of the tiles on the chip times (stages times
 // a stage's time + the rest of a tile), and for K slices their sums' way to memory
 // and back. Times from sweeps of every tile and 1 to 16 slices over 16 sizes (1 to
-// 8192 tokens, 256 x 1024 to 4096 x 28672); the plan's own time was within 5 % of
-// the best of the sweep for most, 14 % at most. Both sides, us: 4096 tokens x 4096 x
-// 28672 forward / dx / dw tiles of 256 723 / 676 / 734, of 128 887 / 816 / 875;
+// 8192 tokens, 256 x 1024 to 4096 x 28672), with a workgroup per tile; the plan's own time
+// was within 5 % of the best of the sweep for most, 14 % at most. Both sides, us: 4096
+// tokens x 4096 x 28672 forward / dx / dw tiles of 256 723 / 676 / 734, of 128 887 / 816 / 875;
 // 777 x 4096 x 4096 dx 64 rows 38.5, 128 rows in 2 slices 42; dw without a ring 36.9,
 // 256 rows 39.3; 333 x 2880 x 5760 dx 128 rows in 6 slices 28.8, 64 in 3 39.
 LinearPlan linear_plan(int mode, int64_t na, int64_t nb, int64_t K) {
@@ -585,8 +700,10 @@ LinearPlan linear_plan(int mode, int64_t na, int64_t nb, int64_t K) {
 // x 4096 x 4096 42.7 (38.9), 1500 x 14336 x 4096 235 (180).
 bool linear_codes(int64_t N, int64_t K, int64_t T) { return T <= 512 && linear_plan(LM_DW, K, N, T).bm == 1; }
 
+// (several tiles per workgroup where no K slice is a single stage)
 template <bool TRA, bool TRB, int BM>
 void launch_big(const LinearGemm& g, dim3 grid, hipStream_t st) {
+  if (g.K % 64 == 0 && grid.y == 1 && g.K > 64 && grid.x > 256) grid.x = 256;
   if (g.K % 64) hipLaunchKernelGGL((linear_big_kernel<TRA, TRB, BM, true>), grid, dim3(256), 0, st, g);
   else hipLaunchKernelGGL((linear_big_kernel<TRA, TRB, BM, false>), grid, dim3(256), 0, st, g);
 }
