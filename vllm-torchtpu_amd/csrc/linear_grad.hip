@@ -8,9 +8,9 @@
 // its 8 significant bits): of up to 512 tokens by the tiles themselves, of more expanded
 // and transposed once on the way to dw (4096 x 4096: 14 us).
 //
-// The products (the layer's own among them) are the same tile: 256 "A" rows x BM "B" rows of a workgroup, a
-// ring of LDS stages of 64 k filled by direct copies, and one operand that lies
-// across K (gemm_across.h):
+// The products (the layer's own among them) are the same tile: 256 "A" rows x BM "B"
+// rows of a workgroup, a ring of LDS stages of 64 k filled by direct copies, and for
+// the gradients an operand that lies across K (gemm_across.h):
 //   dx : A = columns of w (across), B = rows of dy
 //   dw : A = columns of x8 (rows of its transpose, padded with zeros to 64 k, or codes across K), B = columns
 //        of dy (across)

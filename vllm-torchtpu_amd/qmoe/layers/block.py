@@ -76,7 +76,7 @@ class _Block(torch.autograd.Function):
         saved = (y, residual if y is None else h, gate, norm_weight, next_weight, rstd)
         ctx.save_for_backward(*saved)
         ctx.args = args
-        ctx.desc = None if desc is None else ops.block_saved(desc, *saved)
+        ctx.run = None if desc is None else ops.block_saved(desc, *saved)
         ctx.set_materialize_grads(False)
         return h, z
 
@@ -91,8 +91,8 @@ class _Block(torch.autograd.Function):
         if g_h is None and g_z is None:
             return (None,) * 6
         saved, need = ctx.saved_tensors, ctx.needs_input_grad[:5]
-        if ctx.desc is not None and (g_h is None or ops.plain_grad(g_h)) and (g_z is None or ops.plain_grad(g_z)):
-            grads = ops.block_grad_plain(ctx.desc, g_h, g_z, *saved, need)
+        if ctx.run is not None and ops.plain_grad(g_h, g_z):
+            grads = ops.block_grad_plain(ctx.run, g_h, g_z, saved, need)
             if grads is not None:
                 return (*grads, None)
         if ops.eager_call(g_h, g_z, *saved):

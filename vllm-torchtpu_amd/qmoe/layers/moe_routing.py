@@ -164,7 +164,7 @@ class _Balance(torch.autograd.Function):
         ctx.run = None
         if ops.eager_call(logits, bias, token_mask) and logits.numel() and logits.is_contiguous() and \
                 (token_mask is None or token_mask.is_contiguous()):
-            at = (logits.data_ptr(), ids.data_ptr(), counts.data_ptr(), 0 if token_mask is None else token_mask.data_ptr())
+            at = ops._addresses((logits, ids, counts, token_mask))
             ctx.run = (at, *logits.shape, topk, ops._SCORING[args[0]], *args[1:3])
         ctx.mark_non_differentiable(ids, counts)
         ctx.set_materialize_grads(False)
@@ -180,10 +180,9 @@ class _Balance(torch.autograd.Function):
     def _grads(ctx, g_w, g_ids, g_loss, g_counts):
         if g_w is None and g_loss is None:
             return (None,) * 5
-        logits, ids, counts, mask = ctx.saved_tensors
+        logits, ids, counts, mask = saved = ctx.saved_tensors
         run = ctx.run
-        if run is not None and (g_w is None or ops.plain_grad(g_w)) and (g_loss is None or ops.plain_grad(g_loss)) and \
-                (logits.data_ptr(), ids.data_ptr(), counts.data_ptr(), 0 if mask is None else mask.data_ptr()) == run[0]:
+        if run is not None and ops.plain_grad(g_w, g_loss) and ops._addresses(saved) == run[0]:
             return ops.balance_grad_run(logits, ids, counts, g_w, g_loss, *run[1:], mask), None, None, None, None
         fn = ops.moe_balance_grad
         if not ops.eager_call(logits, ids, counts, g_w, g_loss, mask):

@@ -84,14 +84,27 @@ def eager_call(*ts):
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
-def plain_grad(grad):
-    """Whether a gradient that autograd hands to a backward pass is an ordinary
-    contiguous tensor on the current device, and the pass itself runs at once (see
-    `eager_call`). With saved tensors that lie where the forward pass had them, such a
-    call needs no checks but the forward pass's."""
-    return (type(grad) is torch.Tensor and grad.is_contiguous() and grad.get_device() == _current_device()
-            and not _included_keys().raw_repr() & _WATCHING and forward_ad._current_level < 0
+def plain_grad(*grads):
+    """Whether the gradients that autograd hands to a backward pass (None aside) are
+    ordinary contiguous tensors on the current device, and the pass itself runs at once
+    (see `eager_call`). With saved tensors that lie where the forward pass had them, such
+    a call needs no checks but the forward pass's."""
+    dev = _current_device()
+    for g in grads:
+        if g is not None and (type(g) is not torch.Tensor or not g.is_contiguous() or g.get_device() != dev):
+            return False
+    return (not _included_keys().raw_repr() & _WATCHING and forward_ad._current_level < 0
             and not torch.compiler.is_compiling())
+
+
+def _addresses(ts):
+    return [0 if t is None else t.data_ptr() for t in ts]
+
+
+def _like(t):
+    """A contiguous tensor of ``t``'s shape and type (half the time of `new_empty`, which
+    makes the shape's numbers Python objects first)"""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def has_tangent(*ts):
@@ -1181,7 +1194,7 @@ def moe_balance_grad(router_logits, topk_ids, counts, g_weights, g_loss, scoring
 def balance_grad_run(logits, ids, counts, g_weights, g_loss, T, E, k, scoring, renormalize, rsf, mask):
     """`moe_balance_grad` behind its checks, on the current device (few Python objects,
     see `block_grad_run`)."""
-    d = logits.new_empty((T, E))
+    d = _like(logits)
     rc = lib.qmoe_moe_balance_grad(logits.data_ptr(), logits.dtype is torch.float32, T, E, k, scoring, renormalize, rsf,
                                    None if mask is None else mask.data_ptr(), ids.data_ptr(), counts.data_ptr(),
                                    None if g_weights is None else g_weights.data_ptr(),
@@ -1346,26 +1359,25 @@ def block_residual_grad(g_h, g_z, y, h, gate, post_weight, next_weight, rstd, sc
 
 
 def block_saved(d, y, h, gate, post, nxt, rstd):
-    """The descriptor of a forward call where its operands are contiguous and lie where
-    it has read them (not copies that it had to make): its backward pass may take the
-    addresses from there. Else None."""
+    """(descriptor, addresses) of a forward call where its operands are contiguous and lie
+    where it has read them (not copies that it had to make): its backward pass may take
+    the addresses from there. Else None."""
     for t, at in ((y, d.y), (h, d.residual if y is None else d.h), (gate, d.gate), (post, d.post_weight),
                   (nxt, d.next_weight)):
         if t is not None and (t.data_ptr() != at or not t.is_contiguous()):
             return None
     if y is None:
         d.h, d.ldh = d.residual, d.H
-    return d
+    return d, _addresses((y, h, gate, post, nxt, rstd))
 
 
-def block_grad_plain(d, g_h, g_z, y, h, gate, post, nxt, rstd, need):
-    """`block_grad_run` with the descriptor that `block_saved` passed, for contiguous
-    gradients; None where a hook has moved a saved tensor"""
-    if h.data_ptr() != d.h or rstd.data_ptr() != d.rstd_y or (y is not None and y.data_ptr() != d.y) or \
-            (gate is not None and gate.data_ptr() != d.gate) or (post is not None and post.data_ptr() != d.post_weight) or \
-            (nxt is not None and nxt.data_ptr() != d.next_weight):
+def block_grad_plain(run, g_h, g_z, saved, need):
+    """`block_grad_run` with what `block_saved` returned, for contiguous gradients; None
+    where a hook has moved a saved tensor"""
+    d, at = run
+    if _addresses(saved) != at:
         return None
-    return block_grad_run(d, g_h, d.H, g_z, d.H, y, h, gate, post, nxt, need)
+    return block_grad_run(d, g_h, d.H, g_z, d.H, *saved[:5], need)
 
 
 def block_grad_run(d, g_h, ldgh, g_z, ldgz, y, h, gate, post, nxt, need):
@@ -1373,11 +1385,11 @@ def block_grad_run(d, g_h, ldgh, g_z, ldgz, y, h, gate, post, nxt, need):
     operands' addresses). A backward pass calls it from autograd's own thread, where
     every Python object that the forward pass has used comes from another core: it
     touches few."""
-    dy = y.new_empty(y.shape) if need[0] and y is not None else None
-    dr = h.new_empty(h.shape) if need[1] else None
-    dg = gate.new_empty(gate.shape) if need[2] and gate is not None else None
-    dp = post.new_empty(post.shape) if need[3] and post is not None else None
-    dn = nxt.new_empty(nxt.shape) if need[4] and g_z is not None else None
+    dy = _like(y) if need[0] and y is not None else None
+    dr = _like(h) if need[1] else None
+    dg = _like(gate) if need[2] and gate is not None else None
+    dp = _like(post) if need[3] and post is not None else None
+    dn = _like(nxt) if need[4] and g_z is not None else None
     ws, n = None, 0
     if dp is not None or dn is not None or (dg is not None and d.gate_kind == 1):
         n = _block_grad_bytes(d.T, d.H)
@@ -1561,7 +1573,7 @@ def linear_grad_run(dy, ld, shape, T, N, K, weight, codes, scales, need_x, need_
     """`linear_grad` behind its checks, on the current device (few Python objects, see
     `block_grad_run`)."""
     dx = dy.new_empty((*shape[:-1], K)) if need_x else None
-    dw = dy.new_empty((N, K)) if need_weight else None
+    dw = _like(weight) if need_weight else None
     db = None if bias_dtype is None else dy.new_empty(N, dtype=bias_dtype)
     n = _linear_grad_bytes(T, N, K, need_x, need_weight, db is not None)
     ws = dy.new_empty(n, dtype=torch.uint8) if n else None
