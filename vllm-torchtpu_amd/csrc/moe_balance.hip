@@ -21,7 +21,7 @@
 // workgroups' parts in a fixed order, and none at all where one workgroup holds
 // every token. The gradient reads logits again rather than keeping T E scores.
 //
-// 16384 tokens, 256 experts in f32, 8 of 4 of 8 groups by sigmoids: routes 34 us (84 % of
+// 16384 tokens, 256 experts in f32, 8 from the best 4 of 8 groups by sigmoids: routes 34 us (84 % of
 // the vector ALUs' cycles, four wavefronts a SIMD), sums 6, gradient 14 (34 MB, 2.4
 // TB/s); 777 tokens, 128 experts, softmax 4.4, 6.6 and 4.4; 8 tokens 3.9 in one launch.
 
