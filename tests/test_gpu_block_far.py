@@ -76,10 +76,13 @@ def test_linear(dev):
     assert not dx[:-LAST].any()
 
 
-# tiles of more than one for every CU, with ragged ends: of 256 and of 192 rows along K,
-# across it in the input's gradient, and in the weight's
+# more tiles than CUs, with ragged ends: of 256 and of 192 rows along K, across it in the
+# input's gradient, and in the weight's; then each tile where K is short or long for it
 @pytest.mark.parametrize("T,K,N,bias", [(4072, 512, 4104, True), (3000, 512, 8200, False), (3000, 512, 8200, True),
-                                        (4072, 4128, 512, False), (3000, 8224, 512, True), (2048, 5152, 5128, False)])
+                                        (4072, 4128, 512, False), (3000, 8224, 512, True), (2048, 5152, 5128, False),
+                                        (250, 96, 28680, True), (4070, 28672, 72, True), (777, 96, 14344, True),
+                                        (777, 14368, 72, False), (3000, 28640, 72, False), (3000, 96, 28680, False),
+                                        (4070, 96, 28680, True), (4070, 64, 28672, False)])
 def test_linear_of_many_tiles(dev, T, K, N, bias):
     """sums of K, N and T products in float32, one rounding to bf16; what is read behind
     each matrix is its own, so that a wrong place shows"""

@@ -48,26 +48,31 @@ struct LinearGemm {
 };
 
 // B row t of the 64 that a round holds, A row n of it at n ^ vg_row_swz(t): 8
-// consecutive A rows per thread and store. 64 KB of LDS, once no copy or read uses it.
-template <int THREADS, int NI, int MJ>
+// consecutive A rows per thread and store. 64 KB of LDS, once no copy or read uses it,
+// or 128 (HALVES: wavefronts wm = 0 and 1 have the same rows, of half of k each).
+template <int THREADS, int NI, int MJ, bool HALVES = false>
 __device__ __forceinline__ void linear_epilogue(const LinearGemm& p, f32x16 (&acc)[NI][MJ], uint8_t* smem, int n0, int m0,
                                                 int arows, int brows, int wn, int wm) {
   const int tid = threadIdx.x, lane = tid & 63, rl = lane & 31, kh = lane >> 5;
-  float* reg = reinterpret_cast<float*>(smem);  // [64][256]
+  float *reg = reinterpret_cast<float*>(smem), *reg2 = reg + 64 * kAN;  // [64][256]
+  float* to = HALVES && wm ? reg2 : reg;
+  constexpr int ROUND = HALVES ? 2 : 1;  // blocks of a wavefront in 64 rows
 #pragma unroll
-  for (int j = 0; j < MJ; ++j) {
-    const int tl = wm * 32 + rl;
+  for (int j = 0; j < MJ / ROUND; ++j) {
     if (64 * j >= brows) break;
     if (j) __syncthreads();  // the rows before have been read
     const int n1 = opaque_v(wn * NI * 32 + kh * 4);
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
+    for (int jj = 0; jj < ROUND; ++jj)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = n1 + i * 32 + q * 8;
-        *reinterpret_cast<float4*>(reg + tl * kAN + (n ^ vg_row_swz(tl))) =
-            make_float4(acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]);
-      }
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = n1 + i * 32 + q * 8, tl = (HALVES ? jj : wm) * 32 + rl;
+          const f32x16& v = acc[i][j * ROUND + jj];
+          *reinterpret_cast<float4*>(to + tl * kAN + (n ^ vg_row_swz(tl))) =
+              make_float4(v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]);
+        }
     __syncthreads();
     constexpr int CH = kAN / 8;
     const int c = (tid % CH) * 8;
@@ -76,8 +81,13 @@ __device__ __forceinline__ void linear_epilogue(const LinearGemm& p, f32x16 (&ac
       const int64_t row = m0 + 64 * j + t;
       if (64 * j + t >= brows) break;
       if (c >= arows) continue;  // (A rows come in multiples of 8)
-      const float4 lo = *reinterpret_cast<const float4*>(reg + t * kAN + (c ^ vg_row_swz(t)));
-      const float4 hi = *reinterpret_cast<const float4*>(reg + t * kAN + ((c + 4) ^ vg_row_swz(t)));
+      const int at = t * kAN + (c ^ vg_row_swz(t)), at4 = t * kAN + ((c + 4) ^ vg_row_swz(t));
+      float4 lo = *reinterpret_cast<const float4*>(reg + at), hi = *reinterpret_cast<const float4*>(reg + at4);
+      if constexpr (HALVES) {
+        const float4 l = *reinterpret_cast<const float4*>(reg2 + at), h = *reinterpret_cast<const float4*>(reg2 + at4);
+        lo.x += l.x, lo.y += l.y, lo.z += l.z, lo.w += l.w;
+        hi.x += h.x, hi.y += h.y, hi.z += h.z, hi.w += h.w;
+      }
       if (p.kslice) {
         float4* dst = reinterpret_cast<float4*>(p.slices + ((int64_t)blockIdx.y * p.nb + row) * p.na + n0 + c);
         dst[0] = lo;
@@ -106,17 +116,20 @@ __device__ __forceinline__ void linear_slice(LinearGemm& p) {
   p.K = (int)min((int64_t)p.kslice, p.K - k0);
 }
 
-// Tiles of 256 x BM (64 or 128) by eight wavefronts. ONE: a stage at a time,
-// without a ring, so that two workgroups share a CU. 777 tokens, 4096 x 4096: 64 rows,
-// forward / dx 40.2 / 43.9 us (26 and 24 % of the matrix cores' cycles: 208 tiles of 256
-// CUs, and LDS feeds a wavefront of 64 x 32), dw without a ring 30. CODES: the A operand is x8
+// Tiles of 256 x BM (64 or 128) by eight wavefronts of 64 x 64. HALVES (64 B rows): two
+// of them have the same block, of half of every stage's k each, and their sums are added
+// at the end: 64 KB of operands from LDS per stage where wavefronts of 64 x 32 read 96.
+// 777 tokens, 4096 x 4096 forward / dx 38.1 / 39.5 -> 35.5 / 34.9 us (208 tiles of 256 CUs,
+// 740 TFLOP/s); of 128 rows the same 2 to 9 % slower. ONE: a stage at a time, without a
+// ring, so that two workgroups share a CU (that case's dw 30). CODES: the A operand is x8
 // itself, codes and scale bytes across K, expanded on the way to LDS (a thread 32
 // columns of a row): no transposed copy of x8 before the product, whose launch and
 // bytes count where the sums are short.
 template <bool TRA, bool TRB, int BM, bool ONE, bool CODES>
 __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const LinearGemm args) {
-  constexpr int NI = 2, MJ = BM / 64, WB = kAN * 128, STG = WB + BM * 128;
-  constexpr int RING = ONE ? 1 : (163840 / STG < 6 ? 163840 / STG : 6), EPILOGUE = 65536;
+  constexpr bool HALVES = BM == 64;
+  constexpr int NI = 2, MJ = HALVES ? 2 : BM / 64, WB = kAN * 128, STG = WB + BM * 128;
+  constexpr int RING = ONE ? 1 : (163840 / STG < 6 ? 163840 / STG : 6), EPILOGUE = HALVES ? 131072 : 65536;
   __shared__ __align__(1024) uint8_t smem[RING * STG > EPILOGUE ? RING * STG : EPILOGUE];
   static_assert(ONE ? sizeof(smem) <= 81920 : RING >= 3 && sizeof(smem) <= 163840, "workgroups of a CU, ring");
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
@@ -196,33 +209,37 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
   B8 wf[2][NI], xf[2][MJ];
   const uint32_t alane = tr_lane<kAN * 2>(lane), blane = tr_lane<BM * 2>(lane);
   // operands of step q (16 k) of a stage
-  auto read_q = [&](int slot, int q) {
+  constexpr int QS = HALVES ? 2 : 4;  // steps of a wavefront in a stage
+  auto read_q = [&](int slot, int u) {
     const uint8_t* s = smem + slot * STG;
+    const int q = HALVES ? 2 * wm + u : u;
 #pragma unroll
     for (int i = 0; i < NI; ++i)
-      if constexpr (TRA) wf[q & 1][i].u = tr_read<kAN * 2>(s + q * 32 * kAN + (alane ^ (wn * NI + i) * 64));
-      else wf[q & 1][i].u =
+      if constexpr (TRA) wf[u & 1][i].u = tr_read<kAN * 2>(s + q * 32 * kAN + (alane ^ (wn * NI + i) * 64));
+      else wf[u & 1][i].u =
           *reinterpret_cast<const uint4*>(s + (wn * 64 + i * 32 + rl) * 128 + ((2 * q + kh) ^ vg_swz(rl)) * 16);
 #pragma unroll
-    for (int j = 0; j < MJ; ++j)
-      if constexpr (TRB) xf[q & 1][j].u = tr_read<BM * 2>(s + WB + q * 32 * BM + (blane ^ (2 * j + wm) * 64));
-      else xf[q & 1][j].u =
-          *reinterpret_cast<const uint4*>(s + WB + ((2 * j + wm) * 32 + rl) * 128 + ((2 * q + kh) ^ vg_swz(rl)) * 16);
+    for (int j = 0; j < MJ; ++j) {
+      const int b = HALVES ? j : 2 * j + wm;  // block of 32 B rows
+      if constexpr (TRB) xf[u & 1][j].u = tr_read<BM * 2>(s + WB + q * 32 * BM + (blane ^ b * 64));
+      else xf[u & 1][j].u =
+          *reinterpret_cast<const uint4*>(s + WB + (b * 32 + rl) * 128 + ((2 * q + kh) ^ vg_swz(rl)) * 16);
+    }
   };
-  auto mma = [&](int q) {
+  auto mma = [&](int u) {
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int j = 0; j < MJ; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[q & 1][i].v, xf[q & 1][j].v, acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[u & 1][i].v, xf[u & 1][j].v, acc[i][j], 0, 0, 0);
   };
   auto one_stage = [&]() {
     wait_copies_upto<0>();
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      read_q(0, q);
-      mma(q);
+    for (int u = 0; u < QS; ++u) {
+      read_q(0, u);
+      mma(u);
     }
     __syncthreads();
   };
@@ -277,16 +294,16 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
     for (int s = 0; s < KF; ++s) {
       const int next = slot == RING - 1 ? 0 : slot + 1;
 #pragma unroll
-      for (int q = 0; q < 3; ++q) {
-        read_q(slot, q + 1);
-        mma(q);
+      for (int u = 0; u < QS - 1; ++u) {
+        read_q(slot, u + 1);
+        mma(u);
       }
       wait_copies_upto<(RING - 2) * (WI + XI)>();
       stage_barrier();
       copy_stage(s + RING, slot);
       asm volatile("" ::: "memory");
       read_q(next, 0);
-      mma(3);
+      mma(QS - 1);
       slot = next;
     }
     wait_copies_upto<0>();
@@ -296,7 +313,7 @@ __global__ __launch_bounds__(512, ONE ? 4 : 2) void linear_small_kernel(const Li
     copy_tail();
     one_stage();
   }
-  linear_epilogue<512, NI, MJ>(p, acc, smem, n0, m0, arows, brows, wn, wm);
+  linear_epilogue<512, NI, MJ, HALVES>(p, acc, smem, n0, m0, arows, brows, wn, wm);
 }
 
 // The same without slices in 32 KB of LDS (at `region`), waiting for none of the copies
@@ -664,15 +681,16 @@ struct LinearPlan {
 // 8192 tokens, 256 x 1024 to 4096 x 28672), with a workgroup per tile; the plan's own time
 // was within 5 % of the best of the sweep for most, 14 % at most. Both sides, us: 4096
 // tokens x 4096 x 28672 forward / dx / dw tiles of 256 723 / 676 / 734, of 128 887 / 816 / 875;
-// 777 x 4096 x 4096 dx 64 rows 38.5, 128 rows in 2 slices 42; dw without a ring 36.9,
-// 256 rows 39.3; 333 x 2880 x 5760 dx 128 rows in 6 slices 28.8, 64 in 3 39.
+// 777 x 4096 x 4096 dw without a ring 36.9, 256 rows 39.3; forward of 512 x 7168 x 7168 64 rows
+// 58.7, 256 rows in 4 slices 65.7; of 200 x 1024 x 4096 64 rows 13.2, in 4 slices 18.9; of
+// 64 x 4096 x 4096 16.8 in 8 slices.
 LinearPlan linear_plan(int mode, int64_t na, int64_t nb, int64_t K) {
   struct Tile {
     int bm, cus, stage, fixed;  // workgroups of a round, ns of a stage and of the rest of a tile
   };
   // (dw: few stages and the most to write; without a ring one workgroup's stores run under the other's products)
   constexpr Tile kAlong[] = {{256, 256, 1680, 6000}, {192, 256, 1290, 5000}, {128, 256, 1050, 4000}, {1, 512, 2000, 5000},
-                             {64, 256, 700, 2000}};
+                             {64, 256, 510, 5500}};
   constexpr Tile kDw[] = {{256, 256, 1680, 11000}, {128, 256, 1050, 8000}, {1, 512, 1900, 5000}, {64, 256, 700, 4000}};
   LinearPlan best{};
   int64_t least = INT64_MAX;
