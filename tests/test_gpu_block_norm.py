@@ -294,3 +294,19 @@ def test_kept_factors_and_refusals(dev):
         ops.block_residual_grad(None, None, ts[0], h, *ts[2:5], rstd)
     with pytest.raises(ValueError):
         block_residual(ts[0].cpu(), ts[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rows_of_the_lowest_value(dev, dtype):
+    """Their squares' sum is infinite, the row factor zero: zeros behind the norm, with
+    weights and gates above one, and other rows as without them."""
+    H = 512
+    g = torch.Generator(device=dev).manual_seed(3)
+    x = _rand(g, (5, H), dtype)
+    low = x.clone()
+    low[2] = torch.finfo(dtype).min
+    w, gate = torch.full((H,), 2.0, device=dev), torch.full((H,), 3.0, device=dev)
+    z, clean = block_norm(low, w), block_norm(x, w)
+    assert not z[2].any() and torch.equal(z[[0, 1, 3, 4]], clean[[0, 1, 3, 4]])
+    h, want = (block_residual(v, x, gate=gate, norm_weight=w) for v in (low, x))
+    assert torch.equal(h[2], x[2]) and torch.equal(h[[0, 1, 3, 4]], want[[0, 1, 3, 4]])

@@ -102,6 +102,7 @@ __global__ __launch_bounds__(THREADS) void block_residual_kernel(const qmoe_bloc
       for (int k = 0; k < 8; ++k) s[0] += v[k] * v[k];
     }
     row_sums<1>(s, red[0], W);
+    // (multiplied first: of a row of the type's lowest value it is zero, and so is the norm)
     ry = row_factor(s[0], inv, p.eps);
     if (row && p.rstd_y && threadIdx.x == 0) p.rstd_y[t] = ry;
   }
@@ -118,16 +119,14 @@ __global__ __launch_bounds__(THREADS) void block_residual_kernel(const qmoe_bloc
       if (p.post_weight) {
         load8_any<AL>(p.post_weight, p.weight_type, i, H, m);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] *= p.weight_offset + m[k];
+        for (int k = 0; k < 8; ++k) v[k] = v[k] * ry * (p.weight_offset + m[k]);
       }
       if (p.gate_kind == GATE_CHANNEL) load8_any<AL>(p.gate, p.gate_type, i, H, m);
       if (p.gate_kind == GATE_FULL) raw8_values<YT>(gr[c], m);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float g = p.gate_kind == GATE_CHANNEL || p.gate_kind == GATE_FULL ? m[k] : gt;
-        // (value, weight and gate in 16 bits: their product is exact, and the row factor's the
-        // only rounding before the sum's)
-        h[c][k] = round_to<RT>(p.residual_scale * h[c][k] + p.scale * (g * v[k] * ry));
+        h[c][k] = round_to<RT>(p.residual_scale * h[c][k] + p.scale * (g * v[k]));
       }
       store8<RT, AL>(static_cast<uint8_t*>(p.h) + t * p.ldh * rt_size(RT), i, H, h[c]);
     }
@@ -145,7 +144,7 @@ __global__ __launch_bounds__(THREADS) void block_residual_kernel(const qmoe_bloc
     float m[8];
     load8_any<AL>(p.next_weight, p.weight_type, i, H, m);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m[k] = h[c][k] * (p.weight_offset + m[k]) * rh;
+    for (int k = 0; k < 8; ++k) m[k] = h[c][k] * rh * (p.weight_offset + m[k]);
     store8<YT, AL>(static_cast<uint8_t*>(p.z) + t * p.ldz * rt_size(YT), i, H, m);
   }
 }
