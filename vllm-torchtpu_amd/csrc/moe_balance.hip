@@ -288,9 +288,12 @@ __global__ __launch_bounds__(256) void balance_grad_kernel(const BalanceGradPara
       }
       float v = gw * p.rsf;
       if (p.renormalize) {
-        // gw counts only by its differences: taken from the first choice's, so that one
-        // weight, or one that is nearly all, gives no rounding error of gw's own size
-        const float u = gw - __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(gw)));
+        // gw counts only by its differences: taken from that of the choice with the largest
+        // score (the first may have a small one: the correction bias is not in it), so that
+        // one weight, or one that is nearly all, gives no rounding error of gw's own size
+        const float top = wave_max_u(lane < k ? a : -__builtin_inff());
+        const uint64_t at = __ballot(lane < k && a == top);  // (none: a NaN, as is the sum)
+        const float u = gw - lane_f(gw, at ? (int)__builtin_ctzll(at) : 0);
         const float sum = wave_sum_u(lane < k ? a : 0.0f), dot = wave_sum_u(lane < k ? u * a : 0.0f);
         const float q = 1.0f / (sum != sum ? sum : fmaxf(sum, kTiny));
         v = p.rsf * (sum < kTiny ? gw : u - dot * q) * q;
