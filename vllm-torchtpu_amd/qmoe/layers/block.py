@@ -6,10 +6,12 @@ whose inputs wait for the backward pass in 8 bits (``checkpointed_activation``,
 no counterpart.
 
 Each runs straight on the C ABI in eager mode and as a torch custom op
-(``torch.ops.qmoe.block_residual`` ...) under a trace, a dispatch mode, a functorch
-transform and fake tensors, as the vocabulary's operators do. Gradients come from
+(``torch.ops.qmoe.block_residual`` ...) under a trace, a dispatch mode, `torch.vmap` and
+fake tensors, as the vocabulary's operators do. Gradients come from
 `torch.autograd.Function`s; there is no second derivative and no forward-mode
-derivative, and a tangent is refused.
+derivative, and a tangent is refused, as is a gradient that is asked for inside a
+functorch transform (`torch.func.grad` ...; through a batch of `torch.vmap`, whose
+operands do not say that they require one, the backward pass is an error).
 
 8 bits: per 32 columns e4m3 codes and a power of two, the least with which none
 of them saturates. A value is off by at most 2^-4 of itself, or 2^-10 of the
@@ -122,6 +124,7 @@ def block_norm(x, weight, eps=1e-6, weight_offset=0.0, out_dtype=None):
     if weight is None:
         raise ValueError("block_norm: a weight is required")
     if _wants(x, weight):
+        ops.refuse_transforms("block_norm")
         return _Block.apply(None, x, None, None, weight, args)[1]
     return _block(None, x, None, None, weight, args, False)[1]
 
@@ -145,7 +148,11 @@ def block_residual(y, residual, gate=None, norm_weight=None, next_weight=None, s
         raise ValueError("block_residual: needs the block's output")
     args = (float(scale), float(residual_scale), float(eps), float(weight_offset), y.dtype)
     ts = (y, residual, gate, norm_weight, next_weight)
-    h, z = _Block.apply(*ts, args) if _wants(*ts) else _block(*ts, args, False)[:2]
+    if _wants(*ts):
+        ops.refuse_transforms("block_residual")
+        h, z = _Block.apply(*ts, args)
+    else:
+        h, z = _block(*ts, args, False)[:2]
     return h if next_weight is None else (h, z)
 
 
@@ -228,6 +235,7 @@ def checkpointed_activation(gate_up, activation="silu"):
     8-bit values; a clamp passes the gradient up to its limits. The result itself comes
     from the 16-bit values."""
     if _wants(gate_up):
+        ops.refuse_transforms("checkpointed_activation")
         return _Activation.apply(gate_up, activation)
     return _act(gate_up, activation, False)[0]
 
@@ -321,5 +329,6 @@ def checkpointed_linear(x, weight, bias=None):
     bias are exact. bf16 gradients (the bias's in its type) from float32 sums in a
     fixed order."""
     if _wants(x, weight, bias):
+        ops.refuse_transforms("checkpointed_linear")
         return _Linear.apply(x, weight, bias)
     return _linear(x, weight, bias, False)[0]

@@ -215,8 +215,9 @@ def balanced_experts(router_logits, topk, scoring_func="softmax", renormalize=Tr
 
     ``expert_counts`` are those routes. A token outside the mask gets weights 0, and no
     gradient whatever its logits are. Differentiable in the logits through the
-    weights and the loss (through P; the choice and f are constants), in their type;
-    the correction bias only chooses and has no gradient. The sums' order is fixed."""
+    weights and the loss (through P; the choice and f are constants), in their type, by
+    `torch.autograd` (under functorch transforms the call is refused where a gradient is
+    asked for); the correction bias only chooses and has no gradient. The sums' order is fixed."""
     if torch.is_grad_enabled() and e_score_correction_bias is not None and e_score_correction_bias.requires_grad:
         raise NotImplementedError("balanced_experts: no gradient for the correction bias, which only chooses")
     if router_logits.dtype not in (torch.bfloat16, torch.float32) and router_logits.is_floating_point():
@@ -225,5 +226,6 @@ def balanced_experts(router_logits, topk, scoring_func="softmax", renormalize=Tr
             int(topk_group or 1))
     topk = int(topk)
     if torch.is_grad_enabled() and router_logits.requires_grad:
+        ops.refuse_transforms("balanced_experts")
         return _Balance.apply(router_logits, topk, args, e_score_correction_bias, token_mask)
     return _balance(router_logits, topk, args, e_score_correction_bias, token_mask)

@@ -7,10 +7,11 @@ models put behind it, and its gradient for a bf16 or f32 table.
 table of `fp8.py:1679-1681`) without the [T, V] logits, and its gradients.
 
 Both run as torch custom ops (``torch.ops.qmoe.vocab_lookup`` ...) under a
-trace, a dispatch mode, a functorch transform and fake tensors, and straight on
-the C ABI in eager mode: the op's dispatch takes longer than a decode step's
-lookup. Gradients come from `torch.autograd.Function`s around them; there is no
-forward-mode derivative, and a tangent is refused.
+trace, a dispatch mode, `torch.vmap` and fake tensors, and straight on the C ABI
+in eager mode: the op's dispatch takes longer than a decode step's lookup.
+Gradients come from `torch.autograd.Function`s around them; there is no
+forward-mode derivative, and a tangent is refused, as is a gradient that is asked
+for inside a functorch transform (`torch.func.grad` ...).
 """
 
 from typing import Optional, Tuple
@@ -103,6 +104,7 @@ def embedding(ids, weight, weight_scale=None, scale=1.0, padding_idx=None, out_d
             raise NotImplementedError("embedding: no gradient for a table of 1-byte codes or its scales")
         if out_dtype == torch.float16:
             raise NotImplementedError("embedding: gradients flow through bf16 or f32 outputs, not f16")
+        ops.refuse_transforms("embedding")
         return _Embedding.apply(ids, weight, scale, padding_idx, out_dtype)
     return _lookup(ids, weight, weight_scale, scale, out_dtype)
 
@@ -207,5 +209,6 @@ def vocab_cross_entropy(x, weight, targets, weight_scale=None, ignore_index=-100
                                     (weight_scale is not None and weight_scale.requires_grad)):
         if weight_scale is not None and (weight.requires_grad or weight_scale.requires_grad):
             raise NotImplementedError("vocab_cross_entropy: no gradient for a table of 1-byte codes or its scales")
+        ops.refuse_transforms("vocab_cross_entropy")
         return _VocabCrossEntropy.apply(x, weight, targets, weight_scale, ignore_index)
     return _loss(x, weight, targets, weight_scale, ignore_index)

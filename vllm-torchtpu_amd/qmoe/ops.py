@@ -121,6 +121,14 @@ def refuse_tangents(what, *ts):
         raise NotImplementedError(f"{what}: no forward-mode derivative")
 
 
+def refuse_transforms(what):
+    """An error for a call whose gradient is asked for inside a functorch transform: the
+    autograd functions here are for `torch.autograd`."""
+    if not torch.compiler.is_compiling() and torch._C._are_functorch_transforms_active():
+        raise NotImplementedError(f"{what}: no gradients under functorch transforms (torch.func, vmap); without gradients "
+                                  "(torch.no_grad, detached operands) it runs there, and torch.autograd differentiates it")
+
+
 class _NoSecond(torch.autograd.Function):
     @staticmethod
     def forward(ctx, what, *grads):
