@@ -20,7 +20,8 @@ class UnquantizedLinearMethod:
                                                               dtype=params_dtype)))
 
     def process_weights_after_loading(self, layer):
-        layer.weight = _param(layer.weight.data.to(_device(), torch.bfloat16).contiguous())
+        trained = layer.weight.requires_grad  # (frozen unless it was made trainable before)
+        layer.weight = _param(layer.weight.data.to(_device(), torch.bfloat16).contiguous()).requires_grad_(trained)
 
     def apply(self, layer, x, bias=None):
         k = x.shape[-1]
@@ -31,9 +32,22 @@ class UnquantizedLinearMethod:
         return out
 
     def apply_checkpointed(self, layer, x, bias=None):
-        """`apply` with gradients: ``x`` waits for the weight's in 8 bits
-        (`qmoe.layers.block.checkpointed_linear`)."""
-        return checkpointed_linear(x.to(torch.bfloat16), layer.weight, bias)
+        """`apply` with gradients, of ``x``, ``bias`` and a trainable weight, for whose
+        gradient ``x`` waits in 8 bits (`qmoe.layers.block.checkpointed_linear`): bf16,
+        the bias added before the one rounding.
+
+        `create_weights` makes a frozen weight, which gets no gradient and keeps nothing
+        of ``x``; ``layer.weight.requires_grad_()`` makes it trainable, before or after
+        loading. An output size that is not a multiple of 8 is padded with rows of
+        zeros, a copy of the weight in every call."""
+        x, w, n = x.to(torch.bfloat16), layer.weight, layer.weight.shape[0]
+        if bias is not None and bias.dtype not in (torch.bfloat16, torch.float32):
+            bias = bias.float()
+        if n % 8 == 0:
+            return checkpointed_linear(x, w, bias)
+        w = torch.nn.functional.pad(w, (0, 0, 0, -n % 8))
+        bias = None if bias is None else torch.nn.functional.pad(bias, (0, -n % 8))
+        return checkpointed_linear(x, w, bias)[..., :n]
 
     def embedding(self, layer, input_):
         """Rows of a bf16 or f32 ``[vocab, H]`` table (a `VocabParallelEmbedding`
