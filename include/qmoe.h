@@ -661,6 +661,17 @@ int qmoe_linear_grad(const void* dy, int64_t lddy, int64_t T, int64_t N, int64_t
                      void* workspace, int64_t ws_bytes, qmoe_stream_t stream);
 
 /*
+ * The tiles of qmoe_linear (y) and qmoe_linear_grad (dx, dw) for these sizes: rows
+ * of a tile (of x, dy and w's gradient), 64 and 128 by eight wavefronts, 192 and 256
+ * by four, 1 for 128 rows without a stage ring; the slices that each product's summed
+ * axis (K, N, T) is cut into; and whether dw takes the codes as they are. Reads no memory.
+ */
+typedef struct qmoe_linear_tiles {
+  int32_t y, y_slices, dx, dx_slices, dw, dw_slices, dw_codes;
+} qmoe_linear_tiles;
+int qmoe_linear_plan(int64_t T, int64_t N, int64_t K, qmoe_linear_tiles* plan);
+
+/*
  * Plain read of `bytes` (a multiple of 16, 16-byte aligned) at `src` by at
  * most `workgroups` 256-thread workgroups; `sink` receives at most one dword
  * per workgroup ([workgroups] uint32, normally untouched). No counterpart in

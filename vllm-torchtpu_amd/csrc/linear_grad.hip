@@ -817,6 +817,13 @@ extern "C" int qmoe_linear(const void* x, int64_t ldx, int64_t T, int64_t N, int
   return hipGetLastError() == hipSuccess ? QMOE_OK : QMOE_ERR_LAUNCH;
 }
 
+extern "C" int qmoe_linear_plan(int64_t T, int64_t N, int64_t K, qmoe_linear_tiles* plan) {
+  if (!linear_sizes_ok(T, N, K) || !plan) return QMOE_ERR_ARG;
+  const LinearPlan y = linear_plan(LM_FORWARD, N, T, K), dx = linear_plan(LM_DX, K, T, N), dw = linear_plan(LM_DW, K, N, T);
+  *plan = qmoe_linear_tiles{y.bm, y.slices, dx.bm, dx.slices, dw.bm, dw.slices, linear_codes(N, K, T)};
+  return QMOE_OK;
+}
+
 extern "C" int qmoe_linear_grad_workspace_size(int64_t T, int64_t N, int64_t K, int need_dx, int need_dw, int need_dbias,
                                                int64_t* bytes) {
   if (!linear_sizes_ok(T, N, K) || !bytes) return QMOE_ERR_ARG;

@@ -18,7 +18,7 @@ import torch  # noqa: F401  (its HIP runtime first; see above)
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libqmoe.so")
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 QMOE_OK = 0
 STATUS_TEXT = {
@@ -206,6 +206,12 @@ class BlockGrads(ctypes.Structure):
     ]
 
 
+class LinearTiles(ctypes.Structure):
+    """Mirror of `qmoe_linear_tiles`."""
+
+    _fields_ = [(name, _i32) for name in ("y", "y_slices", "dx", "dx_slices", "dw", "dw_slices", "dw_codes")]
+
+
 def _load():
     if not os.path.exists(_LIB_PATH):
         raise ImportError(
@@ -309,6 +315,8 @@ def _load():
     lib.qmoe_linear_grad.restype = ctypes.c_int
     lib.qmoe_linear_grad.argtypes = [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, ctypes.c_int, _vp,
                                      _i64, _vp]
+    lib.qmoe_linear_plan.restype = ctypes.c_int
+    lib.qmoe_linear_plan.argtypes = [_i64, _i64, _i64, ctypes.POINTER(LinearTiles)]
     lib.qmoe_stream_read.restype = ctypes.c_int
     lib.qmoe_stream_read.argtypes = [_vp, _i64, _i32, _vp, _vp]
     v = lib.qmoe_abi_version()
@@ -359,6 +367,7 @@ EXPORTED = (
     "qmoe_linear",
     "qmoe_linear_grad_workspace_size",
     "qmoe_linear_grad",
+    "qmoe_linear_plan",
 )
 
 

@@ -1543,6 +1543,14 @@ def linear_checkpoint(x, weight, bias=None, keep=True):
     return y, codes, scales
 
 
+def linear_plan(T, N, K):
+    """Tiles and slices that `linear_checkpoint` and `linear_grad` take for these
+    sizes (host-side `qmoe_linear_plan`), by name."""
+    tiles = _capi.LinearTiles()
+    check(lib.qmoe_linear_plan(T, N, K, ctypes.byref(tiles)), "linear_plan")
+    return {name: getattr(tiles, name) for name, _ in tiles._fields_}
+
+
 @functools.lru_cache(maxsize=256)
 def _linear_grad_bytes(T, N, K, need_x, need_weight, need_bias):
     need = ctypes.c_int64(0)
