@@ -523,8 +523,8 @@ int qmoe_vocab_loss_grad(const void* x, int64_t ldx, int64_t T, const void* w, i
  * Routing with its balance loss and per-expert counts (no counterpart in the
  * reference, which serves only): routes as qmoe_moe_route with float32 weights,
  * then over the counted tokens (token_mask[t] != 0, or all without a mask), N of
- * them, with p[t, e] = s[t, e] / sum over e of s[t, e] and counts[e] the counted
- * tokens that chose e,
+ * them, with p[t, e] = s[t, e] / max(sum over e of s[t, e], 1e-20) and counts[e] the
+ * counted tokens that chose e,
  *   loss = E / (topk N^2) sum over e of counts[e] sum over t of p[t, e]    (0 for N = 0)
  *   logits      : [T][E] bf16, or f32 with logits_f32; scoring 0..2, bias,
  *                 renormalize, groups as qmoe_moe_route
@@ -543,8 +543,9 @@ int qmoe_moe_balance(const void* logits, int logits_f32, int64_t T, int E, int t
 /*
  * Its gradient: d_logits [T][E] (the logits' type) for the gradients of
  * topk_weights (f32 [T][topk] or NULL) and of loss (f32 [1] or NULL); topk_ids and
- * counts as qmoe_moe_balance wrote them. A token outside the mask gets zeros,
- * whatever its logits are.
+ * counts as qmoe_moe_balance wrote them. A sum below 1e-20 (of the row's scores, or of
+ * the weights that are renormalized) counts as a constant. A token outside the mask
+ * gets zeros, whatever its logits are.
  */
 int qmoe_moe_balance_grad(const void* logits, int logits_f32, int64_t T, int E, int topk, int scoring, int renormalize,
                           float routed_scaling_factor, const uint8_t* token_mask, const int32_t* topk_ids,
@@ -558,7 +559,9 @@ int qmoe_moe_balance_grad(const void* logits, int logits_f32, int64_t T, int E, 
  *   b = n(y; post_weight) or y,  h = residual_scale residual + scale gate b,  z = n(h; next_weight)
  * y NULL: h is the residual itself (the norm before a block alone). Types: 0
  * bf16, 1 f32, 2 f16; residual and h of y_type or f32; z and a gate per element
- * of y_type. h is rounded as it is stored before its norm. Rows may be strided.
+ * of y_type. h is rounded as it is stored before its norm. Rows may be strided. The
+ * mean square is float32: a row whose squares add up to infinity (values beyond
+ * 1.8e19 / sqrt(H) in size) gives zeros behind its norm.
  */
 typedef struct qmoe_block_desc {
   int64_t T, H;            /* rows, 1..2^24; row length, 1..16384 */

@@ -5,8 +5,9 @@
 // What bounds it: two products of 2 T N K operations on the bf16 matrix cores, or,
 // for few tokens, one read of w and one write of dw. The 8-bit values' scales
 // change along the summed axis, so the codes are multiplied as bf16 (exact: 4 of
-// its 8 significant bits): of up to 512 tokens by the tiles themselves, of more expanded
-// and transposed once on the way to dw (4096 x 4096: 14 us).
+// its 8 significant bits): of up to 512 tokens by the tiles without a ring themselves
+// (linear_codes), for other tiles and of more tokens expanded and transposed once on the
+// way to dw (4096 x 4096: 14 us).
 //
 // The products (the layer's own among them) are the same tile: 256 "A" rows x BM "B"
 // rows of a workgroup, a ring of LDS stages of 64 k filled by direct copies, and for
@@ -119,9 +120,10 @@ __device__ __forceinline__ void linear_slice(LinearGemm& p) {
 // Tiles of 256 x BM (64 or 128) by eight wavefronts of 64 x 64. HALVES (64 B rows): two
 // of them have the same block, of half of every stage's k each, and their sums are added
 // at the end: 64 KB of operands from LDS per stage where wavefronts of 64 x 32 read 96.
-// 777 tokens, 4096 x 4096 forward / dx 38.1 / 39.5 -> 35.5 / 34.9 us (208 tiles of 256 CUs,
-// 740 TFLOP/s); of 128 rows the same 2 to 9 % slower. ONE: a stage at a time, without a
-// ring, so that two workgroups share a CU (that case's dw 30). CODES: the A operand is x8
+// 777 tokens, 4096 x 4096 forward / dx, each alone, 38.1 / 39.5 -> 35.5 / 34.9 us (208 tiles of
+// 256 CUs, 740 TFLOP/s; 37.1 / 38.3 in a step, 35.4 / 37.4 at best); of 128 rows the same 2
+// to 9 % slower. ONE: a stage at a time, without a ring, so that two workgroups share a CU
+// (that case's dw 30). CODES: the A operand is x8
 // itself, codes and scale bytes across K, expanded on the way to LDS (a thread 32
 // columns of a row): no transposed copy of x8 before the product, whose launch and
 // bytes count where the sums are short.
@@ -712,7 +714,9 @@ LinearPlan linear_plan(int mode, int64_t na, int64_t nb, int64_t K) {
   return best;
 }
 
-// Whether dw takes the codes as they are: tiles without a ring of up to 512 tokens.
+// Whether dw takes the codes as they are: tiles without a ring of up to 512 tokens. (The
+// plan's times leave the transposed copy out, so that other tiles of so few tokens still
+// make it, where their own time is less: 19 tokens x 2048 x 2048.)
 // Every tile of N expands them again: 19 tokens x 2880 x 2880 10.4 us (13.4 with the
 // transposed copy), 200 x 7168 x 2048 19.6 (22.1), 512 x 4096 x 4096 29.7 (30.0), but 777
 // x 4096 x 4096 42.7 (38.9), 1500 x 14336 x 4096 235 (180).

@@ -1,13 +1,13 @@
 // Routing with its balance loss, per-expert counts and the logits' gradient.
 //
 //   s[t]    = scores of token t, ids / w as qmoe_moe_route (float32 weights; 0 for a token outside the mask)
-//   p[t, e] = s[t, e] / sum_e s[t, e]            (softmax: s itself)
+//   p[t, e] = s[t, e] / max(sum_e s[t, e], 1e-20)   (softmax: s itself)
 //   c[e]    = counted tokens that chose e, N = counted tokens
 //   loss    = E / (k N^2) sum_e c[e] sum_t p[t, e],  0 where N = 0
 //
 // and, with gw and gl the gradients of w and loss, A_j = s[t, ids_j], D = max(sum_j A_j, 1e-20),
 //
-//   g[t, e]  = gl E c[e] / (k N^2)  as the gradient of p, put through p's quotient to s, plus
+//   g[t, e]  = gl E c[e] / (k N^2)  as the gradient of p, put through p's quotient to s (a floor is a constant), plus
 //              rsf (gw_j - sum_i gw_i A_i / D) / D  at e = ids_j     (renormalized; else rsf gw_j)
 //   dlogits  = s (g - sum_e g s)                  softmax
 //              g s (1 - s)                        sigmoid
@@ -22,8 +22,8 @@
 // every token. The gradient reads logits again rather than keeping T E scores.
 //
 // 16384 tokens, 256 experts in f32, 8 from the best 4 of 8 groups by sigmoids: routes 34 us (84 % of
-// the vector ALUs' cycles, four wavefronts a SIMD), sums 6, gradient 14 (34 MB, 2.4
-// TB/s); 777 tokens, 128 experts, softmax 4.4, 6.6 and 4.4; 8 tokens 3.9 in one launch.
+// the vector ALUs' cycles, four wavefronts a SIMD), sums 5.5, gradient 15 (34 MB, 2.3
+// TB/s); 777 tokens, 128 experts, softmax 4.5, 6.5 and 4.5; 8 tokens 3.9 in one launch.
 
 #include "../../include/qmoe.h"
 #include "moe_route.h"
@@ -330,8 +330,14 @@ __global__ __launch_bounds__(256) void balance_grad_kernel(const BalanceGradPara
   }
 }
 
-// workgroups and wavefronts of the forward launch: one token per wavefront while
-// there are fewer than four wavefronts per CU, then sixteen per workgroup, so that the parts stay few
+// workgroups and wavefronts of the forward launch. Up to 32 tokens one workgroup, two tokens
+// per wavefront, and no second launch: 17 tokens x 128, softmax 5.5 us (two launches 7.8), 32
+// tokens 7.5 (8.0), 48 tokens 10.1 (8.0); of 256 experts in groups, whose choice takes
+// longer, 17 tokens 11.6 (11.7), but 24 tokens 12.7 (12.0) and 32 tokens 17.4 (11.7). Then one
+// token per wavefront while there are fewer than four wavefronts per CU, in workgroups
+// of four (of sixteen: 300 x 128 8.7 -> 9.6, 1024 x 256 in groups 12.7 -> 16.5), above that of
+// sixteen, so that the parts stay few (of four: 1025 x 128 10.2 -> 9.4, 4096 x 128 10.5 -> 12.8, 16384
+// x 256 36.8 -> 69.4). 256 workgroups at most: 16384 x 256 by 128 63.7, by 512 41.4.
 int balance_groups(int64_t T, int* waves) {
   if (T <= kOneGroup) {
     *waves = (int)(T < 16 ? T : 16);
@@ -359,6 +365,8 @@ void launch_balance(int scoring, bool grouped, int groups, int waves, const Bala
 
 template <int S>
 void launch_balance_grad(int scoring, const BalanceGradParams& p, hipStream_t st) {
+  // (65536 tokens x 128 / x 256: 28.7 / 37.7 us, by 1024 workgroups 33.4 / 43.7, by 16384 32.5 / 40.3;
+  // no difference up to 16384 tokens)
   const int64_t g = cdiv<int64_t>(p.T, 4);
   const dim3 grid((unsigned)(g < 4096 ? g : 4096)), block(256);
   if (scoring == 0) hipLaunchKernelGGL((balance_grad_kernel<S, 0>), grid, block, 0, st, p);

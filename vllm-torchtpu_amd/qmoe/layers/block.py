@@ -118,7 +118,7 @@ def _block(y, residual, gate, norm_weight, next_weight, args, keep):
 def block_norm(x, weight, eps=1e-6, weight_offset=0.0, out_dtype=None):
     """The norm before a block: x (mean x^2 + eps)^(-1/2) (weight_offset + weight)
     over the last axis of ``x`` [..., H] (bf16, f16 or f32; H up to 16384), statistics in
-    float32, rounded once to ``out_dtype`` (``x``'s type; of a float32 ``x`` also bf16
+    float32 (a row whose squares add up to infinity there gives zeros), rounded once to ``out_dtype`` (``x``'s type; of a float32 ``x`` also bf16
     or f16). Differentiable in ``x`` and ``weight``, with gradients of their types."""
     args = (1.0, 1.0, float(eps), float(weight_offset), x.dtype if out_dtype is None else out_dtype)
     if weight is None:

@@ -209,7 +209,8 @@ def balanced_experts(router_logits, topk, scoring_func="softmax", renormalize=Tr
     Experts and weights as `select_experts` chooses them (scoring "softmax",
     "sigmoid" or "sqrtsoftplus"), the weights not rounded. Over the N tokens of
     ``token_mask`` (bool [T]; None: all), with f[e] the share of their k N routes that
-    expert e has and P[e] the mean of their scores' share of e (softmax: the score):
+    expert e has and P[e] the mean of their scores' share of e (softmax: the score; else
+    over the row's sum, of at least 1e-20):
 
         balance_loss = E sum_e f[e] P[e]          (1 for an even load; 0 for N = 0)
 
@@ -217,7 +218,9 @@ def balanced_experts(router_logits, topk, scoring_func="softmax", renormalize=Tr
     gradient whatever its logits are. Differentiable in the logits through the
     weights and the loss (through P; the choice and f are constants), in their type, by
     `torch.autograd` (under functorch transforms the call is refused where a gradient is
-    asked for); the correction bias only chooses and has no gradient. The sums' order is fixed."""
+    asked for); the correction bias only chooses and has no gradient. The sums' order is
+    fixed. The fused expert layers here serve only: a gradient of the weights comes from
+    experts that are differentiable themselves."""
     if torch.is_grad_enabled() and e_score_correction_bias is not None and e_score_correction_bias.requires_grad:
         raise NotImplementedError("balanced_experts: no gradient for the correction bias, which only chooses")
     if router_logits.dtype not in (torch.bfloat16, torch.float32) and router_logits.is_floating_point():
