@@ -52,15 +52,11 @@ def _eight(x):
 @pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 13, 72])
 @pytest.mark.parametrize("bias", [None, F16, F32])
-@pytest.mark.parametrize("before", [False, True])
-def test_a_loaded_layer_made_trainable(dev, n, bias, before):
+def test_a_loaded_layer_made_trainable(dev, n, bias):
     T, K = 37, 96
     layer, rand = _layer(n, K, dev, n)
-    if before:
-        layer.weight.requires_grad_()
     METHOD.process_weights_after_loading(layer)
-    if not before:
-        layer.weight.requires_grad_()
+    layer.weight.requires_grad_()
     assert layer.weight.requires_grad and layer.weight.is_leaf and layer.weight.is_cuda
     x = (2 * rand(T, K)).round().clamp(-8, 8).to(BF16).requires_grad_()
     b = None if bias is None else rand(n).to(bias).requires_grad_()
@@ -83,8 +79,10 @@ def test_a_loaded_layer_made_trainable(dev, n, bias, before):
 
 @pytest.mark.gpu
 def test_a_loaded_layer_is_frozen(dev):
-    """... as it comes: the input's gradient alone, and nothing of the input kept."""
+    """... as it comes, also where the weight was trainable before: the input's gradient
+    alone, and nothing of the input kept."""
     layer, rand = _layer(72, 96, dev, 1)
+    layer.weight.requires_grad_()
     METHOD.process_weights_after_loading(layer)
     assert not layer.weight.requires_grad
     x = rand(20, 96).to(BF16).requires_grad_()

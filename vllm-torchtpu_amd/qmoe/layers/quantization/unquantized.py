@@ -20,8 +20,7 @@ class UnquantizedLinearMethod:
                                                               dtype=params_dtype)))
 
     def process_weights_after_loading(self, layer):
-        trained = layer.weight.requires_grad  # (frozen unless it was made trainable before)
-        layer.weight = _param(layer.weight.data.to(_device(), torch.bfloat16).contiguous()).requires_grad_(trained)
+        layer.weight = _param(layer.weight.data.to(_device(), torch.bfloat16).contiguous())
 
     def apply(self, layer, x, bias=None):
         k = x.shape[-1]
@@ -36,9 +35,9 @@ class UnquantizedLinearMethod:
         gradient ``x`` waits in 8 bits (`qmoe.layers.block.checkpointed_linear`): bf16,
         the bias added before the one rounding.
 
-        `create_weights` makes a frozen weight, which gets no gradient and keeps nothing
-        of ``x``; ``layer.weight.requires_grad_()`` makes it trainable, before or after
-        loading. An output size that is not a multiple of 8 is padded with rows of
+        Loading leaves a frozen weight, which gets no gradient and keeps nothing of ``x``;
+        ``layer.weight.requires_grad_()`` after `process_weights_after_loading` makes it
+        trainable. An output size that is not a multiple of 8 is padded with rows of
         zeros, a copy of the weight in every call."""
         x, w, n = x.to(torch.bfloat16), layer.weight, layer.weight.shape[0]
         if bias is not None and bias.dtype not in (torch.bfloat16, torch.float32):
