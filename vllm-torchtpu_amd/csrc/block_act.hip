@@ -179,7 +179,8 @@ __global__ __launch_bounds__(512) void pack_kernel(const ActParams p) {
 }
 
 // threads of 8 columns, in whole groups of four: as few workgroups per row as
-// take 512 at most, alike
+// take 512 at most, alike (8192 x 14336: 194 / 189 us, at most 256 192 / 186, at most 128
+// 212 / 194; 777 x 2880 5.4 / 4.7 each)
 dim3 row_grid(int64_t T, int64_t I, dim3* block) {
   const int64_t n = cdiv<int64_t>(I, 32) * 4;
   const int64_t parts = cdiv<int64_t>(n, 512);
